@@ -206,6 +206,87 @@ int    lag_hip_head_argmax(const void *Wc, int w_bf16, const float *x, int S, in
 /* tok[s] = argmax_logits' pick over logits[s, 0..V) alone (c/laguna.c:1159).  0 = ok */
 int    lag_hip_argmax(const float *logits, int S, int V, int *tok);
 
+/* ---------------- attention over a paged cache (device pointers, queued on the backend stream) ----------------
+ * The attention half of a layer's decode step: the projection's heads normalised, turned and
+ * appended to the cache, then one new token of each row against its sequence's cells.  No
+ * counterpart in the reference's lag table (its engines keep attention on the CPU). */
+enum { LAG_HIP_KV_F32 = 0, LAG_HIP_KV_BF16 = 1, LAG_HIP_KV_F16 = 2 };
+/* One layer's cache: pools of n_pages pages of page_size tokens (a power of two, 8 to 4096)
+ * of n_heads heads of head_dim values (a multiple of 32, at most 256).  The values of head g,
+ * slot i of page p begin at element p * page_stride + g * head_stride + i * token_stride of k
+ * and of v; the strides are in elements and a head's values side by side, so a page may be
+ * [head][token][value] or [token][head][value], and both pools may lie in one allocation.
+ * Pools and strides are multiples of 16 bytes, and cells do not overlap. */
+typedef struct {
+    void   *k, *v;
+    int     type;                               /* LAG_HIP_KV_* */
+    int     n_pages, page_size, n_heads, head_dim;
+    int64_t page_stride, head_stride, token_stride;
+} LagHipKvCache;
+/* The rows of a batch (device arrays): row s is the token at position pos[s] of sequence
+ * seq[s] (seq NULL: sequence s), whose token t lies in page table[seq * max_pages +
+ * t / page_size], slot t % page_size.  pos[s] < 0: a free place, no row.  max_pages *
+ * page_size <= 2^30.  What the arrays hold is read on the device, at the time of the launch
+ * or replay: a sequence outside [0, n_seqs), a position beyond the table or a page outside
+ * the pool has no cell (nothing is written there and nothing attended to). */
+typedef struct {
+    const int *pos, *seq, *table;
+    int n_seqs, max_pages;
+} LagHipKvRows;
+/* Rotary positions of the first `dims` values of each head (even, 0: none, at most head_dim):
+ * pair i, values (i, i + dims/2) or, interleaved, (2i, 2i + 1), turns by pos * freq[i] radians
+ * (freq: device, [dims/2] doubles, so that a caller scales them for long contexts as it
+ * likes; the angle is taken in 64 bits), times factor. */
+typedef struct {
+    const double *freq;
+    int   dims, interleaved;
+    float factor;
+} LagHipRope;
+/* qkv [S][ld]: row s holds n_q_heads q heads, then n_heads k heads, then n_heads v heads.  q
+ * and k heads are normalised, x / sqrt(mean(x^2) + eps) * q_norm or k_norm ([head_dim], NULL:
+ * not), and turned; q to q_out [S][n_q_heads][head_dim], k and v rounded to nearest into the
+ * row's cell.  n_q_heads is a multiple of n_heads, ld of 4; qkv and q_out are 16-byte aligned
+ * and do not overlap.  Rows without a place leave q_out and the cache as they were; two rows
+ * of one cell are the caller's mistake (the cell holds values of both).  0 = ok */
+int    lag_hip_qk_rope_append(const LagHipKvCache *c, const LagHipKvRows *r, const LagHipRope *rope, const float *qkv,
+                              int64_t ld, const float *q_norm, const float *k_norm, float eps, int n_q_heads, float *q_out,
+                              int S);
+/* out[s][h] = sum_t p_t v_t, p the softmax of scale * q[s][h] . k_t over the cells t <= pos[s]
+ * of row s (t > pos[s] - window with window > 0), head h reading cache head h / (n_q_heads /
+ * n_heads); q and out [S][n_q_heads][head_dim], 16-byte aligned, not overlapping.  Sums and
+ * the softmax in 32 bits.  A free place, or a row without any cell, gives zeros.  Rows of one
+ * sequence at consecutive positions (a chunk of a prompt, already appended) each see what is
+ * theirs to see.  Infinities and NaN in a cell reach the rows that attend to it, as values
+ * without meaning, and no others; cells that no row attends to may hold anything.  A row's bits depend on S, n_q_heads and max_pages * page_size, not on the
+ * other rows' values.  0 = ok */
+int    lag_hip_attn_paged(const LagHipKvCache *c, const LagHipKvRows *r, const float *q, int n_q_heads, float scale,
+                          int window, float *out, int S);
+/* Page src[i] of every one of n_layers caches (one geometry and type) to page dst[i], k and v:
+ * a fork's last page, or pages moved together.  src and dst are host arrays, free to change
+ * on return; a dst is named once and is no src.  0 = ok */
+int    lag_hip_kv_copy_pages(const LagHipKvCache *layers, int n_layers, const int *src, const int *dst, int n);
+/* x[i] += t[i] for n values: the residual after an output projection.  0 = ok */
+int    lag_hip_add(float *x, const float *t, size_t n);
+
+/* ---------------- sampling ----------------
+ * Settings of a batch's rows, device arrays [S], each may be NULL: temperature (NULL 1; <= 0
+ * or NaN: the greedy pick of lag_hip_argmax), top_k (NULL, <= 0 or >= V: off), top_p (NULL,
+ * >= 1 or NaN: off), min_p (NULL, <= 0 or NaN: off). */
+typedef struct {
+    const float *temperature;
+    const int   *top_k;
+    const float *top_p, *min_p;
+} LagHipSample;
+/* tok[s] = a token of logits[s, 0..V) drawn by u[s] in [0, 1): weights w_i = exp((l_i - max) /
+ * temperature); of the tokens in order of falling logit (equal ones by rising index) the
+ * first top_k, of those the shortest beginning with at least top_p of their weight (at least
+ * one token), of those the weights >= min_p * the largest; the pick is the lowest index at which the
+ * kept weights' sum in order of index exceeds u * their total.  Weights are whole numbers of
+ * 2^-42 of the largest, so the sums are exact and the pick the same in every run and batch;
+ * V <= 2^20.  -inf and NaN are never picked; a row that holds nothing else gives
+ * lag_hip_argmax's pick.  0 = ok */
+int    lag_hip_sample(const float *logits, int S, int V, const LagHipSample *p, const float *u, int *tok);
+
 /* ---------------- memory, stream, timing ---------------- */
 void  *lag_hip_alloc(size_t n);
 int    lag_hip_h2d(void *dst, const void *src, size_t n);

@@ -30,6 +30,7 @@ EXPORTS = [
     "lag_hip_moe_forward_scratch_bytes",
     "lag_hip_moe_block", "lag_hip_route",
     "lag_hip_last_groups", "lag_hip_rmsnorm", "lag_hip_moe_forward_rmsnorm", "lag_hip_head_argmax", "lag_hip_argmax", "lag_hip_set_grouped_kernel",
+    "lag_hip_qk_rope_append", "lag_hip_attn_paged", "lag_hip_kv_copy_pages", "lag_hip_add", "lag_hip_sample",
     "lag_hip_set_q4_mode",
     "lag_hip_alloc", "lag_hip_h2d", "lag_hip_d2h", "lag_hip_d2d", "lag_hip_memset",
     "lag_hip_graph_begin", "lag_hip_graph_end", "lag_hip_graph_launch", "lag_hip_graph_destroy", "lag_hip_sync",
@@ -60,6 +61,31 @@ class LagHipMoeDesc(C.Structure):
 class LagHipMoeWeights(C.Structure):
     _fields_ = [("router", VP), ("corr_bias", VP), ("logit_bias", VP), ("gu_q", VP), ("gu_s", VP),
                 ("dn_q", VP), ("dn_s", VP), ("sg", VP), ("su", VP), ("sd", VP)]
+
+
+KV_TYPES = {"f32": 0, "bf16": 1, "f16": 2}
+
+
+class LagHipKvCache(C.Structure):
+    _fields_ = [("k", VP), ("v", VP), ("type", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int),
+                ("n_heads", C.c_int), ("head_dim", C.c_int), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("token_stride", C.c_int64)]
+
+
+class LagHipKvRows(C.Structure):
+    _fields_ = [("pos", VP), ("seq", VP), ("table", VP), ("n_seqs", C.c_int), ("max_pages", C.c_int)]
+
+
+class LagHipRope(C.Structure):
+    _fields_ = [("freq", VP), ("dims", C.c_int), ("interleaved", C.c_int), ("factor", C.c_float)]
+
+
+class LagHipSample(C.Structure):
+    _fields_ = [("temperature", VP), ("top_k", VP), ("top_p", VP), ("min_p", VP)]
+
+
+def _ptr(b):
+    return int(b) if b is not None else None
 
 
 def desc_of(cfg):
@@ -108,6 +134,12 @@ def load_library(path=None):
     L.lag_hip_rmsnorm.argtypes = [VP, VP, VP, C.c_int, C.c_int, C.c_float]
     L.lag_hip_head_argmax.argtypes = [VP, C.c_int, VP, C.c_int, C.c_int, C.c_int, VP, VP]
     L.lag_hip_argmax.argtypes = [VP, C.c_int, C.c_int, VP]
+    KP, RP = C.POINTER(LagHipKvCache), C.POINTER(LagHipKvRows)
+    L.lag_hip_qk_rope_append.argtypes = [KP, RP, C.POINTER(LagHipRope), VP, C.c_int64, VP, VP, C.c_float, C.c_int, VP, C.c_int]
+    L.lag_hip_attn_paged.argtypes = [KP, RP, VP, C.c_int, C.c_float, C.c_int, VP, C.c_int]
+    L.lag_hip_kv_copy_pages.argtypes = [KP, C.c_int, VP, VP, C.c_int]
+    L.lag_hip_add.argtypes = [VP, VP, C.c_size_t]
+    L.lag_hip_sample.argtypes = [VP, C.c_int, C.c_int, C.POINTER(LagHipSample), VP, VP]
     DP, WP = C.POINTER(LagHipMoeDesc), C.POINTER(LagHipMoeWeights)
     L.lag_hip_moe_forward.argtypes = [DP, WP, VP, VP, C.c_int]
     L.lag_hip_moe_forward_rmsnorm.argtypes = [DP, WP, VP, C.c_float, VP, VP, C.c_int]
@@ -294,6 +326,58 @@ class Backend:
 
     def argmax(self, logits_dev, S, V, tok_dev):
         self.check(self.lib.lag_hip_argmax(VP(int(logits_dev)), S, V, VP(int(tok_dev))), "lag_hip_argmax")
+
+    # ---- attention over a paged cache, sampling (device pointers) ----
+    # The descriptors are plain structs of device addresses: a caller makes them once and keeps
+    # the buffers they name alive.
+    @staticmethod
+    def kv_cache(k, v, type, n_pages, page_size, n_heads, head_dim, strides=None):
+        """one layer's cache; strides: (page, head, token) in elements, default [page][head][token][value]"""
+        ps, hs, ts = strides or (n_heads * page_size * head_dim, page_size * head_dim, head_dim)
+        return LagHipKvCache(int(k), int(v), KV_TYPES[type], n_pages, page_size, n_heads, head_dim, ps, hs, ts)
+
+    @staticmethod
+    def kv_caches(caches):
+        """the caches of several layers as kv_copy_pages takes them"""
+        return (LagHipKvCache * len(caches))(*caches)
+
+    @staticmethod
+    def kv_rows(pos_dev, table_dev, n_seqs, max_pages, seq_dev=None):
+        return LagHipKvRows(int(pos_dev), _ptr(seq_dev), int(table_dev), n_seqs, max_pages)
+
+    @staticmethod
+    def rope(freq_dev, dims, interleaved=False, factor=1.0):
+        return LagHipRope(_ptr(freq_dev), dims, int(interleaved), factor)
+
+    @staticmethod
+    def sample_params(temperature=None, top_k=None, top_p=None, min_p=None):
+        """device arrays of one value per row (f32, int32, f32, f32), None: off"""
+        return LagHipSample(_ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p))
+
+    def qk_rope_append(self, cache, rows, rope, qkv_dev, ld, q_norm, k_norm, eps, n_q_heads, q_out_dev, S):
+        """q and k heads normalised and turned, q to q_out_dev, k and v into the rows' cells"""
+        self.check(self.lib.lag_hip_qk_rope_append(cache, rows, rope, int(qkv_dev), ld, _ptr(q_norm), _ptr(k_norm), eps,
+                                                   n_q_heads, int(q_out_dev), S), "lag_hip_qk_rope_append")
+
+    def attn_paged(self, cache, rows, q_dev, n_q_heads, scale, window, out_dev, S):
+        """one new token of each row against its sequence's cells (window 0: all of them)"""
+        self.check(self.lib.lag_hip_attn_paged(cache, rows, int(q_dev), n_q_heads, scale, window, int(out_dev), S),
+                   "lag_hip_attn_paged")
+
+    def kv_copy_pages(self, caches, src, dst):
+        """pages src[i] -> dst[i] of every layer (caches from kv_caches; host indices)"""
+        src, dst = np.ascontiguousarray(src, np.int32).reshape(-1), np.ascontiguousarray(dst, np.int32).reshape(-1)
+        if src.size != dst.size:
+            raise ValueError("kv_copy_pages: as many destinations as sources")
+        self.check(self.lib.lag_hip_kv_copy_pages(caches, len(caches), src.ctypes.data, dst.ctypes.data, src.size),
+                   "lag_hip_kv_copy_pages")
+
+    def add(self, x_dev, t_dev, n):
+        self.check(self.lib.lag_hip_add(int(x_dev), int(t_dev), n), "lag_hip_add")
+
+    def sample(self, logits_dev, S, V, params, u_dev, tok_dev):
+        """a token of each row by its settings (sample_params, or None) and random number"""
+        self.check(self.lib.lag_hip_sample(int(logits_dev), S, V, params, int(u_dev), int(tok_dev)), "lag_hip_sample")
 
     def last_groups(self, cap=4096):
         G = C.c_int(0)

@@ -8,6 +8,7 @@
 // forward keeps routing, bucketing and the combine on the GPU.
 #include "sw_hip.h"
 #include "sw_shared.h"
+#include "sw_attn.h"
 #include "../../include/sabrewing_hip.h"
 #include <stdio.h>
 #include <stdlib.h>
@@ -934,6 +935,152 @@ extern "C" int lag_hip_head_argmax(const void *Wc, int w_bf16, const float *x, i
         PROF("argmax");
         if (sw_launch_argmax(g_st, logits, S, V, tok)) return fail_msg("argmax launch");
     }
+    return 0;
+}
+
+// ------------------------------------------------------------ attention over a paged cache ----
+// the caller's cache as the kernels take it; NULL or the reason it is refused
+static const char *kv_of(const LagHipKvCache *c, SwKv &o) {
+    if (!c || !c->k || !c->v) return "no pools";
+    if (c->type < LAG_HIP_KV_F32 || c->type > LAG_HIP_KV_F16) return "unknown element type";
+    if (c->n_pages < 1 || c->n_heads < 1 || c->n_heads > 1024) return "page or head count";
+    if (c->head_dim < 32 || c->head_dim > 256 || c->head_dim % 32) return "head_dim (a multiple of 32, at most 256)";
+    if (c->page_size < 8 || c->page_size > 4096 || (c->page_size & (c->page_size - 1)))
+        return "page_size (a power of two, 8 to 4096)";
+    const int64_t per = c->type == LAG_HIP_KV_F32 ? 4 : 8;               // elements in 16 bytes
+    if (((uintptr_t)c->k | (uintptr_t)c->v) % 16 || c->page_stride % per || c->head_stride % per || c->token_stride % per)
+        return "pools and strides must be multiples of 16 bytes";
+    // cells side by side or apart: each stride, in rising order, past the whole extent of the one before
+    struct { int64_t n, s; } d[3] = {{c->page_size, c->token_stride}, {c->n_heads, c->head_stride}, {c->n_pages, c->page_stride}};
+    for (int i = 0; i < 3; i++)
+        for (int j = i + 1; j < 3; j++)
+            if (d[j].s < d[i].s) { const auto t = d[i]; d[i] = d[j]; d[j] = t; }
+    int64_t extent = c->head_dim;
+    for (auto &x : d) {
+        if (x.n == 1) continue;
+        if (x.s < extent || x.s > ((int64_t)1 << 60) / x.n) return "strides that overlap";
+        extent += x.s * (x.n - 1);
+    }
+    o = {c->k, c->v, c->type, c->n_pages, __builtin_ctz((unsigned)c->page_size), c->n_heads, c->head_dim,
+         c->page_stride, c->head_stride, c->token_stride};
+    return nullptr;
+}
+static const char *rows_of(const LagHipKvRows *r, int page_size, int S, SwRows &o) {
+    if (!r || !r->pos || !r->table) return "no positions or page table";
+    if (S < 1 || r->n_seqs < 1 || r->max_pages < 1) return "row, sequence or page count";
+    if (!r->seq && S > r->n_seqs) return "more rows than sequences";
+    if ((int64_t)r->max_pages * page_size > (1 << 30)) return "max_pages * page_size over 2^30";
+    o = {r->pos, r->seq, r->table, r->n_seqs, r->max_pages};
+    return nullptr;
+}
+static int refuse(const char *who, const char *why) {
+    snprintf(g_err, sizeof g_err, "%s: %s", who, why);
+    return -1;
+}
+// (after an entry's checks of its arguments, which need no device)
+static bool not_ready(const char *who) {
+    if (!g_ok) return refuse(who, "backend not initialised") != 0;
+    return fault_injected() && refuse(who, "injected fault") != 0;
+}
+static bool apart(const void *a, size_t na, const void *b, size_t nb) {
+    return (uintptr_t)a + na <= (uintptr_t)b || (uintptr_t)b + nb <= (uintptr_t)a;
+}
+
+extern "C" int lag_hip_qk_rope_append(const LagHipKvCache *c, const LagHipKvRows *r, const LagHipRope *rope, const float *qkv,
+                                      int64_t ld, const float *q_norm, const float *k_norm, float eps, int Hq, float *q_out,
+                                      int S) {
+    static const char *me = "qk_rope_append";
+    SwKv kv;
+    SwRows rows;
+    if (const char *why = kv_of(c, kv)) return refuse(me, why);
+    if (const char *why = rows_of(r, c->page_size, S, rows)) return refuse(me, why);
+    if (!qkv || !q_out || ((uintptr_t)qkv | (uintptr_t)q_out) % 16 || ld % 4) return refuse(me, "qkv and q_out must be 16-byte aligned rows");
+    if (Hq < 1 || Hq > 1024 || Hq % c->n_heads) return refuse(me, "n_q_heads (a multiple of n_heads)");
+    if (ld < (int64_t)(Hq + 2 * c->n_heads) * c->head_dim || ld > (int64_t)1 << 31) return refuse(me, "ld shorter than a row");
+    const int dims = rope ? rope->dims : 0;
+    if (dims < 0 || dims > c->head_dim || dims % 2 || (dims && !rope->freq)) return refuse(me, "rope dims (even, at most head_dim)");
+    if (!apart(qkv, ((size_t)(S - 1) * ld + (Hq + 2 * c->n_heads) * c->head_dim) * 4, q_out, (size_t)S * Hq * c->head_dim * 4))
+        return refuse(me, "qkv and q_out overlap");
+    const SwRope ro = {dims ? rope->freq : nullptr, dims / 2, dims ? rope->interleaved != 0 : 0, dims ? rope->factor : 1.f};
+    if (not_ready(me)) return -1;
+    PROF("qk_rope_append");
+    if (sw_launch_qk_rope_append(g_st, kv, rows, ro, qkv, ld, q_norm, k_norm, eps, Hq, q_out, S)) return fail_msg("qk_rope_append launch");
+    return 0;
+}
+
+extern "C" int lag_hip_attn_paged(const LagHipKvCache *c, const LagHipKvRows *r, const float *q, int Hq, float scale,
+                                  int window, float *out, int S) {
+    static const char *me = "attn_paged";
+    SwKv kv;
+    SwRows rows;
+    if (const char *why = kv_of(c, kv)) return refuse(me, why);
+    if (const char *why = rows_of(r, c->page_size, S, rows)) return refuse(me, why);
+    if (!q || !out || ((uintptr_t)q | (uintptr_t)out) % 16) return refuse(me, "q and out must be 16-byte aligned");
+    if (Hq < 1 || Hq > 1024 || Hq % c->n_heads) return refuse(me, "n_q_heads (a multiple of n_heads)");
+    if (window < 0) return refuse(me, "negative window");
+    const size_t n = (size_t)S * Hq * c->head_dim * 4;
+    if (!apart(q, n, out, n)) return refuse(me, "q and out overlap");
+    if (not_ready(me)) return -1;
+    PROF("attn_paged");
+    if (sw_launch_attn(g_st, kv, rows, q, Hq, scale, window, out, S)) return fail_msg("attn_paged launch");
+    return 0;
+}
+
+extern "C" int lag_hip_kv_copy_pages(const LagHipKvCache *layers, int n_layers, const int *src, const int *dst, int n) {
+    static const char *me = "kv_copy_pages";
+    if (!layers || n_layers < 1 || n < 0 || (n && (!src || !dst))) return refuse(me, "no layers or pages");
+    SwKv kv[SW_COPY_LAYERS];
+    for (int l = 0; l < n_layers; l++) {
+        SwKv one;
+        if (const char *why = kv_of(layers + l, one)) return refuse(me, why);
+        const LagHipKvCache &a = layers[0], &b = layers[l];
+        if (a.type != b.type || a.n_pages != b.n_pages || a.page_size != b.page_size || a.n_heads != b.n_heads ||
+            a.head_dim != b.head_dim || a.page_stride != b.page_stride || a.head_stride != b.head_stride ||
+            a.token_stride != b.token_stride)
+            return refuse(me, "layers of different geometry");
+    }
+    if (n > layers[0].n_pages) return refuse(me, "a destination named twice, or also a source");
+    // each page: 1 a source, 2 a destination
+    unsigned char *mark = (unsigned char *)calloc((size_t)layers[0].n_pages, 1);
+    if (!mark) return refuse(me, "out of host memory");
+    const char *why = nullptr;
+    for (int i = 0; i < n && !why; i++) {
+        if (src[i] < 0 || src[i] >= layers[0].n_pages || dst[i] < 0 || dst[i] >= layers[0].n_pages) why = "a page outside the pool";
+        else mark[src[i]] |= 1;
+    }
+    for (int i = 0; i < n && !why; i++) {
+        if (mark[dst[i]]) why = "a destination named twice, or also a source";
+        else mark[dst[i]] = 2;
+    }
+    free(mark);
+    if (why) return refuse(me, why);
+    if (not_ready(me)) return -1;
+    PROF("kv_copy_pages");
+    for (int l = 0; l < n_layers; l += SW_COPY_LAYERS) {
+        const int nl = n_layers - l < SW_COPY_LAYERS ? n_layers - l : SW_COPY_LAYERS;
+        for (int i = 0; i < nl; i++) (void)kv_of(layers + l + i, kv[i]);
+        for (int i = 0; i < n; i += SW_COPY_PAIRS)
+            if (sw_launch_kv_copy(g_st, kv, nl, src + i, dst + i, n - i < SW_COPY_PAIRS ? n - i : SW_COPY_PAIRS))
+                return fail_msg("kv_copy_pages launch");
+    }
+    return 0;
+}
+
+extern "C" int lag_hip_add(float *x, const float *t, size_t n) {
+    if (!g_ok || fault_injected() || !x || !t || !n) return -1;
+    PROF("add");
+    if (sw_launch_add(g_st, x, t, n)) return fail_msg("add launch");
+    return 0;
+}
+
+extern "C" int lag_hip_sample(const float *logits, int S, int V, const LagHipSample *p, const float *u, int *tok) {
+    static const char *me = "sample";
+    if (!logits || !u || !tok || S < 1 || V < 1) return refuse(me, "no logits, random numbers or tokens");
+    if (V > 1 << 20) return refuse(me, "V over 2^20");
+    const SwSample sp = p ? SwSample{p->temperature, p->top_k, p->top_p, p->min_p} : SwSample{};
+    if (not_ready(me)) return -1;
+    PROF("sample");
+    if (sw_launch_sample(g_st, logits, S, V, sp, u, tok)) return fail_msg("sample launch");
     return 0;
 }
 

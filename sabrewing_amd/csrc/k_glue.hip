@@ -94,3 +94,27 @@ int sw_launch_argmax(hipStream_t st, const float *logits, int S, int V, int *tok
     SW_LAUNCH(k_argmax, dim3((unsigned)S), dim3(AM_NT), 0, st, logits, V, tok);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
+
+// x[i] += t[i], four values per thread where both begin on 16 bytes
+__global__ __launch_bounds__(256) void k_add(float *__restrict__ x, const float *__restrict__ t, size_t n, int by4) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (by4) {
+        if (4 * i + 4 <= n) {
+            sw_f32x4 a = ((sw_f32x4 *)x)[i];
+            const sw_f32x4 b = ((const sw_f32x4 *)t)[i];
+#pragma unroll
+            for (int c = 0; c < 4; c++) a[c] = a[c] + b[c];
+            ((sw_f32x4 *)x)[i] = a;
+        } else {
+            for (size_t j = 4 * i; j < n; j++) x[j] = x[j] + t[j];
+        }
+    } else if (i < n) x[i] = x[i] + t[i];
+}
+
+int sw_launch_add(hipStream_t st, float *x, const float *t, size_t n) {
+    const int by4 = ((uintptr_t)x | (uintptr_t)t) % 16 == 0;
+    const size_t m = by4 ? (n + 3) / 4 : n;
+    if (m > ((size_t)1 << 31) * 128) return -1;
+    SW_LAUNCH(k_add, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, st, x, t, n, by4);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}

@@ -438,6 +438,8 @@ int sw_launch_idot_glu(hipStream_t st, SwQ4 W, const uint32_t *xi, const float *
 int sw_launch_idot_rows(hipStream_t st, SwQ4 W, const uint32_t *xi, const float *xs, SwGroups g, float *Y);
 int sw_launch_rmsnorm(hipStream_t st, const float *x, const float *w, float *out, int S, int D, float eps);
 int sw_launch_argmax(hipStream_t st, const float *logits, int S, int V, int *tok);
+// x[i] += t[i]
+int sw_launch_add(hipStream_t st, float *x, const float *t, size_t n);
 // the shared expert of a batch on the bf16 MFMA (k_shared.hip): the three bf16 parts of
 // rows of x ([S][K/32][3][32]); h = silu(Wg x) * (Wu x) as its parts; out = Wd h (f32)
 int sw_launch_sh_parts(hipStream_t st, const float *x, int S, int K, uint16_t *parts);
