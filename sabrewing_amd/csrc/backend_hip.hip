@@ -1021,8 +1021,10 @@ extern "C" int lag_hip_attn_paged(const LagHipKvCache *c, const LagHipKvRows *r,
     const size_t n = (size_t)S * Hq * c->head_dim * 4;
     if (!apart(q, n, out, n)) return refuse(me, "q and out overlap");
     if (not_ready(me)) return -1;
+    const int64_t np = sw_attn_part_floats(kv, rows, Hq, window, S);
+    if (np && grow_dev(g_arena, (size_t)np * 4)) return -1;
     PROF("attn_paged");
-    if (sw_launch_attn(g_st, kv, rows, q, Hq, scale, window, out, S)) return fail_msg("attn_paged launch");
+    if (sw_launch_attn(g_st, kv, rows, q, Hq, scale, window, out, S, np ? (float *)g_arena.p : nullptr)) return fail_msg("attn_paged launch");
     return 0;
 }
 

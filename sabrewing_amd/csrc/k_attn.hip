@@ -1,63 +1,434 @@
 // k_attn.hip -- attention of one new token of each row over a paged cache:
 // out[s, h] = sum_t p_t v_t, p = softmax over t in (pos - window, pos] of scale * q[s, h] . k_t.
+//
+// One pass over the cells with the running maximum and sum of the softmax.  A cell is read
+// once for all the query heads that share it, and both products run on the matrix cores: 32 tokens by
+// up to 16 heads (16 tokens of a 32-bit cache).  Bytes bound it: 512 bytes of k and v of a
+// token take some 25 cycles of a CU's matrix cores and 55 of its share of the memory.
+//
+// 32-bit accuracy from 16-bit products: q and p are 32-bit and are split into parts of the
+// cache's type, whose products with a cell are exact in the 32-bit sums.  bf16: three parts of 8
+// bits, nothing is lost.  f16: q is first scaled by a power of two to 2^13..2^14 and p by 2^13, so that
+// two parts hold 22 bits (a relative 2^-23) of all that matters beside the largest.  f32
+// caches use the f32 matrix instruction.
+//
+// The layout needs no shared memory between the two products: lane l = 16 g + c of the
+// scores' tile holds head c and tokens 4g .. 4g+3, just what the second product's right
+// operand wants as its elements of the summed index, whose order is free.  So v's rows are
+// loaded for these tokens, 16 bytes of a row per lane, and a lane transposes its
+// 8 tokens x 8 values by byte permutations in registers.
 #include "sw_attn.h"
 
-// One block per (row, head), a wave per token in turn, a lane 1 to 4 of the head's values;
-// each wave keeps the running maximum, sum and output of its tokens, and the waves join at
-// the end.  All in 32 bits.
 #define AT_NT 256
+#define AT_NW (AT_NT / 64)
+
+// bytes of a lane per row: 16-byte pieces first, then 8 and 4; the byte of row `rr` at dword w
+template <int RB>
+__host__ __device__ constexpr int at_vbyte(int w, int rr) {
+    const int full = RB / 256, rem = RB % 256, x = w - 4 * full;
+    return x < 0 ? (w / 4) * 256 + rr * 16 + (w % 4) * 4
+         : rem >= 128 ? (x < 2 ? full * 256 + rr * 8 + x * 4 : full * 256 + 128 + rr * 4)
+                      : full * 256 + rr * 4;
+}
+// a value and its partner's 16 or 32 lanes away (as a pair in no order): each swap exchanges
+// the rows of 16, or the halves, of two registers.  (The second register is hidden from the compiler,
+// which takes the swap of a register with itself for no change.)
+template <int BY>
+__device__ __forceinline__ float2 at_pair(float x) {
+    const uint32_t a = __builtin_bit_cast(uint32_t, x);
+    uint32_t b = a;
+    asm("" : "+v"(b));
+    const auto r = BY == 16 ? __builtin_amdgcn_permlane16_swap(a, b, false, false) : __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    return make_float2(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float at_max4(float x) {           // over the four lanes of a head
+    const float2 a = at_pair<16>(x), b = at_pair<32>(fmaxf(a.x, a.y));
+    return fmaxf(b.x, b.y);
+}
+__device__ __forceinline__ float at_sum4(float x) {
+    const float2 a = at_pair<16>(x), b = at_pair<32>(a.x + a.y);
+    return b.x + b.y;
+}
+
+// parts of 8 values: three bf16 (by truncation: each takes the next 8 bits, exact) or two f16
 template <int TYPE>
-__global__ __launch_bounds__(AT_NT) void k_attn(SwKv c, SwRows r, const float *__restrict__ q, int Hq, float scale, int window,
-                                                float *__restrict__ out) {
-    __shared__ float sm[4], sl[4], so[4][256];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = blockIdx.x, h = blockIdx.y;
-    const int hk = h / (Hq / c.Hkv), pos = r.pos[s], sq = r.seq ? r.seq[s] : s;
-    const int first = window > 0 && pos >= window ? pos - window + 1 : 0;
-    const int last = min(pos, (r.max_pages << c.psh) - 1);             // (the host keeps that below 2^30)
-    const int64_t row = ((int64_t)s * Hq + h) * c.dh;
-    float qv[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+struct AtParts { static constexpr int n = TYPE == SW_KV_BF16 ? 3 : 2; };
+template <int TYPE>
+__device__ __forceinline__ void at_split(const float (&x)[8], sw_u32x4 (&o)[AtParts<TYPE>::n]) {
+    if constexpr (TYPE == SW_KV_BF16) {
+        uint32_t b[8], m[8], z[8];
 #pragma unroll
-    for (int j = 0; j < 4; j++) qv[j] = lane + 64 * j < c.dh ? q[row + lane + 64 * j] : 0.f;
-    for (int t = first + wave; t <= last; t += 4) {
-        const int page = sw_page(c, r, sq, t);
-        if (page < 0) continue;
-        const int64_t cell = (int64_t)page * c.ps + (int64_t)hk * c.hs + (int64_t)(t & ((1 << c.psh) - 1)) * c.ts;
-        float d = 0.f;
+        for (int i = 0; i < 8; i++) {
+            b[i] = __builtin_bit_cast(uint32_t, x[i]);
+            const float r1 = x[i] - __builtin_bit_cast(float, b[i] & 0xFFFF0000u);
+            m[i] = __builtin_bit_cast(uint32_t, r1);
+            z[i] = __builtin_bit_cast(uint32_t, r1 - __builtin_bit_cast(float, m[i] & 0xFFFF0000u));
+        }
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (lane + 64 * j < c.dh) d = __builtin_fmaf(qv[j], sw_kv_load<TYPE>(c.k, cell + lane + 64 * j), d);
-        for (int k = 32; k; k >>= 1) d += __shfl_xor(d, k);
-        d = d * scale;
-        const float nm = d > m || d != d ? d : m;
-        if (nm == -INFINITY) continue;                             // no weight yet
-        const float f = m == nm ? 1.f : expf(m - nm), p = expf(d - nm);
-        l = __builtin_fmaf(l, f, p);
-        m = nm;
+        for (int i = 0; i < 4; i++) {
+            o[0][i] = __builtin_amdgcn_perm(b[2 * i + 1], b[2 * i], 0x07060302);
+            o[1][i] = __builtin_amdgcn_perm(m[2 * i + 1], m[2 * i], 0x07060302);
+            o[2][i] = __builtin_amdgcn_perm(z[2 * i + 1], z[2 * i], 0x07060302);
+        }
+    } else {
+        sw_half8 hi, lo;
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (lane + 64 * j < c.dh) o[j] = __builtin_fmaf(o[j], f, p * sw_kv_load<TYPE>(c.v, cell + lane + 64 * j));
+        for (int i = 0; i < 8; i++) {
+            hi[i] = (_Float16)x[i];
+            lo[i] = (_Float16)(x[i] - (float)hi[i]);
+        }
+        o[0] = __builtin_bit_cast(sw_u32x4, hi);
+        o[1] = __builtin_bit_cast(sw_u32x4, lo);
     }
-    if (lane == 0) { sm[wave] = m; sl[wave] = l; }
+}
+template <int TYPE>
+__device__ __forceinline__ sw_f32x4 at_mfma(sw_u32x4 a, sw_u32x4 b, sw_f32x4 c) {
+    if constexpr (TYPE == SW_KV_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(sw_bf16x8, a), __builtin_bit_cast(sw_bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(sw_half8, a), __builtin_bit_cast(sw_half8, b), c, 0, 0, 0);
+}
+
+// The work of a row: its cells' chunks [c0, c0 + n), `per` of them a part, `parts` parts in use.
+struct AtWork { int first, last, c0, n, per, parts; };
+__device__ __forceinline__ AtWork at_work(const SwKv &c, const SwRows &r, int s, int window, int CT, int n_split, int min_per) {
+    AtWork w;
+    const int pos = r.pos[s], sq = r.seq ? r.seq[s] : s;
+    w.first = window > 0 && pos >= window ? pos - window + 1 : 0;
+    w.last = min(pos, (r.max_pages << c.psh) - 1);                     // (the host keeps that below 2^30)
+    if (sq < 0 || sq >= r.n_seqs) w.last = -1;
+    w.c0 = w.first / CT;
+    w.n = w.last < w.first ? 0 : w.last / CT - w.c0 + 1;
+    w.per = max(min_per, (w.n + n_split - 1) / n_split);
+    w.parts = (w.n + w.per - 1) / w.per;
+    return w;
+}
+
+// One block per (row, cache head, 16 query heads, part of the row's cells); a wave takes every
+// 4th chunk, its k of the next chunk and v of the next chunk in flight while it computes.
+template <int TYPE, int NB>
+__global__ __launch_bounds__(AT_NT, NB > 5 ? 1 : 2) void k_attn(SwKv c, SwRows r, const float *__restrict__ q, int Hq, float sc, int window,
+                                                   float *__restrict__ out, float *__restrict__ part, int n_split, int min_per) {
+    constexpr bool F32 = TYPE == SW_KV_F32;
+    constexpr int DH = 32 * NB, ES = F32 ? 4 : 2, RB = DH * ES, CT = F32 ? 16 : 32;
+    constexpr int NT = CT / 16, NS = RB / 64, ND = RB / 64, NTOK = 4 * NT, NO = DH / 16;
+    constexpr int NP = F32 ? 1 : AtParts<TYPE>::n, QN = NP * NS * 64;
+    constexpr int LD = DH + 4;                                         // a head's row in the waves' join
+    constexpr int SHB = QN * 16 > AT_NW * 16 * LD * 4 ? QN * 16 : AT_NW * 16 * LD * 4;
+    __shared__ __align__(16) char sh[SHB];
+    __shared__ float s_m[AT_NW][16], s_l[AT_NW][16], s_q[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, cl = lane & 15;
+    const int G = Hq / c.Hkv, gt = (G + 15) >> 4, per_s = c.Hkv * gt;
+    const int hg = blockIdx.x % per_s, sp = blockIdx.x / per_s % n_split, s = blockIdx.x / per_s / n_split;
+    const int hk = hg / gt, h0 = hk * G + (hg % gt) * 16, nh = min(16, G - (hg % gt) * 16);
+    const AtWork w = at_work(c, r, s, window, CT, n_split, min_per);
+    float *orow = out + ((int64_t)s * Hq + h0) * DH;
+    if (sp >= w.parts) {
+        if (sp == 0) for (int i = tid; i < nh * DH; i += AT_NT) orow[i] = 0.f;      // no cell at all
+        return;
+    }
+    // ---- q's parts in the right operand's order: [part][step][lane] of 16 bytes
+    const float *qrow = q + ((int64_t)s * Hq + h0) * DH;
+    sw_u32x4 *sq = (sw_u32x4 *)sh;
+    float up = 1.f;
+    if constexpr (TYPE == SW_KV_F16) {
+        float mx = 0.f;                                                // 16 threads a head
+        if ((tid >> 4) < nh)
+            for (int i = tid & 15; i < DH; i += 16) mx = fmaxf(mx, fabsf(qrow[(tid >> 4) * DH + i]));
+        for (int o = 8; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+        if ((tid & 15) == 0) {
+            const int e = mx > 0.f && mx < INFINITY ? 13 - ilogbf(mx) : 0;
+            s_q[tid >> 4] = ldexpf(1.f, min(max(e, -100), 100));
+        }
+        __syncthreads();
+        up = s_q[cl];
+        sc = sc / up;
+    }
+    for (int i = tid; i < NS * 64; i += AT_NT) {
+        const int st = i >> 6, d = st * (64 / ES) + g * (16 / ES);     // (256 threads: the same lane in every round)
+        if constexpr (F32) {
+            sw_f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            if (cl < nh) x = *(const sw_f32x4 *)(qrow + cl * DH + d);
+            sq[i] = __builtin_bit_cast(sw_u32x4, x);
+        } else {
+            float x[8];
 #pragma unroll
-    for (int j = 0; j < 4; j++) so[wave][lane + 64 * j] = o[j];
+            for (int j = 0; j < 8; j++) x[j] = 0.f;
+            if (cl < nh) {
+                const sw_f32x4 a = *(const sw_f32x4 *)(qrow + cl * DH + d), b = *(const sw_f32x4 *)(qrow + cl * DH + d + 4);
+#pragma unroll
+                for (int j = 0; j < 4; j++) { x[j] = a[j] * up; x[j + 4] = b[j] * up; }
+            }
+            sw_u32x4 o[NP];
+            at_split<TYPE>(x, o);
+#pragma unroll
+            for (int p = 0; p < NP; p++) sq[p * NS * 64 + i] = o[p];
+        }
+    }
     __syncthreads();
-    if ((int)threadIdx.x >= c.dh) return;
-    float M = -INFINITY, L = 0.f, O = 0.f;
-    for (int w = 0; w < 4; w++) M = sm[w] > M || sm[w] != sm[w] ? sm[w] : M;
-    for (int w = 0; w < 4; w++) {
-        if (sl[w] == 0.f && sm[w] == -INFINITY) continue;          // a wave without tokens
-        const float f = expf(sm[w] - M);
-        L = __builtin_fmaf(sl[w], f, L);
-        O = __builtin_fmaf(so[w][threadIdx.x], f, O);
+
+    const int seq = r.seq ? r.seq[s] : s, pmask = (1 << c.psh) - 1;
+    const char *kb = (const char *)c.k + (int64_t)hk * c.hs * ES + g * 16;
+    const char *vb = (const char *)c.v + (int64_t)hk * c.hs * ES;
+    struct Pages { int k[NT], v[NT]; };
+    auto pages = [&](int ch) {
+        Pages p;
+        const int t0 = ch * CT;
+        if (pmask >= CT - 1) {                                         // one page, read once for the wave
+            const int x = __builtin_amdgcn_readfirstlane(sw_page(c, r, seq, t0));
+#pragma unroll
+            for (int t = 0; t < NT; t++) p.k[t] = p.v[t] = x;
+        } else {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                p.k[t] = sw_page(c, r, seq, t0 + 16 * t + cl);
+                p.v[t] = sw_page(c, r, seq, t0 + 16 * t + 4 * g);
+            }
+        }
+        return p;
+    };
+    sw_u32x4 K[NT][NS];
+    uint32_t V[NTOK][ND];
+    // (a page that leads nowhere: page 0's cells are read in its place and weigh nothing)
+    auto load_k = [&](int ch, const Pages &p) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const char *a = kb + ((int64_t)max(p.k[t], 0) * c.ps + (int64_t)((ch * CT + 16 * t + cl) & pmask) * c.ts) * ES;
+#pragma unroll
+            for (int i = 0; i < NS; i++) K[t][i] = *(const sw_u32x4 *)(a + i * 64);
+        }
+    };
+    auto load_v = [&](int ch, const Pages &p) {
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const char *a = vb + ((int64_t)max(p.v[t], 0) * c.ps + (int64_t)((ch * CT + 16 * t + 4 * g + j) & pmask) * c.ts) * ES;
+                uint32_t (&d)[ND] = V[4 * t + j];
+#pragma unroll
+                for (int u = 0; u < RB / 256; u++) {
+                    const sw_u32x4 x = *(const sw_u32x4 *)(a + u * 256 + cl * 16);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) d[4 * u + e] = x[e];
+                }
+                constexpr int w0 = 4 * (RB / 256), b0 = RB / 256 * 256;
+                if constexpr (RB % 256 >= 128) {
+                    const uint2 x = *(const uint2 *)(a + b0 + cl * 8);
+                    d[w0] = x.x; d[w0 + 1] = x.y;
+                }
+                if constexpr (RB % 128 == 64) d[ND - 1] = *(const uint32_t *)(a + RB - 64 + cl * 4);
+            }
+    };
+
+    sw_f32x4 O[NO];
+#pragma unroll
+    for (int i = 0; i < NO; i++) O[i] = sw_f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;                                      // head cl: the maximum, this lane's part of the sum
+    const int c1 = w.c0 + min(w.n, (sp + 1) * w.per);
+    int ch = w.c0 + sp * w.per + wave;
+    if (ch < c1) {
+        Pages p = pages(ch), pn = ch + AT_NW < c1 ? pages(ch + AT_NW) : p;
+        load_k(ch, p);
+        load_v(ch, p);
+        for (; ch < c1; ch += AT_NW) {
+            const bool more = ch + AT_NW < c1;
+            Pages pnn = pn;
+            if (ch + 2 * AT_NW < c1) pnn = pages(ch + 2 * AT_NW);
+            // scores of the chunk's tokens 16 t + 4 g + j for head cl
+            sw_f32x4 S[NT];
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                S[t] = sw_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < NS; i++) {
+                    if constexpr (F32) {
+                        const sw_f32x4 a = __builtin_bit_cast(sw_f32x4, K[t][i]), b = __builtin_bit_cast(sw_f32x4, sq[i * 64 + lane]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) S[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], S[t], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < NP; u++) S[t] = at_mfma<TYPE>(K[t][i], sq[(u * NS + i) * 64 + lane], S[t]);
+                    }
+                }
+            }
+            if (more) load_k(ch + AT_NW, pn);
+            bool ok = ch * CT >= w.first && ch * CT + CT - 1 <= w.last;
+#pragma unroll
+            for (int t = 0; t < NT; t++) ok = ok && p.v[t] >= 0;
+            const bool full = __all(ok);
+            float x[NTOK], mx = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    x[4 * t + j] = S[t][j] * sc;
+                    if (!full) {
+                        const int tok = ch * CT + 16 * t + 4 * g + j;
+                        if (tok < w.first || tok > w.last || p.v[t] < 0) {
+                            x[4 * t + j] = -INFINITY;
+#pragma unroll
+                            for (int e = 0; e < ND; e++) V[4 * t + j][e] = 0;
+                        }
+                    }
+                    mx = fmaxf(mx, x[4 * t + j]);
+                }
+            const float nm = fmaxf(m, at_max4(mx));
+            if (__any(nm > m)) {                                       // some head's maximum grew
+                const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - nm);
+                l = l * f;
+#pragma unroll
+                for (int i = 0; i < NO; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) O[i][j] = O[i][j] * f;
+                m = nm;
+            }
+            const float base = m == -INFINITY ? 0.f : TYPE == SW_KV_F16 ? m - 13.f : m;
+            float pr[NTOK];
+#pragma unroll
+            for (int j = 0; j < NTOK; j++) {
+                pr[j] = __builtin_amdgcn_exp2f(x[j] - base);
+                l = l + pr[j];
+            }
+            if constexpr (F32) {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int e = 0; e < ND; e++)
+                        O[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, V[j][e]), pr[j], O[e], 0, 0, 0);
+            } else {
+                sw_u32x4 P[NP];
+                at_split<TYPE>(pr, P);
+#pragma unroll
+                for (int e = 0; e < 2 * ND; e++) {
+                    sw_u32x4 a;
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        a[i] = __builtin_amdgcn_perm(V[2 * i + 1][e / 2], V[2 * i][e / 2], e & 1 ? 0x07060302 : 0x05040100);
+#pragma unroll
+                    for (int u = 0; u < NP; u++) O[e] = at_mfma<TYPE>(a, P[u], O[e]);
+                }
+            }
+            if (more) load_v(ch + AT_NW, pn);
+            p = pn;
+            pn = pnn;
+        }
     }
-    out[row + threadIdx.x] = L == 0.f ? 0.f : O / L;
+    // ---- the waves join: outputs relative to the block's maximum, summed in the waves' order
+    l = at_sum4(l);
+    if (g == 0) { s_m[wave][cl] = m; s_l[wave][cl] = l; }
+    __syncthreads();                                                   // (also: q's parts are done with)
+    float M = s_m[0][cl];
+#pragma unroll
+    for (int i = 1; i < AT_NW; i++) M = fmaxf(M, s_m[i][cl]);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+    float *so = (float *)sh + wave * 16 * LD + cl * LD;
+#pragma unroll
+    for (int e = 0; e < NO; e++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int d = F32 ? at_vbyte<RB>(e, 4 * g + j) / 4 : at_vbyte<RB>(e / 2, 4 * g + j) / 2 + (e & 1);
+            so[d] = O[e][j] * f;
+        }
+    if (tid < 16) {
+        float L = 0.f;
+#pragma unroll
+        for (int i = 0; i < AT_NW; i++) L = __builtin_fmaf(s_l[i][tid], s_m[i][tid] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[i][tid] - M), L);
+        s_q[tid] = L;
+        if (w.parts > 1 && tid < nh) {
+            float *ml = part + (((int64_t)s * Hq + h0 + tid) * n_split + sp) * (DH + 4);
+            ml[0] = M;
+            ml[1] = L;
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < nh * (DH / 4); i += AT_NT) {
+        const int h = i / (DH / 4), d = i % (DH / 4) * 4;
+        sw_f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < AT_NW; v++) {
+            const sw_f32x4 b = *(const sw_f32x4 *)((float *)sh + (v * 16 + h) * LD + d);
+#pragma unroll
+            for (int e = 0; e < 4; e++) a[e] = a[e] + b[e];
+        }
+        if (w.parts > 1) {
+            *(sw_f32x4 *)(part + (((int64_t)s * Hq + h0 + h) * n_split + sp) * (DH + 4) + 4 + d) = a;
+        } else {
+            const float L = s_q[h];
+#pragma unroll
+            for (int e = 0; e < 4; e++) a[e] = L == 0.f ? 0.f : a[e] / L;
+            *(sw_f32x4 *)(orow + h * DH + d) = a;
+        }
+    }
+}
+
+// The parts of a row's head joined, in their order: part [row][head][n_split] of (maximum,
+// sum, -, -, the output's values), one value a thread.
+__global__ __launch_bounds__(256) void k_attn_join(SwKv c, SwRows r, int Hq, int window, int CT, const float *__restrict__ part,
+                                                   int n_split, int min_per, float *__restrict__ out) {
+    const int s = blockIdx.x / Hq;
+    const AtWork w = at_work(c, r, s, window, CT, n_split, min_per);
+    if (w.parts < 2) return;
+    const float *p = part + (int64_t)blockIdx.x * n_split * (c.dh + 4);
+    const int d = threadIdx.x;
+    float M = -INFINITY, L = 0.f, O = 0.f;
+    for (int i = 0; i < w.parts; i++) M = fmaxf(M, p[i * (c.dh + 4)]);
+    for (int i = 0; i < w.parts; i++) {
+        const float mi = p[i * (c.dh + 4)], f = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - M);
+        L = __builtin_fmaf(p[i * (c.dh + 4) + 1], f, L);
+        O = __builtin_fmaf(p[i * (c.dh + 4) + 4 + d], f, O);
+    }
+    out[(int64_t)blockIdx.x * c.dh + d] = L == 0.f ? 0.f : O / L;
+}
+
+// Parts of a row: as many as give the chip about AT_BLOCKS blocks, of at least AT_MIN chunks each.
+#define AT_BLOCKS 2048
+#define AT_MIN 4
+static int at_splits(const SwKv &c, const SwRows &r, int Hq, int window, int S) {
+    const int G = Hq / c.Hkv, CT = c.type == SW_KV_F32 ? 16 : 32;
+    const int64_t base = (int64_t)S * c.Hkv * ((G + 15) / 16);
+    int64_t cells = (int64_t)r.max_pages << c.psh;
+    if (window > 0 && window + CT < cells) cells = window + CT;       // (a window begins anywhere in a chunk)
+    int64_t n = (AT_BLOCKS + base - 1) / base, most = (cells / CT + AT_MIN) / AT_MIN;
+    n = n < most ? n : most;
+    return (int)(n < 1 ? 1 : n);
+}
+int64_t sw_attn_part_floats(const SwKv &c, const SwRows &r, int Hq, int window, int S) {
+    const int n = at_splits(c, r, Hq, window, S);
+    return n > 1 ? (int64_t)S * Hq * n * (c.dh + 4) : 0;
+}
+
+template <int TYPE, int NB>
+static void at_launch(hipStream_t st, unsigned grid, const SwKv &c, const SwRows &r, const float *q, int Hq, float sc, int window,
+                      float *out, float *part, int n) {
+    SW_LAUNCH((k_attn<TYPE, NB>), dim3(grid), dim3(AT_NT), 0, st, c, r, q, Hq, sc, window, out, part, n, AT_MIN);
+}
+template <int TYPE>
+static void at_dispatch(hipStream_t st, unsigned grid, const SwKv &c, const SwRows &r, const float *q, int Hq, float sc, int window,
+                        float *out, float *part, int n) {
+    switch (c.dh / 32) {
+    case 1: at_launch<TYPE, 1>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
+    case 2: at_launch<TYPE, 2>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
+    case 3: at_launch<TYPE, 3>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
+    case 4: at_launch<TYPE, 4>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
+    case 5: at_launch<TYPE, 5>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
+    case 6: at_launch<TYPE, 6>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
+    case 7: at_launch<TYPE, 7>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
+    default: at_launch<TYPE, 8>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
+    }
 }
 
 int sw_launch_attn(hipStream_t st, const SwKv &c, const SwRows &r, const float *q, int Hq, float scale, int window, float *out,
-                   int S) {
-    const dim3 grid((unsigned)S, (unsigned)Hq);
-    if (c.type == SW_KV_F32) SW_LAUNCH(k_attn<SW_KV_F32>, grid, dim3(AT_NT), 0, st, c, r, q, Hq, scale, window, out);
-    else if (c.type == SW_KV_BF16) SW_LAUNCH(k_attn<SW_KV_BF16>, grid, dim3(AT_NT), 0, st, c, r, q, Hq, scale, window, out);
-    else SW_LAUNCH(k_attn<SW_KV_F16>, grid, dim3(AT_NT), 0, st, c, r, q, Hq, scale, window, out);
+                   int S, float *part) {
+    if (c.dh < 32 || c.dh > 256 || c.dh % 32) return -1;
+    const int n = at_splits(c, r, Hq, window, S), gt = (Hq / c.Hkv + 15) / 16;
+    const int64_t grid = (int64_t)S * n * c.Hkv * gt;
+    if (grid >= (int64_t)1 << 31 || (int64_t)S * Hq >= (int64_t)1 << 31 || (n > 1 && !part)) return -1;
+    const float sc = (float)((double)scale * 1.4426950408889634074);   // the softmax in powers of two
+    if (c.type == SW_KV_F32) at_dispatch<SW_KV_F32>(st, (unsigned)grid, c, r, q, Hq, sc, window, out, part, n);
+    else if (c.type == SW_KV_BF16) at_dispatch<SW_KV_BF16>(st, (unsigned)grid, c, r, q, Hq, sc, window, out, part, n);
+    else at_dispatch<SW_KV_F16>(st, (unsigned)grid, c, r, q, Hq, sc, window, out, part, n);
+    if (n > 1)
+        SW_LAUNCH(k_attn_join, dim3((unsigned)(S * Hq)), dim3((unsigned)c.dh), 0, st, c, r, Hq, window, c.type == SW_KV_F32 ? 16 : 32,
+                  part, n, AT_MIN, out);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }

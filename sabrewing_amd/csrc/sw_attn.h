@@ -57,9 +57,11 @@ int sw_launch_qk_rope_append(hipStream_t st, const SwKv &c, const SwRows &r, con
 #define SW_COPY_PAIRS 256
 #define SW_COPY_LAYERS 64
 int sw_launch_kv_copy(hipStream_t st, const SwKv *layers, int n_layers, const int *src, const int *dst, int n);
-// (k_attn.hip) one token of each row against its sequence's cells (pos - window, pos]
+// (k_attn.hip) one token of each row against its sequence's cells (pos - window, pos]; part:
+// scratch of sw_attn_part_floats floats, 16-byte aligned (0: none)
+int64_t sw_attn_part_floats(const SwKv &c, const SwRows &r, int Hq, int window, int S);
 int sw_launch_attn(hipStream_t st, const SwKv &c, const SwRows &r, const float *q, int Hq, float scale, int window, float *out,
-                   int S);
+                   int S, float *part);
 // (k_sample.hip) a pick of each row of logits; each setting may be null
 struct SwSample { const float *temp; const int *top_k; const float *top_p, *min_p; };
 int sw_launch_sample(hipStream_t st, const float *logits, int S, int V, const SwSample &p, const float *u, int *tok);
