@@ -361,27 +361,66 @@ __global__ __launch_bounds__(AT_NT, NB > 5 ? 1 : 2) void k_attn(SwKv c, SwRows r
     }
 }
 
-// The parts of a row's head joined, in their order: part [row][head][n_split] of (maximum,
-// sum, -, -, the output's values), one value a thread.
-__global__ __launch_bounds__(256) void k_attn_join(SwKv c, SwRows r, int Hq, int window, int CT, const float *__restrict__ part,
-                                                   int n_split, int min_per, float *__restrict__ out) {
-    const int s = blockIdx.x / Hq;
+// The parts of a row's head joined: part [row][head][n_split] of (maximum, sum, -, -, the
+// output's values).  A part's weight first, one part a thread; then dh / 4 threads take four values of
+// every (AT_NT / (dh / 4))-th part, and their sums meet in order.
+#define AT_MAXPARTS 2048
+__global__ __launch_bounds__(AT_NT) void k_attn_join(SwKv c, SwRows r, int Hq, int window, int CT, const float *__restrict__ part,
+                                                     int n_split, int min_per, float *__restrict__ out) {
+    __shared__ float s_f[AT_MAXPARTS], s_r[AT_NW];
+    __shared__ sw_f32x4 s_o[AT_NT];
+    const int tid = threadIdx.x, s = blockIdx.x / Hq, nd = c.dh / 4, ng = AT_NT / nd, row = c.dh + 4;
     const AtWork w = at_work(c, r, s, window, CT, n_split, min_per);
     if (w.parts < 2) return;
-    const float *p = part + (int64_t)blockIdx.x * n_split * (c.dh + 4);
-    const int d = threadIdx.x;
-    float M = -INFINITY, L = 0.f, O = 0.f;
-    for (int i = 0; i < w.parts; i++) M = fmaxf(M, p[i * (c.dh + 4)]);
-    for (int i = 0; i < w.parts; i++) {
-        const float mi = p[i * (c.dh + 4)], f = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - M);
-        L = __builtin_fmaf(p[i * (c.dh + 4) + 1], f, L);
-        O = __builtin_fmaf(p[i * (c.dh + 4) + 4 + d], f, O);
+    const float *p = part + (int64_t)blockIdx.x * n_split * row;
+    float M = -INFINITY, L = 0.f;
+    for (int i = tid; i < w.parts; i += AT_NT) {
+        s_f[i] = p[(int64_t)i * row];
+        M = fmaxf(M, s_f[i]);
     }
-    out[(int64_t)blockIdx.x * c.dh + d] = L == 0.f ? 0.f : O / L;
+    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+    if ((tid & 63) == 0) s_r[tid >> 6] = M;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < AT_NW; i++) M = fmaxf(M, s_r[i]);
+    __syncthreads();
+    for (int i = tid; i < w.parts; i += AT_NT) {
+        const float f = s_f[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_f[i] - M);
+        s_f[i] = f;
+        L = __builtin_fmaf(p[(int64_t)i * row + 1], f, L);
+    }
+    for (int o = 32; o; o >>= 1) L = L + __shfl_xor(L, o);
+    if ((tid & 63) == 0) s_r[tid >> 6] = L;
+    __syncthreads();
+    const int gr = tid / nd, d = tid % nd * 4;
+    sw_f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    if (gr < ng) {
+#pragma unroll 4
+        for (int i = gr; i < w.parts; i += ng) {
+            const sw_f32x4 v = *(const sw_f32x4 *)(p + (int64_t)i * row + 4 + d);
+            const float f = s_f[i];
+#pragma unroll
+            for (int e = 0; e < 4; e++) a[e] = __builtin_fmaf(v[e], f, a[e]);
+        }
+        s_o[tid] = a;
+    }
+    __syncthreads();
+    if (tid >= nd) return;
+    L = 0.f;
+#pragma unroll
+    for (int i = 0; i < AT_NW; i++) L = L + s_r[i];
+    for (int i = 1; i < ng; i++) {
+        const sw_f32x4 v = s_o[i * nd + tid];
+#pragma unroll
+        for (int e = 0; e < 4; e++) a[e] = a[e] + v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) a[e] = L == 0.f ? 0.f : a[e] / L;
+    *(sw_f32x4 *)(out + (int64_t)blockIdx.x * c.dh + d) = a;
 }
 
 // Parts of a row: as many as give the chip about AT_BLOCKS blocks, of at least AT_MIN chunks each.
-#define AT_BLOCKS 2048
+#define AT_BLOCKS 1024
 #define AT_MIN 4
 static int at_splits(const SwKv &c, const SwRows &r, int Hq, int window, int S) {
     const int G = Hq / c.Hkv, CT = c.type == SW_KV_F32 ? 16 : 32;
@@ -390,6 +429,7 @@ static int at_splits(const SwKv &c, const SwRows &r, int Hq, int window, int S) 
     if (window > 0 && window + CT < cells) cells = window + CT;       // (a window begins anywhere in a chunk)
     int64_t n = (AT_BLOCKS + base - 1) / base, most = (cells / CT + AT_MIN) / AT_MIN;
     n = n < most ? n : most;
+    n = n < AT_MAXPARTS ? n : AT_MAXPARTS;
     return (int)(n < 1 ? 1 : n);
 }
 int64_t sw_attn_part_floats(const SwKv &c, const SwRows &r, int Hq, int window, int S) {
@@ -428,7 +468,7 @@ int sw_launch_attn(hipStream_t st, const SwKv &c, const SwRows &r, const float *
     else if (c.type == SW_KV_BF16) at_dispatch<SW_KV_BF16>(st, (unsigned)grid, c, r, q, Hq, sc, window, out, part, n);
     else at_dispatch<SW_KV_F16>(st, (unsigned)grid, c, r, q, Hq, sc, window, out, part, n);
     if (n > 1)
-        SW_LAUNCH(k_attn_join, dim3((unsigned)(S * Hq)), dim3((unsigned)c.dh), 0, st, c, r, Hq, window, c.type == SW_KV_F32 ? 16 : 32,
+        SW_LAUNCH(k_attn_join, dim3((unsigned)(S * Hq)), dim3(AT_NT), 0, st, c, r, Hq, window, c.type == SW_KV_F32 ? 16 : 32,
                   part, n, AT_MIN, out);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
