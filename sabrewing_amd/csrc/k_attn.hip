@@ -30,26 +30,6 @@ __host__ __device__ constexpr int at_vbyte(int w, int rr) {
          : rem >= 128 ? (x < 2 ? full * 256 + rr * 8 + x * 4 : full * 256 + 128 + rr * 4)
                       : full * 256 + rr * 4;
 }
-// a value and its partner's 16 or 32 lanes away (as a pair in no order): each swap exchanges
-// the rows of 16, or the halves, of two registers.  (The second register is hidden from the compiler,
-// which takes the swap of a register with itself for no change.)
-template <int BY>
-__device__ __forceinline__ float2 at_pair(float x) {
-    const uint32_t a = __builtin_bit_cast(uint32_t, x);
-    uint32_t b = a;
-    asm("" : "+v"(b));
-    const auto r = BY == 16 ? __builtin_amdgcn_permlane16_swap(a, b, false, false) : __builtin_amdgcn_permlane32_swap(a, b, false, false);
-    return make_float2(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
-}
-__device__ __forceinline__ float at_max4(float x) {           // over the four lanes of a head
-    const float2 a = at_pair<16>(x), b = at_pair<32>(fmaxf(a.x, a.y));
-    return fmaxf(b.x, b.y);
-}
-__device__ __forceinline__ float at_sum4(float x) {
-    const float2 a = at_pair<16>(x), b = at_pair<32>(a.x + a.y);
-    return b.x + b.y;
-}
-
 // parts of 8 values: three bf16 (by truncation: each takes the next 8 bits, exact) or two f16
 template <int TYPE>
 struct AtParts { static constexpr int n = TYPE == SW_KV_BF16 ? 3 : 2; };
@@ -272,7 +252,7 @@ __global__ __launch_bounds__(AT_NT, NB > 5 ? 1 : 2) void k_attn(SwKv c, SwRows r
                     }
                     mx = fmaxf(mx, x[4 * t + j]);
                 }
-            const float nm = fmaxf(m, at_max4(mx));
+            const float nm = fmaxf(m, sw_max4(mx));
             if (__any(nm > m)) {                                       // some head's maximum grew
                 const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - nm);
                 l = l * f;
@@ -314,7 +294,7 @@ __global__ __launch_bounds__(AT_NT, NB > 5 ? 1 : 2) void k_attn(SwKv c, SwRows r
         }
     }
     // ---- the waves join: outputs relative to the block's maximum, summed in the waves' order
-    l = at_sum4(l);
+    l = sw_sum4(l);
     if (g == 0) { s_m[wave][cl] = m; s_l[wave][cl] = l; }
     __syncthreads();                                                   // (also: q's parts are done with)
     float M = s_m[0][cl];

@@ -12,10 +12,10 @@
 //
 // A block per row, in passes over it (the first SP_CACHE tiles stay in LDS, the rest of a
 // larger row comes from the caches again), each for what the settings need:
-//   the largest logit;
-//   a top-k of up to SP_LIST / 2: the k-th largest of the threads' own maxima bounds the k-th
-//     largest logit from below and little more than k logits reach it; they are listed, and all the
-//     rest is done on the list (as is min-p alone, where few weights reach it);
+//   the largest logit, from the maxima of 256 groups of the row's tokens;
+//   a top-k of up to SP_MAXK: the k-th largest group maximum bounds the k-th largest logit from
+//     below and little more than k logits reach it; they are listed, and all the rest is
+//     done on the list (as is min-p alone, where few weights reach it);
 //   else a histogram over the distance to the largest logit, of counts for top-k, then of
 //     weights for top-p; the tokens of the bin in which the beginning ends are listed and ranked;
 //   the kept weights of each tile, then of the one tile in which the sum passes.
@@ -29,27 +29,53 @@
 #define SP_CACHE 8                        // tiles in LDS: 128 KB
 #define SP_BINS 2048
 #define SP_LIST 512
-#define SP_MAXTILES 256                   // 2^20 logits
+#define SP_GROUPS 256
+#define SP_MAXK 192                       // (at random, 355 tokens reach the 192nd of 256 maxima)
+#define SP_STEPS 512
+#define SP_GROUPS_OF_TILES 16
 #define SP_ONE 4398046511104.0            // 2^42
-#define SP_FAR 43.5f                      // log2 of the largest weight over one that rounds to 0
-#define SP_SCALE 47.0f                    // bins per halving
+#define SP_FAR 43.1f                      // log2 of the largest weight over one that rounds to 0
+#define SP_SCALE 47.0f                    // bins per halving (47 x 43.1 < SP_BINS)
 
 typedef unsigned long long u64;
+typedef u64 u64x4 __attribute__((ext_vector_type(4)));
 typedef float sp_f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
+// 2^(j / 32) and 2^(j / 512), rounded to nearest
+__constant__ double SP_POW2[32] = {
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
+    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
+    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0,
+};
+__constant__ double SP_POW2F[16] = {
+    0x1.0000000000000p+0, 0x1.0058c86da1c0ap+0, 0x1.00b1afa5abcbfp+0, 0x1.010ab5b2cbd11p+0,
+    0x1.0163da9fb3335p+0, 0x1.01bd1e77170b4p+0, 0x1.02168143b0281p+0, 0x1.027003103b10ep+0,
+    0x1.02c9a3e778061p+0, 0x1.032363d42b027p+0, 0x1.037d42e11bbccp+0, 0x1.03d7411915a8ap+0,
+    0x1.04315e86e7f85p+0, 0x1.048b9b35659d8p+0, 0x1.04e5f72f654b1p+0, 0x1.0540727fc1762p+0,
+};
+struct SpItem { u64 code, weight; };
 struct SpShared {
     sw_f32x4 tile[SP_CACHE * SP_NT];
-    u64 hist[SP_BINS];                    // (also the tiles' sums)
-    u64 code[SP_LIST], weight[SP_LIST];
-    u64 part[SP_NW], found, before, acc;
-    double pow2[32];                      // 2^(42 + j / 32)
+    u64 hist[SP_BINS];                    // (also the tiles' sums by wave)
+    SpItem item[SP_LIST];
+    float group[SP_GROUPS];
+    u64 part[SP_NW], found, before;
+    double pow2[SP_STEPS];                // 2^(42 + j / SP_STEPS)
     int n, bin, pick;
+    float fmax, bound;
 };
 struct SpRow {
     const float *v;
     int V, ntile;
-    float fmax, c32;                      // the largest logit; log2(e) / T
+    float fmax, c32;                      // the largest logit; bins of distance to it by logit
     double m64, c64;
+    float lf;                             // kept so far: logits above lf, and equal ones up to index li
+    int li;
 };
 
 // tile k of the row, this thread's four (NaN behind its end)
@@ -61,62 +87,105 @@ __device__ __forceinline__ sw_f32x4 sp_load(const SpRow &r, int k) {
     for (int e = 0; e < 4; e++) x[e] = i + e < r.V ? r.v[i + e] : NAN;
     return x;
 }
-// f(logit, index) over all of the row, four tiles' loads ahead; done(tile) after each tile
-template <class F, class G>
-__device__ __forceinline__ void sp_each(const SpShared &sh, const SpRow &r, F f, G done) {
-    for (int k0 = 0; k0 < r.ntile; k0 += 4) {
-        sw_f32x4 x[4];
+// f(four logits, the first's index, tile) over all of the row; tiles beyond LDS are loaded four ahead
+template <class F>
+__device__ __forceinline__ void sp_each(const SpShared &sh, const SpRow &r, F f) {
+    const int i0 = 4 * (int)threadIdx.x;
+    sw_f32x4 x[4];
+    if (r.ntile > SP_CACHE)
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (k0 + j < r.ntile) x[j] = k0 < SP_CACHE ? sh.tile[(k0 + j) * SP_NT + threadIdx.x] : sp_load(r, k0 + j);
+        for (int j = 0; j < 4; j++) x[j] = sp_load(r, min(SP_CACHE + j, r.ntile - 1));
+#pragma unroll 1
+    for (int k = 0; k < min(r.ntile, SP_CACHE); k++) f(sh.tile[k * SP_NT + threadIdx.x], k * SP_TILE + i0, k);
+#pragma unroll 1
+    for (int k = SP_CACHE; k < r.ntile; k++) {
+        const sw_f32x4 y = x[0];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (k0 + j >= r.ntile) break;
-            const int i = (k0 + j) * SP_TILE + 4 * (int)threadIdx.x;
-#pragma unroll
-            for (int e = 0; e < 4; e++) f(x[j][e], i + e);
-            done(k0 + j);
-        }
+        for (int j = 0; j < 3; j++) x[j] = x[j + 1];
+        if (k + 4 < r.ntile) x[3] = sp_load(r, k + 4);
+        f(y, k * SP_TILE + i0, k);
     }
 }
 
 __device__ __forceinline__ u64 sp_code(float f, int i) { return ((u64)ord_f32(f + 0.0f) << 32) | (0xFFFFFFFFu - (uint32_t)i); }
-// log2(largest weight / weight), for bins and for what has no weight: NaN or infinite then
+__device__ __forceinline__ float sp_unkey(uint32_t o) { return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7FFFFFFFu : ~o); }
+// log2(largest weight / weight) in bins: below SP_BINS for what is kept
 __device__ __forceinline__ float sp_dist(float f, const SpRow &r) { return f == r.fmax ? 0.f : (r.fmax - f) * r.c32; }
-__device__ __forceinline__ int sp_bin(float d) { return (int)(d * SP_SCALE); }            // d in [0, SP_FAR]: below SP_BINS
-// 2^42 2^((f - max) c) to the nearest whole number: 32 steps of a halving from a table, the rest (at
-// most 2^-6 of one) by the exponential's series to the fifth power, 2e-15 off
+__device__ __forceinline__ bool sp_kept(float f, int i, const SpRow &r) { return (f > r.lf) | ((f == r.lf) & (i <= r.li)); }
+// 2^42 2^((f - max) c) to the nearest whole number: 512 steps of a halving from a table, the rest
+// (at most 2^-10 of one) by the exponential's series to the third power, 9e-15 off.  For what is kept;
+// infinities count as the largest float, which m64 is then
 __device__ __forceinline__ u64 sp_weight(float f, const SpRow &r, const SpShared &sh) {
-    constexpr double L = 0.69314718055994530942 / 32, MAGIC = 6755399441055744.0;         // 1.5 * 2^52: rounds to whole numbers
-    if (f == r.fmax) return (u64)SP_ONE;
-    const double x = (double)f - r.m64;
+    constexpr double L = 0.69314718055994530942 / SP_STEPS, MAGIC = 6755399441055744.0;   // 1.5 * 2^52: rounds to whole numbers
+    const double x = (double)__builtin_amdgcn_fmed3f(f, -3.402823466e38f, 3.402823466e38f) - r.m64;
     const double t = __builtin_fma(x, r.c64, MAGIC);
     const int k = (int)(uint32_t)__builtin_bit_cast(u64, t);
     const double z = __builtin_fma(x, r.c64, MAGIC - t);
-    const double p = __builtin_fma(z, __builtin_fma(z, __builtin_fma(z, __builtin_fma(z, __builtin_fma(z, L * L * L * L * L / 120, L * L * L * L / 24),
-                                                                                      L * L * L / 6), L * L / 2), L), 1.0);
-    const double w = __builtin_fma(p, __builtin_ldexp(sh.pow2[k & 31], k >> 5), 4503599627370496.0);
+    const double p = __builtin_fma(z, __builtin_fma(z, __builtin_fma(z, L * L * L / 6, L * L / 2), L), 1.0);
+    const u64 b = __builtin_bit_cast(u64, sh.pow2[k & (SP_STEPS - 1)]);       // its exponent lowered by whole halvings
+    const uint32_t hi = (uint32_t)(b >> 32) + ((uint32_t)(k & -SP_STEPS) << 11);
+    const double w = __builtin_fma(p, __builtin_bit_cast(double, ((u64)hi << 32) | (uint32_t)b), 4503599627370496.0);
     return __builtin_bit_cast(u64, w) & 0xFFFFFFFFFFFFFull;
 }
+// the weights of the four with `on`, 0 for the others (side by side: each is a chain of 64-bit operations)
+__device__ __forceinline__ void sp_weights(const sw_f32x4 &x, const bool (&on)[4], const SpRow &r, const SpShared &sh, u64 (&w)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        w[e] = sp_weight(x[e], r, sh);
+        if (!on[e]) w[e] = 0;
+    }
+}
 
-__device__ __forceinline__ u64 sp_wave_sum(u64 v) {
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+// a 64-bit value moved in a row of 16 lanes or to the next rows, 0 where nothing comes from
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ u64 sp_dpp(u64 x) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xF, false);
+    return ((u64)hi << 32) | lo;
+}
+__device__ __forceinline__ u64 sp_weight1(u64 code, const SpRow &r, const SpShared &sh) {
+    return r.fmax == INFINITY ? (u64)SP_ONE : sp_weight(sp_unkey((uint32_t)(code >> 32)), r, sh);
+}
+__device__ __forceinline__ u64 sp_wave_sum(u64 v) {           // (row rotations by 8, 4, 2, 1, then the rows)
+    v += sp_dpp<0x128>(v);
+    v += sp_dpp<0x124>(v);
+    v += sp_dpp<0x122>(v);
+    v += sp_dpp<0x121>(v);
+    uint2 lo = sw_pair<16>((uint32_t)v), hi = sw_pair<16>((uint32_t)(v >> 32));
+    v = (((u64)hi.x << 32) | lo.x) + (((u64)hi.y << 32) | lo.y);
+    lo = sw_pair<32>((uint32_t)v);
+    hi = sw_pair<32>((uint32_t)(v >> 32));
+    return (((u64)hi.x << 32) | lo.x) + (((u64)hi.y << 32) | lo.y);
+}
+__device__ __forceinline__ u64 sp_wave_scan(u64 v) {          // sums up to each lane (shifts by 1, 2, 4, 8, then the rows' last)
+    v += sp_dpp<0x111>(v);
+    v += sp_dpp<0x112>(v);
+    v += sp_dpp<0x114>(v);
+    v += sp_dpp<0x118>(v);
+    v += sp_dpp<0x142, 0xA>(v);
+    v += sp_dpp<0x143, 0xC>(v);
     return v;
+}
+__device__ __forceinline__ float sp_wave_max(float x) {
+    auto ror = [](float f, auto n) {
+        return fmaxf(f, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, f), 0x120 + decltype(n)::v, 0xF, 0xF, false)));
+    };
+    x = ror(x, SwIc<8>{});
+    x = ror(x, SwIc<4>{});
+    x = ror(x, SwIc<2>{});
+    x = ror(x, SwIc<1>{});
+    return sw_max4(x);
 }
 // the block's sum, and with `before` the sum of the threads before this one
 __device__ __forceinline__ u64 sp_block_sum(SpShared &sh, u64 v, u64 *before = nullptr) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    u64 x = v;
-    if (before) {
-        for (int o = 1; o < 64; o <<= 1) { const u64 t = __shfl_up(x, o); if (lane >= o) x += t; }
-    } else {
-        x = sp_wave_sum(x);
-    }
+    const u64 x = before ? sp_wave_scan(v) : sp_wave_sum(v);
     __syncthreads();
     if (lane == 63) sh.part[wave] = x;
     __syncthreads();
     u64 t = 0;
     if (before) *before = x - v;
+#pragma unroll
     for (int q = 0; q < SP_NW; q++) {
         if (before && q < wave) *before += sh.part[q];
         t += sh.part[q];
@@ -124,32 +193,39 @@ __device__ __forceinline__ u64 sp_block_sum(SpShared &sh, u64 v, u64 *before = n
     return t;
 }
 
-// hist[b] += w for the lanes with `on` (lanes of one bin, a row of equal logits say, in one addition)
-__device__ __forceinline__ void sp_add(SpShared &sh, bool on, int b, u64 w) {
-    const u64 any = __ballot(on);
-    if (!any) return;
-    const int b0 = __builtin_amdgcn_readlane(b, __builtin_ctzll(any));
-    if (__ballot(on && b != b0) == 0 && __popcll(any) > 4) {
-        w = sp_wave_sum(on ? w : 0);
-        if ((threadIdx.x & 63) == 0) atomicAdd(&sh.hist[b0], w);
-    } else if (on) {
-        atomicAdd(&sh.hist[b], w);
+// hist[b] += w for the four with `on` (a wave whose first ones share a bin, as in a row of equal logits,
+// adds up its lanes of a bin first)
+__device__ __forceinline__ void sp_add(SpShared &sh, const bool (&on)[4], const int (&b)[4], const u64 (&w)[4]) {
+    const u64 any = __ballot(on[0]);
+    const int b0 = __builtin_amdgcn_readlane(b[0], any ? __builtin_ctzll(any) : 0);
+    if (__popcll(any) > 8 && __ballot(on[0] && b[0] != b0) == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const u64 v = sp_wave_sum(on[e] && b[e] == b0 ? w[e] : 0);
+            if ((threadIdx.x & 63) == 0) atomicAdd(&sh.hist[b0], v);
+            if (on[e] && b[e] != b0) atomicAdd(&sh.hist[b[e]], w[e]);
+        }
+        return;
     }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (on[e]) atomicAdd(&sh.hist[b[e]], w[e]);
 }
 __device__ __forceinline__ void sp_clear(SpShared &sh) {
     __syncthreads();
     sh.hist[threadIdx.x] = sh.hist[threadIdx.x + SP_NT] = 0;
     __syncthreads();
 }
-// The bin in which the histogram's sum, from bin 0 (up: from the last), reaches `limit`, and the sum
-// before it; -1: never.
-__device__ __forceinline__ int sp_find(SpShared &sh, u64 limit, u64 &before, bool up = false) {
+// The bin in which the histogram's sum, from bin 0 (up: from the last), reaches limit(its total), and
+// the sum before it; -1: never.
+template <class F>
+__device__ __forceinline__ int sp_find(SpShared &sh, F limit_of, u64 &limit, u64 &before, bool up = false) {
     const int t = threadIdx.x, b0 = up ? SP_BINS - 1 - 2 * t : 2 * t, b1 = up ? b0 - 1 : b0 + 1;
     __syncthreads();
     const u64 a = sh.hist[b0], b = sh.hist[b1];
     if (t == 0) sh.bin = -1;
     u64 at;
-    sp_block_sum(sh, a + b, &at);
+    limit = limit_of(sp_block_sum(sh, a + b, &at));
     if (at < limit && at + a + b >= limit) {
         const bool first = at + a >= limit;
         sh.bin = first ? b0 : b1;
@@ -159,15 +235,18 @@ __device__ __forceinline__ int sp_find(SpShared &sh, u64 limit, u64 &before, boo
     before = sh.before;
     return sh.bin;
 }
-// the lanes with `on` into the list (beyond its end they are counted)
-__device__ __forceinline__ void sp_list(SpShared &sh, bool on, u64 code, u64 w) {
-    const u64 any = __ballot(on);
-    if (!any) return;
-    const int lane = threadIdx.x & 63, first = __builtin_ctzll(any);
-    int at = 0;
-    if (lane == first) at = atomicAdd(&sh.n, (int)__popcll(any));
-    at = __builtin_amdgcn_readlane(at, first) + (int)__popcll(any & ((1ull << lane) - 1));
-    if (on && at < SP_LIST) { sh.code[at] = code; sh.weight[at] = w; }
+// the tokens with `on` of the wave's four into the list (beyond its end they are counted)
+__device__ __forceinline__ void sp_list(SpShared &sh, const bool (&on)[4], const sw_f32x4 &x, int i) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const u64 b = __ballot(on[e]);
+        if (!b) continue;
+        int at = 0;
+        if ((int)(threadIdx.x & 63) == __builtin_ctzll(b)) at = atomicAdd(&sh.n, (int)__popcll(b));
+        at = __builtin_amdgcn_readlane(at, __builtin_ctzll(b)) +
+             (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+        if (on[e] && at < SP_LIST) sh.item[at].code = sp_code(x[e], i + e);
+    }
 }
 __device__ __forceinline__ u64 sp_share(double part, u64 total, u64 least) {      // ceil(part * total), at least `least`
     const double x = ceil(part * (double)total);
@@ -179,52 +258,93 @@ __device__ __forceinline__ u64 sp_target(float u, u64 total) {                  
     return t < total ? t : total - 1;
 }
 
-// The code at which the beginning ends, among codes >= least: after `limit` tokens, or (mass) with the
-// token at which the weights' sum reaches `limit`.  The histogram's bin holding it is narrowed by bits of
-// the code until the list takes its tokens.  `over`: what counts, of the whole beginning.
-__device__ u64 sp_cut(SpShared &sh, const SpRow &r, int bin, u64 limit, u64 before, bool mass, u64 least, u64 &over) {
+// The code at which the beginning ends, among the kept: after `limit` tokens, or (mass) with the token
+// at which the weights' sum reaches `limit`; `before`: what counts of the bins before `bin`.  The bin's
+// tokens are narrowed by bits of the code until the list takes them.
+__device__ __forceinline__ u64 sp_cut(SpShared &sh, const SpRow &r, int bin, u64 limit, u64 before, bool mass) {
     u64 prefix = 0, mask = 0;
     int shift = 64;
-    for (;;) {
+    const float lo = (float)bin, hi = (float)(bin + 1);
+    for (bool list = true;;) {
+        if (!list) sp_clear(sh);
         __syncthreads();
-        if (threadIdx.x == 0) { sh.n = 0; sh.found = 0; sh.acc = 0; }
+        if (threadIdx.x == 0) { sh.n = 0; sh.found = 0; }
         __syncthreads();
-        sp_each(sh, r, [&](float f, int i) {
-            const float d = sp_dist(f, r);
-            const u64 c = sp_code(f, i);
-            const bool on = d <= SP_FAR && sp_bin(d) == bin && (c & mask) == prefix && c >= least;
-            u64 w = 1;
-            if (mass && __any(on)) w = sp_weight(f, r, sh);
-            sp_list(sh, on, c, w);
-        }, [](int) {});
+        sp_each(sh, r, [&](const sw_f32x4 &x, int i, int) {
+            bool on[4], any = false;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float d = sp_dist(x[e], r);
+                on[e] = (d >= lo) & (d < hi);
+                any |= on[e];
+            }
+            if (!__any(any)) return;
+#pragma unroll
+            for (int e = 0; e < 4; e++) on[e] = on[e] && sp_kept(x[e], i + e, r);
+            if (mask)
+#pragma unroll
+                for (int e = 0; e < 4; e++) on[e] = on[e] && (sp_code(x[e], i + e) & mask) == prefix;
+            if (list) {
+                sp_list(sh, on, x, i);
+                return;
+            }
+            u64 w[4] = {1, 1, 1, 1};
+            int b[4];
+            if (mass) sp_weights(x, on, r, sh, w);
+#pragma unroll
+            for (int e = 0; e < 4; e++) b[e] = (int)(sp_code(x[e], i + e) >> shift) & (SP_BINS - 1);
+            sp_add(sh, on, b, w);
+        });
         __syncthreads();
-        if (sh.n <= SP_LIST) break;
-        shift = shift > 11 ? shift - 11 : 0;                          // 2048 ways by the next bits
-        sp_clear(sh);
-        sp_each(sh, r, [&](float f, int i) {
-            const float d = sp_dist(f, r);
-            const u64 c = sp_code(f, i);
-            const bool on = d <= SP_FAR && sp_bin(d) == bin && (c & mask) == prefix && c >= least;
-            u64 w = 1;
-            if (mass && __any(on)) w = sp_weight(f, r, sh);
-            sp_add(sh, on, (int)(c >> shift) & (SP_BINS - 1), w);
-        }, [](int) {});
-        u64 more;
-        const int b = sp_find(sh, limit - before, more, true);
-        before += more;
-        prefix |= (u64)b << shift;
-        mask |= (u64)(SP_BINS - 1) << shift;
+        if (list) {
+            if (sh.n <= SP_LIST) break;
+            shift = shift > 11 ? shift - 11 : 0;                      // 2048 ways by the next bits
+        } else {
+            u64 more, left;
+            const int b = sp_find(sh, [&](u64) { return limit - before; }, left, more, true);
+            before += more;
+            prefix |= (u64)b << shift;
+            mask |= (u64)(SP_BINS - 1) << shift;
+        }
+        list = !list;
     }
-    const int n = sh.n, t = threadIdx.x;
+    const int t = threadIdx.x;
+    int n = sh.n;
+    u64 c = 0, w = 0;
     if (t < n) {
-        const u64 c = sh.code[t], w = sh.weight[t];
+        c = sh.item[t].code;
+        w = mass ? sp_weight(sp_unkey((uint32_t)(c >> 32)), r, sh) : 1;
+    }
+    if (n > 64) {                                                     // 2048 parts of the bin, and the list of one
+        const int part = min((int)((sp_dist(sp_unkey((uint32_t)(c >> 32)), r) - lo) * SP_BINS), SP_BINS - 1);
+        sp_clear(sh);
+        if (t < n) atomicAdd(&sh.hist[part], w);
+        u64 left, more;
+        const int b = sp_find(sh, [&](u64) { return limit - before; }, left, more);
+        before += more;
+        if (t == 0) sh.n = 0;
+        __syncthreads();
+        const bool on = t < n && part == b;
+        int at = 0;
+        if (on) at = atomicAdd(&sh.n, 1);
+        __syncthreads();
+        if (on) sh.item[at].code = c;
+        n = sh.n;
+        __syncthreads();
+        if (t < n) {
+            c = sh.item[t].code;
+            w = mass ? sp_weight(sp_unkey((uint32_t)(c >> 32)), r, sh) : 1;
+        }
+    }
+    if (t < n) sh.item[t].weight = w;
+    __syncthreads();
+    if (t < n) {
         u64 at = before;
-        for (int j = 0; j < n; j++)
-            if (sh.code[j] > c) at += sh.weight[j];
-        if (at < limit && at + w >= limit) { sh.found = c; sh.acc = at + w; }
+#pragma unroll 4
+        for (int j = 0; j < n; j++) at += sh.item[j].code > c ? sh.item[j].weight : 0;
+        if (at < limit && at + w >= limit) sh.found = c;
     }
     __syncthreads();
-    over = sh.acc;
     return sh.found;
 }
 
@@ -240,180 +360,251 @@ __global__ __launch_bounds__(SP_NT) void k_sample(const float *__restrict__ logi
     int k = p.top_k ? p.top_k[s] : 0;
     const float top_p = p.top_p ? p.top_p[s] : 1.f, min_p = p.min_p ? p.min_p[s] : 0.f;
     if (k <= 0 || k >= V) k = 0;
+    if (tid < SP_STEPS) sh.pow2[tid] = SP_POW2[tid >> 4] * SP_POW2F[tid & 15] * SP_ONE;
     // ---- the largest logit: each thread's first, in order of index
     float best = -INFINITY;
     int bi = -1;
-    for (int k0 = 0; k0 < r.ntile; k0 += 4) {
-        sw_f32x4 x[4];
+    auto take = [&](const sw_f32x4 &x, int t) {
+        if (t < SP_CACHE) sh.tile[t * SP_NT + tid] = x;
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (k0 + j < r.ntile) x[j] = sp_load(r, k0 + j);
+        for (int e = 0; e < 4; e++)
+            if (x[e] > best) { best = x[e]; bi = t * SP_TILE + 4 * tid + e; }
+    };
+    const int whole = V / SP_TILE;
+    const sw_f32x4 last = sp_load(r, r.ntile - 1);
+    for (int k0 = 0; k0 < whole; k0 += 8) {                           // (past the last: that one again)
+        sw_f32x4 x[8];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (k0 + j >= r.ntile) break;
-            if (k0 < SP_CACHE) sh.tile[(k0 + j) * SP_NT + tid] = x[j];
+        for (int j = 0; j < 8; j++) x[j] = *(const sp_f32x4u *)(r.v + min(k0 + j, whole - 1) * SP_TILE + 4 * tid);
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (x[j][e] > best) { best = x[j][e]; bi = (k0 + j) * SP_TILE + 4 * tid + e; }
+        for (int j = 0; j < 8; j++) take(x[j], min(k0 + j, whole - 1));
+    }
+    if (whole < r.ntile) take(last, whole);
+    {   // (a group: 16 lanes of a wave hold the maxima of their four)
+        const float g = sw_max4(best);
+        if (lane < 16) sh.group[wave * 16 + lane] = g;
+    }
+    const bool by_p = top_p < 1.f, by_k = k > 0 && k <= SP_MAXK;
+    const bool few = temp > 0.f && (by_k || (!k && !by_p && min_p > 0.f));
+    __syncthreads();
+    if (wave == 0) {
+        const sw_f32x4 g = ((const sw_f32x4 *)sh.group)[lane];
+        const float top = sp_wave_max(fmaxf(fmaxf(g[0], g[1]), fmaxf(g[2], g[3])));
+        float bound = -INFINITY;
+        if (few && by_k && top < INFINITY) {
+            // the k-th largest of the groups, or a little less: halving the range between a bound that k
+            // groups reach and one that fewer do
+            float least = fminf(fminf(g[0], g[1]), fminf(g[2], g[3]));
+            least = -sp_wave_max(-least);
+            float lo = least, hi = top, at = lo > -INFINITY ? 0.5f * lo + 0.5f * top : top - 1.f;
+            for (int step = 0; step < 40; step++) {
+                int n = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) n += (int)__popcll(__ballot(g[e] >= at));
+                if (n >= k) lo = at; else hi = at;
+                if (n >= k && n <= k + (step < 6 ? 3 : 8)) break;
+                at = lo > -INFINITY ? 0.5f * lo + 0.5f * hi : top - 2.f * (top - hi);
+                if (at == lo || at == hi || !(at > -INFINITY)) break;
+            }
+            bound = lo;
+        }
+        if (lane == 0) {
+            sh.fmax = top;
+            sh.bound = bound;
+            sh.n = 0;
+            sh.pick = 0x7FFFFFFF;
         }
     }
-    u64 top = bi < 0 ? 0 : sp_code(best, bi);
-    for (int o = 32; o; o >>= 1) { const u64 t = __shfl_xor(top, o); top = t > top ? t : top; }
-    if (lane == 0) sh.part[wave] = top;
-    if (tid < 32) sh.pow2[tid] = exp2((double)tid / 32) * SP_ONE;
     __syncthreads();
-    for (int q = 0; q < SP_NW; q++) top = sh.part[q] > top ? sh.part[q] : top;
-    const int arg = top ? (int)(0xFFFFFFFFu - (uint32_t)top) : 0;
-    if (!(temp > 0.f) || !top) {                                      // greedy, or nothing to draw from
-        if (tid == 0) tok[s] = f0 != f0 ? 0 : arg;
+    r.fmax = sh.fmax;
+    if (!(temp > 0.f) || r.fmax == -INFINITY) {                       // greedy, or nothing to draw from
+        if (best == r.fmax && bi >= 0) atomicMin(&sh.pick, bi);
+        __syncthreads();
+        if (tid == 0) tok[s] = f0 != f0 || r.fmax == -INFINITY ? 0 : sh.pick;
         return;
     }
+    r.m64 = (double)fminf(r.fmax, 3.402823466e38f);
+    r.c64 = SP_STEPS * 1.4426950408889634074 / (double)temp;
+    r.c32 = (float)(SP_SCALE * 1.4426950408889634074 / (double)temp);
+    // what rounds to no weight is not kept (a little lower: the weights decide)
     {
-        const uint32_t o = (uint32_t)(top >> 32);                     // back from the order bits
-        r.fmax = __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
+        const float lo = r.fmax - SP_FAR * SP_SCALE / r.c32;
+        r.lf = r.fmax == INFINITY ? 3.402823466e38f : lo - 1e-6f * fabsf(lo);
+        r.li = 0x7FFFFFFF;
     }
-    r.m64 = (double)r.fmax;
-    r.c64 = 32 * 1.4426950408889634074 / (double)temp;                // (in steps of 1/32 halving)
-    r.c32 = (float)(1.4426950408889634074 / (double)temp);
-    const double least_w = min_p > 0.f ? fmin((double)min_p, 1.0) * SP_ONE : 0.0;
+    const u64 least_w = min_p > 0.f ? (u64)ceil(fmin((double)min_p, 1.0) * SP_ONE) : 0;
 
     // ---- few tokens can be kept: list them and stay there
-    const bool by_p = top_p < 1.f;
-    if ((k > 0 && k <= SP_LIST / 2) || (!k && !by_p && min_p > 0.f)) {
-        int bound = SP_BINS - 1;
-        if (k) {
-            sp_clear(sh);
-            const float d = sp_dist(best, r);
-            sp_add(sh, bi >= 0 && d <= SP_FAR, bi >= 0 && d <= SP_FAR ? sp_bin(d) : 0, 1);
-            u64 before;
-            const int b = sp_find(sh, (u64)k, before);
-            if (b >= 0) bound = b;
+    if (few) {
+        float bound = sh.bound;                                       // the list's tokens reach it
+        if (!by_p && min_p > 0.f) {                                   // (a little lower: the weights decide)
+            const float lo = r.fmax - (0.05f - log2f(fminf(min_p, 1.f))) * SP_SCALE / r.c32;
+            bound = fmaxf(bound, lo - 1e-6f * fabsf(lo));
         }
-        if (!by_p && min_p > 0.f) bound = min(bound, sp_bin(fminf(-log2f(fminf(min_p, 1.f)) + 0.05f, SP_FAR)) + 1);
-        __syncthreads();
-        if (tid == 0) { sh.n = 0; sh.pick = 0x7FFFFFFF; }
-        __syncthreads();
-        sp_each(sh, r, [&](float f, int i) {
-            const float d = sp_dist(f, r);
-            const bool on = d <= SP_FAR && sp_bin(d) <= bound;
-            u64 w = 0;
-            if (__any(on)) w = sp_weight(f, r, sh);
-            sp_list(sh, on, sp_code(f, i), w);
-        }, [](int) {});
+        sp_each(sh, r, [&](const sw_f32x4 &x, int i, int) {
+            if (__all(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) < bound)) return;
+            bool on[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) on[e] = (x[e] >= bound) & (x[e] > r.lf);
+            sp_list(sh, on, x, i);
+        });
         __syncthreads();
         const int n = sh.n;
+        if (n <= 64) {                                                // one wave does the rest
+            if (wave) return;
+            u64 code = 0, w = 0, at = 0;
+            int rank = 0;
+            if (lane < n) {
+                code = sh.item[lane].code;
+                w = sp_weight(sp_unkey((uint32_t)(code >> 32)), r, sh);
+            }
+            for (int j0 = 0; j0 < n; j0 += 8)                         // (lanes behind the list hold 0)
+#pragma unroll
+            for (int j = j0; j < j0 + 8; j++) {
+                const u64 cj = ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(code >> 32), j) << 32) |
+                               (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)code, j);
+                const u64 wj = ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(w >> 32), j) << 32) |
+                               (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)w, j);
+                rank += cj > code;
+                at += cj > code ? wj : 0;
+            }
+            if (lane >= n || (k && rank >= k)) w = 0;
+            if (by_p && at >= sp_share((double)top_p, sp_wave_sum(w), 1)) w = 0;
+            if (w < least_w) w = 0;
+            const u64 target = sp_target(us, sp_wave_sum(w));
+            u64 sum = 0;                                              // the kept weights up to this index
+            for (int j0 = 0; j0 < n; j0 += 8)
+#pragma unroll
+            for (int j = j0; j < j0 + 8; j++) {
+                const uint32_t cj = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)code, j);
+                const u64 wj = ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(w >> 32), j) << 32) |
+                               (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)w, j);
+                sum += cj >= (uint32_t)code ? wj : 0;
+            }
+            // the least index past the target: the one token whose own weight crosses it
+            if (w && sum > target && sum - w <= target) tok[s] = (int)(0xFFFFFFFFu - (uint32_t)code);
+            return;
+        }
         if (n <= SP_LIST) {
             u64 code = 0, w = 0, at = 0;
             int rank = 0;
             if (tid < n) {
-                code = sh.code[tid];
-                w = sh.weight[tid];
-                for (int j = 0; j < n; j++)
-                    if (sh.code[j] > code) { rank++; at += sh.weight[j]; }
+                code = sh.item[tid].code;
+                w = sp_weight(sp_unkey((uint32_t)(code >> 32)), r, sh);
+                sh.item[tid].weight = w;
             }
-            bool kept = tid < n && (!k || rank < k);
+            __syncthreads();
+            if (tid < n) {
+#pragma unroll 4
+                for (int j = 0; j < n; j++) {
+                    const SpItem o = sh.item[j];
+                    rank += o.code > code;
+                    at += o.code > code ? o.weight : 0;
+                }
+            }
+            if (k && rank >= k) w = 0;
             if (by_p) {
-                const u64 total = sp_block_sum(sh, kept ? w : 0);
-                kept = kept && at < sp_share((double)top_p, total, 1);
+                const u64 total = sp_block_sum(sh, w);
+                if (at >= sp_share((double)top_p, total, 1)) w = 0;
             }
-            kept = kept && (double)w >= least_w;
-            const u64 total = sp_block_sum(sh, kept ? w : 0);
-            const u64 target = sp_target(us, total);
+            if (w < least_w) w = 0;
+            const u64 target = sp_target(us, sp_block_sum(sh, w));
+            if (tid < n) sh.item[tid].weight = w;
             __syncthreads();
-            if (tid < n && !kept) sh.weight[tid] = 0;
-            __syncthreads();
-            if (kept && w) {                                          // the kept weights up to this index
+            if (w) {
                 u64 sum = 0;
-                for (int j = 0; j < n; j++)
-                    if ((uint32_t)sh.code[j] >= (uint32_t)code) sum += sh.weight[j];
-                if (sum > target) atomicMin(&sh.pick, (int)(0xFFFFFFFFu - (uint32_t)code));
+#pragma unroll 4
+                for (int j = 0; j < n; j++) sum += (uint32_t)sh.item[j].code >= (uint32_t)code ? sh.item[j].weight : 0;
+                if (sum > target && sum - w <= target) tok[s] = (int)(0xFFFFFFFFu - (uint32_t)code);
             }
-            __syncthreads();
-            if (tid == 0) tok[s] = sh.pick;
             return;
         }
     }
 
-    // ---- the least code that is kept
-    u64 least = 0, total = 0;
-    if (k) {
+    // ---- the least token that is kept: by counts, then by weights
+    for (int by = k ? 0 : 1; by < (by_p ? 2 : 1); by++) {
         sp_clear(sh);
-        sp_each(sh, r, [&](float f, int) {
-            const float d = sp_dist(f, r);
-            sp_add(sh, d <= SP_FAR, d <= SP_FAR ? sp_bin(d) : 0, 1);
-        }, [](int) {});
-        u64 before, n;
-        const int b = sp_find(sh, (u64)k, before);
-        if (b >= 0) least = sp_cut(sh, r, b, (u64)k, before, false, 0, n);
-    }
-    if (by_p) {
-        sp_clear(sh);
-        u64 sum = 0;
-        sp_each(sh, r, [&](float f, int i) {
-            const float d = sp_dist(f, r);
-            const bool on = d <= SP_FAR && sp_code(f, i) >= least;
-            u64 w = 0;
-            if (__any(on)) w = sp_weight(f, r, sh);
-            if (!on) w = 0;
-            sum += w;
-            sp_add(sh, on, on ? sp_bin(d) : 0, w);
-        }, [](int) {});
-        total = sp_block_sum(sh, sum);
-        u64 before, over;
-        const u64 limit = sp_share((double)top_p, total, 1);
-        const int b = sp_find(sh, limit, before);
+        sp_each(sh, r, [&](const sw_f32x4 &x, int i, int) {
+            bool on[4];
+            int d[4];
+            u64 w[4] = {1, 1, 1, 1};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                on[e] = sp_kept(x[e], i + e, r);
+                d[e] = on[e] ? min((int)sp_dist(x[e], r), SP_BINS - 1) : 0;
+            }
+            if (by) sp_weights(x, on, r, sh, w);
+            sp_add(sh, on, d, w);
+        });
+        u64 limit, before;
+        const int b = sp_find(sh, [&](u64 total) { return by ? sp_share((double)top_p, total, 1) : (u64)k; }, limit, before);
         if (b >= 0) {
-            const u64 c = sp_cut(sh, r, b, limit, before, true, least, over);
-            least = c > least ? c : least;
+            const u64 c = sp_cut(sh, r, b, limit, before, by);
+            r.lf = sp_unkey((uint32_t)(c >> 32));
+            r.li = (int)(0xFFFFFFFFu - (uint32_t)c);
         }
     }
-    // ---- the kept weights by tile, in order of index
-    __syncthreads();
-    if (tid < SP_MAXTILES) sh.hist[tid] = 0;
-    __syncthreads();
-    u64 w4 = 0;
-    sp_each(sh, r, [&](float f, int i) {
-        const bool on = sp_dist(f, r) <= SP_FAR && sp_code(f, i) >= least;
-        if (!__any(on)) return;
-        const u64 w = sp_weight(f, r, sh);
-        if (on && (double)w >= least_w) w4 += w;
-    }, [&](int t) {
-        if (__any(w4 != 0)) {
-            const u64 x = sp_wave_sum(w4);
-            if (lane == 0) atomicAdd(&sh.hist[t], x);
+    // ---- the kept weights by group of tiles, in order of index: hist[group][wave]
+    const int per = (r.ntile + SP_GROUPS_OF_TILES - 1) / SP_GROUPS_OF_TILES;
+    auto kept4 = [&](const sw_f32x4 &x, int i) -> u64x4 {
+        bool on[4], any = false;
+        u64x4 w = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            on[e] = sp_kept(x[e], i + e, r);
+            any |= on[e];
         }
-        w4 = 0;
+        if (__any(any)) {
+            u64 v[4];
+            sp_weights(x, on, r, sh, v);
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = v[e];
+            if (least_w)
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = v[e] < least_w ? 0 : v[e];
+        }
+        return w;
+    };
+    __syncthreads();
+    u64 acc = 0;
+    int left = per, group = 0;
+    sp_each(sh, r, [&](const sw_f32x4 &x, int i, int t) {
+        const u64x4 w = kept4(x, i);
+        acc += (w[0] + w[1]) + (w[2] + w[3]);
+        if (--left && t + 1 < r.ntile) return;
+        const u64 v = sp_wave_sum(acc);
+        if (lane == 0) sh.hist[group * SP_NW + wave] = v;
+        acc = 0;
+        left = per;
+        group++;
     });
     __syncthreads();
-    u64 before;
-    const u64 mine = tid < r.ntile ? sh.hist[tid] : 0;
-    total = sp_block_sum(sh, mine, &before);
-    const u64 target = sp_target(us, total);
-    if (before <= target && target < before + mine) { sh.bin = tid; sh.before = before; }
+    u64 base, mine = 0;
+    if (tid < group)
+#pragma unroll
+        for (int q = 0; q < SP_NW; q++) mine += sh.hist[tid * SP_NW + q];
+    u64 target = sp_target(us, sp_block_sum(sh, mine, &base));
+    if (base <= target && target < base + mine) { sh.bin = tid; sh.before = base; }
     __syncthreads();
-    const int t = sh.bin;
-    const u64 base = sh.before;
-    // ---- the tile's four of each thread
-    const sw_f32x4 x = t < SP_CACHE ? sh.tile[t * SP_NT + tid] : sp_load(r, t);
-    u64 w[4], sum = 0;
+    target -= sh.before;
+    // ---- that group's tiles one by one
+    for (int t = sh.bin * per; t < r.ntile; t++) {
+        const sw_f32x4 x = t < SP_CACHE ? sh.tile[t * SP_NT + tid] : sp_load(r, t);
+        const u64x4 w = kept4(x, t * SP_TILE + 4 * tid);
+        const u64 sum = (w[0] + w[1]) + (w[2] + w[3]);
+        u64 at;
+        const u64 all = sp_block_sum(sh, sum, &at);
+        if (all <= target) { target -= all; continue; }
+        if (at <= target && target < at + sum) {
+            int e = 0;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        const bool on = sp_dist(x[e], r) <= SP_FAR && sp_code(x[e], t * SP_TILE + 4 * tid + e) >= least;
-        w[e] = on ? sp_weight(x[e], r, sh) : 0;
-        if ((double)w[e] < least_w) w[e] = 0;
-        sum += w[e];
-    }
-    u64 at;
-    sp_block_sum(sh, sum, &at);
-    at += base;
-    if (at <= target && target < at + sum) {
-        int e = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            at += w[j];
-            e += at <= target;
+            for (int j = 0; j < 4; j++) {
+                at += w[j];
+                e += at <= target;
+            }
+            tok[s] = t * SP_TILE + 4 * tid + e;
         }
-        tok[s] = t * SP_TILE + 4 * tid + e;
+        return;
     }
 }
 

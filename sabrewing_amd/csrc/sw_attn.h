@@ -46,6 +46,28 @@ __device__ __forceinline__ float sw_kv_load(const void *p, int64_t i) {
     else return (float)((const _Float16 *)p)[i];
 }
 
+// A value and its partner's 16 or 32 lanes away (as a pair in no order): each swap exchanges
+// the rows of 16, or the halves, of two registers.  (The second register is hidden from the
+// compiler, which takes the swap of a register with itself for no change.)
+template <int BY>
+__device__ __forceinline__ uint2 sw_pair(uint32_t a) {
+    uint32_t b = a;
+    asm("" : "+v"(b));
+    const auto r = BY == 16 ? __builtin_amdgcn_permlane16_swap(a, b, false, false) : __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    return make_uint2((uint32_t)r[0], (uint32_t)r[1]);
+}
+// over the four lanes 16 apart
+__device__ __forceinline__ float sw_max4(float x) {
+    const uint2 a = sw_pair<16>(__builtin_bit_cast(uint32_t, x));
+    const uint2 b = sw_pair<32>(__builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a.x), __builtin_bit_cast(float, a.y))));
+    return fmaxf(__builtin_bit_cast(float, b.x), __builtin_bit_cast(float, b.y));
+}
+__device__ __forceinline__ float sw_sum4(float x) {
+    const uint2 a = sw_pair<16>(__builtin_bit_cast(uint32_t, x));
+    const uint2 b = sw_pair<32>(__builtin_bit_cast(uint32_t, __builtin_bit_cast(float, a.x) + __builtin_bit_cast(float, a.y)));
+    return __builtin_bit_cast(float, b.x) + __builtin_bit_cast(float, b.y);
+}
+
 // ---- launch wrappers (async on `st`) ----
 // (k_cache.hip) the q and k heads of S projected rows normalised (wq, wk null: not) and
 // turned (np pairs of a head, freq in radians per position), q to q_out, k and v to the cache
