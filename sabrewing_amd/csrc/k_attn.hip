@@ -21,6 +21,8 @@
 
 #define AT_NT 256
 #define AT_NW (AT_NT / 64)
+#define AT_BLOCKS 512                     // two blocks on each CU
+#define AT_MIN 4                          // chunks of a part: one a wave
 
 // bytes of a lane per row: 16-byte pieces first, then 8 and 4; the byte of row `rr` at dword w
 template <int RB>
@@ -69,165 +71,271 @@ __device__ __forceinline__ sw_f32x4 at_mfma(sw_u32x4 a, sw_u32x4 b, sw_f32x4 c) 
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(sw_half8, a), __builtin_bit_cast(sw_half8, b), c, 0, 0, 0);
 }
 
-// The work of a row: its cells' chunks [c0, c0 + n), `per` of them a part, `parts` parts in use.
-struct AtWork { int first, last, c0, n, per, parts; };
-__device__ __forceinline__ AtWork at_work(const SwKv &c, const SwRows &r, int s, int window, int CT, int n_split, int min_per) {
-    AtWork w;
+// A row's cells as chunks of CT tokens: n of them from chunk c0.
+struct AtRow { int first, last, c0, n; };
+__device__ __forceinline__ AtRow at_row(const SwKv &c, const SwRows &r, int s, int window, int CT) {
+    AtRow w;
     const int pos = r.pos[s], sq = r.seq ? r.seq[s] : s;
     w.first = window > 0 && pos >= window ? pos - window + 1 : 0;
     w.last = min(pos, (r.max_pages << c.psh) - 1);                     // (the host keeps that below 2^30)
     if (sq < 0 || sq >= r.n_seqs) w.last = -1;
     w.c0 = w.first / CT;
     w.n = w.last < w.first ? 0 : w.last / CT - w.c0 + 1;
-    w.per = max(min_per, (w.n + n_split - 1) / n_split);
-    w.parts = (w.n + w.per - 1) / w.per;
     return w;
 }
 
-// One block per (row, cache head, 16 query heads, part of the row's cells); a wave takes every
-// 4th chunk, its k of the next chunk and v of the next chunk in flight while it computes.
+// (the same in every lane: kept in scalar registers)
+__device__ __forceinline__ int at_uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t at_uni(int64_t x) {
+    return (int64_t)(((uint64_t)(uint32_t)at_uni((int)(x >> 32)) << 32) | (uint32_t)at_uni((int)x));
+}
+
+// How the rows' chunks are dealt to the B blocks of a cache head.  Laid end to end they are N, and
+// block b takes those from b q to (b + 1) q, whatever rows they fall in: parts of rows, joined
+// by k_attn_join, and the same work for each block however the lengths differ.  Where whole rows
+// (b, b + B, ...) are as even, within a fifth, they are dealt whole.  The lengths are on the device
+// alone, so each block counts them.
+struct AtPlan { int64_t N, q, before; bool whole; };                   // before: the chunks of rows before row `upto`
+__device__ __forceinline__ AtPlan at_plan(const SwKv &c, const SwRows &r, int S, int window, int CT, int B, int upto, int64_t *s_scan) {
+    AtPlan p;
+    int64_t mx;
+    if (S == 1) {
+        p.N = mx = at_row(c, r, 0, window, CT).n;
+        p.before = 0;
+    } else {
+        int64_t n = 0, before = 0;
+        mx = 0;
+        for (int i = threadIdx.x; i < S; i += AT_NT) {
+            const int64_t x = at_row(c, r, i, window, CT).n;
+            n += x;
+            before += i < upto ? x : 0;
+            mx = x > mx ? x : mx;
+        }
+        for (int o = 32; o; o >>= 1) {
+            n += __shfl_xor(n, o);
+            before += __shfl_xor(before, o);
+            const int64_t t = __shfl_xor(mx, o);
+            mx = t > mx ? t : mx;
+        }
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) {
+            s_scan[threadIdx.x >> 6] = n;
+            s_scan[AT_NW + (threadIdx.x >> 6)] = before;
+            s_scan[2 * AT_NW + (threadIdx.x >> 6)] = mx;
+        }
+        __syncthreads();
+        p.N = p.before = 0;
+        for (int i = 0; i < AT_NW; i++) {
+            p.N += s_scan[i];
+            p.before += s_scan[AT_NW + i];
+            mx = s_scan[2 * AT_NW + i] > mx ? s_scan[2 * AT_NW + i] : mx;
+        }
+    }
+    p.N = at_uni(p.N);
+    p.before = at_uni(p.before);
+    mx = at_uni(mx);
+    p.q = (p.N + B - 1) / B;
+    p.whole = 5 * mx * ((S + B - 1) / B) <= 6 * p.q;
+    if (p.q < AT_MIN) p.q = AT_MIN;
+    return p;
+}
+// the row in which chunk `at` of all lies, and the chunks of rows before it
+__device__ __forceinline__ int at_find(const SwKv &c, const SwRows &r, int S, int window, int CT, int64_t at, int64_t &before,
+                                       int64_t *s_scan) {
+    if (S == 1) { before = 0; return 0; }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t base = 0;
+    for (int i0 = 0;; i0 += AT_NT) {                                   // (`at` is below the rows' sum: it ends)
+        const int i = i0 + (int)threadIdx.x;
+        const int64_t n = i < S ? at_row(c, r, i, window, CT).n : 0;
+        int64_t x = n;
+        for (int o = 1; o < 64; o <<= 1) { const int64_t t = __shfl_up(x, o); if (lane >= o) x += t; }
+        __syncthreads();
+        if (lane == 63) s_scan[wave] = x;
+        __syncthreads();
+        int64_t all = 0;
+        x += base - n;
+        for (int q = 0; q < AT_NW; q++) {
+            if (q < wave) x += s_scan[q];
+            all += s_scan[q];
+        }
+        if (x <= at && at < x + n) { s_scan[AT_NW] = i; s_scan[AT_NW + 1] = x; }
+        base += all;
+        if (base > at || i0 + AT_NT >= S) break;
+    }
+    __syncthreads();
+    before = at_uni(s_scan[AT_NW + 1]);
+    return at_uni((int)s_scan[AT_NW]);
+}
+
+// One block per cache head (16 query heads of it) and share of the rows' chunks; of a row's part a
+// wave takes every 4th chunk, its k of the next chunk and v of the next chunk in flight while
+// it computes.
 template <int TYPE, int NB>
-__global__ __launch_bounds__(AT_NT, NB > 5 ? 1 : 2) void k_attn(SwKv c, SwRows r, const float *__restrict__ q, int Hq, float sc, int window,
-                                                   float *__restrict__ out, float *__restrict__ part, int n_split, int min_per) {
+__global__ __launch_bounds__(AT_NT, NB > 4 ? 1 : 2) void k_attn(SwKv c, SwRows r, const float *__restrict__ q, int S, int Hq, float sc0,
+                                                                int window, float *__restrict__ out, float *__restrict__ part, int B) {
     constexpr bool F32 = TYPE == SW_KV_F32;
     constexpr int DH = 32 * NB, ES = F32 ? 4 : 2, RB = DH * ES, CT = F32 ? 16 : 32;
     constexpr int NT = CT / 16, NS = RB / 64, ND = RB / 64, NTOK = 4 * NT, NO = DH / 16;
-    constexpr int NP = F32 ? 1 : AtParts<TYPE>::n, QN = NP * NS * 64;
+    constexpr int NP = F32 ? 1 : AtParts<TYPE>::n, QN = NP * NS * 64, QI = (NS * 64 + AT_NT - 1) / AT_NT;
     constexpr int LD = DH + 4;                                         // a head's row in the waves' join
     constexpr int SHB = QN * 16 > AT_NW * 16 * LD * 4 ? QN * 16 : AT_NW * 16 * LD * 4;
     __shared__ __align__(16) char sh[SHB];
     __shared__ float s_m[AT_NW][16], s_l[AT_NW][16], s_q[16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, cl = lane & 15;
+    __shared__ int64_t s_scan[3 * AT_NW];
+    const int tid = threadIdx.x, lane = tid & 63, wave = at_uni(tid >> 6), g = lane >> 4, cl = lane & 15;
     const int G = Hq / c.Hkv, gt = (G + 15) >> 4, per_s = c.Hkv * gt;
-    const int hg = blockIdx.x % per_s, sp = blockIdx.x / per_s % n_split, s = blockIdx.x / per_s / n_split;
+    const int hg = blockIdx.x % per_s, b = blockIdx.x / per_s;
     const int hk = hg / gt, h0 = hk * G + (hg % gt) * 16, nh = min(16, G - (hg % gt) * 16);
-    const AtWork w = at_work(c, r, s, window, CT, n_split, min_per);
-    float *orow = out + ((int64_t)s * Hq + h0) * DH;
-    if (sp >= w.parts) {
-        if (sp == 0) for (int i = tid; i < nh * DH; i += AT_NT) orow[i] = 0.f;      // no cell at all
-        return;
-    }
-    // ---- q's parts in the right operand's order: [part][step][lane] of 16 bytes
-    const float *qrow = q + ((int64_t)s * Hq + h0) * DH;
-    sw_u32x4 *sq = (sw_u32x4 *)sh;
-    float up = 1.f;
-    if constexpr (TYPE == SW_KV_F16) {
-        float mx = 0.f;                                                // 16 threads a head
-        if ((tid >> 4) < nh)
-            for (int i = tid & 15; i < DH; i += 16) mx = fmaxf(mx, fabsf(qrow[(tid >> 4) * DH + i]));
-        for (int o = 8; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-        if ((tid & 15) == 0) {
-            const int e = mx > 0.f && mx < INFINITY ? 13 - ilogbf(mx) : 0;
-            s_q[tid >> 4] = ldexpf(1.f, min(max(e, -100), 100));
-        }
-        __syncthreads();
-        up = s_q[cl];
-        sc = sc / up;
-    }
-    for (int i = tid; i < NS * 64; i += AT_NT) {
-        const int st = i >> 6, d = st * (64 / ES) + g * (16 / ES);     // (256 threads: the same lane in every round)
-        if constexpr (F32) {
-            sw_f32x4 x = {0.f, 0.f, 0.f, 0.f};
-            if (cl < nh) x = *(const sw_f32x4 *)(qrow + cl * DH + d);
-            sq[i] = __builtin_bit_cast(sw_u32x4, x);
-        } else {
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[j] = 0.f;
-            if (cl < nh) {
-                const sw_f32x4 a = *(const sw_f32x4 *)(qrow + cl * DH + d), b = *(const sw_f32x4 *)(qrow + cl * DH + d + 4);
-#pragma unroll
-                for (int j = 0; j < 4; j++) { x[j] = a[j] * up; x[j + 4] = b[j] * up; }
-            }
-            sw_u32x4 o[NP];
-            at_split<TYPE>(x, o);
-#pragma unroll
-            for (int p = 0; p < NP; p++) sq[p * NS * 64 + i] = o[p];
-        }
-    }
-    __syncthreads();
-
-    const int seq = r.seq ? r.seq[s] : s, pmask = (1 << c.psh) - 1;
+    for (int64_t s = b + (int64_t)B * tid; s < S; s += (int64_t)B * AT_NT)             // rows without any cell: zeros
+        if (at_row(c, r, (int)s, window, CT).n == 0)
+            for (int i = 0; i < nh * DH; i += 4) *(sw_f32x4 *)(out + (s * Hq + h0) * DH + i) = sw_f32x4{0.f, 0.f, 0.f, 0.f};
+    const AtPlan plan = at_plan(c, r, S, window, CT, B, 0, s_scan);
+    int64_t at = (int64_t)b * plan.q, end = at + plan.q < plan.N ? at + plan.q : plan.N, before = 0;
+    if (!plan.whole && at >= end) return;
+    int s = plan.whole ? b : at_find(c, r, S, window, CT, at, before, s_scan);
+    const int pmask = (1 << c.psh) - 1;
     const char *kb = (const char *)c.k + (int64_t)hk * c.hs * ES + g * 16;
     const char *vb = (const char *)c.v + (int64_t)hk * c.hs * ES;
-    struct Pages { int k[NT], v[NT]; };
-    auto pages = [&](int ch) {
-        Pages p;
-        const int t0 = ch * CT;
-        if (pmask >= CT - 1) {                                         // one page, read once for the wave
-            const int x = __builtin_amdgcn_readfirstlane(sw_page(c, r, seq, t0));
+    sw_u32x4 *sq = (sw_u32x4 *)sh;
+
+    for (; s < S && (plan.whole || at < end); s += plan.whole ? B : 1) {
+        const AtRow w = at_row(c, r, s, window, CT);
+        if (w.n == 0) continue;
+        // this block's chunks of the row
+        const int from = plan.whole ? 0 : (int)(at - before), len = plan.whole ? w.n : (int)(end - at < w.n - from ? end - at : w.n - from);
+        const int c1 = w.c0 + from + len;
+        int ch = w.c0 + from + wave;
+        before += w.n;
+        at += len;
+        // ---- q's rows on their way, then the first chunk's cells
+        const float *qrow = q + ((int64_t)s * Hq + h0) * DH;
+        sw_f32x4 qx[QI][F32 ? 1 : 2];
 #pragma unroll
-            for (int t = 0; t < NT; t++) p.k[t] = p.v[t] = x;
-        } else {
+        for (int i = 0; i < QI; i++) {
+            const int d = ((tid + i * AT_NT) >> 6) * (64 / ES) + g * (16 / ES);
+#pragma unroll
+            for (int j = 0; j < (F32 ? 1 : 2); j++) {
+                qx[i][j] = sw_f32x4{0.f, 0.f, 0.f, 0.f};
+                if (tid + i * AT_NT < NS * 64 && cl < nh) qx[i][j] = *(const sw_f32x4 *)(qrow + cl * DH + d + 4 * j);
+            }
+        }
+        const int seq = r.seq ? r.seq[s] : s;
+        struct Pages { int k[NT], v[NT]; };
+        auto pages = [&](int x) {
+            Pages p;
+            const int t0 = x * CT;
+            if (pmask >= CT - 1) {                                     // one page, read once for the wave
+                const int y = __builtin_amdgcn_readfirstlane(sw_page(c, r, seq, t0));
+#pragma unroll
+                for (int t = 0; t < NT; t++) p.k[t] = p.v[t] = y;
+            } else {
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    p.k[t] = sw_page(c, r, seq, t0 + 16 * t + cl);
+                    p.v[t] = sw_page(c, r, seq, t0 + 16 * t + 4 * g);
+                }
+            }
+            return p;
+        };
+        sw_u32x4 K[NT][NS];
+        uint32_t V[NTOK][ND];
+        // (a page that leads nowhere: page 0's cells are read in its place and weigh nothing)
+        auto load_k = [&](int x, const Pages &p) {
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                p.k[t] = sw_page(c, r, seq, t0 + 16 * t + cl);
-                p.v[t] = sw_page(c, r, seq, t0 + 16 * t + 4 * g);
+                const char *a = kb + ((int64_t)max(p.k[t], 0) * c.ps + (int64_t)((x * CT + 16 * t + cl) & pmask) * c.ts) * ES;
+#pragma unroll
+                for (int i = 0; i < NS; i++) K[t][i] = *(const sw_u32x4 *)(a + i * 64);
+            }
+        };
+        auto load_v = [&](int x, const Pages &p) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const char *a = vb + ((int64_t)max(p.v[t], 0) * c.ps + (int64_t)((x * CT + 16 * t + 4 * g + j) & pmask) * c.ts) * ES;
+                    uint32_t (&d)[ND] = V[4 * t + j];
+#pragma unroll
+                    for (int u = 0; u < RB / 256; u++) {
+                        const sw_u32x4 y = *(const sw_u32x4 *)(a + u * 256 + cl * 16);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) d[4 * u + e] = y[e];
+                    }
+                    constexpr int w0 = 4 * (RB / 256), b0 = RB / 256 * 256;
+                    if constexpr (RB % 256 >= 128) {
+                        const uint2 y = *(const uint2 *)(a + b0 + cl * 8);
+                        d[w0] = y.x; d[w0 + 1] = y.y;
+                    }
+                    if constexpr (RB % 128 == 64) d[ND - 1] = *(const uint32_t *)(a + RB - 64 + cl * 4);
+                }
+        };
+        Pages p, pn;
+        if (ch < c1) {
+            p = pages(ch);
+            pn = ch + AT_NW < c1 ? pages(ch + AT_NW) : p;
+            load_k(ch, p);
+            load_v(ch, p);
+        }
+        // ---- q's parts in the right operand's order: [part][step][lane] of 16 bytes
+        float sc = sc0, up = 1.f;
+        if constexpr (TYPE == SW_KV_F16) {
+            float mx = 0.f;
+#pragma unroll
+            for (int i = 0; i < QI; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(qx[i][j / 4][j % 4]));
+            mx = sw_max4(mx);
+            __syncthreads();                                           // (the row before is done with)
+            if (lane < 16) s_m[wave][cl] = mx;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < AT_NW; i++) mx = fmaxf(mx, s_m[i][cl]);
+            const int e = mx > 0.f && mx < INFINITY ? 13 - ilogbf(mx) : 0;
+            up = ldexpf(1.f, min(max(e, -100), 100));
+            sc = sc0 / up;
+        } else {
+            __syncthreads();                                           // (the row before is done with)
+        }
+#pragma unroll
+        for (int i = 0; i < QI; i++) {
+            if (tid + i * AT_NT >= NS * 64) break;
+            if constexpr (F32) {
+                sq[tid + i * AT_NT] = __builtin_bit_cast(sw_u32x4, qx[i][0]);
+            } else {
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = qx[i][j / 4][j % 4] * up;
+                sw_u32x4 o[NP];
+                at_split<TYPE>(x, o);
+#pragma unroll
+                for (int u = 0; u < NP; u++) sq[u * NS * 64 + tid + i * AT_NT] = o[u];
             }
         }
-        return p;
-    };
-    sw_u32x4 K[NT][NS];
-    uint32_t V[NTOK][ND];
-    // (a page that leads nowhere: page 0's cells are read in its place and weigh nothing)
-    auto load_k = [&](int ch, const Pages &p) {
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const char *a = kb + ((int64_t)max(p.k[t], 0) * c.ps + (int64_t)((ch * CT + 16 * t + cl) & pmask) * c.ts) * ES;
-#pragma unroll
-            for (int i = 0; i < NS; i++) K[t][i] = *(const sw_u32x4 *)(a + i * 64);
-        }
-    };
-    auto load_v = [&](int ch, const Pages &p) {
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const char *a = vb + ((int64_t)max(p.v[t], 0) * c.ps + (int64_t)((ch * CT + 16 * t + 4 * g + j) & pmask) * c.ts) * ES;
-                uint32_t (&d)[ND] = V[4 * t + j];
-#pragma unroll
-                for (int u = 0; u < RB / 256; u++) {
-                    const sw_u32x4 x = *(const sw_u32x4 *)(a + u * 256 + cl * 16);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) d[4 * u + e] = x[e];
-                }
-                constexpr int w0 = 4 * (RB / 256), b0 = RB / 256 * 256;
-                if constexpr (RB % 256 >= 128) {
-                    const uint2 x = *(const uint2 *)(a + b0 + cl * 8);
-                    d[w0] = x.x; d[w0 + 1] = x.y;
-                }
-                if constexpr (RB % 128 == 64) d[ND - 1] = *(const uint32_t *)(a + RB - 64 + cl * 4);
-            }
-    };
+        __syncthreads();
 
-    sw_f32x4 O[NO];
+        sw_f32x4 O[NO];
 #pragma unroll
-    for (int i = 0; i < NO; i++) O[i] = sw_f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;                                      // head cl: the maximum, this lane's part of the sum
-    const int c1 = w.c0 + min(w.n, (sp + 1) * w.per);
-    int ch = w.c0 + sp * w.per + wave;
-    if (ch < c1) {
-        Pages p = pages(ch), pn = ch + AT_NW < c1 ? pages(ch + AT_NW) : p;
-        load_k(ch, p);
-        load_v(ch, p);
+        for (int i = 0; i < NO; i++) O[i] = sw_f32x4{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;                                  // head cl: the maximum, this lane's part of the sum
         for (; ch < c1; ch += AT_NW) {
             const bool more = ch + AT_NW < c1;
             Pages pnn = pn;
             if (ch + 2 * AT_NW < c1) pnn = pages(ch + 2 * AT_NW);
             // scores of the chunk's tokens 16 t + 4 g + j for head cl
-            sw_f32x4 S[NT];
+            sw_f32x4 Sc[NT];
 #pragma unroll
             for (int t = 0; t < NT; t++) {
-                S[t] = sw_f32x4{0.f, 0.f, 0.f, 0.f};
+                Sc[t] = sw_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < NS; i++) {
                     if constexpr (F32) {
-                        const sw_f32x4 a = __builtin_bit_cast(sw_f32x4, K[t][i]), b = __builtin_bit_cast(sw_f32x4, sq[i * 64 + lane]);
+                        const sw_f32x4 a = __builtin_bit_cast(sw_f32x4, K[t][i]), y = __builtin_bit_cast(sw_f32x4, sq[i * 64 + lane]);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) S[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], S[t], 0, 0, 0);
+                        for (int e = 0; e < 4; e++) Sc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], y[e], Sc[t], 0, 0, 0);
                     } else {
 #pragma unroll
-                        for (int u = 0; u < NP; u++) S[t] = at_mfma<TYPE>(K[t][i], sq[(u * NS + i) * 64 + lane], S[t]);
+                        for (int u = 0; u < NP; u++) Sc[t] = at_mfma<TYPE>(K[t][i], sq[(u * NS + i) * 64 + lane], Sc[t]);
                     }
                 }
             }
@@ -241,7 +349,7 @@ __global__ __launch_bounds__(AT_NT, NB > 5 ? 1 : 2) void k_attn(SwKv c, SwRows r
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    x[4 * t + j] = S[t][j] * sc;
+                    x[4 * t + j] = Sc[t][j] * sc;
                     if (!full) {
                         const int tok = ch * CT + 16 * t + 4 * g + j;
                         if (tok < w.first || tok > w.last || p.v[t] < 0) {
@@ -292,70 +400,77 @@ __global__ __launch_bounds__(AT_NT, NB > 5 ? 1 : 2) void k_attn(SwKv c, SwRows r
             p = pn;
             pn = pnn;
         }
-    }
-    // ---- the waves join: outputs relative to the block's maximum, summed in the waves' order
-    l = sw_sum4(l);
-    if (g == 0) { s_m[wave][cl] = m; s_l[wave][cl] = l; }
-    __syncthreads();                                                   // (also: q's parts are done with)
-    float M = s_m[0][cl];
+        // ---- the waves join: outputs relative to the block's maximum, summed in the waves' order
+        l = sw_sum4(l);
+        __syncthreads();                                               // q's parts (and the maxima of q) are done with
+        if (g == 0) { s_m[wave][cl] = m; s_l[wave][cl] = l; }
+        __syncthreads();
+        float M = s_m[0][cl];
 #pragma unroll
-    for (int i = 1; i < AT_NW; i++) M = fmaxf(M, s_m[i][cl]);
-    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
-    float *so = (float *)sh + wave * 16 * LD + cl * LD;
+        for (int i = 1; i < AT_NW; i++) M = fmaxf(M, s_m[i][cl]);
+        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+        float *so = (float *)sh + wave * 16 * LD + cl * LD;
 #pragma unroll
-    for (int e = 0; e < NO; e++)
+        for (int e = 0; e < NO; e++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int d = F32 ? at_vbyte<RB>(e, 4 * g + j) / 4 : at_vbyte<RB>(e / 2, 4 * g + j) / 2 + (e & 1);
-            so[d] = O[e][j] * f;
+            for (int j = 0; j < 4; j++) {
+                const int d = F32 ? at_vbyte<RB>(e, 4 * g + j) / 4 : at_vbyte<RB>(e / 2, 4 * g + j) / 2 + (e & 1);
+                so[d] = O[e][j] * f;
+            }
+        const bool all = len == w.n;
+        float *prow = all ? nullptr : part + ((int64_t)(b + s) * Hq + h0) * (DH + 4);      // (one more for each row or block)
+        if (tid < 16) {
+            float L = 0.f;
+#pragma unroll
+            for (int i = 0; i < AT_NW; i++) L = __builtin_fmaf(s_l[i][tid], s_m[i][tid] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[i][tid] - M), L);
+            s_q[tid] = L;
+            if (!all && tid < nh) {
+                prow[tid * (DH + 4)] = M;
+                prow[tid * (DH + 4) + 1] = L;
+            }
         }
-    if (tid < 16) {
-        float L = 0.f;
+        __syncthreads();
+        for (int i = tid; i < nh * (DH / 4); i += AT_NT) {
+            const int h = i / (DH / 4), d = i % (DH / 4) * 4;
+            sw_f32x4 a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < AT_NW; i++) L = __builtin_fmaf(s_l[i][tid], s_m[i][tid] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[i][tid] - M), L);
-        s_q[tid] = L;
-        if (w.parts > 1 && tid < nh) {
-            float *ml = part + (((int64_t)s * Hq + h0 + tid) * n_split + sp) * (DH + 4);
-            ml[0] = M;
-            ml[1] = L;
-        }
-    }
-    __syncthreads();
-    for (int i = tid; i < nh * (DH / 4); i += AT_NT) {
-        const int h = i / (DH / 4), d = i % (DH / 4) * 4;
-        sw_f32x4 a = {0.f, 0.f, 0.f, 0.f};
+            for (int v = 0; v < AT_NW; v++) {
+                const sw_f32x4 y = *(const sw_f32x4 *)((float *)sh + (v * 16 + h) * LD + d);
 #pragma unroll
-        for (int v = 0; v < AT_NW; v++) {
-            const sw_f32x4 b = *(const sw_f32x4 *)((float *)sh + (v * 16 + h) * LD + d);
+                for (int e = 0; e < 4; e++) a[e] = a[e] + y[e];
+            }
+            if (!all) {
+                *(sw_f32x4 *)(prow + h * (DH + 4) + 4 + d) = a;
+            } else {
+                const float L = s_q[h];
 #pragma unroll
-            for (int e = 0; e < 4; e++) a[e] = a[e] + b[e];
-        }
-        if (w.parts > 1) {
-            *(sw_f32x4 *)(part + (((int64_t)s * Hq + h0 + h) * n_split + sp) * (DH + 4) + 4 + d) = a;
-        } else {
-            const float L = s_q[h];
-#pragma unroll
-            for (int e = 0; e < 4; e++) a[e] = L == 0.f ? 0.f : a[e] / L;
-            *(sw_f32x4 *)(orow + h * DH + d) = a;
+                for (int e = 0; e < 4; e++) a[e] = L == 0.f ? 0.f : a[e] / L;
+                *(sw_f32x4 *)(out + ((int64_t)s * Hq + h0 + h) * DH + d) = a;
+            }
         }
     }
 }
 
-// The parts of a row's head joined: part [row][head][n_split] of (maximum, sum, -, -, the
+// The parts of a row's head joined: part [block + row][head] of (maximum, sum, -, -, the
 // output's values).  A part's weight first, one part a thread; then dh / 4 threads take four values of
 // every (AT_NT / (dh / 4))-th part, and their sums meet in order.
-#define AT_MAXPARTS 2048
-__global__ __launch_bounds__(AT_NT) void k_attn_join(SwKv c, SwRows r, int Hq, int window, int CT, const float *__restrict__ part,
-                                                     int n_split, int min_per, float *__restrict__ out) {
-    __shared__ float s_f[AT_MAXPARTS], s_r[AT_NW];
+__global__ __launch_bounds__(AT_NT) void k_attn_join(SwKv c, SwRows r, int S, int Hq, int window, int CT, const float *__restrict__ part,
+                                                     int B, float *__restrict__ out) {
+    __shared__ float s_f[AT_BLOCKS], s_r[AT_NW];
     __shared__ sw_f32x4 s_o[AT_NT];
-    const int tid = threadIdx.x, s = blockIdx.x / Hq, nd = c.dh / 4, ng = AT_NT / nd, row = c.dh + 4;
-    const AtWork w = at_work(c, r, s, window, CT, n_split, min_per);
-    if (w.parts < 2) return;
-    const float *p = part + (int64_t)blockIdx.x * n_split * row;
+    __shared__ int64_t s_scan[3 * AT_NW];
+    const int tid = threadIdx.x, s = blockIdx.x / Hq, h = blockIdx.x % Hq, nd = c.dh / 4, ng = AT_NT / nd;
+    const int n = at_row(c, r, s, window, CT).n;
+    if (n == 0) return;
+    const AtPlan plan = at_plan(c, r, S, window, CT, B, s, s_scan);
+    if (plan.whole) return;
+    const int b0 = (int)(plan.before / plan.q), parts = (int)((plan.before + n - 1) / plan.q) - b0 + 1;
+    if (parts < 2) return;
+    const int64_t row = (int64_t)Hq * (c.dh + 4);                      // from a part to the next
+    const float *p = part + ((int64_t)(b0 + s) * Hq + h) * (c.dh + 4);
     float M = -INFINITY, L = 0.f;
-    for (int i = tid; i < w.parts; i += AT_NT) {
-        s_f[i] = p[(int64_t)i * row];
+    for (int i = tid; i < parts; i += AT_NT) {
+        s_f[i] = p[i * row];
         M = fmaxf(M, s_f[i]);
     }
     for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
@@ -364,10 +479,10 @@ __global__ __launch_bounds__(AT_NT) void k_attn_join(SwKv c, SwRows r, int Hq, i
 #pragma unroll
     for (int i = 0; i < AT_NW; i++) M = fmaxf(M, s_r[i]);
     __syncthreads();
-    for (int i = tid; i < w.parts; i += AT_NT) {
+    for (int i = tid; i < parts; i += AT_NT) {
         const float f = s_f[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_f[i] - M);
         s_f[i] = f;
-        L = __builtin_fmaf(p[(int64_t)i * row + 1], f, L);
+        L = __builtin_fmaf(p[i * row + 1], f, L);
     }
     for (int o = 32; o; o >>= 1) L = L + __shfl_xor(L, o);
     if ((tid & 63) == 0) s_r[tid >> 6] = L;
@@ -376,8 +491,8 @@ __global__ __launch_bounds__(AT_NT) void k_attn_join(SwKv c, SwRows r, int Hq, i
     sw_f32x4 a = {0.f, 0.f, 0.f, 0.f};
     if (gr < ng) {
 #pragma unroll 4
-        for (int i = gr; i < w.parts; i += ng) {
-            const sw_f32x4 v = *(const sw_f32x4 *)(p + (int64_t)i * row + 4 + d);
+        for (int i = gr; i < parts; i += ng) {
+            const sw_f32x4 v = *(const sw_f32x4 *)(p + i * row + 4 + d);
             const float f = s_f[i];
 #pragma unroll
             for (int e = 0; e < 4; e++) a[e] = __builtin_fmaf(v[e], f, a[e]);
@@ -399,56 +514,51 @@ __global__ __launch_bounds__(AT_NT) void k_attn_join(SwKv c, SwRows r, int Hq, i
     *(sw_f32x4 *)(out + (int64_t)blockIdx.x * c.dh + d) = a;
 }
 
-// Parts of a row: as many as give the chip about AT_BLOCKS blocks, of at least AT_MIN chunks each.
-#define AT_BLOCKS 1024
-#define AT_MIN 4
-static int at_splits(const SwKv &c, const SwRows &r, int Hq, int window, int S) {
-    const int G = Hq / c.Hkv, CT = c.type == SW_KV_F32 ? 16 : 32;
-    const int64_t base = (int64_t)S * c.Hkv * ((G + 15) / 16);
+// Blocks of a cache head: so many that all of them are AT_BLOCKS, no more than chunks for them.
+static int at_blocks(const SwKv &c, const SwRows &r, int Hq, int window, int S) {
+    const int per_s = c.Hkv * ((Hq / c.Hkv + 15) / 16), CT = c.type == SW_KV_F32 ? 16 : 32;
     int64_t cells = (int64_t)r.max_pages << c.psh;
-    if (window > 0 && window + CT < cells) cells = window + CT;       // (a window begins anywhere in a chunk)
-    int64_t n = (AT_BLOCKS + base - 1) / base, most = (cells / CT + AT_MIN) / AT_MIN;
-    n = n < most ? n : most;
-    n = n < AT_MAXPARTS ? n : AT_MAXPARTS;
-    return (int)(n < 1 ? 1 : n);
+    if (window > 0 && (int64_t)window + CT < cells) cells = (int64_t)window + CT;      // (a window begins anywhere in a chunk)
+    const int64_t most = (S * (cells / CT + 1) + AT_MIN - 1) / AT_MIN, n = AT_BLOCKS / per_s;
+    return (int)(n < 1 ? 1 : n < most ? n : most);
 }
 int64_t sw_attn_part_floats(const SwKv &c, const SwRows &r, int Hq, int window, int S) {
-    const int n = at_splits(c, r, Hq, window, S);
-    return n > 1 ? (int64_t)S * Hq * n * (c.dh + 4) : 0;
+    const int B = at_blocks(c, r, Hq, window, S);
+    return B > 1 ? (int64_t)(B + S) * Hq * (c.dh + 4) : 0;
 }
 
 template <int TYPE, int NB>
-static void at_launch(hipStream_t st, unsigned grid, const SwKv &c, const SwRows &r, const float *q, int Hq, float sc, int window,
-                      float *out, float *part, int n) {
-    SW_LAUNCH((k_attn<TYPE, NB>), dim3(grid), dim3(AT_NT), 0, st, c, r, q, Hq, sc, window, out, part, n, AT_MIN);
+static void at_launch(hipStream_t st, unsigned grid, const SwKv &c, const SwRows &r, const float *q, int S, int Hq, float sc, int window,
+                      float *out, float *part, int B) {
+    SW_LAUNCH((k_attn<TYPE, NB>), dim3(grid), dim3(AT_NT), 0, st, c, r, q, S, Hq, sc, window, out, part, B);
 }
 template <int TYPE>
-static void at_dispatch(hipStream_t st, unsigned grid, const SwKv &c, const SwRows &r, const float *q, int Hq, float sc, int window,
-                        float *out, float *part, int n) {
+static void at_dispatch(hipStream_t st, unsigned grid, const SwKv &c, const SwRows &r, const float *q, int S, int Hq, float sc,
+                        int window, float *out, float *part, int B) {
     switch (c.dh / 32) {
-    case 1: at_launch<TYPE, 1>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
-    case 2: at_launch<TYPE, 2>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
-    case 3: at_launch<TYPE, 3>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
-    case 4: at_launch<TYPE, 4>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
-    case 5: at_launch<TYPE, 5>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
-    case 6: at_launch<TYPE, 6>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
-    case 7: at_launch<TYPE, 7>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
-    default: at_launch<TYPE, 8>(st, grid, c, r, q, Hq, sc, window, out, part, n); break;
+    case 1: at_launch<TYPE, 1>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
+    case 2: at_launch<TYPE, 2>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
+    case 3: at_launch<TYPE, 3>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
+    case 4: at_launch<TYPE, 4>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
+    case 5: at_launch<TYPE, 5>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
+    case 6: at_launch<TYPE, 6>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
+    case 7: at_launch<TYPE, 7>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
+    default: at_launch<TYPE, 8>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
     }
 }
 
 int sw_launch_attn(hipStream_t st, const SwKv &c, const SwRows &r, const float *q, int Hq, float scale, int window, float *out,
                    int S, float *part) {
     if (c.dh < 32 || c.dh > 256 || c.dh % 32) return -1;
-    const int n = at_splits(c, r, Hq, window, S), gt = (Hq / c.Hkv + 15) / 16;
-    const int64_t grid = (int64_t)S * n * c.Hkv * gt;
-    if (grid >= (int64_t)1 << 31 || (int64_t)S * Hq >= (int64_t)1 << 31 || (n > 1 && !part)) return -1;
+    const int B = at_blocks(c, r, Hq, window, S);
+    const int64_t grid = (int64_t)B * c.Hkv * ((Hq / c.Hkv + 15) / 16);
+    if ((int64_t)S * Hq >= (int64_t)1 << 31 || (B > 1 && !part)) return -1;
     const float sc = (float)((double)scale * 1.4426950408889634074);   // the softmax in powers of two
-    if (c.type == SW_KV_F32) at_dispatch<SW_KV_F32>(st, (unsigned)grid, c, r, q, Hq, sc, window, out, part, n);
-    else if (c.type == SW_KV_BF16) at_dispatch<SW_KV_BF16>(st, (unsigned)grid, c, r, q, Hq, sc, window, out, part, n);
-    else at_dispatch<SW_KV_F16>(st, (unsigned)grid, c, r, q, Hq, sc, window, out, part, n);
-    if (n > 1)
-        SW_LAUNCH(k_attn_join, dim3((unsigned)(S * Hq)), dim3(AT_NT), 0, st, c, r, Hq, window, c.type == SW_KV_F32 ? 16 : 32,
-                  part, n, AT_MIN, out);
+    if (c.type == SW_KV_F32) at_dispatch<SW_KV_F32>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B);
+    else if (c.type == SW_KV_BF16) at_dispatch<SW_KV_BF16>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B);
+    else at_dispatch<SW_KV_F16>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B);
+    if (B > 1)
+        SW_LAUNCH(k_attn_join, dim3((unsigned)(S * Hq)), dim3(AT_NT), 0, st, c, r, S, Hq, window, c.type == SW_KV_F32 ? 16 : 32, part, B,
+                  out);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
