@@ -23,6 +23,9 @@
 #define AT_NW (AT_NT / 64)
 #define AT_BLOCKS 512                     // two blocks on each CU
 #define AT_MIN 4                          // chunks of a part: one a wave
+// A row's parts are joined by the block that finishes last (one launch), with up to this many blocks
+// of a cache head; by k_attn_join, over more blocks, where there can be more parts than that
+#define AT_FUSE 64
 
 // bytes of a lane per row: 16-byte pieces first, then 8 and 4; the byte of row `rr` at dword w
 template <int RB>
@@ -168,6 +171,23 @@ __device__ __forceinline__ int at_find(const SwKv &c, const SwRows &r, int S, in
     return at_uni((int)s_scan[AT_NW]);
 }
 
+// What one block writes for another of the same launch goes through to memory and is read from there,
+// eight bytes at a time (agent-scope accesses): no cache has to be written back or dropped for it, as a
+// fence would, 20 us and more over a launch of 512 blocks.  The writer waits for its
+// stores before it counts itself done.
+__device__ __forceinline__ void at_put(float *p, float a, float b) {
+    const uint64_t v = ((uint64_t)__builtin_bit_cast(uint32_t, b) << 32) | __builtin_bit_cast(uint32_t, a);
+    __hip_atomic_store((uint64_t *)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 at_get(const float *p) {
+    const uint64_t v = __hip_atomic_load((const uint64_t *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__builtin_bit_cast(float, (uint32_t)v), __builtin_bit_cast(float, (uint32_t)(v >> 32)));
+}
+
+// Parts that are written, of the split row that begins in a block (no two begin in one): counted up by
+// its blocks, and zero again when the last has joined them.  Launches are in one stream's order.
+static __device__ int g_at_done[AT_BLOCKS];
+
 // One block per cache head (16 query heads of it) and share of the rows' chunks; of a row's part a
 // wave takes every 4th chunk, its k of the next chunk and v of the next chunk in flight while
 // it computes.
@@ -179,7 +199,8 @@ __global__ __launch_bounds__(AT_NT, NB > 4 ? 1 : 2) void k_attn(SwKv c, SwRows r
     constexpr int NT = CT / 16, NS = RB / 64, ND = RB / 64, NTOK = 4 * NT, NO = DH / 16;
     constexpr int NP = F32 ? 1 : AtParts<TYPE>::n, QN = NP * NS * 64, QI = (NS * 64 + AT_NT - 1) / AT_NT;
     constexpr int LD = DH + 4;                                         // a head's row in the waves' join
-    constexpr int SHB = QN * 16 > AT_NW * 16 * LD * 4 ? QN * 16 : AT_NW * 16 * LD * 4;
+    constexpr int SHJ = AT_NW * 16 * LD * 4, SHB = QN * 16 > SHJ ? QN * 16 : SHJ;
+    static_assert(SHJ >= AT_FUSE * 16 * 4 + AT_NT * 16, "the parts' weights and sums");
     __shared__ __align__(16) char sh[SHB];
     __shared__ float s_m[AT_NW][16], s_l[AT_NW][16], s_q[16];
     __shared__ int64_t s_scan[3 * AT_NW];
@@ -206,6 +227,7 @@ __global__ __launch_bounds__(AT_NT, NB > 4 ? 1 : 2) void k_attn(SwKv c, SwRows r
         const int from = plan.whole ? 0 : (int)(at - before), len = plan.whole ? w.n : (int)(end - at < w.n - from ? end - at : w.n - from);
         const int c1 = w.c0 + from + len;
         int ch = w.c0 + from + wave;
+        const int64_t begin = before;
         before += w.n;
         at += len;
         // ---- q's rows on their way, then the first chunk's cells
@@ -424,10 +446,7 @@ __global__ __launch_bounds__(AT_NT, NB > 4 ? 1 : 2) void k_attn(SwKv c, SwRows r
 #pragma unroll
             for (int i = 0; i < AT_NW; i++) L = __builtin_fmaf(s_l[i][tid], s_m[i][tid] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_m[i][tid] - M), L);
             s_q[tid] = L;
-            if (!all && tid < nh) {
-                prow[tid * (DH + 4)] = M;
-                prow[tid * (DH + 4) + 1] = L;
-            }
+            if (!all && tid < nh) at_put(prow + tid * (DH + 4), M, L);
         }
         __syncthreads();
         for (int i = tid; i < nh * (DH / 4); i += AT_NT) {
@@ -440,8 +459,88 @@ __global__ __launch_bounds__(AT_NT, NB > 4 ? 1 : 2) void k_attn(SwKv c, SwRows r
                 for (int e = 0; e < 4; e++) a[e] = a[e] + y[e];
             }
             if (!all) {
-                *(sw_f32x4 *)(prow + h * (DH + 4) + 4 + d) = a;
+                at_put(prow + h * (DH + 4) + 4 + d, a[0], a[1]);
+                at_put(prow + h * (DH + 4) + 6 + d, a[2], a[3]);
             } else {
+                const float L = s_q[h];
+#pragma unroll
+                for (int e = 0; e < 4; e++) a[e] = L == 0.f ? 0.f : a[e] / L;
+                *(sw_f32x4 *)(out + ((int64_t)s * Hq + h0 + h) * DH + d) = a;
+            }
+        }
+        if (all || B > AT_FUSE) continue;
+        // ---- the last of the row's blocks joins its parts, in their order
+        const int b0 = (int)(begin / plan.q), parts = (int)((before - 1) / plan.q) - b0 + 1;
+        int *done = g_at_done + hg * B + b0;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();                                               // the block's part is in memory
+        if (tid == 0) s_q[0] = __hip_atomic_fetch_add(done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1 ? 1.f : 0.f;
+        __syncthreads();
+        if (s_q[0] == 0.f) continue;
+        if (tid == 0) __hip_atomic_store(done, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int64_t prs = (int64_t)Hq * (DH + 4);                    // from a part to the next
+        const float *p0 = part + ((int64_t)(b0 + s) * Hq + h0) * (DH + 4);
+        float *s_f = (float *)sh;                                      // [part][head] weights
+        sw_f32x4 *s_o = (sw_f32x4 *)(sh + AT_FUSE * 16 * 4);
+        const int items = nh * (DH / 4), ng = items < AT_NT ? AT_NT / items : 1;       // groups of parts, where few values
+        const int it0 = ng > 1 ? tid % items : tid, gr = ng > 1 ? tid / items : 0;
+        for (int i0 = 0; i0 < items; i0 += AT_NT) {
+            const int it = i0 + it0, h = it / (DH / 4), d = it % (DH / 4) * 4;
+            const bool mine = it < items && gr < ng;
+            const float *po = p0 + h * (DH + 4) + 4 + d;
+            sw_f32x4 a = {0.f, 0.f, 0.f, 0.f};
+            for (int j0 = gr; j0 < parts || j0 == gr; j0 += 8 * ng) {
+                float2 y[8], z[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    y[j] = z[j] = make_float2(0.f, 0.f);
+                    if (mine && j0 + j * ng < parts) {
+                        y[j] = at_get(po + (j0 + j * ng) * prs);
+                        z[j] = at_get(po + (j0 + j * ng) * prs + 2);
+                    }
+                }
+                if (i0 == 0 && j0 == gr) {                             // (meanwhile) the parts' weights, 16 threads a head
+                    const int hh = tid >> 4;
+                    float2 ml[AT_FUSE / 16];
+                    float M2 = -INFINITY, L = 0.f;
+#pragma unroll
+                    for (int i = 0; i < AT_FUSE / 16; i++) {
+                        ml[i] = make_float2(-INFINITY, 0.f);
+                        if (hh < nh && (tid & 15) + 16 * i < parts) ml[i] = at_get(p0 + ((tid & 15) + 16 * i) * prs + hh * (DH + 4));
+                        M2 = fmaxf(M2, ml[i].x);
+                    }
+                    for (int o = 8; o; o >>= 1) M2 = fmaxf(M2, __shfl_xor(M2, o));
+#pragma unroll
+                    for (int i = 0; i < AT_FUSE / 16; i++) {
+                        const float x = ml[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[i].x - M2);
+                        if (hh < nh) s_f[((tid & 15) + 16 * i) * 16 + hh] = x;
+                        L = __builtin_fmaf(ml[i].y, x, L);
+                    }
+                    for (int o = 8; o; o >>= 1) L = L + __shfl_xor(L, o);
+                    __syncthreads();                                   // (s_q[0] is read)
+                    if ((tid & 15) == 0 && hh < nh) s_q[hh] = L;
+                    __syncthreads();
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float x = mine && j0 + j * ng < parts ? s_f[(j0 + j * ng) * 16 + h] : 0.f;
+                    a[0] = __builtin_fmaf(y[j].x, x, a[0]);
+                    a[1] = __builtin_fmaf(y[j].y, x, a[1]);
+                    a[2] = __builtin_fmaf(z[j].x, x, a[2]);
+                    a[3] = __builtin_fmaf(z[j].y, x, a[3]);
+                }
+            }
+            if (ng > 1) {
+                s_o[tid] = a;
+                __syncthreads();
+                for (int i = 1; i < ng && gr == 0; i++) {
+                    const sw_f32x4 y = s_o[i * items + it];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) a[e] = a[e] + y[e];
+                }
+            }
+            if (mine && gr == 0) {
                 const float L = s_q[h];
 #pragma unroll
                 for (int e = 0; e < 4; e++) a[e] = L == 0.f ? 0.f : a[e] / L;
@@ -557,7 +656,7 @@ int sw_launch_attn(hipStream_t st, const SwKv &c, const SwRows &r, const float *
     if (c.type == SW_KV_F32) at_dispatch<SW_KV_F32>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B);
     else if (c.type == SW_KV_BF16) at_dispatch<SW_KV_BF16>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B);
     else at_dispatch<SW_KV_F16>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B);
-    if (B > 1)
+    if (B > AT_FUSE)
         SW_LAUNCH(k_attn_join, dim3((unsigned)(S * Hq)), dim3(AT_NT), 0, st, c, r, S, Hq, window, c.type == SW_KV_F32 ? 16 : 32, part, B,
                   out);
     return hipGetLastError() == hipSuccess ? 0 : -1;
