@@ -256,9 +256,11 @@ int    lag_hip_qk_rope_append(const LagHipKvCache *c, const LagHipKvRows *r, con
  * n_heads); q and out [S][n_q_heads][head_dim], 16-byte aligned, not overlapping.  Sums and
  * the softmax in 32 bits.  A free place, or a row without any cell, gives zeros.  Rows of one
  * sequence at consecutive positions (a chunk of a prompt, already appended) each see what is
- * theirs to see.  Infinities and NaN in a cell reach the rows that attend to it, as values
- * without meaning, and no others; cells that no row attends to may hold anything.  A row's bits depend on S, n_q_heads and max_pages * page_size, not on the
- * other rows' values.  0 = ok */
+ * theirs to see.  max_pages * page_size times S, or 64 if that is less, is below 2^36.  Infinities and NaN in a cell reach the rows that attend to it, as values
+ * without meaning, and no others; cells that no row attends to may hold anything.  The
+ * same call gives the same bits; how a row's cells are cut into parts, and with that its
+ * last bits, depends on the batch's positions, S, n_q_heads, window and max_pages * page_size, not on what
+ * the other rows' cells hold.  0 = ok */
 int    lag_hip_attn_paged(const LagHipKvCache *c, const LagHipKvRows *r, const float *q, int n_q_heads, float scale,
                           int window, float *out, int S);
 /* Page src[i] of every one of n_layers caches (one geometry and type) to page dst[i], k and v:

@@ -74,101 +74,81 @@ __device__ __forceinline__ sw_f32x4 at_mfma(sw_u32x4 a, sw_u32x4 b, sw_f32x4 c) 
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(sw_half8, a), __builtin_bit_cast(sw_half8, b), c, 0, 0, 0);
 }
 
-// A row's cells as chunks of CT tokens: n of them from chunk c0.
-struct AtRow { int first, last, c0, n; };
-__device__ __forceinline__ AtRow at_row(const SwKv &c, const SwRows &r, int s, int window, int CT) {
-    AtRow w;
-    const int pos = r.pos[s], sq = r.seq ? r.seq[s] : s;
-    w.first = window > 0 && pos >= window ? pos - window + 1 : 0;
-    w.last = min(pos, (r.max_pages << c.psh) - 1);                     // (the host keeps that below 2^30)
-    if (sq < 0 || sq >= r.n_seqs) w.last = -1;
-    w.c0 = w.first / CT;
-    w.n = w.last < w.first ? 0 : w.last / CT - w.c0 + 1;
-    return w;
-}
-
 // (the same in every lane: kept in scalar registers)
 __device__ __forceinline__ int at_uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int64_t at_uni(int64_t x) {
     return (int64_t)(((uint64_t)(uint32_t)at_uni((int)(x >> 32)) << 32) | (uint32_t)at_uni((int)x));
 }
+// Row s's position, -1 for a row without cells to look for
+__device__ __forceinline__ int at_pos(const SwRows &r, int s) {
+    const int sq = r.seq ? r.seq[s] : s;
+    return sq < 0 || sq >= r.n_seqs ? -1 : r.pos[s];
+}
+// A row's cells as chunks of CT tokens: n of them from chunk c0.
+struct AtRow { int first, last, c0, n; };
+__device__ __forceinline__ AtRow at_row(const SwKv &c, const SwRows &r, int pos, int window, int CT) {
+    AtRow w;
+    w.first = window > 0 && pos >= window ? pos - window + 1 : 0;
+    w.last = min(pos, (r.max_pages << c.psh) - 1);                     // (the host keeps that below 2^30)
+    w.c0 = w.first / CT;
+    w.n = w.last < w.first ? 0 : w.last / CT - w.c0 + 1;
+    return w;
+}
 
 // How the rows' chunks are dealt to the B blocks of a cache head.  Laid end to end they are N, and
 // block b takes those from b q to (b + 1) q, whatever rows they fall in: parts of rows, joined
-// by k_attn_join, and the same work for each block however the lengths differ.  Where whole rows
-// (b, b + B, ...) are as even, within a fifth, they are dealt whole.  The lengths are on the device
-// alone, so each block counts them.
-struct AtPlan { int64_t N, q, before; bool whole; };                   // before: the chunks of rows before row `upto`
-__device__ __forceinline__ AtPlan at_plan(const SwKv &c, const SwRows &r, int S, int window, int CT, int B, int upto, int64_t *s_scan) {
+// at the end, and the same work for each block however the lengths differ.  Where whole rows (b,
+// b + B, ...) are as even, within a fifth, they are dealt whole.  The lengths are on the device alone, so
+// each wave counts them, 64 rows at a time; up to 64 rows their positions then stay in registers.
+struct AtPlan {
+    int64_t N, q;
+    bool whole;
+    int pos, n;                                                        // lane i: row i's position and chunks (S <= 64)
+    uint32_t upto;                                                     //         the chunks of rows up to it
+};
+__device__ __forceinline__ AtPlan at_plan(const SwKv &c, const SwRows &r, int S, int window, int CT, int B) {
     AtPlan p;
-    int64_t mx;
+    const int lane = threadIdx.x & 63;
+    int64_t mx = 0;
+    p.N = 0;
     if (S == 1) {
-        p.N = mx = at_row(c, r, 0, window, CT).n;
-        p.before = 0;
-    } else {
-        int64_t n = 0, before = 0;
-        mx = 0;
-        for (int i = threadIdx.x; i < S; i += AT_NT) {
-            const int64_t x = at_row(c, r, i, window, CT).n;
-            n += x;
-            before += i < upto ? x : 0;
-            mx = x > mx ? x : mx;
-        }
-        for (int o = 32; o; o >>= 1) {
-            n += __shfl_xor(n, o);
-            before += __shfl_xor(before, o);
-            const int64_t t = __shfl_xor(mx, o);
-            mx = t > mx ? t : mx;
-        }
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) {
-            s_scan[threadIdx.x >> 6] = n;
-            s_scan[AT_NW + (threadIdx.x >> 6)] = before;
-            s_scan[2 * AT_NW + (threadIdx.x >> 6)] = mx;
-        }
-        __syncthreads();
-        p.N = p.before = 0;
-        for (int i = 0; i < AT_NW; i++) {
-            p.N += s_scan[i];
-            p.before += s_scan[AT_NW + i];
-            mx = s_scan[2 * AT_NW + i] > mx ? s_scan[2 * AT_NW + i] : mx;
-        }
+        p.pos = at_uni(at_pos(r, 0));
+        p.n = at_row(c, r, p.pos, window, CT).n;
+        p.upto = (uint32_t)p.n;
+        p.N = mx = p.n;
+    } else
+    for (int i0 = 0; i0 < S; i0 += 64) {                               // (the host keeps 64 rows below 2^32 chunks)
+        p.pos = i0 + lane < S ? at_pos(r, i0 + lane) : -1;
+        p.n = at_row(c, r, p.pos, window, CT).n;
+        p.upto = sw_wave_scan((uint32_t)p.n);
+        p.N += (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)p.upto, 63);
+        const int m = at_uni((int)sw_wave_max((uint32_t)p.n));
+        mx = m > mx ? m : mx;
     }
-    p.N = at_uni(p.N);
-    p.before = at_uni(p.before);
-    mx = at_uni(mx);
     p.q = (p.N + B - 1) / B;
     p.whole = 5 * mx * ((S + B - 1) / B) <= 6 * p.q;
     if (p.q < AT_MIN) p.q = AT_MIN;
     return p;
 }
-// the row in which chunk `at` of all lies, and the chunks of rows before it
-__device__ __forceinline__ int at_find(const SwKv &c, const SwRows &r, int S, int window, int CT, int64_t at, int64_t &before,
-                                       int64_t *s_scan) {
-    if (S == 1) { before = 0; return 0; }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// the row in which chunk `at` (below N) of all lies, and the chunks of rows before it
+__device__ __forceinline__ int at_find(const AtPlan &plan, const SwKv &c, const SwRows &r, int S, int window, int CT, int64_t at,
+                                       int64_t &before) {
+    const int lane = threadIdx.x & 63;
     int64_t base = 0;
-    for (int i0 = 0;; i0 += AT_NT) {                                   // (`at` is below the rows' sum: it ends)
-        const int i = i0 + (int)threadIdx.x;
-        const int64_t n = i < S ? at_row(c, r, i, window, CT).n : 0;
-        int64_t x = n;
-        for (int o = 1; o < 64; o <<= 1) { const int64_t t = __shfl_up(x, o); if (lane >= o) x += t; }
-        __syncthreads();
-        if (lane == 63) s_scan[wave] = x;
-        __syncthreads();
-        int64_t all = 0;
-        x += base - n;
-        for (int q = 0; q < AT_NW; q++) {
-            if (q < wave) x += s_scan[q];
-            all += s_scan[q];
+    uint32_t upto = plan.upto;
+    int n = plan.n, i0 = 0;
+    for (;; i0 += 64) {
+        if (S > 64) {
+            n = i0 + lane < S ? at_row(c, r, at_pos(r, i0 + lane), window, CT).n : 0;
+            upto = sw_wave_scan((uint32_t)n);
         }
-        if (x <= at && at < x + n) { s_scan[AT_NW] = i; s_scan[AT_NW + 1] = x; }
+        const int64_t all = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+        if (base + all > at || i0 + 64 >= S) break;
         base += all;
-        if (base > at || i0 + AT_NT >= S) break;
     }
-    __syncthreads();
-    before = at_uni(s_scan[AT_NW + 1]);
-    return at_uni((int)s_scan[AT_NW]);
+    const int i = __builtin_ctzll(__ballot((int64_t)upto > at - base) | (1ull << 63));
+    before = base + (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(upto - (uint32_t)n), i);
+    return i0 + i;
 }
 
 // What one block writes for another of the same launch goes through to memory and is read from there,
@@ -203,25 +183,25 @@ __global__ __launch_bounds__(AT_NT, NB > 4 ? 1 : 2) void k_attn(SwKv c, SwRows r
     static_assert(SHJ >= AT_FUSE * 16 * 4 + AT_NT * 16, "the parts' weights and sums");
     __shared__ __align__(16) char sh[SHB];
     __shared__ float s_m[AT_NW][16], s_l[AT_NW][16], s_q[16];
-    __shared__ int64_t s_scan[3 * AT_NW];
     const int tid = threadIdx.x, lane = tid & 63, wave = at_uni(tid >> 6), g = lane >> 4, cl = lane & 15;
     const int G = Hq / c.Hkv, gt = (G + 15) >> 4, per_s = c.Hkv * gt;
     const int hg = blockIdx.x % per_s, b = blockIdx.x / per_s;
     const int hk = hg / gt, h0 = hk * G + (hg % gt) * 16, nh = min(16, G - (hg % gt) * 16);
+    const AtPlan plan = at_plan(c, r, S, window, CT, B);
+    auto row_at = [&](int s) { return at_row(c, r, S <= 64 ? __builtin_amdgcn_readlane(plan.pos, s) : at_uni(at_pos(r, s)), window, CT); };
     for (int64_t s = b + (int64_t)B * tid; s < S; s += (int64_t)B * AT_NT)             // rows without any cell: zeros
-        if (at_row(c, r, (int)s, window, CT).n == 0)
+        if (at_row(c, r, at_pos(r, (int)s), window, CT).n == 0)
             for (int i = 0; i < nh * DH; i += 4) *(sw_f32x4 *)(out + (s * Hq + h0) * DH + i) = sw_f32x4{0.f, 0.f, 0.f, 0.f};
-    const AtPlan plan = at_plan(c, r, S, window, CT, B, 0, s_scan);
     int64_t at = (int64_t)b * plan.q, end = at + plan.q < plan.N ? at + plan.q : plan.N, before = 0;
     if (!plan.whole && at >= end) return;
-    int s = plan.whole ? b : at_find(c, r, S, window, CT, at, before, s_scan);
+    int s = plan.whole ? b : at_find(plan, c, r, S, window, CT, at, before);
     const int pmask = (1 << c.psh) - 1;
     const char *kb = (const char *)c.k + (int64_t)hk * c.hs * ES + g * 16;
     const char *vb = (const char *)c.v + (int64_t)hk * c.hs * ES;
     sw_u32x4 *sq = (sw_u32x4 *)sh;
 
     for (; s < S && (plan.whole || at < end); s += plan.whole ? B : 1) {
-        const AtRow w = at_row(c, r, s, window, CT);
+        const AtRow w = row_at(s);
         if (w.n == 0) continue;
         // this block's chunks of the row
         const int from = plan.whole ? 0 : (int)(at - before), len = plan.whole ? w.n : (int)(end - at < w.n - from ? end - at : w.n - from);
@@ -557,13 +537,17 @@ __global__ __launch_bounds__(AT_NT) void k_attn_join(SwKv c, SwRows r, int S, in
                                                      int B, float *__restrict__ out) {
     __shared__ float s_f[AT_BLOCKS], s_r[AT_NW];
     __shared__ sw_f32x4 s_o[AT_NT];
-    __shared__ int64_t s_scan[3 * AT_NW];
     const int tid = threadIdx.x, s = blockIdx.x / Hq, h = blockIdx.x % Hq, nd = c.dh / 4, ng = AT_NT / nd;
-    const int n = at_row(c, r, s, window, CT).n;
+    const int n = at_row(c, r, at_uni(at_pos(r, s)), window, CT).n;
     if (n == 0) return;
-    const AtPlan plan = at_plan(c, r, S, window, CT, B, s, s_scan);
+    const AtPlan plan = at_plan(c, r, S, window, CT, B);
     if (plan.whole) return;
-    const int b0 = (int)(plan.before / plan.q), parts = (int)((plan.before + n - 1) / plan.q) - b0 + 1;
+    int64_t before = 0;                                                // the chunks of rows before it
+    for (int i0 = 0; i0 < s; i0 += 64) {
+        const int i = i0 + (tid & 63);
+        before += (uint32_t)__builtin_amdgcn_readlane((int)sw_wave_scan(i < s ? (uint32_t)at_row(c, r, at_pos(r, i), window, CT).n : 0u), 63);
+    }
+    const int b0 = (int)(before / plan.q), parts = (int)((before + n - 1) / plan.q) - b0 + 1;
     if (parts < 2) return;
     const int64_t row = (int64_t)Hq * (c.dh + 4);                      // from a part to the next
     const float *p = part + ((int64_t)(b0 + s) * Hq + h) * (c.dh + 4);

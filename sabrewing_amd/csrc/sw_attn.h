@@ -56,6 +56,26 @@ __device__ __forceinline__ uint2 sw_pair(uint32_t a) {
     const auto r = BY == 16 ? __builtin_amdgcn_permlane16_swap(a, b, false, false) : __builtin_amdgcn_permlane32_swap(a, b, false, false);
     return make_uint2((uint32_t)r[0], (uint32_t)r[1]);
 }
+// sums up to each lane of a wave (shifts by 1, 2, 4, 8 in rows of 16, then the rows' last), the wave's maximum
+__device__ __forceinline__ uint32_t sw_wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+__device__ __forceinline__ uint32_t sw_wave_max(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xF, 0xF, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xF, 0xF, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xF, 0xF, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xF, 0xF, false));
+    uint2 p = sw_pair<16>(v);
+    v = max(p.x, p.y);
+    p = sw_pair<32>(v);
+    return max(p.x, p.y);
+}
 // over the four lanes 16 apart
 __device__ __forceinline__ float sw_max4(float x) {
     const uint2 a = sw_pair<16>(__builtin_bit_cast(uint32_t, x));

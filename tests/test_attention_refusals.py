@@ -130,3 +130,10 @@ def test_good_arguments_reach_the_device(lib):
     assert "not initialised" in lib.lag_hip_last_error().decode()
     for f in (lambda: rope_call(lib), lambda: attn_call(lib), lambda: copy_call(lib, [0], [1])):
         refused(lib, f(), "not initialised")
+
+
+def test_too_many_cells(lib):
+    """64 rows of tables of 2^30 cells are refused, one is not"""
+    r = dict(n_seqs=64, max_pages=1 << 26)
+    refused(lib, attn_call(lib, r=rows(**r), S=64, out=1024 * A), "2^30")
+    assert attn_call(lib, r=rows(**r), S=1) == -1 and "2^30" not in lib.lag_hip_last_error().decode()
