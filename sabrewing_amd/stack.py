@@ -3,6 +3,10 @@ decode step: for every layer h += MoE(rmsnorm(h, w_l)), then rmsnorm(h, w_f),
 the bf16 head and a greedy pick (c/laguna.c forward_span / argmax_logits,
 c/laguna.c:1156-1160; rmsnorm_row c/moe_math.h:58-62).
 
+With attention layers (attn=) a layer is h += attention(rmsnorm(h)), then the MoE half, over a
+PagedCache (attention.py); with draw= a step ends in a random pick (lag_hip_sample) in place of the
+greedy one.
+
 Synthetic stacks are seeded like the layers: norm weights 1 + N(0, 0.02)
 (tensor T_NORM of layer l, the final norm as layer L), the head N(0, 0.02)
 bf16 [V, D] (tensor T_HEAD).
@@ -10,6 +14,7 @@ bf16 [V, D] (tensor T_HEAD).
 import numpy as np
 
 from . import synth
+from .attention import AttnScratch, DeviceAttention, Rope
 from .backend import DeviceLayer, desc_of
 from .configs import WEIGHT_SIGMA
 
@@ -21,6 +26,24 @@ class DeviceStack:
         self.be, self.cfg, self.V = be, cfg, V
         self.layers, self.norms, self.bufs = [], [], []
         self.final_norm = self.head = None
+        self.attn, self.rope, self.scratch = [], None, None
+
+    def add_attention(self, acfg, layers=None, seed=0):
+        """attention layers in front of the MoE ones: DeviceAttention's (sharing self.rope), or seeded
+        ones made on the device"""
+        self.rope = self.rope or Rope(self.be, acfg)
+        self.attn = list(layers) if layers is not None else [
+            DeviceAttention.generate(self.be, acfg, self.cfg.D, seed, l, self.rope) for l in range(len(self.layers))]
+        if len(self.attn) != len(self.layers):
+            raise ValueError("add_attention: as many attention layers as MoE layers")
+        return self
+
+    def reserve(self, S):
+        """scratch for steps of up to S rows (a step grows it, which a recording cannot)"""
+        if self.attn and (self.scratch is None or self.scratch.S < S):
+            if self.scratch:
+                self.scratch.free()
+            self.scratch = AttnScratch(self.be, self.attn[0].acfg, self.cfg.D, S)
 
     @classmethod
     def from_host(cls, be, cfg, host_layers, norms, final_norm, head_bf16):
@@ -60,24 +83,38 @@ class DeviceStack:
         self.bufs.append(b)
         return b
 
-    def step(self, h, xn, logits, tok, S, fused=True):
+    def step(self, h, xn, logits, tok, S, fused=True, cache=None, rows=None, draw=None):
         """h [S, D] (device, updated in place), xn [S, D] scratch, logits [S, V], tok [S] int32;
         fused: each layer's RMSNorm inside its routing launch (lag_hip_moe_forward_rmsnorm,
-        the same bits as the separate rmsnorm + forward)"""
+        the same bits as the separate rmsnorm + forward); cache, rows: the PagedCache and the
+        descriptor of its rows() for the S tokens (a stack with attention layers); draw: (settings
+        from Backend.sample_params or None, random numbers [S] on the device)"""
         be, D = self.be, self.cfg.D
         desc = desc_of(self.cfg)
+        if self.attn:
+            if cache is None or rows is None or cache.n_layers != len(self.attn):
+                raise ValueError("step: a stack with attention needs a cache of its layers, and rows")
+            self.reserve(S)
         for l, dl in enumerate(self.layers):
+            if self.attn:
+                self.attn[l].forward(h, xn, S, cache.layers[l], rows, self.scratch)
             if fused:
                 be.moe_forward_rmsnorm(desc, dl.weights(), self.norms[l], NORM_EPS, xn, h, S)
             else:
                 be.rmsnorm(h, self.norms[l], xn, S, D, NORM_EPS)
                 be.moe_forward(desc, dl.weights(), xn, h, S)
         be.rmsnorm(h, self.final_norm, xn, S, D, NORM_EPS)
-        be.head_argmax(self.head, True, xn, S, D, self.V, logits, tok)
+        be.head_argmax(self.head, True, xn, S, D, self.V, logits, None if draw else tok)
+        if draw:
+            be.sample(logits, S, self.V, draw[0], draw[1], tok)
 
     def free(self):
-        for dl in self.layers:
+        for dl in self.layers + self.attn:
             dl.free()
+        for b in (self.rope, self.scratch):
+            if b:
+                b.free()
+        self.attn, self.rope, self.scratch = [], None, None
         for b in self.bufs:
             b.free()
         self.layers, self.bufs = [], []
