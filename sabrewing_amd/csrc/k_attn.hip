@@ -23,6 +23,7 @@
 #define AT_NW (AT_NT / 64)
 #define AT_BLOCKS 512                     // two blocks on each CU
 #define AT_MIN 4                          // chunks of a part: one a wave
+#define AT_ROW 12
 // A row's parts are joined by the block that finishes last (one launch), with up to this many blocks
 // of a cache head; by k_attn_join, over more blocks, where there can be more parts than that
 #define AT_FUSE 64
@@ -74,6 +75,27 @@ __device__ __forceinline__ sw_f32x4 at_mfma(sw_u32x4 a, sw_u32x4 b, sw_f32x4 c) 
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(sw_half8, a), __builtin_bit_cast(sw_half8, b), c, 0, 0, 0);
 }
 
+// the same over 16 of the summed index: elements 4 (l / 16) + 0 .. 3 of a lane
+typedef _Float16 at_half4 __attribute__((ext_vector_type(4)));
+typedef short at_short4 __attribute__((ext_vector_type(4)));
+template <int TYPE>
+__device__ __forceinline__ sw_f32x4 at_mfma16(uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1, sw_f32x4 c) {
+    const uint2 a = make_uint2(a0, a1), b = make_uint2(b0, b1);
+    if constexpr (TYPE == SW_KV_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(at_short4, a), __builtin_bit_cast(at_short4, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(at_half4, a), __builtin_bit_cast(at_half4, b), c, 0, 0, 0);
+}
+
+// Tokens of a wave's chunk: two tiles; one where two would leave room for one block on a CU and one for two
+// (bf16 heads of 224 and 256 spill at two: 127 us against 106 for 8 rows of 8192 tokens)
+__host__ __device__ constexpr int at_chunk(int type, int dh) {
+    return type == SW_KV_F32 || (dh > 160 && (type == SW_KV_F16 || dh <= 192)) ? 16 : 32;
+}
+__host__ __device__ constexpr int at_blocks_cu(int type, int dh) {
+    return (type == SW_KV_F32 && dh > 160) || (type == SW_KV_BF16 && dh > 192) ? 1 : 2;
+}
+
 // (the same in every lane: kept in scalar registers)
 __device__ __forceinline__ int at_uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int64_t at_uni(int64_t x) {
@@ -97,16 +119,16 @@ __device__ __forceinline__ AtRow at_row(const SwKv &c, const SwRows &r, int pos,
 
 // How the rows' chunks are dealt to the B blocks of a cache head.  Laid end to end they are N, and
 // block b takes those from b q to (b + 1) q, whatever rows they fall in: parts of rows, joined
-// at the end, and the same work for each block however the lengths differ.  Where whole rows (b,
-// b + B, ...) are as even, within a fifth, they are dealt whole.  The lengths are on the device alone, so
-// each wave counts them, 64 rows at a time; up to 64 rows their positions then stay in registers.
+// at the end, and the same work for each block however the lengths differ.  Or whole rows (b, b + B,
+// ...), where that is less: a row costs a block its chunks and about AT_ROW more for its beginning
+// and end, a join as much again.  The lengths are on the device alone, so each wave counts them, 64 rows at a time; up to 64 rows their positions then stay in registers.
 struct AtPlan {
     int64_t N, q;
     bool whole;
     int pos, n;                                                        // lane i: row i's position and chunks (S <= 64)
     uint32_t upto;                                                     //         the chunks of rows up to it
 };
-__device__ __forceinline__ AtPlan at_plan(const SwKv &c, const SwRows &r, int S, int window, int CT, int B) {
+__device__ __forceinline__ AtPlan at_plan(const SwKv &c, const SwRows &r, int S, int Hq, int window, int CT, int B) {
     AtPlan p;
     const int lane = threadIdx.x & 63;
     int64_t mx = 0;
@@ -126,8 +148,12 @@ __device__ __forceinline__ AtPlan at_plan(const SwKv &c, const SwRows &r, int S,
         mx = m > mx ? m : mx;
     }
     p.q = (p.N + B - 1) / B;
-    p.whole = 5 * mx * ((S + B - 1) / B) <= 6 * p.q;
+    // a part's chunks take a wave a third of a microsecond each, and its outputs the join some 30 KB a
+    // microsecond: the long row's parts are not made shorter than where the two together are least
+    const int best = at_uni((int)sqrtf((float)mx * (float)(min(Hq / c.Hkv, 16) * c.dh) / 2500.f));
     if (p.q < AT_MIN) p.q = AT_MIN;
+    if (p.q < best) p.q = best;
+    p.whole = ((S + B - 1) / B) * (AT_ROW + mx) <= p.q + AT_ROW * (2 + S / B);
     return p;
 }
 // the row in which chunk `at` (below N) of all lies, and the chunks of rows before it
@@ -172,10 +198,10 @@ static __device__ int g_at_done[AT_BLOCKS];
 // wave takes every 4th chunk, its k of the next chunk and v of the next chunk in flight while
 // it computes.
 template <int TYPE, int NB>
-__global__ __launch_bounds__(AT_NT, NB > 4 ? 1 : 2) void k_attn(SwKv c, SwRows r, const float *__restrict__ q, int S, int Hq, float sc0,
+__global__ __launch_bounds__(AT_NT, at_blocks_cu(TYPE, 32 * NB)) void k_attn(SwKv c, SwRows r, const float *__restrict__ q, int S, int Hq, float sc0,
                                                                 int window, float *__restrict__ out, float *__restrict__ part, int B) {
     constexpr bool F32 = TYPE == SW_KV_F32;
-    constexpr int DH = 32 * NB, ES = F32 ? 4 : 2, RB = DH * ES, CT = F32 ? 16 : 32;
+    constexpr int DH = 32 * NB, ES = F32 ? 4 : 2, RB = DH * ES, CT = at_chunk(TYPE, DH);
     constexpr int NT = CT / 16, NS = RB / 64, ND = RB / 64, NTOK = 4 * NT, NO = DH / 16;
     constexpr int NP = F32 ? 1 : AtParts<TYPE>::n, QN = NP * NS * 64, QI = (NS * 64 + AT_NT - 1) / AT_NT;
     constexpr int LD = DH + 4;                                         // a head's row in the waves' join
@@ -187,7 +213,7 @@ __global__ __launch_bounds__(AT_NT, NB > 4 ? 1 : 2) void k_attn(SwKv c, SwRows r
     const int G = Hq / c.Hkv, gt = (G + 15) >> 4, per_s = c.Hkv * gt;
     const int hg = blockIdx.x % per_s, b = blockIdx.x / per_s;
     const int hk = hg / gt, h0 = hk * G + (hg % gt) * 16, nh = min(16, G - (hg % gt) * 16);
-    const AtPlan plan = at_plan(c, r, S, window, CT, B);
+    const AtPlan plan = at_plan(c, r, S, Hq, window, CT, B);
     auto row_at = [&](int s) { return at_row(c, r, S <= 64 ? __builtin_amdgcn_readlane(plan.pos, s) : at_uni(at_pos(r, s)), window, CT); };
     for (int64_t s = b + (int64_t)B * tid; s < S; s += (int64_t)B * AT_NT)             // rows without any cell: zeros
         if (at_row(c, r, at_pos(r, (int)s), window, CT).n == 0)
@@ -386,16 +412,22 @@ __global__ __launch_bounds__(AT_NT, NB > 4 ? 1 : 2) void k_attn(SwKv c, SwRows r
                     for (int e = 0; e < ND; e++)
                         O[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, V[j][e]), pr[j], O[e], 0, 0, 0);
             } else {
+                float p8[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) p8[j] = j < NTOK ? pr[j] : 0.f;
                 sw_u32x4 P[NP];
-                at_split<TYPE>(pr, P);
+                at_split<TYPE>(p8, P);
 #pragma unroll
                 for (int e = 0; e < 2 * ND; e++) {
-                    sw_u32x4 a;
+                    uint32_t a[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
+                    for (int i = 0; i < NTOK / 2; i++)
                         a[i] = __builtin_amdgcn_perm(V[2 * i + 1][e / 2], V[2 * i][e / 2], e & 1 ? 0x07060302 : 0x05040100);
 #pragma unroll
-                    for (int u = 0; u < NP; u++) O[e] = at_mfma<TYPE>(a, P[u], O[e]);
+                    for (int u = 0; u < NP; u++) {
+                        if constexpr (NT == 2) O[e] = at_mfma<TYPE>(sw_u32x4{a[0], a[1], a[2], a[3]}, P[u], O[e]);
+                        else O[e] = at_mfma16<TYPE>(a[0], a[1], P[u][0], P[u][1], O[e]);
+                    }
                 }
             }
             if (more) load_v(ch + AT_NW, pn);
@@ -540,7 +572,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_join(SwKv c, SwRows r, int S, in
     const int tid = threadIdx.x, s = blockIdx.x / Hq, h = blockIdx.x % Hq, nd = c.dh / 4, ng = AT_NT / nd;
     const int n = at_row(c, r, at_uni(at_pos(r, s)), window, CT).n;
     if (n == 0) return;
-    const AtPlan plan = at_plan(c, r, S, window, CT, B);
+    const AtPlan plan = at_plan(c, r, S, Hq, window, CT, B);
     if (plan.whole) return;
     int64_t before = 0;                                                // the chunks of rows before it
     for (int i0 = 0; i0 < s; i0 += 64) {
@@ -597,13 +629,14 @@ __global__ __launch_bounds__(AT_NT) void k_attn_join(SwKv c, SwRows r, int S, in
     *(sw_f32x4 *)(out + (int64_t)blockIdx.x * c.dh + d) = a;
 }
 
-// Blocks of a cache head: so many that all of them are AT_BLOCKS, no more than chunks for them.
+// Blocks of a cache head: so many that all of them are AT_BLOCKS, no more than rows or least parts for them.
 static int at_blocks(const SwKv &c, const SwRows &r, int Hq, int window, int S) {
-    const int per_s = c.Hkv * ((Hq / c.Hkv + 15) / 16), CT = c.type == SW_KV_F32 ? 16 : 32;
+    const int per_s = c.Hkv * ((Hq / c.Hkv + 15) / 16), CT = at_chunk(c.type, c.dh);
     int64_t cells = (int64_t)r.max_pages << c.psh;
     if (window > 0 && (int64_t)window + CT < cells) cells = (int64_t)window + CT;      // (a window begins anywhere in a chunk)
     const int64_t most = (S * (cells / CT + 1) + AT_MIN - 1) / AT_MIN, n = AT_BLOCKS / per_s;
-    return (int)(n < 1 ? 1 : n < most ? n : most);
+    const int64_t use = S > most ? S : most;
+    return (int)(n < 1 ? 1 : n < use ? n : use);
 }
 int64_t sw_attn_part_floats(const SwKv &c, const SwRows &r, int Hq, int window, int S) {
     const int B = at_blocks(c, r, Hq, window, S);
@@ -641,7 +674,6 @@ int sw_launch_attn(hipStream_t st, const SwKv &c, const SwRows &r, const float *
     else if (c.type == SW_KV_BF16) at_dispatch<SW_KV_BF16>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B);
     else at_dispatch<SW_KV_F16>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B);
     if (B > AT_FUSE)
-        SW_LAUNCH(k_attn_join, dim3((unsigned)(S * Hq)), dim3(AT_NT), 0, st, c, r, S, Hq, window, c.type == SW_KV_F32 ? 16 : 32, part, B,
-                  out);
+        SW_LAUNCH(k_attn_join, dim3((unsigned)(S * Hq)), dim3(AT_NT), 0, st, c, r, S, Hq, window, at_chunk(c.type, c.dh), part, B, out);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
