@@ -24,6 +24,9 @@
 #define AT_BLOCKS 512                     // two blocks on each CU
 #define AT_MIN 4                          // chunks of a part: one a wave
 #define AT_ROW 12
+// Beyond so many rows they are dealt whole, a block each, without counting them: there are blocks enough
+// to even out, and each would count them all
+#define AT_COUNT 256
 // A row's parts are joined by the block that finishes last (one launch), with up to this many blocks
 // of a cache head; by k_attn_join, over more blocks, where there can be more parts than that
 #define AT_FUSE 64
@@ -129,7 +132,8 @@ struct AtPlan {
     uint32_t upto;                                                     //         the chunks of rows up to it
 };
 __device__ __forceinline__ AtPlan at_plan(const SwKv &c, const SwRows &r, int S, int Hq, int window, int CT, int B) {
-    AtPlan p;
+    AtPlan p = {};
+    if (S > AT_COUNT) { p.whole = true; return p; }
     const int lane = threadIdx.x & 63;
     int64_t mx = 0;
     p.N = 0;
@@ -631,6 +635,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_join(SwKv c, SwRows r, int S, in
 
 // Blocks of a cache head: so many that all of them are AT_BLOCKS, no more than rows or least parts for them.
 static int at_blocks(const SwKv &c, const SwRows &r, int Hq, int window, int S) {
+    if (S > AT_COUNT) return S;
     const int per_s = c.Hkv * ((Hq / c.Hkv + 15) / 16), CT = at_chunk(c.type, c.dh);
     int64_t cells = (int64_t)r.max_pages << c.psh;
     if (window > 0 && (int64_t)window + CT < cells) cells = (int64_t)window + CT;      // (a window begins anywhere in a chunk)
@@ -640,7 +645,7 @@ static int at_blocks(const SwKv &c, const SwRows &r, int Hq, int window, int S) 
 }
 int64_t sw_attn_part_floats(const SwKv &c, const SwRows &r, int Hq, int window, int S) {
     const int B = at_blocks(c, r, Hq, window, S);
-    return B > 1 ? (int64_t)(B + S) * Hq * (c.dh + 4) : 0;
+    return B > 1 && S <= AT_COUNT ? (int64_t)(B + S) * Hq * (c.dh + 4) : 0;
 }
 
 template <int TYPE, int NB>
@@ -668,12 +673,13 @@ int sw_launch_attn(hipStream_t st, const SwKv &c, const SwRows &r, const float *
     if (c.dh < 32 || c.dh > 256 || c.dh % 32) return -1;
     const int B = at_blocks(c, r, Hq, window, S);
     const int64_t grid = (int64_t)B * c.Hkv * ((Hq / c.Hkv + 15) / 16);
-    if ((int64_t)S * Hq >= (int64_t)1 << 31 || (B > 1 && !part)) return -1;
+    if ((int64_t)S * Hq >= (int64_t)1 << 31 || grid >= (int64_t)1 << 31 || (B > 1 && S <= AT_COUNT && !part))
+        return -1;
     const float sc = (float)((double)scale * 1.4426950408889634074);   // the softmax in powers of two
     if (c.type == SW_KV_F32) at_dispatch<SW_KV_F32>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B);
     else if (c.type == SW_KV_BF16) at_dispatch<SW_KV_BF16>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B);
     else at_dispatch<SW_KV_F16>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B);
-    if (B > AT_FUSE)
+    if (B > AT_FUSE && S <= AT_COUNT)
         SW_LAUNCH(k_attn_join, dim3((unsigned)(S * Hq)), dim3(AT_NT), 0, st, c, r, S, Hq, window, at_chunk(c.type, c.dh), part, B, out);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }

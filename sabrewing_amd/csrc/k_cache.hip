@@ -136,9 +136,8 @@ __global__ __launch_bounds__(RP_NT) void k_qk_rope(SwKv c, SwRows r, SwRope rope
     }
     const int page = sw_page(c, r, r.seq ? r.seq[s] : s, pos);
     if (tid < rope.np) rp_angle(rope.freq[tid], pos, rope.factor, s_cs[tid], s_sn[tid]);
-    else if (tid < 128) { s_cs[tid] = 1.f; s_sn[tid] = 0.f; }
     __syncthreads();
-    const sw_f32x4 cs = *(const sw_f32x4 *)(s_cs + 4 * u), sn = *(const sw_f32x4 *)(s_sn + 4 * u);
+    const sw_f32x4 cs = *(const sw_f32x4 *)(s_cs + 4 * u), sn = *(const sw_f32x4 *)(s_sn + 4 * u);     // (used below np alone)
     const int64_t cell = (int64_t)page * c.ps + (int64_t)(pos & ((1 << c.psh) - 1)) * c.ts;
 #pragma unroll
     for (int j = 0; j < PB; j++) {
@@ -172,10 +171,14 @@ __global__ __launch_bounds__(RP_NT) void k_qk_rope(SwKv c, SwRows r, SwRope rope
 #pragma unroll
                 for (int e = 0; e < 4; e += 2) {
                     const float p = a[e], q = a[e + 1], y = b[e], z = b[e + 1];
-                    a[e] = __builtin_fmaf(p, cs[e / 2], -(q * sn[e / 2]));
-                    a[e + 1] = __builtin_fmaf(q, cs[e / 2], p * sn[e / 2]);
-                    b[e] = __builtin_fmaf(y, cs[2 + e / 2], -(z * sn[2 + e / 2]));
-                    b[e + 1] = __builtin_fmaf(z, cs[2 + e / 2], y * sn[2 + e / 2]);
+                    if (4 * u + e / 2 < rope.np) {
+                        a[e] = __builtin_fmaf(p, cs[e / 2], -(q * sn[e / 2]));
+                        a[e + 1] = __builtin_fmaf(q, cs[e / 2], p * sn[e / 2]);
+                    }
+                    if (4 * u + 2 + e / 2 < rope.np) {
+                        b[e] = __builtin_fmaf(y, cs[2 + e / 2], -(z * sn[2 + e / 2]));
+                        b[e + 1] = __builtin_fmaf(z, cs[2 + e / 2], y * sn[2 + e / 2]);
+                    }
                 }
             }
         }

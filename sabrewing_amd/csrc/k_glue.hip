@@ -114,7 +114,7 @@ __global__ __launch_bounds__(256) void k_add(float *__restrict__ x, const float 
 int sw_launch_add(hipStream_t st, float *x, const float *t, size_t n) {
     const int by4 = ((uintptr_t)x | (uintptr_t)t) % 16 == 0;
     const size_t m = by4 ? (n + 3) / 4 : n;
-    if (m > ((size_t)1 << 31) * 128) return -1;
+    if (m >= (size_t)1 << 32) return -1;               // (threads of a launch)
     SW_LAUNCH(k_add, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, st, x, t, n, by4);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }

@@ -181,6 +181,34 @@ def test_rows_of_zeros_and_large_values(be):
     c.free()
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dims", [2, 6, 10, 16, 50])
+def test_values_behind_the_turned_part(be, dims, interleaved):
+    """they pass through bit for bit, whatever stands beside them: infinities, NaN, zeros of either sign"""
+    S, Hq, Hkv, dh, P = 3, 2, 1, 64, 8
+    rng = np.random.default_rng(dims)
+    qkv = rng.standard_normal((S, (Hq + 2 * Hkv) * dh)).astype(np.float32)
+    x = qkv.reshape(S, Hq + 2 * Hkv, dh)
+    x[:, :, dims] = [[np.inf], [-0.0], [np.nan]]
+    x[:, :, dims + 3] = -0.0
+    c = Cache(be, "f32", S, P, Hkv, dh, *[np.zeros((S, Hkv, P, dh), np.float32)] * 2)
+    f = freqs(dims)
+    bufs = [be.upload(a) for a in (qkv, np.zeros(S * Hq * dh, np.float32), np.full(S, 5, np.int32),
+                                   np.arange(S, dtype=np.int32)[:, None].copy(), f)]
+    rows = be.kv_rows(bufs[2], bufs[3], S, 1)
+    be.qk_rope_append(c.c, rows, be.rope(bufs[4], dims, interleaved), bufs[0], qkv.shape[1], None, None, 1e-6, Hq, bufs[1], S)
+    q = be.d2h(bufs[1], (S, Hq, dh), np.float32)
+    k, v = c.read()
+    for b in bufs:
+        b.free()
+    c.free()
+    bits = lambda a: np.ascontiguousarray(a).view(np.uint32)
+    assert np.array_equal(bits(q[..., dims:]), bits(x[:, :Hq, dims:]))
+    assert np.array_equal(bits(k[np.arange(S), 0, 5, dims:]), bits(x[:, Hq, dims:]))
+    assert np.array_equal(bits(v[np.arange(S), 0, 5]), bits(x[:, Hq + 1]))
+    assert np.all(np.isfinite(q[..., :dims])) and np.all(np.isfinite(k[np.arange(S), 0, 5, :dims]))
+
+
 # ------------------------------------------------------------- page copies ----
 
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])

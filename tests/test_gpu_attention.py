@@ -120,6 +120,17 @@ def test_many_rows(be):
     one(be, 2, "bf16", 4, 2, 64, 16, list(rng.integers(0, 300, 200)))
 
 
+@pytest.mark.parametrize("S", [63, 64, 65, 128, 129, 255, 256, 257, 700])
+@pytest.mark.parametrize("most,Hq,Hkv", [(40, 4, 2), (700, 2, 1)])
+def test_row_counts(be, S, most, Hq, Hkv):
+    """rows of any number, long ones and free places among them: the positions are counted in rounds of 64 rows, and
+    beyond 256 rows not at all"""
+    rng = np.random.default_rng(S)
+    lens = rng.integers(0, most, S)
+    lens[rng.integers(0, S, 3)] = [0, 3000, 1]
+    one(be, S, "bf16", Hq, Hkv, 32, 16, [int(n) for n in lens])
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 def test_a_chunk_of_one_sequence(be, kind):
     """rows of the same sequences in any order: each sees the cells up to its own position"""
