@@ -18,7 +18,7 @@
 //     done on the list (as is min-p alone, where few weights reach it);
 //   else a histogram over the distance to the largest logit, of counts for top-k, then of
 //     weights for top-p; the tokens of the bin in which the beginning ends are listed and ranked;
-//   the kept weights of each tile, then of the one tile in which the sum passes.
+//   the kept weights of each group of tiles, then tile by tile of the group in which the sum passes.
 // Weights are what costs in the passes over all of a large row (some 20 64-bit operations each).
 #include "sw_attn.h"
 #include "sw_gate.h"
@@ -34,7 +34,7 @@
 #define SP_STEPS 512
 #define SP_GROUPS_OF_TILES 16
 #define SP_ONE 4398046511104.0            // 2^42
-#define SP_FAR 43.1f                      // log2 of the largest weight over one that rounds to 0
+#define SP_FAR 43.1                       // log2 of the largest weight over one that rounds to 0
 #define SP_SCALE 47.0f                    // bins per halving (47 x 43.1 < SP_BINS)
 
 typedef unsigned long long u64;
@@ -110,7 +110,9 @@ __device__ __forceinline__ void sp_each(const SpShared &sh, const SpRow &r, F f)
 __device__ __forceinline__ u64 sp_code(float f, int i) { return ((u64)ord_f32(f + 0.0f) << 32) | (0xFFFFFFFFu - (uint32_t)i); }
 __device__ __forceinline__ float sp_unkey(uint32_t o) { return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7FFFFFFFu : ~o); }
 // log2(largest weight / weight) in bins: below SP_BINS for what is kept
-__device__ __forceinline__ float sp_dist(float f, const SpRow &r) { return f == r.fmax ? 0.f : (r.fmax - f) * r.c32; }
+__device__ __forceinline__ float sp_dist(float f, const SpRow &r) {
+    return f == r.fmax ? 0.f : fminf(r.fmax - f, 3.402823466e38f) * r.c32;           // (of finite ones the difference may not be)
+}
 __device__ __forceinline__ bool sp_kept(float f, int i, const SpRow &r) { return (f > r.lf) | ((f == r.lf) & (i <= r.li)); }
 // 2^42 2^((f - max) c) to the nearest whole number: 512 steps of a halving from a table, the rest
 // (at most 2^-10 of one) by the exponential's series to the third power, 9e-15 off.  For what is kept;
@@ -425,12 +427,18 @@ __global__ __launch_bounds__(SP_NT) void k_sample(const float *__restrict__ logi
     }
     r.m64 = (double)fminf(r.fmax, 3.402823466e38f);
     r.c64 = SP_STEPS * 1.4426950408889634074 / (double)temp;
-    r.c32 = (float)(SP_SCALE * 1.4426950408889634074 / (double)temp);
-    // what rounds to no weight is not kept (a little lower: the weights decide)
+    r.c32 = fminf((float)(SP_SCALE * 1.4426950408889634074 / (double)temp), 3.402823466e38f);
+    // what rounds to no weight is not kept: logits more than SP_FAR halvings below the largest.  In 64 bits, and no
+    // lower than that: at temperatures near 0 a neighbour of the largest can be 1000 halvings away
     {
-        const float lo = r.fmax - SP_FAR * SP_SCALE / r.c32;
-        r.lf = r.fmax == INFINITY ? 3.402823466e38f : lo - 1e-6f * fabsf(lo);
-        r.li = 0x7FFFFFFF;
+        const double far = r.m64 - SP_FAR * 0.69314718055994530942 * (double)temp;
+        float lo = (float)far;                                        // (the float below it, and below the largest logit)
+        if ((double)lo > far || lo >= r.fmax) {
+            const int b = __builtin_bit_cast(int, lo);
+            lo = __builtin_bit_cast(float, lo > 0.f ? b - 1 : lo < 0.f ? b + 1 : (int)0x80000001);
+        }
+        r.lf = r.fmax == INFINITY ? 3.402823466e38f : lo;
+        r.li = -1;
     }
     const u64 least_w = min_p > 0.f ? (u64)ceil(fmin((double)min_p, 1.0) * SP_ONE) : 0;
 

@@ -132,6 +132,7 @@ def exact_pick(l, u, temp=1.0, top_k=0, top_p=1.0, min_p=0.0):
         order = order[:top_k]
     with np.errstate(invalid="ignore"):
         w = np.where(x[order] == top, 1.0, np.exp((x[order] - top) / np.float64(np.float32(temp))))
+    w[x[order] == -np.inf] = 0.0                       # (at an infinite temperature the quotient is none)
     if top_p < 1:
         want = float(np.float32(top_p)) * w.sum()
         before = np.concatenate([[0.0], np.cumsum(w)[:-1]])

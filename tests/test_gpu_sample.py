@@ -109,6 +109,26 @@ def test_masked_and_special_logits(be):
         both(be, x, u, **kw)
 
 
+@pytest.mark.parametrize("temp", [1e-45, 1e-38, 1e-20, 1e-9, 1e-8, 1e-7, 3e-6, 1e36, 1e38, np.inf])
+def test_extreme_temperatures(be, temp):
+    """neighbours of the largest logit, a few units of the last place below it, at temperatures at which they weigh
+    anything from nothing to nearly as much; differences beyond the largest float at temperatures of its size"""
+    rng = np.random.default_rng(8)
+    V, tops = 2000, (0.0, 5.0, -3.0, 100.0, 1e-30, 1e-40, 2e38, -2e38)
+    x = np.zeros((len(tops), V), np.float32)
+    for row, top in zip(x, tops):
+        row[:] = np.float32(top) - np.float32(abs(top) * 0.5 + 1e-3) * (1 + rng.random(V, dtype=np.float32))
+        at, f = rng.permutation(V)[:60], np.float32(top)
+        for i, j in enumerate(at):
+            row[j] = f
+            if i % 3 == 2:
+                f = np.nextafter(f, np.float32(-np.inf))
+    x[6, ::2] = -3e38
+    u = rng.random(len(x), dtype=np.float32)
+    for kw in (dict(), dict(top_k=20), dict(top_k=700), dict(top_p=0.6), dict(min_p=0.3), dict(top_k=900, top_p=0.7, min_p=0.01)):
+        both(be, x, u, temp=temp, **kw)
+
+
 def test_ends_of_the_random_numbers(be):
     rng = np.random.default_rng(5)
     x = rng.standard_normal((6, 3000)).astype(np.float32)
