@@ -141,9 +141,9 @@ class PagedCache:
     # ---- a step ----
     def rows(self, batch):
         """The next tokens of a batch: entries are a sequence (one token), (sequence, n) (its next
-        n tokens, rows in order) or None (a free place).  Returns (rows descriptor, number of rows);
-        appending through them is the caller's next calls, for every layer.  CacheFull leaves
-        everything as it was."""
+        n tokens, rows in order), None or (None, n) (free places).  Returns (rows descriptor, number
+        of rows); appending through them is the caller's next calls, for every layer.  CacheFull
+        leaves everything as it was."""
         batch = [(e, 1) if e is None or np.isscalar(e) else tuple(e) for e in batch]
         named = [s for s, _ in batch if s is not None]
         total = sum(n for _, n in batch)
@@ -172,8 +172,8 @@ class PagedCache:
         src, dst, at = [], [], 0
         for s, n in batch:
             if s is None:
-                self._rows[:, at] = -1
-                at += 1
+                self._rows[:, at:at + n] = -1
+                at += n
                 continue
             pages, ln = self._pages[s], self._len[s]
             if ln % P and self._users[pages[-1]] > 1:

@@ -168,6 +168,16 @@ def test_a_fork_copies_one_page():
     assert c.compact() == 1 and contents(be, c, b) == [0, 1, 11]
 
 
+def test_free_places():
+    be = FakeBackend()
+    c = PagedCache(be, 1, 4, 8, 1, 32, max_seqs=3, max_rows=9)
+    a, b = c.open(), c.open()
+    desc, S = c.rows([(None, 2), (a, 3), None, b])
+    assert S == 7
+    assert list(be.read(desc.pos, 9)) == [-1, -1, 0, 1, 2, -1, 0, -1, -1]
+    assert list(be.read(desc.seq, 9)) == [-1, -1, a, a, a, -1, b, -1, -1]
+
+
 def test_refusals():
     be = FakeBackend()
     c = PagedCache(be, 1, 4, 8, 1, 32, max_seqs=2, max_len=16, max_rows=20)
