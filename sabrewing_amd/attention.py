@@ -142,8 +142,8 @@ class PagedCache:
     def rows(self, batch):
         """The next tokens of a batch: entries are a sequence (one token), (sequence, n) (its next
         n tokens, rows in order), None or (None, n) (free places).  Returns (rows descriptor, number
-        of rows); appending through them is the caller's next calls, for every layer.  CacheFull
-        leaves everything as it was."""
+        of rows); appending through them is the caller's next calls, for every layer.  CacheFull,
+        or a copy that fails, leaves everything as it was."""
         batch = [(e, 1) if e is None or np.isscalar(e) else tuple(e) for e in batch]
         named = [s for s, _ in batch if s is not None]
         total = sum(n for _, n in batch)
@@ -169,18 +169,30 @@ class PagedCache:
             need += -(-(ln + n) // P) - len(pages)
         if need > len(self._free):
             raise CacheFull(f"{need} pages needed, {len(self._free)} free")
-        src, dst, at = [], [], 0
+        # the shared last pages are copied first: where that fails, nothing has changed
+        src, of = [], {}
+        for s, _ in batch:
+            if s is not None and self._len[s] % P and self._users[self._pages[s][-1]] > 1:
+                src.append(self._pages[s][-1])
+                of[s] = self._free.pop()
+                self._users[src[-1]] -= 1
+        if src:
+            try:
+                self.be.kv_copy_pages(self.layers, src, list(of.values()))
+            except Exception:
+                for p, q in zip(reversed(src), reversed(of.values())):
+                    self._users[p] += 1
+                    self._free.append(q)
+                raise
+        at = 0
         for s, n in batch:
             if s is None:
                 self._rows[:, at:at + n] = -1
                 at += n
                 continue
             pages, ln = self._pages[s], self._len[s]
-            if ln % P and self._users[pages[-1]] > 1:
-                p = self._free.pop()
-                src.append(pages[-1])
-                dst.append(p)
-                self._users[pages[-1]] -= 1
+            if s in of:
+                p = of[s]
                 self._users[p] = 1
                 pages[-1] = p
                 self._table[s, len(pages) - 1] = p
@@ -196,8 +208,6 @@ class PagedCache:
             self._len[s] = ln + n
             at += n
         self._rows[:, at:] = -1
-        if src:
-            self.be.kv_copy_pages(self.layers, src, dst)
         self._upload()
         self.be.h2d(self.dev_rows, self._rows)
         return self.desc, total

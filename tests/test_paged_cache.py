@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from sabrewing_amd.attention import AttnConfig, CacheFull, PagedCache, rope_frequencies
-from sabrewing_amd.backend import Backend
+from sabrewing_amd.backend import Backend, BackendError
 
 
 class Buf:
@@ -166,6 +166,31 @@ def test_a_fork_copies_one_page():
     c.close(a)
     c.close(d)
     assert c.compact() == 1 and contents(be, c, b) == [0, 1, 11]
+
+
+def test_a_failed_copy_changes_nothing():
+    be = FakeBackend()
+    c = PagedCache(be, 1, 8, 8, 1, 32, max_seqs=4, max_rows=9)
+    a = c.open()
+    desc, S = c.rows([(a, 2)])
+    append(be, desc, S, 8, [0, 1])
+    b, d = c.fork(a), c.fork(a)
+
+    def state():
+        return c._users.tolist(), list(c._free), list(c._len), [list(p) if p is not None else None for p in c._pages], c._table.tolist()
+    before = state()
+
+    def broken(*_):
+        raise BackendError("injected fault")
+    be.kv_copy_pages = broken
+    with pytest.raises(BackendError):
+        c.rows([a, (b, 7), d])
+    assert state() == before
+    del be.kv_copy_pages
+    desc, S = c.rows([a, (b, 7), d])
+    append(be, desc, S, 8, list(range(10, 19)))
+    invariants(c)
+    assert [contents(be, c, s) for s in (a, b, d)] == [[0, 1, 10], [0, 1] + list(range(11, 18)), [0, 1, 18]]
 
 
 def test_free_places():
