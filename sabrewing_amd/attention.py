@@ -309,6 +309,10 @@ class DeviceAttention:
     def forward(self, h, xn, S, cache_layer, rows, scratch):
         """h [S, D] += attention of its normalised rows (device; xn [S, D] scratch)"""
         be, a, D = self.be, self.acfg, self.D
+        if (cache_layer.n_heads, cache_layer.head_dim) != (a.n_kv, a.head_dim):
+            raise ValueError("DeviceAttention: a cache of other heads")
+        if S > scratch.S or scratch.shape != (a.n_q, a.n_kv, a.head_dim, D):
+            raise ValueError("DeviceAttention: scratch for fewer rows or other heads")
         be.rmsnorm(h, self.norm, xn, S, D, a.eps)
         be.head_argmax(self.wqkv, True, xn, S, D, a.qkv_rows, scratch.qkv)
         be.qk_rope_append(cache_layer, rows, self.rope.desc, scratch.qkv, a.qkv_rows, self.q_norm, self.k_norm, a.eps, a.n_q,
@@ -341,7 +345,7 @@ class AttnScratch:
     """what a layer's attention keeps between its calls, for up to S rows (the layers of a stack share it)"""
 
     def __init__(self, be, acfg, D, S):
-        self.S = S
+        self.S, self.shape = S, (acfg.n_q, acfg.n_kv, acfg.head_dim, D)
         heads = acfg.n_q * acfg.head_dim
         self.qkv, self.q, self.ctx, self.out = (be.alloc(4 * S * n) for n in (acfg.qkv_rows, heads, heads, D))
 

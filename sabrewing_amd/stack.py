@@ -30,12 +30,14 @@ class DeviceStack:
 
     def add_attention(self, acfg, layers=None, seed=0):
         """attention layers in front of the MoE ones: DeviceAttention's (sharing self.rope), or seeded
-        ones made on the device"""
+        ones made on the device; once per stack"""
+        if self.attn:
+            raise ValueError("add_attention: the stack has its attention layers")
+        if layers is not None and len(layers) != len(self.layers):
+            raise ValueError("add_attention: as many attention layers as MoE layers")
         self.rope = self.rope or Rope(self.be, acfg)
         self.attn = list(layers) if layers is not None else [
             DeviceAttention.generate(self.be, acfg, self.cfg.D, seed, l, self.rope) for l in range(len(self.layers))]
-        if len(self.attn) != len(self.layers):
-            raise ValueError("add_attention: as many attention layers as MoE layers")
         return self
 
     def reserve(self, S):
@@ -94,6 +96,8 @@ class DeviceStack:
         if self.attn:
             if cache is None or rows is None or cache.n_layers != len(self.attn):
                 raise ValueError("step: a stack with attention needs a cache of its layers, and rows")
+            if rows is cache.desc and S > cache.max_rows:
+                raise ValueError("step: more rows than the cache has places for")
             self.reserve(S)
         for l, dl in enumerate(self.layers):
             if self.attn:
