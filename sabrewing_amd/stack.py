@@ -26,7 +26,7 @@ class DeviceStack:
         self.be, self.cfg, self.V = be, cfg, V
         self.layers, self.norms, self.bufs = [], [], []
         self.final_norm = self.head = None
-        self.attn, self.rope, self.scratch = [], None, None
+        self.attn, self.rope, self.scratch, self.kept = [], None, None, []
 
     def add_attention(self, acfg, layers=None, seed=0):
         """attention layers in front of the MoE ones: DeviceAttention's (sharing self.rope), or seeded
@@ -41,10 +41,11 @@ class DeviceStack:
         return self
 
     def reserve(self, S):
-        """scratch for steps of up to S rows (a step grows it, which a recording cannot)"""
+        """scratch for steps of up to S rows (a step grows it, which a recording cannot); what it
+        replaces stays until free(): a recorded step may replay over it"""
         if self.attn and (self.scratch is None or self.scratch.S < S):
             if self.scratch:
-                self.scratch.free()
+                self.kept.append(self.scratch)
             self.scratch = AttnScratch(self.be, self.attn[0].acfg, self.cfg.D, S)
 
     @classmethod
@@ -115,10 +116,10 @@ class DeviceStack:
     def free(self):
         for dl in self.layers + self.attn:
             dl.free()
-        for b in (self.rope, self.scratch):
+        for b in [self.rope, self.scratch] + self.kept:
             if b:
                 b.free()
-        self.attn, self.rope, self.scratch = [], None, None
+        self.attn, self.rope, self.scratch, self.kept = [], None, None, []
         for b in self.bufs:
             b.free()
         self.layers, self.bufs = [], []

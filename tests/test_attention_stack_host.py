@@ -104,3 +104,18 @@ def test_attention_is_added_once():
     with pytest.raises(ValueError):
         st2.add_attention(A, st.attn)
     assert not st2.attn
+
+
+def test_scratch_outlives_its_growth():
+    """a recorded step of three rows goes on replaying over its scratch after a step of five"""
+    be = Recorder()
+    st = stack(be, [A])
+    cache = PagedCache(be, 1, 8, 8, 2, 32, max_seqs=8)
+    step(be, st, cache, cache.desc, 3)
+    old = st.scratch
+    step(be, st, cache, cache.desc, 5)
+    assert st.scratch is not old and not any(b.freed for b in (old.qkv, old.q, old.ctx, old.out))
+    step(be, st, cache, cache.desc, 2)
+    new = st.scratch
+    st.free()
+    assert all(b.freed for s in (old, new) for b in (s.qkv, s.q, s.ctx, s.out))
