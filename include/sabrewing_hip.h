@@ -246,8 +246,9 @@ typedef struct {
  * and k heads are normalised, x / sqrt(mean(x^2) + eps) * q_norm or k_norm ([head_dim], NULL:
  * not), and turned; q to q_out [S][n_q_heads][head_dim], k and v rounded to nearest into the
  * row's cell.  n_q_heads is a multiple of n_heads, ld of 4; qkv and q_out are 16-byte aligned
- * and do not overlap.  Rows without a place leave q_out and the cache as they were; two rows
- * of one cell are the caller's mistake (the cell holds values of both).  0 = ok */
+ * and do not overlap.  A free place leaves q_out and the cache as they were; a row whose
+ * position has no cell has its q in q_out and leaves the cache.  Two rows of one cell are the
+ * caller's mistake (the cell holds values of both).  0 = ok */
 int    lag_hip_qk_rope_append(const LagHipKvCache *c, const LagHipKvRows *r, const LagHipRope *rope, const float *qkv,
                               int64_t ld, const float *q_norm, const float *k_norm, float eps, int n_q_heads, float *q_out,
                               int S);
@@ -256,11 +257,12 @@ int    lag_hip_qk_rope_append(const LagHipKvCache *c, const LagHipKvRows *r, con
  * n_heads); q and out [S][n_q_heads][head_dim], 16-byte aligned, not overlapping.  Sums and
  * the softmax in 32 bits.  A free place, or a row without any cell, gives zeros.  Rows of one
  * sequence at consecutive positions (a chunk of a prompt, already appended) each see what is
- * theirs to see.  max_pages * page_size times S, or 64 if that is less, is below 2^36.  Infinities and NaN in a cell reach the rows that attend to it, as values
- * without meaning, and no others; cells that no row attends to may hold anything.  The
- * same call gives the same bits; how a row's cells are cut into parts, and with that its
- * last bits, depends on the batch's positions, S, n_q_heads, window and max_pages * page_size, not on what
- * the other rows' cells hold.  0 = ok */
+ * theirs to see.  max_pages * page_size times S, or 64 if that is less, is below 2^36.
+ * Infinities and NaN in a cell reach the rows that attend to it, as values without meaning,
+ * and no others; cells that no row attends to may hold anything.  The same call gives the same
+ * bits; how a row's cells are cut into parts, and with that its last bits, depends on the
+ * batch's positions, S, n_q_heads, window and max_pages * page_size, not on what the other
+ * rows' cells hold.  Its scratch is the arena's.  0 = ok */
 int    lag_hip_attn_paged(const LagHipKvCache *c, const LagHipKvRows *r, const float *q, int n_q_heads, float scale,
                           int window, float *out, int S);
 /* Page src[i] of every one of n_layers caches (one geometry and type) to page dst[i], k and v:
@@ -303,7 +305,8 @@ void   lag_hip_event_destroy(void *ev);
 
 /* ---------------- graphs ----------------
  * Record the device-pointer entries (lag_hip_moe_forward, lag_hip_route,
- * lag_hip_d2d) issued between begin and end into one graph, replayed with a
+ * lag_hip_d2d, the stack glue, attention, page copies and sampling) issued
+ * between begin and end into one graph, replayed with a
  * single submission by lag_hip_graph_launch (async on the backend stream).
  * Pointers and shapes are fixed at recording; scratch must already be large
  * enough (issue the same shapes once first), else the entry fails.  A

