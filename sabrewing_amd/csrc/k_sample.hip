@@ -15,16 +15,19 @@
 //   the largest logit, from the maxima of 256 groups of the row's tokens;
 //   a top-k of up to SP_MAXK: the k-th largest group maximum bounds the k-th largest logit from
 //     below and little more than k logits reach it; they are listed, and all the rest is
-//     done on the list (as is min-p alone, where few weights reach it);
+//     done on the list, a thread a token (as is min-p alone, where few weights reach it);
+//   one of up to SP_LIST: the threads' own maxima bound it, and where that leaves too many for the list,
+//     a histogram of counts says which bins hold the first k;
 //   else a histogram over the distance to the largest logit, of counts for top-k, then of
 //     weights for top-p; the tokens of the bin in which the beginning ends are listed and ranked;
 //   the kept weights of each group of tiles, then tile by tile of the group in which the sum passes.
 // Weights are what costs in the passes over all of a large row (some 20 64-bit operations each).
 //
-// Measured: one row of 32,000 logits, top-k 50, 11.5 us; 200 rows of 131,072 of all settings 112 us (0.94 TB/s),
-// which is what one row of top-p alone takes: 45 us the histogram of weights (47 cycles of an LDS
-// atomic for a wave), 29 us the groups' sums (64-bit operations), the rest the row's reading three times.  A
-// row of a batch has a CU to itself, so up to 256 rows take no longer than one.
+// Measured: one row of 32,000 logits, top-k 50, 11.5 us; of 128,000: greedy 7, top-k 50 19, top-k 500 39, top-k
+// 1000 62, top-p alone 93, no limit 41.  200 rows of 131,072 of all settings 108 us (0.97 TB/s), which is what one
+// row of top-p takes: 45 us the histogram of weights (47 cycles of an LDS atomic for a wave), 29 us the
+// groups' sums (64-bit operations), the rest the row's reading three times.  A row of a batch has a CU to
+// itself, so up to 256 rows take no longer than one.
 #include "sw_attn.h"
 #include "sw_gate.h"
 
@@ -33,9 +36,10 @@
 #define SP_TILE (4 * SP_NT)
 #define SP_CACHE 8                        // tiles in LDS: 128 KB
 #define SP_BINS 2048
-#define SP_LIST 512
+#define SP_LIST 1024                      // a thread each
 #define SP_GROUPS 256
-#define SP_MAXK 192                       // (at random, 355 tokens reach the 192nd of 256 maxima)
+#define SP_MAXK 192                       // (at random, 355 tokens reach the 192nd of 256 maxima,
+#define SP_MAXK2 600                      // 900 the 600th of the threads' 1024)
 #define SP_STEPS 512
 #define SP_GROUPS_OF_TILES 16
 #define SP_ONE 4398046511104.0            // 2^42
@@ -63,11 +67,10 @@ __constant__ double SP_POW2F[16] = {
     0x1.02c9a3e778061p+0, 0x1.032363d42b027p+0, 0x1.037d42e11bbccp+0, 0x1.03d7411915a8ap+0,
     0x1.04315e86e7f85p+0, 0x1.048b9b35659d8p+0, 0x1.04e5f72f654b1p+0, 0x1.0540727fc1762p+0,
 };
-struct SpItem { u64 code, weight; };
 struct SpShared {
     sw_f32x4 tile[SP_CACHE * SP_NT];
-    u64 hist[SP_BINS];                    // (also the tiles' sums by wave)
-    SpItem item[SP_LIST];
+    u64 hist[SP_BINS];                    // (also the weights beside a short list, the tiles' sums by wave)
+    u64 item[SP_LIST];
     float group[SP_GROUPS];
     u64 part[SP_NW], found, before;
     double pow2[SP_STEPS];                // 2^(42 + j / SP_STEPS)
@@ -114,7 +117,7 @@ __device__ __forceinline__ void sp_each(const SpShared &sh, const SpRow &r, F f)
 
 __device__ __forceinline__ u64 sp_code(float f, int i) { return ((u64)ord_f32(f + 0.0f) << 32) | (0xFFFFFFFFu - (uint32_t)i); }
 __device__ __forceinline__ float sp_unkey(uint32_t o) { return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7FFFFFFFu : ~o); }
-// log2(largest weight / weight) in bins: below SP_BINS for what is kept
+// log2(largest weight / weight) in bins
 __device__ __forceinline__ float sp_dist(float f, const SpRow &r) {
     return f == r.fmax ? 0.f : fminf(r.fmax - f, 3.402823466e38f) * r.c32;           // (of finite ones the difference may not be)
 }
@@ -252,7 +255,7 @@ __device__ __forceinline__ void sp_list(SpShared &sh, const bool (&on)[4], const
         if ((int)(threadIdx.x & 63) == __builtin_ctzll(b)) at = atomicAdd(&sh.n, (int)__popcll(b));
         at = __builtin_amdgcn_readlane(at, __builtin_ctzll(b)) +
              (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
-        if (on[e] && at < SP_LIST) sh.item[at].code = sp_code(x[e], i + e);
+        if (on[e] && at < SP_LIST) sh.item[at] = sp_code(x[e], i + e);
     }
 }
 __device__ __forceinline__ u64 sp_share(double part, u64 total, u64 least) {      // ceil(part * total), at least `least`
@@ -265,13 +268,40 @@ __device__ __forceinline__ u64 sp_target(float u, u64 total) {                  
     return t < total ? t : total - 1;
 }
 
+// Of the threads with `on`, in order of rising bin and in a bin of falling code: the code at which the sum of
+// w reaches limit (0: nowhere).  A histogram finds the bin, its few are ranked.
+__device__ __forceinline__ u64 sp_border(SpShared &sh, bool on, int bin, u64 code, u64 w, u64 limit) {
+    sp_clear(sh);                                                     // (the list is read)
+    if (on) atomicAdd(&sh.hist[bin], w);
+    u64 left, at;
+    const int b = sp_find(sh, [&](u64) { return limit; }, left, at);
+    if (b < 0) return 0;
+    on = on && bin == b;
+    if (threadIdx.x == 0) { sh.n = 0; sh.found = 0; }
+    __syncthreads();
+    if (on) {
+        const int i = atomicAdd(&sh.n, 1);
+        sh.item[i] = code;
+        sh.hist[i] = w;
+    }
+    __syncthreads();
+    if (on) {
+        const int n = sh.n;
+#pragma unroll 4
+        for (int j = 0; j < n; j++) at += sh.item[j] > code ? sh.hist[j] : 0;
+        if (at < limit && at + w >= limit) sh.found = code;
+    }
+    __syncthreads();
+    return sh.found;
+}
+
 // The code at which the beginning ends, among the kept: after `limit` tokens, or (mass) with the token
 // at which the weights' sum reaches `limit`; `before`: what counts of the bins before `bin`.  The bin's
 // tokens are narrowed by bits of the code until the list takes them.
 __device__ __forceinline__ u64 sp_cut(SpShared &sh, const SpRow &r, int bin, u64 limit, u64 before, bool mass) {
     u64 prefix = 0, mask = 0;
     int shift = 64;
-    const float lo = (float)bin, hi = (float)(bin + 1);
+    const float lo = (float)bin, hi = bin == SP_BINS - 1 ? NAN : (float)(bin + 1);     // (the last bin has no end)
     for (bool list = true;;) {
         if (!list) sp_clear(sh);
         __syncthreads();
@@ -282,7 +312,7 @@ __device__ __forceinline__ u64 sp_cut(SpShared &sh, const SpRow &r, int bin, u64
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const float d = sp_dist(x[e], r);
-                on[e] = (d >= lo) & (d < hi);
+                on[e] = (d >= lo) & !(d >= hi);
                 any |= on[e];
             }
             if (!__any(any)) return;
@@ -315,44 +345,16 @@ __device__ __forceinline__ u64 sp_cut(SpShared &sh, const SpRow &r, int bin, u64
         }
         list = !list;
     }
-    const int t = threadIdx.x;
-    int n = sh.n;
-    u64 c = 0, w = 0;
-    if (t < n) {
-        c = sh.item[t].code;
-        w = mass ? sp_weight(sp_unkey((uint32_t)(c >> 32)), r, sh) : 1;
+    u64 c = 0, w = 0;                                                 // 2048 parts of the bin
+    int part = 0;
+    const bool on = (int)threadIdx.x < sh.n;
+    if (on) {
+        c = sh.item[threadIdx.x];
+        const float f = sp_unkey((uint32_t)(c >> 32));
+        w = mass ? sp_weight(f, r, sh) : 1;
+        part = min((int)((sp_dist(f, r) - lo) * SP_BINS), SP_BINS - 1);
     }
-    if (n > 64) {                                                     // 2048 parts of the bin, and the list of one
-        const int part = min((int)((sp_dist(sp_unkey((uint32_t)(c >> 32)), r) - lo) * SP_BINS), SP_BINS - 1);
-        sp_clear(sh);
-        if (t < n) atomicAdd(&sh.hist[part], w);
-        u64 left, more;
-        const int b = sp_find(sh, [&](u64) { return limit - before; }, left, more);
-        before += more;
-        if (t == 0) sh.n = 0;
-        __syncthreads();
-        const bool on = t < n && part == b;
-        int at = 0;
-        if (on) at = atomicAdd(&sh.n, 1);
-        __syncthreads();
-        if (on) sh.item[at].code = c;
-        n = sh.n;
-        __syncthreads();
-        if (t < n) {
-            c = sh.item[t].code;
-            w = mass ? sp_weight(sp_unkey((uint32_t)(c >> 32)), r, sh) : 1;
-        }
-    }
-    if (t < n) sh.item[t].weight = w;
-    __syncthreads();
-    if (t < n) {
-        u64 at = before;
-#pragma unroll 4
-        for (int j = 0; j < n; j++) at += sh.item[j].code > c ? sh.item[j].weight : 0;
-        if (at < limit && at + w >= limit) sh.found = c;
-    }
-    __syncthreads();
-    return sh.found;
+    return sp_border(sh, on, part, c, w, limit - before);
 }
 
 __global__ __launch_bounds__(SP_NT) void k_sample(const float *__restrict__ logits, int V, SwSample p, const float *__restrict__ u,
@@ -398,7 +400,10 @@ __global__ __launch_bounds__(SP_NT) void k_sample(const float *__restrict__ logi
         const sw_f32x4 g = ((const sw_f32x4 *)sh.group)[lane];
         const float top = sp_wave_max(fmaxf(fmaxf(g[0], g[1]), fmaxf(g[2], g[3])));
         float bound = -INFINITY;
-        if (few && by_k && top < INFINITY) {
+        int some = 0;                                                 // groups that hold anything
+#pragma unroll
+        for (int e = 0; e < 4; e++) some += (int)__popcll(__ballot(g[e] > -INFINITY));
+        if (few && by_k && top < INFINITY && some >= k) {
             // the k-th largest of the groups, or a little less: halving the range between a bound that k
             // groups reach and one that fewer do
             float least = fminf(fminf(g[0], g[1]), fminf(g[2], g[3]));
@@ -448,10 +453,11 @@ __global__ __launch_bounds__(SP_NT) void k_sample(const float *__restrict__ logi
     const u64 least_w = min_p > 0.f ? (u64)ceil(fmin((double)min_p, 1.0) * SP_ONE) : 0;
 
     // ---- few tokens can be kept: list them and stay there
+    int listed = -1;                                                  // tokens of the list, where it holds all that can be kept
     if (few) {
         float bound = sh.bound;                                       // the list's tokens reach it
         if (!by_p && min_p > 0.f) {                                   // (a little lower: the weights decide)
-            const float lo = r.fmax - (0.05f - log2f(fminf(min_p, 1.f))) * SP_SCALE / r.c32;
+            const float lo = r.fmax - (0.05f - log2f(fminf(min_p, 1.f))) * 0.6931472f * temp;
             bound = fmaxf(bound, lo - 1e-6f * fabsf(lo));
         }
         sp_each(sh, r, [&](const sw_f32x4 &x, int i, int) {
@@ -468,7 +474,7 @@ __global__ __launch_bounds__(SP_NT) void k_sample(const float *__restrict__ logi
             u64 code = 0, w = 0, at = 0;
             int rank = 0;
             if (lane < n) {
-                code = sh.item[lane].code;
+                code = sh.item[lane];
                 w = sp_weight(sp_unkey((uint32_t)(code >> 32)), r, sh);
             }
             for (int j0 = 0; j0 < n; j0 += 8)                         // (lanes behind the list hold 0)
@@ -498,61 +504,129 @@ __global__ __launch_bounds__(SP_NT) void k_sample(const float *__restrict__ logi
             if (w && sum > target && sum - w <= target) tok[s] = (int)(0xFFFFFFFFu - (uint32_t)code);
             return;
         }
-        if (n <= SP_LIST) {
-            u64 code = 0, w = 0, at = 0;
-            int rank = 0;
-            if (tid < n) {
-                code = sh.item[tid].code;
-                w = sp_weight(sp_unkey((uint32_t)(code >> 32)), r, sh);
-                sh.item[tid].weight = w;
+        if (n <= SP_LIST) listed = n;
+    }
+    if (listed < 0) {
+        // bins as fine as the range of the row's first tiles allows (what lies below is in the last one)
+        {
+            float m = INFINITY;
+            for (int t = 0; t < min(r.ntile, SP_CACHE); t++) {
+                const sw_f32x4 x = sh.tile[t * SP_NT + tid];
+                m = fminf(fminf(fminf(m, x[0]), fminf(x[1], x[2])), x[3]);
             }
+            m = -sp_wave_max(-m);
             __syncthreads();
-            if (tid < n) {
-#pragma unroll 4
-                for (int j = 0; j < n; j++) {
-                    const SpItem o = sh.item[j];
-                    rank += o.code > code;
-                    at += o.code > code ? o.weight : 0;
+            if (lane == 0) sh.group[wave] = m;
+            __syncthreads();
+            float lo = sh.group[0];
+#pragma unroll
+            for (int q = 1; q < SP_NW; q++) lo = fminf(lo, sh.group[q]);
+            r.c32 = fminf(fmaxf(r.c32, (SP_BINS - 1) / (r.fmax - fmaxf(lo, r.lf))), 3.402823466e38f);
+        }
+        if (k) {
+            // the k-th largest of the threads' maxima bounds the k-th largest token from below: all above `bound` (the
+            // end of a bin, or a little lower) are looked at
+            float bound = -INFINITY;
+            auto end_of = [&](int b) {
+                const float x = r.fmax - (float)(b + 1) / r.c32;
+                return b < SP_BINS - 1 && r.fmax < INFINITY ? x - 1e-6f * (fabsf(x) + fabsf(r.fmax)) : -INFINITY;
+            };
+            u64 limit, before;
+            if (k <= SP_LIST) {
+                sp_clear(sh);
+                if (best > r.lf) atomicAdd(&sh.hist[min((int)sp_dist(best, r), SP_BINS - 1)], 1ull);
+                const int b = sp_find(sh, [&](u64) { return (u64)k; }, limit, before);
+                if (b >= 0) bound = end_of(b);
+            }
+            // a list of these, if they are few enough; else they are counted by bin, and the k-th token's bin is the
+            // last of the list, or its tokens are ranked
+            for (bool count = k > SP_MAXK2, again = false;; again = count, count = true) {
+                if (count) {
+                    sp_clear(sh);
+                    sp_each(sh, r, [&](const sw_f32x4 &x, int i, int) {
+                        if (__all(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) < bound)) return;
+                        bool on[4];
+                        int d[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            d[e] = min((int)sp_dist(x[e], r), SP_BINS - 1);
+                            on[e] = (x[e] > r.lf) & (x[e] >= bound);
+                        }
+                        const u64 one[4] = {1, 1, 1, 1};
+                        sp_add(sh, on, d, one);
+                    });
+                    const int b = sp_find(sh, [&](u64) { return (u64)k; }, limit, before);
+                    if (b >= 0 && !again && before + sh.hist[b] <= SP_LIST - 8) {
+                        bound = fmaxf(bound, end_of(b));
+                    } else if (b >= 0) {
+                        const u64 c = sp_cut(sh, r, b, limit, before, false);
+                        r.lf = sp_unkey((uint32_t)(c >> 32));
+                        r.li = (int)(0xFFFFFFFFu - (uint32_t)c);
+                    }
+                    if (k > SP_LIST) break;
+                }
+                __syncthreads();
+                if (tid == 0) sh.n = 0;
+                __syncthreads();
+                sp_each(sh, r, [&](const sw_f32x4 &x, int i, int) {
+                    if (__all(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) < bound)) return;
+                    bool on[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) on[e] = sp_kept(x[e], i + e, r) & (x[e] >= bound);
+                    sp_list(sh, on, x, i);
+                });
+                __syncthreads();
+                if (sh.n <= SP_LIST) {
+                    listed = sh.n;
+                    break;
                 }
             }
-            if (k && rank >= k) w = 0;
-            if (by_p) {
-                const u64 total = sp_block_sum(sh, w);
-                if (at >= sp_share((double)top_p, total, 1)) w = 0;
-            }
-            if (w < least_w) w = 0;
-            const u64 target = sp_target(us, sp_block_sum(sh, w));
-            if (tid < n) sh.item[tid].weight = w;
-            __syncthreads();
-            if (w) {
-                u64 sum = 0;
-#pragma unroll 4
-                for (int j = 0; j < n; j++) sum += (uint32_t)sh.item[j].code >= (uint32_t)code ? sh.item[j].weight : 0;
-                if (sum > target && sum - w <= target) tok[s] = (int)(0xFFFFFFFFu - (uint32_t)code);
-            }
-            return;
         }
     }
+    if (listed >= 0) {
+        u64 code = 0, w = 0;
+        int d = 0;
+        if (tid < listed) {
+            code = sh.item[tid];
+            const float f = sp_unkey((uint32_t)(code >> 32));
+            w = sp_weight(f, r, sh);
+            d = min((int)sp_dist(f, r), SP_BINS - 1);
+        }
+        if (k && k < listed && code < sp_border(sh, tid < listed, d, code, 1, (u64)k)) w = 0;
+        if (by_p) {
+            const u64 limit = sp_share((double)top_p, sp_block_sum(sh, w), 1);
+            if (code < sp_border(sh, w != 0, d, code, w, limit)) w = 0;
+        }
+        if (w < least_w) w = 0;
+        // the pick: the same in order of index
+        const int bits = 32 - __builtin_clz(V), shift = bits > 11 ? bits - 11 : 0;
+        const u64 target = sp_target(us, sp_block_sum(sh, w));
+        const u64 c = sp_border(sh, w != 0, (int)((0xFFFFFFFFu - (uint32_t)code) >> shift) & (SP_BINS - 1), (uint32_t)code, w, target + 1);
+        if (tid == 0) tok[s] = (int)(0xFFFFFFFFu - (uint32_t)c);
+        return;
+    }
 
-    // ---- the least token that is kept: by counts, then by weights
-    for (int by = k ? 0 : 1; by < (by_p ? 2 : 1); by++) {
+    // ---- top-p: the least token that is kept, by weights
+    if (by_p) {
         sp_clear(sh);
         sp_each(sh, r, [&](const sw_f32x4 &x, int i, int) {
-            bool on[4];
+            bool on[4], any = false;
             int d[4];
-            u64 w[4] = {1, 1, 1, 1};
+            u64 w[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 on[e] = sp_kept(x[e], i + e, r);
                 d[e] = on[e] ? min((int)sp_dist(x[e], r), SP_BINS - 1) : 0;
+                any |= on[e];
             }
-            if (by) sp_weights(x, on, r, sh, w);
+            if (!__any(any)) return;
+            sp_weights(x, on, r, sh, w);
             sp_add(sh, on, d, w);
         });
         u64 limit, before;
-        const int b = sp_find(sh, [&](u64 total) { return by ? sp_share((double)top_p, total, 1) : (u64)k; }, limit, before);
+        const int b = sp_find(sh, [&](u64 total) { return sp_share((double)top_p, total, 1); }, limit, before);
         if (b >= 0) {
-            const u64 c = sp_cut(sh, r, b, limit, before, by);
+            const u64 c = sp_cut(sh, r, b, limit, before, true);
             r.lf = sp_unkey((uint32_t)(c >> 32));
             r.li = (int)(0xFFFFFFFFu - (uint32_t)c);
         }

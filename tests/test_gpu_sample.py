@@ -4,7 +4,7 @@
 import numpy as np
 import pytest
 
-from paged import exact_pick
+from paged import exact_pick, from_bits, to_type
 
 pytestmark = pytest.mark.gpu
 
@@ -107,6 +107,41 @@ def test_masked_and_special_logits(be):
     for kw in (dict(), dict(temp=0.7, top_k=50), dict(top_p=0.9), dict(min_p=0.1), dict(temp=0.0), dict(top_k=1, top_p=0.5, min_p=0.5),
                dict(temp=1e-30), dict(temp=1e30)):
         both(be, x, u, **kw)
+
+
+def shapes_of_rows(rng, S, V):
+    """rows of many kinds: smooth, rounded to 8 bits (many equal), flat but for a few, a beginning that is
+    narrower or wider than the rest, masked by -inf or the lowest value"""
+    x = np.empty((S, V), np.float32)
+    for i, row in enumerate(x):
+        row[:] = rng.choice([0.5, 2.5, 6.0]) * rng.standard_normal(V)
+        kind = i % 8
+        if kind == 1:
+            row[:] = from_bits(to_type(row, "bf16")[0])
+        elif kind == 2:
+            row[:] = np.round(row)
+        elif kind == 3:
+            row[:] = 0.25
+            row[rng.integers(0, V, 5)] += rng.standard_normal(5).astype(np.float32)
+        elif kind == 4:
+            row[:40000] = row.max() - 1e-3 * rng.random(row[:40000].size, dtype=np.float32)
+        elif kind == 5:
+            row[:40000] *= 3
+        elif kind == 6:
+            row[rng.random(V) < 0.9] = -np.inf
+        elif kind == 7:
+            row[rng.random(V) < 0.6] = np.finfo(np.float32).min
+    return x
+
+
+@pytest.mark.parametrize("top_k", [0, 30, 192, 193, 400, 600, 601, 1000, 1024, 1025, 3000])
+@pytest.mark.parametrize("V", [260, 700, 1200, 5000, 40001, 70003])
+def test_kinds_of_rows(be, V, top_k):
+    rng = np.random.default_rng(V + top_k)
+    S = 32
+    x, u = shapes_of_rows(rng, S, V), rng.random(S, dtype=np.float32)
+    for temp, top_p, min_p in ((1.0, 1.0, 0.0), (0.6, 0.93, 0.0), (1.7, 0.71, 0.03), (30.0, 0.52, 0.0)):
+        both(be, x, u, temp=temp, top_k=top_k, top_p=top_p, min_p=min_p)
 
 
 @pytest.mark.parametrize("temp", [1e-45, 1e-38, 1e-20, 1e-9, 1e-8, 1e-7, 3e-6, 1e36, 1e38, np.inf])
