@@ -34,8 +34,7 @@
 // Beyond so many rows they are dealt whole, a block each, without counting them: there are blocks enough
 // to even out, and each would count them all
 #define AT_COUNT 256
-// A row's parts are joined by the block that finishes last (one launch), with up to this many blocks
-// of a cache head; by k_attn_join, over more blocks, where there can be more parts than that
+// A row's parts, up to this many, are joined by the block that finishes last (one launch), else by k_attn_join
 #define AT_FUSE 64
 
 // bytes of a lane per row: 16-byte pieces first, then 8 and 4; the byte of row `rr` at dword w
@@ -127,6 +126,14 @@ __device__ __forceinline__ AtRow at_row(const SwKv &c, const SwRows &r, int pos,
     return w;
 }
 
+// The least chunks of a part: one a wave, and a part's chunks take a wave a third of a microsecond each, its outputs
+// the join some 30 KB a microsecond, so the longest row's (mx chunks) are no shorter than where the two
+// together are least.
+__host__ __device__ inline int at_least(int64_t mx, int G, int dh) {
+    const int best = (int)sqrtf((float)mx * (float)((G < 16 ? G : 16) * dh) / 2500.f);
+    return best < AT_MIN ? AT_MIN : best;
+}
+
 // How the rows' chunks are dealt to the B blocks of a cache head.  Laid end to end they are N, and
 // block b takes those from b q to (b + 1) q, whatever rows they fall in: parts of rows, joined
 // at the end, and the same work for each block however the lengths differ.  Or whole rows (b, b + B,
@@ -139,7 +146,7 @@ struct AtPlan {
     int pos, n;                                                        // lane i: row i's position and chunks (S <= 64)
     uint32_t upto;                                                     //         the chunks of rows up to it
 };
-__device__ __forceinline__ AtPlan at_plan(const SwKv &c, const SwRows &r, int S, int Hq, int window, int CT, int B) {
+__device__ __forceinline__ AtPlan at_plan(const SwKv &c, const SwRows &r, int S, int Hq, int window, int CT, int B, int fuse) {
     AtPlan p = {};
     if (S > AT_COUNT) { p.whole = true; return p; }
     const int lane = threadIdx.x & 63;
@@ -160,11 +167,9 @@ __device__ __forceinline__ AtPlan at_plan(const SwKv &c, const SwRows &r, int S,
         mx = m > mx ? m : mx;
     }
     p.q = (p.N + B - 1) / B;
-    // a part's chunks take a wave a third of a microsecond each, and its outputs the join some 30 KB a
-    // microsecond: the long row's parts are not made shorter than where the two together are least
-    const int best = at_uni((int)sqrtf((float)mx * (float)(min(Hq / c.Hkv, 16) * c.dh) / 2500.f));
-    if (p.q < AT_MIN) p.q = AT_MIN;
+    const int best = at_uni(at_least(mx, Hq / c.Hkv, c.dh));
     if (p.q < best) p.q = best;
+    if (fuse && B > AT_FUSE && p.q * (AT_FUSE - 2) < mx) p.q = (mx + AT_FUSE - 3) / (AT_FUSE - 2);      // (no row has more parts)
     p.whole = ((S + B - 1) / B) * (AT_ROW + mx) <= p.q + AT_ROW * (2 + S / B);
     return p;
 }
@@ -211,7 +216,7 @@ static __device__ int g_at_done[AT_BLOCKS];
 // it computes.
 template <int TYPE, int NB>
 __global__ __launch_bounds__(AT_NT, at_blocks_cu(TYPE, 32 * NB)) void k_attn(SwKv c, SwRows r, const float *__restrict__ q, int S, int Hq, float sc0,
-                                                                int window, float *__restrict__ out, float *__restrict__ part, int B) {
+                                                                int window, float *__restrict__ out, float *__restrict__ part, int B, int fuse) {
     constexpr bool F32 = TYPE == SW_KV_F32;
     constexpr int DH = 32 * NB, ES = F32 ? 4 : 2, RB = DH * ES, CT = at_chunk(TYPE, DH);
     constexpr int NT = CT / 16, NS = RB / 64, ND = RB / 64, NTOK = 4 * NT, NO = DH / 16;
@@ -225,7 +230,7 @@ __global__ __launch_bounds__(AT_NT, at_blocks_cu(TYPE, 32 * NB)) void k_attn(SwK
     const int G = Hq / c.Hkv, gt = (G + 15) >> 4, per_s = c.Hkv * gt;
     const int hg = blockIdx.x % per_s, b = blockIdx.x / per_s;
     const int hk = hg / gt, h0 = hk * G + (hg % gt) * 16, nh = min(16, G - (hg % gt) * 16);
-    const AtPlan plan = at_plan(c, r, S, Hq, window, CT, B);
+    const AtPlan plan = at_plan(c, r, S, Hq, window, CT, B, fuse);
     auto row_at = [&](int s) { return at_row(c, r, S <= 64 ? __builtin_amdgcn_readlane(plan.pos, s) : at_uni(at_pos(r, s)), window, CT); };
     for (int64_t s = b + (int64_t)B * tid; s < S; s += (int64_t)B * AT_NT)             // rows without any cell: zeros
         if (at_row(c, r, at_pos(r, (int)s), window, CT).n == 0)
@@ -492,7 +497,7 @@ __global__ __launch_bounds__(AT_NT, at_blocks_cu(TYPE, 32 * NB)) void k_attn(SwK
                 *(sw_f32x4 *)(out + ((int64_t)s * Hq + h0 + h) * DH + d) = a;
             }
         }
-        if (all || B > AT_FUSE) continue;
+        if (all || !fuse) continue;
         // ---- the last of the row's blocks joins its parts, in their order
         const int b0 = (int)(begin / plan.q), parts = (int)((before - 1) / plan.q) - b0 + 1;
         int *done = g_at_done + hg * B + b0;
@@ -584,7 +589,7 @@ __global__ __launch_bounds__(AT_NT) void k_attn_join(SwKv c, SwRows r, int S, in
     const int tid = threadIdx.x, s = blockIdx.x / Hq, h = blockIdx.x % Hq, nd = c.dh / 4, ng = AT_NT / nd;
     const int n = at_row(c, r, at_uni(at_pos(r, s)), window, CT).n;
     if (n == 0) return;
-    const AtPlan plan = at_plan(c, r, S, Hq, window, CT, B);
+    const AtPlan plan = at_plan(c, r, S, Hq, window, CT, B, 0);
     if (plan.whole) return;
     int64_t before = 0;                                                // the chunks of rows before it
     for (int i0 = 0; i0 < s; i0 += 64) {
@@ -641,13 +646,16 @@ __global__ __launch_bounds__(AT_NT) void k_attn_join(SwKv c, SwRows r, int S, in
     *(sw_f32x4 *)(out + (int64_t)blockIdx.x * c.dh + d) = a;
 }
 
+// cells of the longest row there can be
+static int64_t at_cells(const SwKv &c, const SwRows &r, int window) {
+    const int64_t cells = (int64_t)r.max_pages << c.psh, most = (int64_t)window + at_chunk(c.type, c.dh);
+    return window > 0 && most < cells ? most : cells;                  // (a window begins anywhere in a chunk)
+}
 // Blocks of a cache head: so many that all of them are AT_BLOCKS, no more than rows or least parts for them.
 static int at_blocks(const SwKv &c, const SwRows &r, int Hq, int window, int S) {
     if (S > AT_COUNT) return S;
     const int per_s = c.Hkv * ((Hq / c.Hkv + 15) / 16), CT = at_chunk(c.type, c.dh);
-    int64_t cells = (int64_t)r.max_pages << c.psh;
-    if (window > 0 && (int64_t)window + CT < cells) cells = (int64_t)window + CT;      // (a window begins anywhere in a chunk)
-    const int64_t most = (S * (cells / CT + 1) + AT_MIN - 1) / AT_MIN, n = AT_BLOCKS / per_s;
+    const int64_t most = (S * (at_cells(c, r, window) / CT + 1) + AT_MIN - 1) / AT_MIN, n = AT_BLOCKS / per_s;
     const int64_t use = S > most ? S : most;
     return (int)(n < 1 ? 1 : n < use ? n : use);
 }
@@ -658,21 +666,21 @@ int64_t sw_attn_part_floats(const SwKv &c, const SwRows &r, int Hq, int window, 
 
 template <int TYPE, int NB>
 static void at_launch(hipStream_t st, unsigned grid, const SwKv &c, const SwRows &r, const float *q, int S, int Hq, float sc, int window,
-                      float *out, float *part, int B) {
-    SW_LAUNCH((k_attn<TYPE, NB>), dim3(grid), dim3(AT_NT), 0, st, c, r, q, S, Hq, sc, window, out, part, B);
+                      float *out, float *part, int B, int fuse) {
+    SW_LAUNCH((k_attn<TYPE, NB>), dim3(grid), dim3(AT_NT), 0, st, c, r, q, S, Hq, sc, window, out, part, B, fuse);
 }
 template <int TYPE>
 static void at_dispatch(hipStream_t st, unsigned grid, const SwKv &c, const SwRows &r, const float *q, int S, int Hq, float sc,
-                        int window, float *out, float *part, int B) {
+                        int window, float *out, float *part, int B, int fuse) {
     switch (c.dh / 32) {
-    case 1: at_launch<TYPE, 1>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
-    case 2: at_launch<TYPE, 2>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
-    case 3: at_launch<TYPE, 3>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
-    case 4: at_launch<TYPE, 4>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
-    case 5: at_launch<TYPE, 5>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
-    case 6: at_launch<TYPE, 6>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
-    case 7: at_launch<TYPE, 7>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
-    default: at_launch<TYPE, 8>(st, grid, c, r, q, S, Hq, sc, window, out, part, B); break;
+    case 1: at_launch<TYPE, 1>(st, grid, c, r, q, S, Hq, sc, window, out, part, B, fuse); break;
+    case 2: at_launch<TYPE, 2>(st, grid, c, r, q, S, Hq, sc, window, out, part, B, fuse); break;
+    case 3: at_launch<TYPE, 3>(st, grid, c, r, q, S, Hq, sc, window, out, part, B, fuse); break;
+    case 4: at_launch<TYPE, 4>(st, grid, c, r, q, S, Hq, sc, window, out, part, B, fuse); break;
+    case 5: at_launch<TYPE, 5>(st, grid, c, r, q, S, Hq, sc, window, out, part, B, fuse); break;
+    case 6: at_launch<TYPE, 6>(st, grid, c, r, q, S, Hq, sc, window, out, part, B, fuse); break;
+    case 7: at_launch<TYPE, 7>(st, grid, c, r, q, S, Hq, sc, window, out, part, B, fuse); break;
+    default: at_launch<TYPE, 8>(st, grid, c, r, q, S, Hq, sc, window, out, part, B, fuse); break;
     }
 }
 
@@ -684,10 +692,16 @@ int sw_launch_attn(hipStream_t st, const SwKv &c, const SwRows &r, const float *
     if ((int64_t)S * Hq >= (int64_t)1 << 31 || grid >= (int64_t)1 << 31 || (B > 1 && S <= AT_COUNT && !part))
         return -1;
     const float sc = (float)((double)scale * 1.4426950408889634074);   // the softmax in powers of two
-    if (c.type == SW_KV_F32) at_dispatch<SW_KV_F32>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B);
-    else if (c.type == SW_KV_BF16) at_dispatch<SW_KV_BF16>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B);
-    else at_dispatch<SW_KV_F16>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B);
-    if (B > AT_FUSE && S <= AT_COUNT)
+    // over more blocks the join in the same launch pays where no row can have many parts: below 72 KB of them (112
+    // rows of one token, 3 cache heads of 96: 13.2 -> 8.5 us; 13 parts of 12 heads of 128, 80 KB: 19.2 -> 20.1)
+    const int G = Hq / c.Hkv, nh = G < 16 ? G : 16;
+    const int64_t mx = at_cells(c, r, window) / at_chunk(c.type, c.dh) + 1;              // chunks of the longest row there can be
+    const int64_t parts = mx / at_least(mx, G, c.dh) + 2;
+    const int fuse = B <= AT_FUSE || S > AT_COUNT || (parts <= AT_FUSE && parts * nh * c.dh <= 18432);
+    if (c.type == SW_KV_F32) at_dispatch<SW_KV_F32>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B, fuse);
+    else if (c.type == SW_KV_BF16) at_dispatch<SW_KV_BF16>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B, fuse);
+    else at_dispatch<SW_KV_F16>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B, fuse);
+    if (!fuse)
         SW_LAUNCH(k_attn_join, dim3((unsigned)(S * Hq)), dim3(AT_NT), 0, st, c, r, S, Hq, window, at_chunk(c.type, c.dh), part, B, out);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
