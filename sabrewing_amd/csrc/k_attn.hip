@@ -693,11 +693,12 @@ int sw_launch_attn(hipStream_t st, const SwKv &c, const SwRows &r, const float *
         return -1;
     const float sc = (float)((double)scale * 1.4426950408889634074);   // the softmax in powers of two
     // over more blocks the join in the same launch pays where no row can have many parts: below 72 KB of them (112
-    // rows of one token, 3 cache heads of 96: 13.2 -> 8.5 us; 13 parts of 12 heads of 128, 80 KB: 19.2 -> 20.1)
+    // rows of one token, 3 cache heads of 96: 13.2 -> 8.5 us; 8 rows, 13 parts of 12 heads of 128, 80 KB: 19.2 ->
+    // 20.1), 160 KB of many rows (32 rows, 23 parts of 8 heads of 192, 138 KB: 56.1 -> 52.8)
     const int G = Hq / c.Hkv, nh = G < 16 ? G : 16;
     const int64_t mx = at_cells(c, r, window) / at_chunk(c.type, c.dh) + 1;              // chunks of the longest row there can be
     const int64_t parts = mx / at_least(mx, G, c.dh) + 2;
-    const int fuse = B <= AT_FUSE || S > AT_COUNT || (parts <= AT_FUSE && parts * nh * c.dh <= 18432);
+    const int fuse = B <= AT_FUSE || S > AT_COUNT || (parts <= AT_FUSE && parts * nh * c.dh <= (S < 32 ? 18432 : 40960));
     if (c.type == SW_KV_F32) at_dispatch<SW_KV_F32>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B, fuse);
     else if (c.type == SW_KV_BF16) at_dispatch<SW_KV_BF16>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B, fuse);
     else at_dispatch<SW_KV_F16>(st, (unsigned)grid, c, r, q, S, Hq, sc, window, out, part, B, fuse);

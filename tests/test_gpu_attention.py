@@ -134,7 +134,7 @@ def test_row_counts(be, S, most, Hq, Hkv):
 @pytest.mark.parametrize("kind,Hq,Hkv,dh,P,lens", [
     ("bf16", 1, 1, 32, 32, [7900, 7900]), ("bf16", 1, 1, 32, 32, [7936, 5, 7936]), ("f16", 2, 1, 64, 16, [4000, 0, 3999, 17]),
     ("f32", 3, 3, 32, 64, [1500] * 7), ("bf16", 4, 2, 96, 128, [600, 1, 599, 300] * 9), ("f16", 5, 1, 128, 256, [3100, 2000]),
-    ("bf16", 5, 5, 64, 8, [3, 90, 400] * 30)])
+    ("bf16", 5, 5, 64, 8, [3, 90, 400] * 30), ("bf16", 8, 1, 128, 64, [2500, 1, 900, 40, 0] * 8), ("f16", 12, 1, 256, 16, [370, 31] * 16)])
 def test_joins_over_more_blocks(be, kind, Hq, Hkv, dh, P, lens):
     """few cache heads: more than 64 blocks for each, whose parts are joined in the same launch where no row has many"""
     one(be, 11, kind, Hq, Hkv, dh, P, lens)
