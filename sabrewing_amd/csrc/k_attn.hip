@@ -21,7 +21,7 @@
 // Measured (bf16, 8 cache heads of 128, 32 query heads; a page copy of the same size runs at 6.0 TB/s):
 // one row of 131,072 tokens 102 us (5.2 TB/s), 30 rows of 1 to 8,192 tokens 92 to 106 us by the card
 // (4.9 to 5.7 TB/s); 64 rows of a window of 512, heads of 64, 19.3 us (3.6 TB/s, 3.8 us of it the launch); f32, 16 heads of
-// 128, 7 rows of 600 to 3,000 tokens 50.6 us (4.5 TB/s); one row of 900 tokens 9.7 us, where the page table's, q's and the first
+// 128, 7 rows of 600 to 3,000 tokens 50.6 us (4.5 TB/s); one row of 900 tokens 10.0 us, where the page table's, q's and the first
 // cells' latencies and the join follow each other.  In the long ones the matrix cores are busy a tenth
 // of the time, the vector units a fifth: the rest waits for memory.
 #include "sw_attn.h"
