@@ -9,6 +9,7 @@ engines keep this half on the CPU (SDPA over their own caches).
 """
 import math
 from dataclasses import dataclass
+from operator import index
 
 import numpy as np
 
@@ -60,9 +61,13 @@ class PagedCache:
         self.n_heads, self.head_dim, self.kind = n_heads, head_dim, kind
         if min(n_layers, n_pages, page_size, n_heads, head_dim, max_seqs) < 1 or page_size & (page_size - 1):
             raise ValueError("PagedCache: sizes must be positive, page_size a power of two")
+        if not 8 <= page_size <= 4096 or head_dim % 32 or head_dim > 256 or n_heads > 1024 or kind not in KV_TYPES:
+            raise ValueError("PagedCache: page_size 8 to 4096, head_dim a multiple of 32 up to 256, at most 1024 heads, f32, bf16 or f16")
         item = 4 if KV_TYPES[kind] == 0 else 2
         self.max_seqs, self.max_rows = max_seqs, max_rows or max_seqs
         self.max_pages = -(-(max_len or n_pages * page_size) // page_size)
+        if self.max_pages * page_size > 1 << 30:
+            raise ValueError("PagedCache: sequences of more than 2^30 tokens (max_len)")
         one = n_pages * n_heads * page_size * head_dim * item              # one layer's keys or values
         self.pool = be.alloc(2 * n_layers * one)
         base = int(self.pool)
@@ -145,6 +150,7 @@ class PagedCache:
         of rows); appending through them is the caller's next calls, for every layer.  CacheFull,
         or a copy that fails, leaves everything as it was."""
         batch = [(e, 1) if e is None or np.isscalar(e) else tuple(e) for e in batch]
+        batch = [(s if s is None else index(s), index(n)) for s, n in batch]
         named = [s for s, _ in batch if s is not None]
         total = sum(n for _, n in batch)
         if len(set(named)) != len(named) or any(n < 1 for _, n in batch):

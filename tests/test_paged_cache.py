@@ -223,7 +223,11 @@ def test_refusals():
     for f in (c.close, c.fork, c.length):
         with pytest.raises(ValueError):
             f(a)
-    for kw in (dict(page_size=12), dict(n_pages=0), dict(max_seqs=0)):
+    with pytest.raises(TypeError):
+        c.rows([(c.open(), 2.0)])                      # before anything changes
+    assert c.pages_free() == 4 and not c._table[c._table >= 0].size
+    for kw in (dict(page_size=12), dict(n_pages=0), dict(max_seqs=0), dict(page_size=4), dict(page_size=8192), dict(head_dim=48),
+               dict(head_dim=288), dict(n_heads=1025), dict(kind="f64"), dict(max_len=(1 << 30) + 1)):
         d = dict(n_layers=1, n_pages=4, page_size=8, n_heads=1, head_dim=32)
         d.update(kw)
         with pytest.raises(ValueError):
