@@ -122,6 +122,15 @@ static int grow_pinned(Buf &b, size_t need) {
     return 0;
 }
 static Buf g_arena, g_hin, g_hout;
+// The last forward's expert groups (lag_hip_last_groups): 1, their lists on the device, in the arena or the fixed
+// region; 0, a count alone.  What next takes the arena writes over them, or frees them as it grows.
+static int g_last_G_dev = 0, g_last_ng = 0;
+static const int *g_last_lists[4];      // G, gexp, gbeg, gcnt
+static int take_arena(size_t need) {
+    const char *p = (const char *)g_last_lists[0], *a = (const char *)g_arena.p;
+    if (g_last_G_dev && p >= a && p < a + g_arena.cap) g_last_G_dev = g_last_ng = 0;
+    return grow_dev(g_arena, need);
+}
 
 // carve aligned sub-buffers out of the arena
 struct Carve {
@@ -273,7 +282,7 @@ static int grouped_host(float *outh, const float *x, int S, const void *gu_q, co
     const size_t o_xl = cv.take((size_t)S * (D / 32) * SW_NL * 16), o_xs = cv.take((size_t)S * (D / 32) * 4);
     size_t o_xd = 0, o_hd = 0;
     if (mf) { o_xd = cv.take((size_t)S * (D / 32) * 128); o_hd = cv.take((size_t)T * (I / 32) * 128); }
-    if (grow_dev(g_arena, cv.off)) return -1;
+    if (take_arena(cv.off)) return -1;
     char *A = (char *)g_arena.p;
     // one pinned image of the arena's head, one upload: x | gexp gbeg gcnt grow rowof w [| items P]
     const size_t xn = (size_t)S * D * 4, up = o_idx + idxn;
@@ -384,7 +393,7 @@ static int lanes_host(float *y, const float *x, const void *W, int wkind, int dp
     if (S <= 0 || I <= 0 || O <= 0 || !W) return -1;
     Carve cv;
     const size_t o_x = cv.take((size_t)S * I * 4), o_y = cv.take((size_t)S * O * 4);
-    if (grow_dev(g_arena, cv.off) || grow_pinned(g_hin, (size_t)S * I * 4) || grow_pinned(g_hout, (size_t)S * O * 4)) return -1;
+    if (take_arena(cv.off) || grow_pinned(g_hin, (size_t)S * I * 4) || grow_pinned(g_hout, (size_t)S * O * 4)) return -1;
     char *A = (char *)g_arena.p;
     memcpy(g_hin.p, x, (size_t)S * I * 4);
     CK(sw_xfer(g_st, A + o_x, g_hin.p, (size_t)S * I * 4, hipMemcpyHostToDevice), "x upload");
@@ -465,9 +474,10 @@ struct FwdScratch {
     uint32_t *xq, *hq;      // IDOT int8 activations of x [S][D/32][8] and of h [T][I/32][8]
     float *xqs, *hqs, *hf;  // their block scales; h [T][I] f32
 };
-static int g_last_G_dev = 0;            // 1: last forward's groups live in the arena
-static FwdScratch g_last;
-static int g_last_ng = 0;
+static void groups_on_device(const FwdScratch &f) {
+    g_last_G_dev = 1; g_last_ng = 0;
+    g_last_lists[0] = f.G; g_last_lists[1] = f.gexp; g_last_lists[2] = f.gbeg; g_last_lists[3] = f.gcnt;
+}
 
 // router rows and the Inkling gate pool; the shared experts of a layer
 static int ink_ns(const LagHipMoeDesc *d) { return d->route_act == SW_ROUTE_INKLING ? d->n_shared : 0; }
@@ -546,7 +556,7 @@ static int carve_fwd(const LagHipMoeDesc *d, int S, FwdScratch &f, const Scratch
         }
         A = src.fixed;
     } else {
-        if (grow_dev(g_arena, cv.off)) return -1;
+        if (take_arena(cv.off)) return -1;
         A = (char *)g_arena.p;
     }
     f.xq = idot ? (uint32_t *)(A + o_xq) : nullptr; f.xqs = idot ? (float *)(A + o_xqs) : nullptr;
@@ -692,8 +702,7 @@ static int forward_idot(const LagHipMoeDesc *d, const LagHipMoeWeights *w, const
       if (sw_launch_combine(g_st, f.slots, f.rowof, f.w, S, K, D, combine_scale(d), f.sout, out, 1,
                             gated ? f.wsh : nullptr, gated ? d->n_shared : 0))
           return fail_msg("combine launch"); }
-    g_last_G_dev = 1; g_last_ng = 0;
-    g_last = f;
+    groups_on_device(f);
     return 0;
 }
 
@@ -798,7 +807,7 @@ static int forward(const LagHipMoeDesc *d, const LagHipMoeWeights *w, const floa
         { PROF("combine");
           if (sw_launch_combine(g_st, f.slots, f.rowof, f.w, S, K, D, rs_c, sh || gated ? f.sout : nullptr, out, 1, wsh, nsg))
               return fail_msg("combine launch"); }
-        g_last_G_dev = 1; g_last_ng = 0;
+        groups_on_device(f);
     } else {
         // tokens per pass of the grouped kernels: one when the pairs number at most 0.3 E
         // (about one token per group: C5's 64 pairs of 256 experts, 7.19 -> 6.91 ms per
@@ -841,9 +850,8 @@ static int forward(const LagHipMoeDesc *d, const LagHipMoeWeights *w, const floa
             if (sw_launch_combine(g_st, f.slots, f.rowof, f.w, S, K, D, rs_c, sh || gated ? f.sout : nullptr, out, 1, wsh, nsg))
                 return fail_msg("combine launch");
         }
-        g_last_G_dev = 1; g_last_ng = 0;
+        groups_on_device(f);
     }
-    g_last = f;
     return 0;
 }
 
@@ -1024,7 +1032,7 @@ extern "C" int lag_hip_attn_paged(const LagHipKvCache *c, const LagHipKvRows *r,
     if (!apart(q, n, out, n)) return refuse(me, "q and out overlap");
     if (not_ready(me)) return -1;
     const int64_t np = sw_attn_part_floats(kv, rows, Hq, window, S);
-    if (np && grow_dev(g_arena, (size_t)np * 4)) return -1;
+    if (np && take_arena((size_t)np * 4)) return -1;
     PROF("attn_paged");
     if (sw_launch_attn(g_st, kv, rows, q, Hq, scale, window, out, S, np ? (float *)g_arena.p : nullptr)) return fail_msg("attn_paged launch");
     return 0;
@@ -1092,12 +1100,12 @@ extern "C" int lag_hip_last_groups(int *G, int *gexp, int *gbeg, int *gcnt, int 
     if (!g_ok) return -1;
     CK(hipStreamSynchronize(g_st), "stream sync");
     if (!g_last_G_dev) { *G = g_last_ng; return 0; }
-    CK(hipMemcpy(G, g_last.G, 4, hipMemcpyDeviceToHost), "G download");
+    CK(hipMemcpy(G, g_last_lists[0], 4, hipMemcpyDeviceToHost), "G download");
     const int n = *G < cap ? *G : cap;
     if (n > 0) {
-        CK(hipMemcpy(gexp, g_last.gexp, (size_t)n * 4, hipMemcpyDeviceToHost), "gexp download");
-        CK(hipMemcpy(gbeg, g_last.gbeg, (size_t)n * 4, hipMemcpyDeviceToHost), "gbeg download");
-        CK(hipMemcpy(gcnt, g_last.gcnt, (size_t)n * 4, hipMemcpyDeviceToHost), "gcnt download");
+        CK(hipMemcpy(gexp, g_last_lists[1], (size_t)n * 4, hipMemcpyDeviceToHost), "gexp download");
+        CK(hipMemcpy(gbeg, g_last_lists[2], (size_t)n * 4, hipMemcpyDeviceToHost), "gbeg download");
+        CK(hipMemcpy(gcnt, g_last_lists[3], (size_t)n * 4, hipMemcpyDeviceToHost), "gcnt download");
     }
     return 0;
 }

@@ -215,3 +215,51 @@ def test_forked_streams_agree(be, orc):
     cache.free()
     for q in (hd, xn, lg, tok):
         q.free()
+
+
+def test_groups_after_attention(be, orc):
+    """lag_hip_last_groups tells of the last forward until another call takes the scratch its lists lie in: an attention whose
+    rows have parts, a matmul of host arrays, a routing; then there are none.  What takes no scratch, or
+    other scratch than the lists lie in, leaves them."""
+    from paged import Cache
+    from sabrewing_amd.backend import DeviceLayer, desc_of
+    cfg = cf.scaled(cf.C5_LAYER, D=512, E=32, K=8, I=384)
+    layer = synth.make_layer(orc, cfg, 91)
+    dl, S = DeviceLayer.from_host(be, cfg, layer), 5
+    x = synth.make_x(orc, cfg, 92, S)
+    xd, od = be.upload(x), be.upload(np.zeros_like(x))
+    P, dh, far = 16, 64, 20000                         # one row of 20,000 tokens: split, and more scratch than the forward
+    n_pages = -(-far // P)
+    c = Cache(be, "bf16", n_pages, P, 1, dh, *[np.zeros((n_pages, 1, P, dh), np.uint16)] * 2)
+    bufs = [be.upload(a) for a in (np.array([far - 1], np.int32), np.arange(n_pages, dtype=np.int32)[None].copy(),
+                                   np.ones((1, 16, dh), np.float32), np.ones((1, 16, dh), np.float32))]
+    rows, head = be.kv_rows(bufs[0], bufs[1], 1, n_pages), be.upload(np.zeros((8, cfg.D), np.uint16))
+    attend = lambda: be.attn_paged(c.c, rows, bufs[2], 16, 0.125, 0, bufs[3], 1)
+    forward = lambda: be.moe_forward(desc_of(cfg), dl.weights(), xd, od, S)
+    _, sel, _ = be.route(desc_of(cfg), dl.weights(), xd, S)
+    want = orc.bucket(sel, S, cfg.K, cfg.E)
+
+    def same():
+        got = be.last_groups()
+        assert got[0] == want[0] and all(np.array_equal(a, b) for a, b in zip(got[1:], want[1:4]))
+    forward()
+    same()
+    be.add(od, xd, x.size)                             # no scratch
+    same()
+    attend()
+    assert be.last_groups()[0] == 0
+    forward()
+    same()
+    be.route(desc_of(cfg), dl.weights(), xd, S)
+    assert be.last_groups()[0] == 0
+    forward()
+    be.matmul_bf16(x, head, 8)
+    assert be.last_groups()[0] == 0
+    be.moe_forward_noalloc(desc_of(cfg), dl.weights(), xd, od, S)
+    same()
+    attend()                                           # its lists lie in the static region
+    same()
+    for b in [xd, od, head] + bufs:
+        b.free()
+    c.free()
+    dl.free()
