@@ -323,7 +323,8 @@ __global__ __launch_bounds__(AT_NT, at_blocks_cu(TYPE, 32 * NB)) void k_attn(SwK
             load_v(ch, p);
         }
         // ---- q's parts in the right operand's order: [part][step][lane] of 16 bytes
-        float sc = sc0, up = 1.f;
+        float sc = sc0;
+        int up = 0;                                                    // the power of two that q is scaled by
         if constexpr (TYPE == SW_KV_F16) {
             float mx = 0.f;
 #pragma unroll
@@ -336,9 +337,9 @@ __global__ __launch_bounds__(AT_NT, at_blocks_cu(TYPE, 32 * NB)) void k_attn(SwK
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < AT_NW; i++) mx = fmaxf(mx, s_m[i][cl]);
-            const int e = mx > 0.f && mx < INFINITY ? 13 - ilogbf(mx) : 0;
-            up = ldexpf(1.f, min(max(e, -100), 100));
-            sc = sc0 / up;
+            up = mx > 0.f && mx < INFINITY ? 13 - ilogbf(mx) : 0;      // (-114 to 162: no float holds them all)
+            sc = ldexpf(sc0, -up);
+            if (fabsf(sc) == INFINITY && fabsf(sc0) < INFINITY) sc = copysignf(3.402823466e38f, sc0);   // (a score of 0 stays one)
         } else {
             __syncthreads();                                           // (the row before is done with)
         }
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(AT_NT, at_blocks_cu(TYPE, 32 * NB)) void k_attn(SwK
             } else {
                 float x[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) x[j] = qx[i][j / 4][j % 4] * up;
+                for (int j = 0; j < 8; j++) x[j] = TYPE == SW_KV_F16 ? ldexpf(qx[i][j / 4][j % 4], up) : qx[i][j / 4][j % 4];
                 sw_u32x4 o[NP];
                 at_split<TYPE>(x, o);
 #pragma unroll

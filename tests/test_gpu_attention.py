@@ -285,3 +285,49 @@ def test_same_bits_every_time(be):
     a = one(be, 11, "bf16", 8, 2, 128, 16, [3000, 10, 700])
     b = one(be, 11, "bf16", 8, 2, 128, 16, [3000, 10, 700])
     assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_queries_near_the_largest_float(be, kind):
+    """queries whose largest values lie between 2^119 and 2^123: the scores are finite in 32 bits, and so far apart that
+    one cell takes everything, so each output is that cell's v, exactly.  (That the two largest scores are further
+    apart than the errors of 32-bit sums, 2 (dh + 2) e sum |q k|, and than 200, is asserted of the inputs.)"""
+    rng = np.random.default_rng(12)
+    P, Hkv, dh, Hq, scale = 16, 2, 128, 6, 0.0883883461
+    lens = [300, 65, 1, 1000]
+    table, n_pages = random_pages(rng, lens, P)
+    k, v = pools(rng, kind, n_pages, P, Hkv, dh)
+    pos, seq = np.asarray(lens) - 1, np.arange(4)
+    q = (1e36 * rng.standard_normal((4, Hq, dh))).astype(np.float32)
+    want = np.zeros(q.shape)
+    for s, n in enumerate(lens):
+        t = np.arange(n)
+        for h in range(Hq):
+            kk, vv = (from_bits(a)[table[s, t // P], h // 3, t % P] for a in (k, v))
+            x, size = kk @ q[s, h].astype(np.float64) * scale, np.abs(kk) @ np.abs(q[s, h].astype(np.float64)) * scale
+            top = np.argmax(x)
+            gap = x[top] - np.delete(x, top)
+            assert np.all(gap > 2 * (dh + 2) * 2.0 ** -24 * size.max() + 200) and np.abs(x).max() < 1e38
+            want[s, h] = vv[top]
+    c = Cache(be, kind, n_pages, P, Hkv, dh, k, v)
+    got = run(be, c, table, pos, q, Hq, scale, seq=seq)
+    c.free()
+    assert np.array_equal(got, want.astype(np.float32))
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-36])
+def test_tiny_queries_and_a_large_scale(be, size):
+    """an f16 cache's queries are scaled to f16's range whatever their size: with a scale that makes up for it the
+    scores are ordinary ones, in the same bounds"""
+    rng = np.random.default_rng(13)
+    P, Hkv, dh, Hq = 16, 2, 64, 4
+    lens = [200, 33, 700]
+    table, n_pages = random_pages(rng, lens, P)
+    k, v = pools(rng, "f16", n_pages, P, Hkv, dh)
+    pos, seq = np.asarray(lens) - 1, np.arange(3)
+    q = (1.5 * size * rng.standard_normal((3, Hq, dh))).astype(np.float32)
+    scale = float(np.float32(0.125 / size))
+    c = Cache(be, "f16", n_pages, P, Hkv, dh, k, v)
+    got = run(be, c, table, pos, q, Hq, scale, seq=seq)
+    c.free()
+    check(got, *exact_attention(from_bits(k), from_bits(v), table, P, pos, seq, q.astype(np.float64), scale))
