@@ -259,7 +259,8 @@ int    lag_hip_qk_rope_append(const LagHipKvCache *c, const LagHipKvRows *r, con
  * n_heads); q and out [S][n_q_heads][head_dim], 16-byte aligned, not overlapping.  Sums and
  * the softmax in 32 bits.  A free place, or a row without any cell, gives zeros.  Rows of one
  * sequence at consecutive positions (a chunk of a prompt, already appended) each see what is
- * theirs to see.  max_pages * page_size times S, or 64 if that is less, is below 2^36.
+ * theirs to see.  max_pages * page_size (of f32 caches, or heads over 160, rounded up to
+ * a multiple of 16) times S, or 64 if that is less, is below 2^36.
  * Infinities and NaN in a cell reach the rows that attend to it, as values without meaning,
  * and no others; cells that no row attends to may hold anything.  The same call gives the same
  * bits; how a row's cells are cut into parts, and with that its last bits, depends on the

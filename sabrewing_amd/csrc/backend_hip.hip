@@ -1026,7 +1026,8 @@ extern "C" int lag_hip_attn_paged(const LagHipKvCache *c, const LagHipKvRows *r,
     if (!q || !out || ((uintptr_t)q | (uintptr_t)out) % 16) return refuse(me, "q and out must be 16-byte aligned");
     if (Hq < 1 || Hq > 1024 || Hq % c->n_heads) return refuse(me, "n_q_heads (a multiple of n_heads)");
     if (window < 0) return refuse(me, "negative window");
-    if ((int64_t)r->max_pages * c->page_size * (S < 64 ? S : 64) >= (int64_t)1 << 36)        // (its counts of 64 rows' cells)
+    const int counted = S < 64 ? S : 64;                               // (rows counted together, in 32 bits)
+    if ((int64_t)r->max_pages * c->page_size * counted >= (int64_t)1 << 36 || sw_attn_row_chunks(kv, rows) * counted >= (int64_t)1 << 32)
         return refuse(me, "64 rows of 2^30 cells");
     const size_t n = (size_t)S * Hq * c->head_dim * 4;
     if (!apart(q, n, out, n)) return refuse(me, "q and out overlap");

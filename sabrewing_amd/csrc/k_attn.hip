@@ -652,6 +652,10 @@ static int64_t at_cells(const SwKv &c, const SwRows &r, int window) {
     const int64_t cells = (int64_t)r.max_pages << c.psh, most = (int64_t)window + at_chunk(c.type, c.dh);
     return window > 0 && most < cells ? most : cells;                  // (a window begins anywhere in a chunk)
 }
+int64_t sw_attn_row_chunks(const SwKv &c, const SwRows &r) {
+    const int CT = at_chunk(c.type, c.dh);
+    return (((int64_t)r.max_pages << c.psh) + CT - 1) / CT;
+}
 // Blocks of a cache head: so many that all of them are AT_BLOCKS, no more than rows or least parts for them.
 static int at_blocks(const SwKv &c, const SwRows &r, int Hq, int window, int S) {
     if (S > AT_COUNT) return S;

@@ -101,6 +101,7 @@ int sw_launch_qk_rope_append(hipStream_t st, const SwKv &c, const SwRows &r, con
 int sw_launch_kv_copy(hipStream_t st, const SwKv *layers, int n_layers, const int *src, const int *dst, int n);
 // (k_attn.hip) one token of each row against its sequence's cells (pos - window, pos]; part:
 // scratch of sw_attn_part_floats floats, 16-byte aligned (0: none)
+int64_t sw_attn_row_chunks(const SwKv &c, const SwRows &r);           // chunks of the longest row there can be: 64 rows' fit 32 bits
 int64_t sw_attn_part_floats(const SwKv &c, const SwRows &r, int Hq, int window, int S);
 int sw_launch_attn(hipStream_t st, const SwKv &c, const SwRows &r, const float *q, int Hq, float scale, int window, float *out,
                    int S, float *part);

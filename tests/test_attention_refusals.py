@@ -137,3 +137,20 @@ def test_too_many_cells(lib):
     r = dict(n_seqs=64, max_pages=1 << 26)
     refused(lib, attn_call(lib, r=rows(**r), S=64, out=1024 * A), "2^30")
     assert attn_call(lib, r=rows(**r), S=1) == -1 and "2^30" not in lib.lag_hip_last_error().decode()
+
+
+def test_cells_that_round_up_to_too_many(lib):
+    """a row of 2^30 - 8 cells is 2^26 chunks where they are of 16 tokens, and 64 such rows no number of 32 bits; one page
+    less is, and so are chunks of 32"""
+    if lib.lag_hip_alloc(16):
+        pytest.skip("a device is initialised in this process")
+    n, out = 1 << 27, 1024 * A
+    for kw in (dict(type="f32", head_dim=64), dict(type="f16", head_dim=192), dict(type="bf16", head_dim=192)):
+        c = cache(page_size=8, **kw)
+        refused(lib, attn_call(lib, c, rows(n_seqs=64, max_pages=n - 1), S=64, out=out), "2^30")
+        refused(lib, attn_call(lib, c, rows(n_seqs=300, max_pages=n - 1), S=300, out=out), "2^30")
+        for S, pages in ((64, n - 2), (63, n - 1), (1, n)):
+            assert attn_call(lib, c, rows(n_seqs=64, max_pages=pages), S=S, out=out) == -1
+            assert "2^30" not in lib.lag_hip_last_error().decode()
+    assert attn_call(lib, cache(page_size=8), rows(n_seqs=64, max_pages=n - 1), S=64, out=out) == -1
+    assert "2^30" not in lib.lag_hip_last_error().decode()
