@@ -279,7 +279,7 @@ class DeviceAttention:
             raise ValueError("DeviceAttention: D and n_q * head_dim must be multiples of 128, n_q of n_kv")
         if (q_norm is None or k_norm is None) == acfg.qk_norm:
             raise ValueError("DeviceAttention: q_norm and k_norm belong to a config with qk_norm, and to no other")
-        self.be, self.acfg, self.D = be, acfg, D
+        self.be, self.acfg, self.D, self.shape = be, acfg, D, (acfg.n_q, acfg.n_kv, acfg.head_dim, D)
         self.norm, self.wqkv, self.wo, self.q_norm, self.k_norm, self.rope = norm, wqkv, wo, q_norm, k_norm, rope
         self.bufs = [b for b in (norm, wqkv, wo, q_norm, k_norm) if isinstance(b, DevBuf)]
 
@@ -317,7 +317,7 @@ class DeviceAttention:
         be, a, D = self.be, self.acfg, self.D
         if (cache_layer.n_heads, cache_layer.head_dim) != (a.n_kv, a.head_dim):
             raise ValueError("DeviceAttention: a cache of other heads")
-        if S > scratch.S or scratch.shape != (a.n_q, a.n_kv, a.head_dim, D):
+        if S > scratch.S or scratch.shape != self.shape:
             raise ValueError("DeviceAttention: scratch for fewer rows or other heads")
         be.rmsnorm(h, self.norm, xn, S, D, a.eps)
         be.head_argmax(self.wqkv, True, xn, S, D, a.qkv_rows, scratch.qkv)

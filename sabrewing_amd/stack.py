@@ -35,6 +35,8 @@ class DeviceStack:
             raise ValueError("add_attention: the stack has its attention layers")
         if layers is not None and len(layers) != len(self.layers):
             raise ValueError("add_attention: as many attention layers as MoE layers")
+        if layers and any(a.shape != layers[0].shape or a.D != self.cfg.D for a in layers):
+            raise ValueError("add_attention: layers of one width and of the same heads")
         self.rope = self.rope or Rope(self.be, acfg)
         self.attn = list(layers) if layers is not None else [
             DeviceAttention.generate(self.be, acfg, self.cfg.D, seed, l, self.rope) for l in range(len(self.layers))]

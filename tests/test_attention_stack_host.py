@@ -119,3 +119,22 @@ def test_scratch_outlives_its_growth():
     new = st.scratch
     st.free()
     assert all(b.freed for s in (old, new) for b in (s.qkv, s.q, s.ctx, s.out))
+
+
+@pytest.mark.parametrize("second,D", [(AttnConfig(8, 2, 32, 32), None), (AttnConfig(4, 4, 32, 32), None), (AttnConfig(4, 2, 64, 32), None),
+                                      (A, 640)], ids=str)
+def test_layers_of_other_shapes_run_nothing(second, D):
+    """they are refused before a first layer has changed h or appended its keys and values"""
+    be = Recorder()
+    cache = PagedCache(be, 2, 8, 8, 2, 32, max_seqs=3)
+    cfg = cf.scaled(cf.C5_LAYER, D=512, E=32, K=8, I=384)
+    rope = Rope(be, A)
+    layers = [attention(be, A, D or cfg.D, rope), attention(be, second, D or cfg.D, rope)]
+    st = DeviceStack(be, cfg, 1000)
+    st.layers, st.norms = [Layer(), Layer()], [be.alloc(4 * cfg.D) for _ in range(2)]
+    st.final_norm, st.head = be.alloc(4), be.alloc(4)
+    be.calls.clear()
+    with pytest.raises(ValueError):
+        st.add_attention(A, layers)
+        step(be, st, cache, cache.desc, 2)
+    assert not be.calls
