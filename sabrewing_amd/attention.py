@@ -136,6 +136,12 @@ class PagedCache:
             if not self._users[p]:
                 self._free.append(p)
 
+    def _take(self, took):
+        p = self._free.pop()
+        self._users[p] = 1
+        took.append(p)
+        return p
+
     def length(self, seq):
         self._check(seq)
         return self._len[seq]
@@ -148,7 +154,7 @@ class PagedCache:
         """The next tokens of a batch: entries are a sequence (one token), (sequence, n) (its next
         n tokens, rows in order), None or (None, n) (free places).  Returns (rows descriptor, number
         of rows); appending through them is the caller's next calls, for every layer.  CacheFull,
-        or a copy that fails, leaves everything as it was."""
+        or a copy or an upload that fails, leaves everything as it was."""
         batch = [(e, 1) if e is None or np.isscalar(e) else tuple(e) for e in batch]
         batch = [(s if s is None else index(s), index(n)) for s, n in batch]
         named = [s for s, _ in batch if s is not None]
@@ -160,11 +166,12 @@ class PagedCache:
         if not 1 <= total <= self.max_rows:
             raise ValueError(f"PagedCache.rows: {total} rows (at most {self.max_rows})")
         # what it takes: copies of shared last pages, then new ones
-        P, users, need = self.page_size, {}, 0
+        P, users, need, old = self.page_size, {}, 0, {}                    # (old: the lengths before)
         for s, n in batch:
             if s is None:
                 continue
             pages, ln = self._pages[s], self._len[s]
+            old[s] = ln
             if ln + n > self.max_pages * P:
                 raise CacheFull(f"sequence {s}: {ln + n} tokens, at most {self.max_pages * P}")
             if ln % P:
@@ -175,47 +182,51 @@ class PagedCache:
             need += -(-(ln + n) // P) - len(pages)
         if need > len(self._free):
             raise CacheFull(f"{need} pages needed, {len(self._free)} free")
-        # the shared last pages are copied first: where that fails, nothing has changed
-        src, of = [], {}
-        for s, _ in batch:
-            if s is not None and self._len[s] % P and self._users[self._pages[s][-1]] > 1:
-                src.append(self._pages[s][-1])
-                of[s] = self._free.pop()
-                self._users[src[-1]] -= 1
-        if src:
-            try:
+        took, src, of = [], [], {}                                         # pages taken, shared ones left, and those in their place
+        try:
+            for s, ln in old.items():                                      # the shared last pages are copied first
+                if ln % P and self._users[self._pages[s][-1]] > 1:
+                    src.append(self._pages[s][-1])
+                    of[s] = self._take(took)
+                    self._users[src[-1]] -= 1
+            if src:
                 self.be.kv_copy_pages(self.layers, src, list(of.values()))
-            except Exception:
-                for p, q in zip(reversed(src), reversed(of.values())):
-                    self._users[p] += 1
-                    self._free.append(q)
-                raise
-        at = 0
-        for s, n in batch:
-            if s is None:
-                self._rows[:, at:at + n] = -1
+            at = 0
+            for s, n in batch:
+                if s is None:
+                    self._rows[:, at:at + n] = -1
+                    at += n
+                    continue
+                pages, ln = self._pages[s], self._len[s]
+                if s in of:
+                    pages[-1] = of[s]
+                    self._table[s, len(pages) - 1] = of[s]
+                    self._dirty.add(s)
+                while len(pages) * P < ln + n:
+                    p = self._take(took)
+                    self._table[s, len(pages)] = p
+                    pages.append(p)
+                    self._dirty.add(s)
+                self._rows[0, at:at + n] = np.arange(ln, ln + n)
+                self._rows[1, at:at + n] = s
+                self._len[s] = ln + n
                 at += n
-                continue
-            pages, ln = self._pages[s], self._len[s]
-            if s in of:
-                p = of[s]
-                self._users[p] = 1
-                pages[-1] = p
-                self._table[s, len(pages) - 1] = p
+            self._rows[:, at:] = -1
+            self._upload()
+            self.be.h2d(self.dev_rows, self._rows)
+        except BaseException:
+            for s, ln in old.items():                                      # as it was
+                n = -(-ln // P)
+                del self._pages[s][n:]
+                self._table[s, n:], self._len[s] = -1, ln
                 self._dirty.add(s)
-            while len(pages) * P < ln + n:
-                p = self._free.pop()
-                self._users[p] = 1
-                self._table[s, len(pages)] = p
-                pages.append(p)
-                self._dirty.add(s)
-            self._rows[0, at:at + n] = np.arange(ln, ln + n)
-            self._rows[1, at:at + n] = s
-            self._len[s] = ln + n
-            at += n
-        self._rows[:, at:] = -1
-        self._upload()
-        self.be.h2d(self.dev_rows, self._rows)
+            for s, p in zip(of, src):
+                self._pages[s][-1] = self._table[s, len(self._pages[s]) - 1] = p
+                self._users[p] += 1
+            for p in reversed(took):
+                self._users[p] = 0
+                self._free.append(p)
+            raise
         return self.desc, total
 
     def _upload(self):

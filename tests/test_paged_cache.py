@@ -193,6 +193,41 @@ def test_a_failed_copy_changes_nothing():
     assert [contents(be, c, s) for s in (a, b, d)] == [[0, 1, 10], [0, 1] + list(range(11, 18)), [0, 1, 18]]
 
 
+@pytest.mark.parametrize("nth", range(5))
+def test_a_failed_upload_changes_nothing(nth):
+    """the nth upload of a step fails (a changed sequence's table, or the rows): the call again gives the same step, and
+    what lies on the device afterwards is right"""
+    be = FakeBackend()
+    c = PagedCache(be, 1, 12, 8, 1, 32, max_seqs=5, max_rows=30)
+    a, e = c.open(), c.open()
+    desc, S = c.rows([(a, 10), (e, 8)])
+    append(be, desc, S, 8, list(range(18)))
+    b, d = c.fork(a), c.fork(a)
+
+    def state():
+        return c._users.tolist(), list(c._free), list(c._len), [list(p) if p is not None else None for p in c._pages], c._table.tolist()
+    before, batch, h2d, left = state(), [a, (b, 9), None, d, (e, 2)], be.h2d, [nth]
+
+    def broken(*args):
+        if not left[0]:
+            raise BackendError("injected fault")
+        left[0] -= 1
+        h2d(*args)
+    be.h2d = broken
+    with pytest.raises(BackendError):
+        c.rows(batch)
+    assert state() == before
+    invariants(c)
+    be.h2d = h2d
+    desc, S = c.rows(batch)
+    assert S == 14
+    append(be, desc, S, 8, list(range(100, 114)))
+    invariants(c)
+    ten = list(range(10))
+    assert [contents(be, c, s) for s in (a, b, d, e)] == [ten + [100], ten + list(range(101, 110)), ten + [111],
+                                                         list(range(10, 18)) + [112, 113]]
+
+
 def test_free_places():
     be = FakeBackend()
     c = PagedCache(be, 1, 4, 8, 1, 32, max_seqs=3, max_rows=9)
