@@ -272,7 +272,8 @@ int    lag_hip_attn_paged(const LagHipKvCache *c, const LagHipKvRows *r, const f
  * a fork's last page, or pages moved together.  src and dst are host arrays, free to change
  * on return; a dst is named once and is no src.  0 = ok */
 int    lag_hip_kv_copy_pages(const LagHipKvCache *layers, int n_layers, const int *src, const int *dst, int n);
-/* x[i] += t[i] for n values: the residual after an output projection.  0 = ok */
+/* x[i] += t[i] for n values: the residual after an output projection.  t may be x, or does
+ * not overlap it.  0 = ok */
 int    lag_hip_add(float *x, const float *t, size_t n);
 
 /* ---------------- sampling ----------------

@@ -1080,7 +1080,10 @@ extern "C" int lag_hip_kv_copy_pages(const LagHipKvCache *layers, int n_layers, 
 }
 
 extern "C" int lag_hip_add(float *x, const float *t, size_t n) {
-    if (!g_ok || fault_injected() || !x || !t || !n) return -1;
+    static const char *me = "add";
+    if (!x || !t || !n) return refuse(me, "no values");
+    if (x != t && !apart(x, n * 4, t, n * 4)) return refuse(me, "x and t overlap");
+    if (not_ready(me)) return -1;
     PROF("add");
     if (sw_launch_add(g_st, x, t, n)) return fail_msg("add launch");
     return 0;

@@ -95,8 +95,8 @@ int sw_launch_argmax(hipStream_t st, const float *logits, int S, int V, int *tok
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
-// x[i] += t[i], four values per thread where both begin on 16 bytes (a launch's time at a decode step's sizes)
-__global__ __launch_bounds__(256) void k_add(float *__restrict__ x, const float *__restrict__ t, size_t n, int by4) {
+// x[i] += t[i], four values per thread where both begin on 16 bytes (a launch's time at a decode step's sizes); t may be x
+__global__ __launch_bounds__(256) void k_add(float *x, const float *t, size_t n, int by4) {
     const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (by4) {
         if (4 * i + 4 <= n) {

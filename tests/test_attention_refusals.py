@@ -119,6 +119,15 @@ def test_bad_sampling(lib):
         refused(lib, lib.lag_hip_sample(*args), word)
 
 
+def test_bad_sums(lib):
+    for args, word in [((0, A, 8), "no values"), ((A, 0, 8), "no values"), ((A, 2 * A, 0), "no values"), ((A, A + 4, 8), "overlap"), ((A, A - 28, 8), "overlap")]:
+        lib.lag_hip_sample(0, 1, 1, None, A, A)        # (leaves another reason)
+        refused(lib, lib.lag_hip_add(*args), word)
+    if not lib.lag_hip_alloc(16):                      # (none is initialised in this process)
+        for args in [(A, A, 8), (A, A + 32, 8), (A + 32, A, 8)]:
+            refused(lib, lib.lag_hip_add(*args), "not initialised")
+
+
 def test_good_arguments_reach_the_device(lib):
     """the same calls with nothing wrong are refused for want of a device alone (run where none is initialised)"""
     if lib.lag_hip_alloc(16):

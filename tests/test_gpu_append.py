@@ -298,3 +298,13 @@ def test_add(be, n, off):
     assert np.array_equal(got, x)
     xd.free()
     td.free()
+
+
+@pytest.mark.parametrize("n,off", [(4096, 0), (1021, 0), (777, 4)])
+def test_add_to_itself(be, n, off):
+    x = np.random.default_rng(n).standard_normal(n + 8).astype(np.float32)
+    xd = be.upload(x)
+    be.add(int(xd) + off, int(xd) + off, n)
+    x[off // 4:off // 4 + n] *= 2
+    assert np.array_equal(be.d2h(xd, (n + 8,), np.float32), x)
+    xd.free()
