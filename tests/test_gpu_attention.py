@@ -331,3 +331,67 @@ def test_tiny_queries_and_a_large_scale(be, size):
     got = run(be, c, table, pos, q, Hq, scale, seq=seq)
     c.free()
     check(got, *exact_attention(from_bits(k), from_bits(v), table, P, pos, seq, q.astype(np.float64), scale))
+
+
+@pytest.mark.parametrize("kind,Hq,Hkv,dh,lens,window", [
+    ("bf16", 8, 2, 128, [3000, 10, 700, 0, 61], 0), ("f16", 32, 8, 64, [900, 40, 2000, 333], 512), ("f32", 4, 4, 64, [600, 1, 77, 1500], 0),
+    ("bf16", 1, 1, 32, [7900, 60, 7900], 0), ("f16", 20, 1, 128, [20000, 333, 9000], 0), ("bf16", 4, 1, 64, [130, 9, 1] * 100, 0)])
+def test_bits_do_not_depend_on_other_rows_contents(be, kind, Hq, Hkv, dh, lens, window):
+    """one row's cells and query stay, all others change: whole rows, parts joined in the launch and behind it"""
+    rng = np.random.default_rng(14)
+    P = 16
+    table, n_pages = random_pages(rng, lens, P)
+    pos, S = np.asarray(lens) - 1, len(lens)
+    k, v = pools(rng, kind, n_pages, P, Hkv, dh)
+    q = rng.standard_normal((S, Hq, dh)).astype(np.float32)
+    c = Cache(be, kind, n_pages, P, Hkv, dh, k, v)
+    first = run(be, c, table, pos, q, Hq, 0.125, window)
+    c.free()
+    for keep in range(min(S, 5)):
+        k2, v2 = pools(rng, kind, n_pages, P, Hkv, dh)
+        q2 = (30 * rng.standard_normal((S, Hq, dh))).astype(np.float32)
+        own = table[keep][table[keep] >= 0]
+        k2[own], v2[own], q2[keep] = k[own], v[own], q[keep]
+        c = Cache(be, kind, n_pages, P, Hkv, dh, k2, v2)
+        again = run(be, c, table, pos, q2, Hq, 0.125, window)
+        c.free()
+        assert np.array_equal(first[keep].view(np.uint32), again[keep].view(np.uint32)), keep
+        assert not np.array_equal(np.delete(first, keep, 0), np.delete(again, keep, 0))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_infinities(be, kind, sign):
+    """in cells that no row attends to they change nothing; in one that a row attends to (as an append into f16 gives for
+    values beyond its largest) they reach that row's heads that read it alone"""
+    rng = np.random.default_rng(15)
+    P, Hkv, dh, Hq, window = 16, 2, 64, 6, 90
+    lens = [120, 50, 64, 0, 700]
+    table, n_pages = random_pages(rng, lens, P)
+    k, v = pools(rng, kind, n_pages, P, Hkv, dh)
+    pos, seq = np.asarray(lens) - 1, np.arange(5)
+    q = rng.standard_normal((5, Hq, dh)).astype(np.float32)
+    inf = sign * np.inf if kind != "bf16" else np.uint16(0x7F80 if sign > 0 else 0xFF80)
+
+    def attend(k, v):
+        c = Cache(be, kind, n_pages, P, Hkv, dh, k, v)
+        got = run(be, c, table, pos, q, Hq, 0.125, window)
+        c.free()
+        return got
+    clean = attend(k, v)
+    live = np.zeros((n_pages, P), bool)
+    for s, p in enumerate(pos):
+        for t in range(max(0, p - window + 1), p + 1):
+            live[table[s, t // P], t % P] = True
+    k2, v2 = k.copy(), v.copy()
+    for a in (k2, v2):
+        a.transpose(0, 2, 1, 3)[~live] = inf
+    assert np.array_equal(clean.view(np.uint32), attend(k2, v2).view(np.uint32))
+    for which in (0, 1):
+        a = [k2.copy(), v2.copy()]
+        a[which][table[0, 5], 1, 3] = inf              # token 83 of row 0, heads 3 to 5
+        got = attend(*a)
+        others = np.ones((5, Hq), bool)
+        others[0, 3:] = False
+        assert np.array_equal(got[others].view(np.uint32), clean[others].view(np.uint32))
+        assert not np.any(np.isfinite(got[0, 3:]))
