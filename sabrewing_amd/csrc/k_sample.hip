@@ -153,9 +153,6 @@ __device__ __forceinline__ u64 sp_dpp(u64 x) {
     const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xF, false);
     return ((u64)hi << 32) | lo;
 }
-__device__ __forceinline__ u64 sp_weight1(u64 code, const SpRow &r, const SpShared &sh) {
-    return r.fmax == INFINITY ? (u64)SP_ONE : sp_weight(sp_unkey((uint32_t)(code >> 32)), r, sh);
-}
 __device__ __forceinline__ u64 sp_wave_sum(u64 v) {           // (row rotations by 8, 4, 2, 1, then the rows)
     v += sp_dpp<0x128>(v);
     v += sp_dpp<0x124>(v);

@@ -39,12 +39,6 @@ __device__ __forceinline__ void sw_kv_store(void *p, int64_t i, float f) {
     else if constexpr (TYPE == SW_KV_BF16) ((uint16_t *)p)[i] = sw_bf16_rne(f);
     else ((_Float16 *)p)[i] = (_Float16)f;
 }
-template <int TYPE>
-__device__ __forceinline__ float sw_kv_load(const void *p, int64_t i) {
-    if constexpr (TYPE == SW_KV_F32) return ((const float *)p)[i];
-    else if constexpr (TYPE == SW_KV_BF16) return __builtin_bit_cast(float, (uint32_t)((const uint16_t *)p)[i] << 16);
-    else return (float)((const _Float16 *)p)[i];
-}
 
 // A value and its partner's 16 or 32 lanes away (as a pair in no order): each swap exchanges
 // the rows of 16, or the halves, of two registers.  (The second register is hidden from the
