@@ -308,3 +308,46 @@ def test_add_to_itself(be, n, off):
     x[off // 4:off // 4 + n] *= 2
     assert np.array_equal(be.d2h(xd, (n + 8,), np.float32), x)
     xd.free()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dims", [0, 24, 50, 128])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_norm_weights_anywhere(be, interleaved, dims, kind):
+    """norm weights that do not begin on 16 bytes give what aligned ones give, to the errors of two orders of summing and of
+    one more rounding into the cache; one of the two may be left out"""
+    S, Hq, Hkv, dh, P = 3, 6, 2, 128, 8
+    rng = np.random.default_rng(dims)
+    qkv = rng.standard_normal((S, (Hq + 2 * Hkv) * dh)).astype(np.float32)
+    w = (1 + 0.1 * rng.standard_normal((2, dh))).astype(np.float32)
+    f = freqs(dims)
+    host = [qkv, np.array([5, 70, 0], np.int32), np.arange(27, dtype=np.int32).reshape(3, 9), np.concatenate([[0], w.ravel()]).astype(np.float32),
+            w]
+    bufs = [be.upload(np.ascontiguousarray(a)) for a in host]
+    fd = be.upload(f) if dims else None
+    rows = be.kv_rows(bufs[1], bufs[2], 3, 9)
+
+    def call(qn, kn):
+        c = Cache(be, kind, 27, P, Hkv, dh, *[np.zeros((27, Hkv, P, dh), np.float32 if kind == "f32" else np.uint16)] * 2)
+        out = be.upload(np.zeros(S * Hq * dh, np.float32))
+        be.qk_rope_append(c.c, rows, be.rope(fd, dims, interleaved, 1.2), bufs[0], qkv.shape[1], qn, kn, 1e-6, Hq, out, S)
+        q = be.d2h(out, (S, Hq, dh), np.float32)
+        k, v = (from_bits(a)[[0, 17, 18], :, [5, 6, 0]] for a in c.read())
+        out.free()
+        c.free()
+        return q, k, v
+    even, odd = int(bufs[4]), int(bufs[3]) + 4
+    q, k, v = call(even, even + 4 * dh)
+    q2, k2, v2 = call(odd, odd + 4 * dh)
+    x = qkv.astype(np.float64).reshape(S, -1, dh)
+    sq, sk = (pair_size(exact_rope(h, np.zeros(S), f, 0, 0, 1, g, 1e-6), dims, interleaved) * 1.2 for h, g in
+              ((x[:, :Hq], w[0]), (x[:, Hq:Hq + Hkv], w[1])))
+    tol = 2 * (dh / 2 + 16) * E
+    assert np.all(np.abs(q - q2) <= tol * sq)
+    assert np.all(np.abs(k - k2) <= tol * sk + 2 * HALF_STEP[kind] * (1 + tol) * sk)
+    assert np.array_equal(v, v2) and np.array_equal(v, to_type(x[:, Hq + Hkv:], kind)[1])
+    plain = call(None, None)
+    for a, b in ((call(even, None), (q, plain[1])), (call(None, even + 4 * dh), (plain[0], k))):
+        assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+    for b in bufs + ([fd] if dims else []):
+        b.free()

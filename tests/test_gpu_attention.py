@@ -395,3 +395,26 @@ def test_infinities(be, kind, sign):
         others[0, 3:] = False
         assert np.array_equal(got[others].view(np.uint32), clean[others].view(np.uint32))
         assert not np.any(np.isfinite(got[0, 3:]))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("window", [0, 40])
+def test_a_prompt_of_more_than_256_rows(be, kind, window):
+    """a chunk of 230 rows of one sequence beside 70 of others, free places and places that lead nowhere among them"""
+    rng = np.random.default_rng(16)
+    P, Hkv, dh, Hq = 8, 2, 96, 8
+    lens = [260] + [int(n) for n in rng.integers(1, 120, 70)]
+    table, n_pages = random_pages(rng, lens, P)
+    k, v = pools(rng, kind, n_pages, P, Hkv, dh)
+    seq = np.concatenate([np.zeros(230, int), np.arange(1, 71)])
+    pos = np.concatenate([np.arange(30, 260), np.asarray(lens[1:]) - 1])
+    at = rng.permutation(300)
+    seq, pos = seq[at], pos[at]
+    pos[[3, 250, 299]], seq[[7, 280]] = -1, [71, -1]
+    q = rng.standard_normal((300, Hq, dh)).astype(np.float32)
+    c = Cache(be, kind, n_pages, P, Hkv, dh, k, v)
+    got = run(be, c, table, pos, q, Hq, 0.102, window, seq=seq)
+    c.free()
+    scale = float(np.float32(0.102))
+    check(got, *exact_attention(from_bits(k), from_bits(v), table, P, pos, seq, q.astype(np.float64), scale, window))
+    assert not np.any(got[[3, 250, 299, 7, 280]])
