@@ -28,7 +28,8 @@ def rope_frequencies(dims, theta=10000.0, factor=1.0, trained=0, fast=32.0, slow
     factor > 1 stretches a model trained on `trained` positions: pairs that turn more than `fast`
     times over them keep their frequency, pairs that turn less than `slow` times are slowed by
     `factor`, those between along a ramp, and cos and sin grow by 0.1 ln(factor) + 1 (the "by
-    parts" interpolation of the YaRN paper).  trained = 0: every pair slowed alike, factor 1."""
+    parts" interpolation of the YaRN paper).  trained = 0: every pair slowed alike, factor 1.  A model with
+    another ramp or factor gives Backend.rope frequencies of its own."""
     if dims % 2 or dims < 0 or factor <= 0:
         raise ValueError("rope_frequencies: dims must be even, factor positive")
     f = float(theta) ** (-2.0 * np.arange(dims // 2, dtype=np.float64) / max(1, dims))

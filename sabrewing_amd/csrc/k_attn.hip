@@ -20,10 +20,11 @@
 //
 // Measured (bf16, 8 cache heads of 128, 32 query heads; a page copy of the same size runs at 6.0 TB/s):
 // one row of 131,072 tokens 102 us (5.2 TB/s), 30 rows of 1 to 8,192 tokens 92 to 106 us by the card
-// (4.9 to 5.7 TB/s); 64 rows of a window of 512, heads of 64, 19.3 us (3.6 TB/s, 3.8 us of it the launch); f32, 16 heads of
-// 128, 7 rows of 600 to 3,000 tokens 50.6 us (4.5 TB/s); one row of 900 tokens 10.0 us, where the page table's, q's and the first
-// cells' latencies and the join follow each other.  In the long ones the matrix cores are busy a tenth
-// of the time, the vector units a fifth: the rest waits for memory.
+// (4.9 to 5.7 TB/s); 64 rows of a window of 512, heads of 64, 19.5 us (3.6 TB/s, 3.8 us of it the launch); f32, 16 heads of
+// 128, 7 rows of 600 to 3,000 tokens 45 to 55 us by the run (4.1 to 5.0 TB/s); one row of 900 tokens 9.9 us, where the page
+// table's, q's and the first cells' latencies and the join follow each other.  In the long ones the matrix cores are busy a
+// tenth of the time, the vector units a fifth: the rest waits for memory.  A prompt's rows each read their cells again,
+// through the caches: 2,048 rows from position 0 take 690 us, from 8,000 on 5.1 ms.
 #include "sw_attn.h"
 
 #define AT_NT 256
@@ -31,8 +32,10 @@
 #define AT_BLOCKS 512                     // two blocks on each CU
 #define AT_MIN 4                          // chunks of a part: one a wave
 #define AT_ROW 12
-// Beyond so many rows they are dealt whole, a block each, without counting them: there are blocks enough
-// to even out, and each would count them all
+// Beyond so many rows they are dealt whole, a block of each cache head a row, without counting them (32 query heads, 8
+// of 128).  That suits a prompt's rows (257 from position 0: 35 us, counted 71; 2,048: 690 and 1,270) and rows of like
+// lengths (257 of 1 to 500 tokens: 56 us, counted 63).  It does not suit a row far longer than the others, which stays with its
+// one block: 257 rows of 1 to 500 and one of 65,536 take 950 us, counted 128.
 #define AT_COUNT 256
 // A row's parts, up to this many, are joined by the block that finishes last (one launch), else by k_attn_join
 #define AT_FUSE 64
@@ -97,7 +100,9 @@ __device__ __forceinline__ sw_f32x4 at_mfma16(uint32_t a0, uint32_t a1, uint32_t
 }
 
 // Tokens of a wave's chunk: two tiles; one where two would leave room for one block on a CU and one for two
-// (bf16 heads of 224 and 256 spill at two: 127 us against 106 for 8 rows of 8192 tokens)
+// (bf16 heads of 224 and 256 spill at two: 127 us against 106 for 8 rows of 8192 tokens).  bf16 heads of 160 and f16 of 256
+// spill 11 and 6 registers at two and are no better off at one: 49 rows of 469 tokens 24.0 us against 30.4 and 33.4
+// against 41.6, 8 rows of 8192 68 against 71 and 106 against 104.
 __host__ __device__ constexpr int at_chunk(int type, int dh) {
     return type == SW_KV_F32 || (dh > 160 && (type == SW_KV_F16 || dh <= 192)) ? 16 : 32;
 }

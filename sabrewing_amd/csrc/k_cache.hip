@@ -14,8 +14,9 @@ __device__ __forceinline__ void rp_angle(double freq, int pos, float factor, flo
 }
 
 #define RP_NT 256
-// The form for any pairs (two halves of a part whose halves are no multiple of 4 values): a wave a head,
-// a lane the pairs lane and lane + 64.
+// The form for any pairs (two halves of a part whose halves are no multiple of 4 values) and norm weights that do not begin
+// on 16 bytes: a wave a head, a lane the pairs lane and lane + 64.  Each head takes its angles again: 2048 rows of 32 + 2 x
+// 8 heads of 128 take 34 to 35 us (18.5 in the other form), one row and 48 what a launch takes.
 template <int TYPE>
 __global__ __launch_bounds__(RP_NT) void k_qk_rope_any(SwKv c, SwRows r, SwRope rope, const float *__restrict__ qkv, int64_t ld,
                                                           const float *__restrict__ wq, const float *__restrict__ wk, float eps,

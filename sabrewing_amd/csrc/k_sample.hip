@@ -23,11 +23,12 @@
 //   the kept weights of each group of tiles, then tile by tile of the group in which the sum passes.
 // Weights are what costs in the passes over all of a large row (some 20 64-bit operations each).
 //
-// Measured: one row of 32,000 logits, top-k 50, 11.5 us; of 128,000: greedy 7, top-k 50 19, top-k 500 39, top-k
-// 1000 62, top-p alone 93, no limit 41.  200 rows of 131,072 of all settings 108 us (0.97 TB/s), which is what one
+// Measured: one row of 32,000 logits, top-k 50, 11.5 us; 8 of 128,000: greedy 7, top-k 50 20, top-k 500 37, top-k
+// 1000 59, top-p alone 91, no limit 41.  200 rows of 131,072 of all settings 108 us (0.97 TB/s), which is what one
 // row of top-p takes: 45 us the histogram of weights (47 cycles of an LDS atomic for a wave), 29 us the
 // groups' sums (64-bit operations), the rest the row's reading three times.  A row of a batch has a CU to
-// itself, so up to 256 rows take no longer than one.
+// itself, so up to 256 rows take no longer than the slowest of them, and few rows leave most CUs idle.  (One register of
+// 128 spills.)
 #include "sw_attn.h"
 #include "sw_gate.h"
 
