@@ -180,9 +180,10 @@ int    lag_hip_moe_block(const LagHipMoeDesc *d, const LagHipMoeWeights *w, cons
 int    lag_hip_route(const LagHipMoeDesc *d, const LagHipMoeWeights *w, const float *x, int S,
                      float *logits, int *sel, float *wts);
 /* the last forward's expert groups: G (host out), gexp/gbeg/gcnt [G] host copies (one token:
- * G alone).  They lie in the backend's scratch: the next call that takes scratch ends them
- * (another forward or lag_hip_route, lag_hip_attn_paged of up to 256 rows, an entry with host
- * pointers), as does the end of a recording; G is 0 from then on. */
+ * G alone).  They lie in the backend's scratch: a later call that takes so much of it that it
+ * reaches them, or makes it grow, ends them (another forward, a lag_hip_route of more tokens,
+ * lag_hip_attn_paged of up to 256 rows, an entry with host pointers), as does the end of a
+ * recording; G is 0 from then on. */
 int    lag_hip_last_groups(int *G, int *gexp, int *gbeg, int *gcnt, int cap);
 
 /* ---------------- stack glue (device pointers, queued on the backend stream) ----------------

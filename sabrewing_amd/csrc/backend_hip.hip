@@ -123,14 +123,16 @@ static int grow_pinned(Buf &b, size_t need) {
 }
 static Buf g_arena, g_hin, g_hout;
 // The last forward's expert groups (lag_hip_last_groups): 1, their lists on the device, in the arena or the fixed
-// region; 0, a count alone.  What next takes the arena writes over them, or frees them as it grows.
+// region; 0, a count alone.  What takes the arena next writes its first bytes, and frees it where it has to grow.
 static int g_last_G_dev = 0, g_last_ng = 0;
 static const int *g_last_lists[4];      // G, gexp, gbeg, gcnt
-static int take_arena(size_t need) {
-    const char *p = (const char *)g_last_lists[0], *a = (const char *)g_arena.p;
-    if (g_last_G_dev && p >= a && p < a + g_arena.cap) g_last_G_dev = g_last_ng = 0;
+static int take_arena(size_t need, size_t written) {
+    const char *p = (const char *)g_last_lists[1], *a = (const char *)g_arena.p;           // (gexp is the first of them)
+    const bool there = g_last_G_dev && p >= a && p < a + g_arena.cap;
+    if (there && (need > g_arena.cap ? !g_capturing : a + written > p)) g_last_G_dev = g_last_ng = 0;
     return grow_dev(g_arena, need);
 }
+static int take_arena(size_t need) { return take_arena(need, need); }
 
 // carve aligned sub-buffers out of the arena
 struct Carve {
@@ -513,9 +515,10 @@ static int desc_ok(const LagHipMoeDesc *d, const LagHipMoeWeights *w) {
 struct ScratchSrc { char *fixed; size_t cap; };
 static const ScratchSrc kArena = {nullptr, 0};
 
-// need: only report the bytes the layout takes (nothing allocated or assigned)
+// need: only report the bytes the layout takes (nothing allocated or assigned); scores_only: the caller
+// writes no more of it than the logits and scores
 static int carve_fwd(const LagHipMoeDesc *d, int S, FwdScratch &f, const ScratchSrc &src, bool idot = false,
-                     size_t *need = nullptr) {
+                     size_t *need = nullptr, bool scores_only = false) {
     const int E = d->n_experts, K = d->topk, D = d->hidden, I = d->moe_inter, Is = d->shared_inter;
     const int T = S * K, R = router_rows(d), nsx = shared_count(d);
     Carve cv;
@@ -556,7 +559,7 @@ static int carve_fwd(const LagHipMoeDesc *d, int S, FwdScratch &f, const Scratch
         }
         A = src.fixed;
     } else {
-        if (take_arena(cv.off)) return -1;
+        if (take_arena(cv.off, scores_only ? o_sc + (size_t)S * R * 4 : cv.off)) return -1;
         A = (char *)g_arena.p;
     }
     f.xq = idot ? (uint32_t *)(A + o_xq) : nullptr; f.xqs = idot ? (float *)(A + o_xqs) : nullptr;
@@ -658,7 +661,7 @@ extern "C" int lag_hip_route(const LagHipMoeDesc *d, const LagHipMoeWeights *w, 
                              float *logits, int *sel, float *wts) {
     if (!g_ok || fault_injected() || !desc_ok(d, w) || S <= 0) return -1;
     FwdScratch f;
-    if (carve_fwd(d, S, f, kArena)) return -1;
+    if (carve_fwd(d, S, f, kArena, false, nullptr, true)) return -1;
     return route_dev(d, w, x, S, logits ? logits : f.logits, f.scores, sel, wts);
 }
 

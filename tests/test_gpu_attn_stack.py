@@ -218,9 +218,9 @@ def test_forked_streams_agree(be, orc):
 
 
 def test_groups_after_attention(be, orc):
-    """lag_hip_last_groups tells of the last forward until another call takes the scratch its lists lie in: an attention whose
-    rows have parts, a matmul of host arrays, a routing; then there are none.  What takes no scratch, or
-    other scratch than the lists lie in, leaves them."""
+    """lag_hip_last_groups tells of the last forward until another call takes the scratch its lists lie in, or makes it grow:
+    an attention whose rows have parts, a matmul of host arrays, a routing of more tokens; then there are none.
+    What takes no scratch, or other scratch than the lists lie in, leaves them, a routing of the same tokens among it."""
     from paged import Cache
     from sabrewing_amd.backend import DeviceLayer, desc_of
     cfg = cf.scaled(cf.C5_LAYER, D=512, E=32, K=8, I=384)
@@ -234,6 +234,7 @@ def test_groups_after_attention(be, orc):
     bufs = [be.upload(a) for a in (np.array([far - 1], np.int32), np.arange(n_pages, dtype=np.int32)[None].copy(),
                                    np.ones((1, 16, dh), np.float32), np.ones((1, 16, dh), np.float32))]
     rows, head = be.kv_rows(bufs[0], bufs[1], 1, n_pages), be.upload(np.zeros((8, cfg.D), np.uint16))
+    many = be.upload(np.tile(x, (120, 1)))
     attend = lambda: be.attn_paged(c.c, rows, bufs[2], 16, 0.125, 0, bufs[3], 1)
     forward = lambda: be.moe_forward(desc_of(cfg), dl.weights(), xd, od, S)
     _, sel, _ = be.route(desc_of(cfg), dl.weights(), xd, S)
@@ -251,15 +252,19 @@ def test_groups_after_attention(be, orc):
     forward()
     same()
     be.route(desc_of(cfg), dl.weights(), xd, S)
+    same()
+    be.route(desc_of(cfg), dl.weights(), many, 600)    # its scores reach further than the lists
     assert be.last_groups()[0] == 0
     forward()
+    be.matmul_bf16(x[:1, :128], head, 1)               # 516 bytes: the lists lie behind 5 rows' scores
+    same()
     be.matmul_bf16(x, head, 8)
     assert be.last_groups()[0] == 0
     be.moe_forward_noalloc(desc_of(cfg), dl.weights(), xd, od, S)
     same()
     attend()                                           # its lists lie in the static region
     same()
-    for b in [xd, od, head] + bufs:
+    for b in [xd, od, head, many] + bufs:
         b.free()
     c.free()
     dl.free()
