@@ -269,6 +269,38 @@ int    lag_hip_qk_rope_append(const LagHipKvCache *c, const LagHipKvRows *r, con
  * rows' cells hold.  Its scratch is the arena's.  0 = ok */
 int    lag_hip_attn_paged(const LagHipKvCache *c, const LagHipKvRows *r, const float *q, int n_q_heads, float scale,
                           int window, float *out, int S);
+/* Trees of drafted tokens (device arrays), to be verified in one step: tree i's nodes are rows first[i] ..
+ * first[i + 1] - 1 of the batch (first: [n_trees + 1], from 0 on and rising; at most max_nodes of a tree, itself at most 64).
+ * base[i] cells of sequence seq[i] (NULL: sequence i) come before the tree, and node j's k and v lie in cell base[i] + j,
+ * whatever its depth; bit j of sees[s] says that row s attends to node j of its tree (itself and its ancestors, as a
+ * rule).  pos[s] (NULL where no window is used): the row's position, base plus its depth.  base[i] < 0: a free place.  Tables as
+ * LagHipKvRows'.  What the arrays hold is read on the device: rows outside the batch, sequences and pages that lead
+ * nowhere have no cells. */
+typedef struct {
+    const int *first, *base, *seq, *pos, *table;
+    const uint64_t *sees;
+    int n_trees, n_seqs, max_pages, max_nodes;
+} LagHipTrees;
+/* lag_hip_attn_paged for trees: out[s][h] = sum_t p_t v_t over the cells t < base of row s's tree (with window > 0 those with t >
+ * max(pos[s], base) - window) and the cells base + j of the nodes that sees[s] names.  A tree's cells are read once for all of its
+ * nodes.  q, out, scale and the accuracy as there; S rows in all.  A row that attends to nothing, or of a free
+ * place, gives zeros; rows of no tree are left as they were.  An infinity or NaN in a cell reaches the rows that attend to it, as
+ * outputs without meaning, and no others.  max_pages * page_size <= 2^30.  0 = ok */
+int    lag_hip_attn_tree(const LagHipKvCache *c, const LagHipTrees *t, const float *q, int n_q_heads, float scale, int window,
+                         float *out, int S);
+/* lag_hip_qk_rope_append with positions of their own for the turn: row s's q and k turn by at[s], and its cell is that of
+ * token r->pos[s] (a tree's node: cell base + j, position base + its depth).  0 = ok */
+int    lag_hip_qk_rope_append_at(const LagHipKvCache *c, const LagHipKvRows *r, const int *at, const LagHipRope *rope,
+                                 const float *qkv, int64_t ld, const float *q_norm, const float *k_norm, float eps, int n_q_heads,
+                                 float *q_out, int S);
+/* The accepted path of each tree: from node 0 on, the lowest later node whose parent (parent[s], an index in its tree) is
+ * the path's last node and whose drafted token (draft[s]) is the one picked there (tok[s]), until there is none.  Writes
+ * path [n_trees][max_nodes] (indices of the path's nodes, then -1), count [n_trees] (its length; a free place or a tree without
+ * nodes: 0) and next [n_trees] (the pick at its last node; -1 without one), and moves the cells of the path's nodes together: node
+ * path[i]'s k and v to cell base + i, in every one of n_layers caches (one geometry and type).  Cells behind base + count
+ * hold what they held.  Cells that lead nowhere are left out.  parent, draft, tok: [S].  sees and pos of t are not used.  0 = ok */
+int    lag_hip_tree_commit(const LagHipKvCache *layers, int n_layers, const LagHipTrees *t, const int *parent, const int *draft,
+                           const int *tok, int *path, int *count, int *next, int S);
 /* Page src[i] of every one of n_layers caches (one geometry and type) to page dst[i], k and v:
  * a fork's last page, or pages moved together.  src and dst are host arrays, free to change
  * on return; a dst is named once and is no src.  0 = ok */

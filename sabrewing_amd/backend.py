@@ -31,6 +31,7 @@ EXPORTS = [
     "lag_hip_moe_block", "lag_hip_route",
     "lag_hip_last_groups", "lag_hip_rmsnorm", "lag_hip_moe_forward_rmsnorm", "lag_hip_head_argmax", "lag_hip_argmax", "lag_hip_set_grouped_kernel",
     "lag_hip_qk_rope_append", "lag_hip_attn_paged", "lag_hip_kv_copy_pages", "lag_hip_add", "lag_hip_sample",
+    "lag_hip_attn_tree", "lag_hip_qk_rope_append_at", "lag_hip_tree_commit",
     "lag_hip_set_q4_mode",
     "lag_hip_alloc", "lag_hip_h2d", "lag_hip_d2h", "lag_hip_d2d", "lag_hip_memset",
     "lag_hip_graph_begin", "lag_hip_graph_end", "lag_hip_graph_launch", "lag_hip_graph_destroy", "lag_hip_sync",
@@ -74,6 +75,11 @@ class LagHipKvCache(C.Structure):
 
 class LagHipKvRows(C.Structure):
     _fields_ = [("pos", VP), ("seq", VP), ("table", VP), ("n_seqs", C.c_int), ("max_pages", C.c_int)]
+
+
+class LagHipTrees(C.Structure):
+    _fields_ = [("first", VP), ("base", VP), ("seq", VP), ("pos", VP), ("table", VP), ("sees", VP), ("n_trees", C.c_int),
+                ("n_seqs", C.c_int), ("max_pages", C.c_int), ("max_nodes", C.c_int)]
 
 
 class LagHipRope(C.Structure):
@@ -137,6 +143,10 @@ def load_library(path=None):
     KP, RP = C.POINTER(LagHipKvCache), C.POINTER(LagHipKvRows)
     L.lag_hip_qk_rope_append.argtypes = [KP, RP, C.POINTER(LagHipRope), VP, C.c_int64, VP, VP, C.c_float, C.c_int, VP, C.c_int]
     L.lag_hip_attn_paged.argtypes = [KP, RP, VP, C.c_int, C.c_float, C.c_int, VP, C.c_int]
+    TP = C.POINTER(LagHipTrees)
+    L.lag_hip_attn_tree.argtypes = [KP, TP, VP, C.c_int, C.c_float, C.c_int, VP, C.c_int]
+    L.lag_hip_qk_rope_append_at.argtypes = [KP, RP, VP, C.POINTER(LagHipRope), VP, C.c_int64, VP, VP, C.c_float, C.c_int, VP, C.c_int]
+    L.lag_hip_tree_commit.argtypes = [KP, C.c_int, TP, VP, VP, VP, VP, VP, VP, C.c_int]
     L.lag_hip_kv_copy_pages.argtypes = [KP, C.c_int, VP, VP, C.c_int]
     L.lag_hip_add.argtypes = [VP, VP, C.c_size_t]
     L.lag_hip_sample.argtypes = [VP, C.c_int, C.c_int, C.POINTER(LagHipSample), VP, VP]
@@ -346,6 +356,12 @@ class Backend:
         return LagHipKvRows(int(pos_dev), _ptr(seq_dev), int(table_dev), n_seqs, max_pages)
 
     @staticmethod
+    def trees(first_dev, base_dev, sees_dev, table_dev, n_trees, n_seqs, max_pages, max_nodes, seq_dev=None, pos_dev=None):
+        """trees of drafted tokens: rows first[i] .. first[i + 1] - 1 are tree i's nodes, node j in cell base[i] + j"""
+        return LagHipTrees(int(first_dev), int(base_dev), _ptr(seq_dev), _ptr(pos_dev), int(table_dev), _ptr(sees_dev), n_trees, n_seqs,
+                           max_pages, max_nodes)
+
+    @staticmethod
     def rope(freq_dev, dims, interleaved=False, factor=1.0):
         return LagHipRope(_ptr(freq_dev), dims, int(interleaved), factor)
 
@@ -363,6 +379,21 @@ class Backend:
         """one new token of each row against its sequence's cells (window 0: all of them)"""
         self.check(self.lib.lag_hip_attn_paged(cache, rows, int(q_dev), n_q_heads, scale, window, int(out_dev), S),
                    "lag_hip_attn_paged")
+
+    def qk_rope_append_at(self, cache, rows, at_dev, rope, qkv_dev, ld, q_norm, k_norm, eps, n_q_heads, q_out_dev, S):
+        """qk_rope_append, turned by positions of their own"""
+        self.check(self.lib.lag_hip_qk_rope_append_at(cache, rows, int(at_dev), rope, int(qkv_dev), ld, _ptr(q_norm), _ptr(k_norm), eps,
+                                                      n_q_heads, int(q_out_dev), S), "lag_hip_qk_rope_append_at")
+
+    def attn_tree(self, cache, trees, q_dev, n_q_heads, scale, window, out_dev, S):
+        """the S nodes of all trees against their sequences' cells and the nodes they see"""
+        self.check(self.lib.lag_hip_attn_tree(cache, trees, int(q_dev), n_q_heads, scale, window, int(out_dev), S), "lag_hip_attn_tree")
+
+    def tree_commit(self, caches, trees, parent_dev, draft_dev, tok_dev, path_dev, count_dev, next_dev, S):
+        """each tree's accepted path, its length and the token after it; its cells moved together in every layer (caches from
+        kv_caches)"""
+        self.check(self.lib.lag_hip_tree_commit(caches, len(caches), trees, int(parent_dev), int(draft_dev), int(tok_dev), int(path_dev),
+                                                int(count_dev), int(next_dev), S), "lag_hip_tree_commit")
 
     def kv_copy_pages(self, caches, src, dst):
         """pages src[i] -> dst[i] of every layer (caches from kv_caches; host indices)"""

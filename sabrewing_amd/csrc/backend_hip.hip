@@ -997,10 +997,8 @@ static bool apart(const void *a, size_t na, const void *b, size_t nb) {
     return (uintptr_t)a + na <= (uintptr_t)b || (uintptr_t)b + nb <= (uintptr_t)a;
 }
 
-extern "C" int lag_hip_qk_rope_append(const LagHipKvCache *c, const LagHipKvRows *r, const LagHipRope *rope, const float *qkv,
-                                      int64_t ld, const float *q_norm, const float *k_norm, float eps, int Hq, float *q_out,
-                                      int S) {
-    static const char *me = "qk_rope_append";
+static int rope_append(const char *me, const LagHipKvCache *c, const LagHipKvRows *r, const int *at, const LagHipRope *rope, const float *qkv,
+                       int64_t ld, const float *q_norm, const float *k_norm, float eps, int Hq, float *q_out, int S) {
     SwKv kv;
     SwRows rows;
     if (const char *why = kv_of(c, kv)) return refuse(me, why);
@@ -1014,9 +1012,21 @@ extern "C" int lag_hip_qk_rope_append(const LagHipKvCache *c, const LagHipKvRows
         return refuse(me, "qkv and q_out overlap");
     const SwRope ro = {dims ? rope->freq : nullptr, dims / 2, dims ? rope->interleaved != 0 : 0, dims ? rope->factor : 1.f};
     if (not_ready(me)) return -1;
-    PROF("qk_rope_append");
-    if (sw_launch_qk_rope_append(g_st, kv, rows, ro, qkv, ld, q_norm, k_norm, eps, Hq, q_out, S)) return fail_msg("qk_rope_append launch");
+    PROF(me);
+    if (sw_launch_qk_rope_append(g_st, kv, rows, at, ro, qkv, ld, q_norm, k_norm, eps, Hq, q_out, S)) return refuse(me, "launch");
     return 0;
+}
+extern "C" int lag_hip_qk_rope_append(const LagHipKvCache *c, const LagHipKvRows *r, const LagHipRope *rope, const float *qkv,
+                                      int64_t ld, const float *q_norm, const float *k_norm, float eps, int Hq, float *q_out,
+                                      int S) {
+    return rope_append("qk_rope_append", c, r, nullptr, rope, qkv, ld, q_norm, k_norm, eps, Hq, q_out, S);
+}
+extern "C" int lag_hip_qk_rope_append_at(const LagHipKvCache *c, const LagHipKvRows *r, const int *at, const LagHipRope *rope,
+                                         const float *qkv, int64_t ld, const float *q_norm, const float *k_norm, float eps, int Hq,
+                                         float *q_out, int S) {
+    static const char *me = "qk_rope_append_at";
+    if (!at) return refuse(me, "no positions to turn by");
+    return rope_append(me, c, r, at, rope, qkv, ld, q_norm, k_norm, eps, Hq, q_out, S);
 }
 
 extern "C" int lag_hip_attn_paged(const LagHipKvCache *c, const LagHipKvRows *r, const float *q, int Hq, float scale,
@@ -1042,19 +1052,80 @@ extern "C" int lag_hip_attn_paged(const LagHipKvCache *c, const LagHipKvRows *r,
     return 0;
 }
 
-extern "C" int lag_hip_kv_copy_pages(const LagHipKvCache *layers, int n_layers, const int *src, const int *dst, int n) {
-    static const char *me = "kv_copy_pages";
-    if (!layers || n_layers < 1 || n < 0 || (n && (!src || !dst))) return refuse(me, "no layers or pages");
-    SwKv kv[SW_COPY_LAYERS];
+static const char *trees_of(const LagHipTrees *t, int page_size, int S, bool reads, SwTrees &o) {
+    if (!t || !t->first || !t->base || !t->table) return "no rows, bases or page table";
+    if (reads && !t->sees) return "no nodes to attend to";
+    if (S < 1 || t->n_trees < 1 || t->n_trees > 65535 || t->n_seqs < 1 || t->max_pages < 1) return "row, tree, sequence or page count";
+    if (t->max_nodes < 1 || t->max_nodes > 64) return "max_nodes (1 to 64)";
+    if (!t->seq && t->n_trees > t->n_seqs) return "more trees than sequences";
+    if ((int64_t)t->max_pages * page_size > (1 << 30)) return "max_pages * page_size over 2^30";
+    o = {t->first, t->base, t->seq, t->pos, t->table, t->sees, t->n_trees, t->n_seqs, t->max_pages, t->max_nodes};
+    return nullptr;
+}
+extern "C" int lag_hip_attn_tree(const LagHipKvCache *c, const LagHipTrees *t, const float *q, int Hq, float scale, int window, float *out,
+                                 int S) {
+    static const char *me = "attn_tree";
+    SwKv kv;
+    SwTrees trees;
+    if (const char *why = kv_of(c, kv)) return refuse(me, why);
+    if (const char *why = trees_of(t, c->page_size, S, true, trees)) return refuse(me, why);
+    if (!q || !out || ((uintptr_t)q | (uintptr_t)out) % 16) return refuse(me, "q and out must be 16-byte aligned");
+    if (Hq < 1 || Hq > 1024 || Hq % c->n_heads) return refuse(me, "n_q_heads (a multiple of n_heads)");
+    if (window < 0) return refuse(me, "negative window");
+    if (window > 0 && !t->pos) return refuse(me, "a window needs the rows' positions");
+    const size_t n = (size_t)S * Hq * c->head_dim * 4;
+    if (!apart(q, n, out, n)) return refuse(me, "q and out overlap");
+    if (not_ready(me)) return -1;
+    const int64_t np = sw_attn_tree_part_floats(kv, trees, Hq);
+    if (np && take_arena((size_t)np * 4)) return -1;
+    PROF("attn_tree");
+    if (sw_launch_attn_tree(g_st, kv, trees, q, Hq, scale, window, out, S, np ? (float *)g_arena.p : nullptr)) return fail_msg("attn_tree launch");
+    return 0;
+}
+static const char *layers_of(const LagHipKvCache *layers, int n_layers) {
+    SwKv one;
     for (int l = 0; l < n_layers; l++) {
-        SwKv one;
-        if (const char *why = kv_of(layers + l, one)) return refuse(me, why);
+        if (const char *why = kv_of(layers + l, one)) return why;
         const LagHipKvCache &a = layers[0], &b = layers[l];
         if (a.type != b.type || a.n_pages != b.n_pages || a.page_size != b.page_size || a.n_heads != b.n_heads ||
             a.head_dim != b.head_dim || a.page_stride != b.page_stride || a.head_stride != b.head_stride ||
             a.token_stride != b.token_stride)
-            return refuse(me, "layers of different geometry");
+            return "layers of different geometry";
     }
+    return nullptr;
+}
+extern "C" int lag_hip_tree_commit(const LagHipKvCache *layers, int n_layers, const LagHipTrees *t, const int *parent, const int *draft,
+                                   const int *tok, int *path, int *count, int *next, int S) {
+    static const char *me = "tree_commit";
+    SwTrees trees;
+    if (!layers || n_layers < 1) return refuse(me, "no layers");
+    if (const char *why = layers_of(layers, n_layers)) return refuse(me, why);
+    if (const char *why = trees_of(t, layers->page_size, S, false, trees)) return refuse(me, why);
+    if (!parent || !draft || !tok) return refuse(me, "no parents, drafted tokens or picks");
+    if (!path || !count || !next) return refuse(me, "no place for the paths, their lengths or the next tokens");
+    const struct { const int *p; size_t n; } reads[] = {{parent, (size_t)S}, {draft, (size_t)S}, {tok, (size_t)S},
+                                                        {t->first, (size_t)t->n_trees + 1}, {t->base, (size_t)t->n_trees}},
+        writes[] = {{path, (size_t)t->n_trees * t->max_nodes}, {count, (size_t)t->n_trees}, {next, (size_t)t->n_trees}};
+    for (auto &w : writes) {
+        for (auto &r : reads) if (!apart(w.p, w.n * 4, r.p, r.n * 4)) return refuse(me, "results that overlap what is read");
+        for (auto &v : writes) if (&v != &w && !apart(w.p, w.n * 4, v.p, v.n * 4)) return refuse(me, "results that overlap");
+    }
+    if (not_ready(me)) return -1;
+    PROF("tree_commit");
+    SwKv kv[SW_COPY_LAYERS];
+    for (int l = 0; l < n_layers; l += SW_COPY_LAYERS) {
+        const int nl = n_layers - l < SW_COPY_LAYERS ? n_layers - l : SW_COPY_LAYERS;
+        for (int i = 0; i < nl; i++) (void)kv_of(layers + l + i, kv[i]);
+        if (sw_launch_tree_commit(g_st, kv, nl, trees, parent, draft, tok, path, count, next, S)) return fail_msg("tree_commit launch");
+    }
+    return 0;
+}
+
+extern "C" int lag_hip_kv_copy_pages(const LagHipKvCache *layers, int n_layers, const int *src, const int *dst, int n) {
+    static const char *me = "kv_copy_pages";
+    if (!layers || n_layers < 1 || n < 0 || (n && (!src || !dst))) return refuse(me, "no layers or pages");
+    SwKv kv[SW_COPY_LAYERS];
+    if (const char *why = layers_of(layers, n_layers)) return refuse(me, why);
     if (n > layers[0].n_pages) return refuse(me, "a destination named twice, or also a source");
     // each page: 1 a source, 2 a destination
     unsigned char *mark = (unsigned char *)calloc((size_t)layers[0].n_pages, 1);

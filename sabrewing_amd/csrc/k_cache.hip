@@ -18,13 +18,14 @@ __device__ __forceinline__ void rp_angle(double freq, int pos, float factor, flo
 // on 16 bytes: a wave a head, a lane the pairs lane and lane + 64.  Each head takes its angles again: 2048 rows of 32 + 2 x
 // 8 heads of 128 take 34 to 35 us (18.5 in the other form), one row and 48 what a launch takes.
 template <int TYPE>
-__global__ __launch_bounds__(RP_NT) void k_qk_rope_any(SwKv c, SwRows r, SwRope rope, const float *__restrict__ qkv, int64_t ld,
-                                                          const float *__restrict__ wq, const float *__restrict__ wk, float eps,
+__global__ __launch_bounds__(RP_NT) void k_qk_rope_any(SwKv c, SwRows r, const int *__restrict__ turn_at, SwRope rope,
+                                                          const float *__restrict__ qkv, int64_t ld, const float *__restrict__ wq, const float *__restrict__ wk, float eps,
                                                           int Hq, float *__restrict__ q_out) {
     const int lane = threadIdx.x & 63, s = blockIdx.x;
     const int H = Hq + 2 * c.Hkv, h = blockIdx.y * (RP_NT / 64) + (threadIdx.x >> 6);
     const int pos = r.pos[s];
     if (pos < 0 || h >= H) return;
+    const int turn = turn_at ? turn_at[s] : pos;
     const int page = sw_page(c, r, r.seq ? r.seq[s] : s, pos);
     const int64_t cell = (int64_t)page * c.ps + (int64_t)(pos & ((1 << c.psh) - 1)) * c.ts;
     float cs[2], sn[2];
@@ -32,7 +33,7 @@ __global__ __launch_bounds__(RP_NT) void k_qk_rope_any(SwKv c, SwRows r, SwRope 
     for (int j = 0; j < 2; j++) {
         const int i = lane + 64 * j;
         cs[j] = 1.f; sn[j] = 0.f;
-        if (i < rope.np) rp_angle(rope.freq[i], pos, rope.factor, cs[j], sn[j]);
+        if (i < rope.np) rp_angle(rope.freq[i], turn, rope.factor, cs[j], sn[j]);
     }
     const float *x = qkv + (int64_t)s * ld;
     const bool is_v = h >= Hq + c.Hkv;
@@ -112,14 +113,15 @@ __device__ __forceinline__ float rp_sum(float x, int lanes) {
 // of 128 (92 MB) take 18.5 us (5.0 TB/s; 37.9 us by single values), 48 rows and one row what a launch takes,
 // 4.5 us.
 template <int TYPE, int PB>
-__global__ __launch_bounds__(RP_NT) void k_qk_rope(SwKv c, SwRows r, SwRope rope, const float *__restrict__ qkv, int64_t ld,
-                                                   const float *__restrict__ wq, const float *__restrict__ wk, float eps, int Hq,
+__global__ __launch_bounds__(RP_NT) void k_qk_rope(SwKv c, SwRows r, const int *__restrict__ turn_at, SwRope rope,
+                                                   const float *__restrict__ qkv, int64_t ld, const float *__restrict__ wq, const float *__restrict__ wk, float eps, int Hq,
                                                    float *__restrict__ q_out, int lanes) {
     __shared__ __align__(16) float s_cs[128], s_sn[128];
     const int tid = threadIdx.x, s = blockIdx.x, H = Hq + 2 * c.Hkv, per = RP_NT / lanes;      // heads a round
     const int u = tid & (lanes - 1), h0 = blockIdx.y * PB * per + tid / lanes;
     const int pos = r.pos[s];
     if (pos < 0) return;
+    const int turn = turn_at ? turn_at[s] : pos;
     // this lane's places in a turned head: ia .. ia + 3 and ib .. ib + 3
     const bool turned = 4 * u < rope.np, halves = turned && !rope.interleaved;
     const int ia = halves ? 4 * u : 8 * u, ib = halves ? rope.np + 4 * u : 8 * u + 4;
@@ -137,7 +139,7 @@ __global__ __launch_bounds__(RP_NT) void k_qk_rope(SwKv c, SwRows r, SwRope rope
         }
     }
     const int page = sw_page(c, r, r.seq ? r.seq[s] : s, pos);
-    if (tid < rope.np) rp_angle(rope.freq[tid], pos, rope.factor, s_cs[tid], s_sn[tid]);
+    if (tid < rope.np) rp_angle(rope.freq[tid], turn, rope.factor, s_cs[tid], s_sn[tid]);
     __syncthreads();
     const sw_f32x4 cs = *(const sw_f32x4 *)(s_cs + 4 * u), sn = *(const sw_f32x4 *)(s_sn + 4 * u);     // (used below np alone)
     const int64_t cell = (int64_t)page * c.ps + (int64_t)(pos & ((1 << c.psh) - 1)) * c.ts;
@@ -197,30 +199,30 @@ __global__ __launch_bounds__(RP_NT) void k_qk_rope(SwKv c, SwRows r, SwRope rope
 }
 
 template <int TYPE>
-static int rp_launch(hipStream_t st, const SwKv &c, const SwRows &r, const SwRope &rope, const float *qkv, int64_t ld, const float *wq,
+static int rp_launch(hipStream_t st, const SwKv &c, const SwRows &r, const int *at, const SwRope &rope, const float *qkv, int64_t ld, const float *wq,
                      const float *wk, float eps, int Hq, float *q_out, int S) {
     const int H = Hq + 2 * c.Hkv;
     if ((!rope.interleaved && rope.np % 4) || (((uintptr_t)wq | (uintptr_t)wk) & 15)) {
-        SW_LAUNCH(k_qk_rope_any<TYPE>, dim3((unsigned)S, (unsigned)((H + 3) / 4)), dim3(RP_NT), 0, st, c, r, rope, qkv, ld, wq, wk, eps, Hq,
+        SW_LAUNCH(k_qk_rope_any<TYPE>, dim3((unsigned)S, (unsigned)((H + 3) / 4)), dim3(RP_NT), 0, st, c, r, at, rope, qkv, ld, wq, wk, eps, Hq,
                   q_out);
     } else {
         const int lanes = c.dh <= 32 ? 4 : c.dh <= 64 ? 8 : c.dh <= 128 ? 16 : 32, rounds = (H * lanes + RP_NT - 1) / RP_NT;
         // four rounds of heads a block where the rows alone fill the chip, else one (an angle is taken by more blocks)
         if ((int64_t)S * ((rounds + 3) / 4) >= 512)
-            SW_LAUNCH((k_qk_rope<TYPE, 4>), dim3((unsigned)S, (unsigned)((rounds + 3) / 4)), dim3(RP_NT), 0, st, c, r, rope, qkv, ld, wq, wk,
+            SW_LAUNCH((k_qk_rope<TYPE, 4>), dim3((unsigned)S, (unsigned)((rounds + 3) / 4)), dim3(RP_NT), 0, st, c, r, at, rope, qkv, ld, wq, wk,
                       eps, Hq, q_out, lanes);
         else
-            SW_LAUNCH((k_qk_rope<TYPE, 1>), dim3((unsigned)S, (unsigned)rounds), dim3(RP_NT), 0, st, c, r, rope, qkv, ld, wq, wk, eps, Hq,
+            SW_LAUNCH((k_qk_rope<TYPE, 1>), dim3((unsigned)S, (unsigned)rounds), dim3(RP_NT), 0, st, c, r, at, rope, qkv, ld, wq, wk, eps, Hq,
                       q_out, lanes);
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
-int sw_launch_qk_rope_append(hipStream_t st, const SwKv &c, const SwRows &r, const SwRope &rope, const float *qkv, int64_t ld,
+int sw_launch_qk_rope_append(hipStream_t st, const SwKv &c, const SwRows &r, const int *at, const SwRope &rope, const float *qkv, int64_t ld,
                              const float *wq, const float *wk, float eps, int Hq, float *q_out, int S) {
-    if (c.type == SW_KV_F32) return rp_launch<SW_KV_F32>(st, c, r, rope, qkv, ld, wq, wk, eps, Hq, q_out, S);
-    if (c.type == SW_KV_BF16) return rp_launch<SW_KV_BF16>(st, c, r, rope, qkv, ld, wq, wk, eps, Hq, q_out, S);
-    return rp_launch<SW_KV_F16>(st, c, r, rope, qkv, ld, wq, wk, eps, Hq, q_out, S);
+    if (c.type == SW_KV_F32) return rp_launch<SW_KV_F32>(st, c, r, at, rope, qkv, ld, wq, wk, eps, Hq, q_out, S);
+    if (c.type == SW_KV_BF16) return rp_launch<SW_KV_BF16>(st, c, r, at, rope, qkv, ld, wq, wk, eps, Hq, q_out, S);
+    return rp_launch<SW_KV_F16>(st, c, r, at, rope, qkv, ld, wq, wk, eps, Hq, q_out, S);
 }
 
 // A page is n2 x n1 runs of `run` 16-byte pieces (one run where its cells lie side by side).
@@ -261,5 +263,78 @@ int sw_launch_kv_copy(hipStream_t st, const SwKv *layers, int n_layers, const in
     for (int i = 0; i < n; i++) { a.src[i] = src[i]; a.dst[i] = dst[i]; }
     SW_LAUNCH(k_kv_copy, dim3((unsigned)((total + KC_NT - 1) / KC_NT), (unsigned)n, (unsigned)(2 * n_layers)), dim3(KC_NT), 0, st, a,
               c.ps / per, n1, s1 / per, s2 / per, (int)(run / per), (int)total);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+// A tree's accepted path and its cells.  The walk takes a ballot a step (a node a lane) and is taken by every wave of every
+// layer's block: nothing to wait for.  A path's nodes rise, so node path[i]'s cell lies at or behind its place i and is
+// nobody's place before i: a thread moves one piece of 16 bytes of all cells in turn, eight reads and then their writes.
+#define TC_NT 256
+struct SwCommit { void *pool[2 * SW_COPY_LAYERS]; };
+__global__ __launch_bounds__(TC_NT) void k_tree_commit(SwCommit a, SwKv c, SwTrees t, const int *__restrict__ parent, const int *__restrict__ draft,
+                                                       const int *__restrict__ tok, int *__restrict__ path, int *__restrict__ count,
+                                                       int *__restrict__ next, int S, int es, int run) {
+    __shared__ int64_t s_src[64], s_dst[64];
+    const int tid = threadIdx.x, lane = tid & 63, i = blockIdx.x;
+    const int row = t.first[i], end = t.first[i + 1], base = t.base[i], seq = t.seq ? t.seq[i] : i;
+    const int n = base < 0 || row < 0 || row >= S || end <= row ? 0 : min(min(end, S) - row, t.max_nodes);
+    const bool node = lane < n;
+    const int p = node ? parent[row + lane] : -2, d = node ? draft[row + lane] : 0, k = node ? tok[row + lane] : 0;
+    int at = 0, len = n ? 1 : 0, mine = -1;
+    if (lane == 0 && n) mine = 0;
+    while (n) {
+        const int pick = __builtin_amdgcn_readlane(k, at);
+        const uint64_t kids = __ballot(lane > at && p == at && d == pick);
+        if (!kids) break;
+        at = __builtin_ctzll(kids);
+        if (lane == len) mine = at;
+        len++;
+    }
+    if (blockIdx.y == 0 && tid < 64) {
+        if (lane < t.max_nodes) path[(int64_t)i * t.max_nodes + lane] = mine;
+        if (lane == 0) {
+            count[i] = len;
+            next[i] = n ? __builtin_amdgcn_readlane(k, at) : -1;
+        }
+    }
+    // the cells that move: their offsets, side by side
+    const SwRows r = {nullptr, nullptr, t.table, t.n_seqs, t.max_pages};
+    const int64_t from = (int64_t)base + mine, to = (int64_t)base + lane;
+    int pf = -1, pt = -1;
+    if (mine > lane && from < (int64_t)t.max_pages << c.psh) { pf = sw_page(c, r, seq, (int)from); pt = sw_page(c, r, seq, (int)to); }
+    const bool moves = pf >= 0 && pt >= 0;
+    const uint64_t all = __ballot(moves);
+    const int cells = __builtin_popcountll(all), pmask = (1 << c.psh) - 1;
+    if (moves && tid < 64) {
+        const int x = __builtin_popcountll(all & ((1ull << lane) - 1));
+        s_src[x] = (pf * c.ps + (from & pmask) * c.ts) * es;
+        s_dst[x] = (pt * c.ps + (to & pmask) * c.ts) * es;
+    }
+    if (!cells) return;
+    __syncthreads();
+    const int pieces = 2 * c.Hkv * run;                                // of 16 bytes: both pools, heads of `run`
+    for (int x = tid; x < pieces; x += TC_NT) {
+        const int v = x >= c.Hkv * run, y = x - v * c.Hkv * run, h = y / run;
+        char *pool = (char *)a.pool[2 * blockIdx.y + v] + h * c.hs * es + (y - h * run) * 16;
+        for (int j0 = 0; j0 < cells; j0 += 8) {
+            sw_u32x4 b[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (j0 + j < cells) b[j] = *(const sw_u32x4 *)(pool + s_src[j0 + j]);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (j0 + j < cells) *(sw_u32x4 *)(pool + s_dst[j0 + j]) = b[j];
+        }
+    }
+}
+
+int sw_launch_tree_commit(hipStream_t st, const SwKv *layers, int n_layers, const SwTrees &t, const int *parent, const int *draft, const int *tok,
+                          int *path, int *count, int *next, int S) {
+    if (n_layers < 1 || n_layers > SW_COPY_LAYERS) return -1;
+    SwCommit a = {};
+    for (int l = 0; l < n_layers; l++) { a.pool[2 * l] = layers[l].k; a.pool[2 * l + 1] = layers[l].v; }
+    const int es = layers[0].type == SW_KV_F32 ? 4 : 2;
+    SW_LAUNCH(k_tree_commit, dim3((unsigned)t.n_trees, (unsigned)n_layers), dim3(TC_NT), 0, st, a, layers[0], t, parent, draft, tok, path, count,
+              next, S, es, layers[0].dh * es / 16);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }

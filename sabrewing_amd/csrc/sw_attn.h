@@ -19,6 +19,13 @@ struct SwRows {
     const int *pos, *seq, *table;
     int n_seqs, max_pages;
 };
+// Trees of drafted tokens: tree i's nodes are rows first[i] .. first[i + 1] - 1, node j in cell base[i] + j of sequence
+// seq[i] (null: i); bit j of sees[s]: row s attends to node j.  pos: the rows' positions, for a window.
+struct SwTrees {
+    const int *first, *base, *seq, *pos, *table;
+    const uint64_t *sees;
+    int n_trees, n_seqs, max_pages, max_nodes;
+};
 
 // the page of token t of sequence q, or -1 where the table or its entry leads nowhere
 __device__ __forceinline__ int sw_page(const SwKv &c, const SwRows &r, int q, int t) {
@@ -84,9 +91,9 @@ __device__ __forceinline__ float sw_sum4(float x) {
 
 // ---- launch wrappers (async on `st`) ----
 // (k_cache.hip) the q and k heads of S projected rows normalised (wq, wk null: not) and
-// turned (np pairs of a head, freq in radians per position), q to q_out, k and v to the cache
+// turned (np pairs of a head, freq in radians per position, by at[s] or, null, pos[s]), q to q_out, k and v to the cache
 struct SwRope { const double *freq; int np, interleaved; float factor; };
-int sw_launch_qk_rope_append(hipStream_t st, const SwKv &c, const SwRows &r, const SwRope &rope, const float *qkv, int64_t ld,
+int sw_launch_qk_rope_append(hipStream_t st, const SwKv &c, const SwRows &r, const int *at, const SwRope &rope, const float *qkv, int64_t ld,
                              const float *wq, const float *wk, float eps, int Hq, float *q_out, int S);
 // pages src[i] to dst[i] of n_layers caches of one geometry (host arrays, n <= SW_COPY_PAIRS,
 // n_layers <= SW_COPY_LAYERS: they travel with the launch)
@@ -99,6 +106,14 @@ int64_t sw_attn_row_chunks(const SwKv &c, const SwRows &r);           // chunks 
 int64_t sw_attn_part_floats(const SwKv &c, const SwRows &r, int Hq, int window, int S);
 int sw_launch_attn(hipStream_t st, const SwKv &c, const SwRows &r, const float *q, int Hq, float scale, int window, float *out,
                    int S, float *part);
+// (k_tree.hip) nodes of trees against their sequences' cells and the nodes they see; part: scratch of
+// sw_attn_tree_part_floats floats (0: none)
+int64_t sw_attn_tree_part_floats(const SwKv &c, const SwTrees &t, int Hq);
+int sw_launch_attn_tree(hipStream_t st, const SwKv &c, const SwTrees &t, const float *q, int Hq, float scale, int window, float *out, int S,
+                        float *part);
+// (k_cache.hip) the accepted path of each tree and its cells moved together in n_layers <= SW_COPY_LAYERS caches
+int sw_launch_tree_commit(hipStream_t st, const SwKv *layers, int n_layers, const SwTrees &t, const int *parent, const int *draft,
+                          const int *tok, int *path, int *count, int *next, int S);
 // (k_sample.hip) a pick of each row of logits; each setting may be null
 struct SwSample { const float *temp; const int *top_k; const float *top_p, *min_p; };
 int sw_launch_sample(hipStream_t st, const float *logits, int S, int V, const SwSample &p, const float *u, int *tok);
