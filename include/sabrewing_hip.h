@@ -305,6 +305,47 @@ int    lag_hip_tree_commit(const LagHipKvCache *layers, int n_layers, const LagH
  * a fork's last page, or pages moved together.  src and dst are host arrays, free to change
  * on return; a dst is named once and is no src.  0 = ok */
 int    lag_hip_kv_copy_pages(const LagHipKvCache *layers, int n_layers, const int *src, const int *dst, int n);
+/* ---- latent attention: a token's keys and values of all heads come from one vector ----
+ * k_t[h] = (Wk[h] c_t, r_t) and v_t[h] = Wv[h] c_t, c_t a latent of `rank` values, r_t a rotary part of `rope_dims` that the
+ * heads share.  The cache holds (c_t, r_t) alone.  Two forms of one attention: absorbed, for single new tokens (queries go
+ * into the latent space, Wk[h]^T q, outputs come back from it, Wv[h] o: lag_hip_latent_heads before and after
+ * lag_hip_attn_latent), and expanded, for a prompt (lag_hip_attn_latent_prompt).  No counterpart in the reference's lag table; the
+ * GLM engine's attention slots (include/sabrewing_coli.h) are other entries.
+ *
+ * One layer's cache: n_pages pages of page_size tokens (a power of two, 8 to 4096), a cell's rank + rope_dims values side
+ * by side at c + page * page_stride + slot * token_stride (elements; strides and c multiples of 16 bytes, cells do not overlap).
+ * type: LAG_HIP_KV_BF16 or LAG_HIP_KV_F16.  rank: 128, 256, 384 or 512; rope_dims: a multiple of 16 up to 64, or 0. */
+typedef struct {
+    void   *c;
+    int     type, n_pages, page_size, rank, rope_dims;
+    int64_t page_stride, token_stride;
+} LagHipLatentCache;
+/* Heads of rows: the values of row s's head h begin at element s * row_stride + h * head_stride of p. */
+typedef struct {
+    void   *p;
+    int64_t row_stride, head_stride;
+} LagHipHeads;
+/* S rows (positions and tables as for the paged cache).  ckv [S][ld_c]: rank values, normalised (c / sqrt(mean(c^2) + eps) * norm;
+ * norm NULL: not), and rope_dims values, turned (rope NULL: not; its dims rope_dims), both rounded to nearest into the row's
+ * cell.  q [S][ld_q]: n_heads heads of `nope` values and a rotary part of rope_dims, rounded to the cache's type: the first to q_nope, the
+ * second, turned, to q_rope (for the absorbed form behind the rank values of each head, for the expanded one behind the
+ * nope values of the same head).  nope: a multiple of 16 up to 256 or, with n_heads 0 and q NULL, unused.  ckv, q and what is written
+ * are 16-byte aligned, strides of inputs multiples of 4 elements, of outputs of 8.  A free place leaves everything as it was, a position without a
+ * cell the cache.  0 = ok */
+int    lag_hip_latent_append(const LagHipLatentCache *c, const LagHipKvRows *r, const LagHipRope *rope, const float *ckv, int64_t ld_c,
+                             const float *norm, float eps, const float *q, int64_t ld_q, int n_heads, int nope, const LagHipHeads *q_nope,
+                             const LagHipHeads *q_rope, int S);
+/* y[s][h] = W[h] x[s][h] for S rows of n_heads heads: x of n_in values and W [n_heads][n_out][n_in] in `type` (BF16 or
+ * F16), sums in 32 bits, y of n_out values in f32 (y_f32) or rounded to the type.  n_in and n_out are multiples of 32 up to 1024.  A
+ * head_stride of 0 gives every head the same x.  Pointers are 16-byte aligned, strides multiples of 8 elements; x and y do not overlap.
+ * 0 = ok */
+int    lag_hip_latent_heads(int type, const LagHipHeads *x, const void *W, int n_heads, int n_in, int n_out, const LagHipHeads *y, int y_f32,
+                            int S);
+/* out[s][h] = sum_t p_t c_t, p the softmax of scale * q[s][h] . (c_t, r_t) over the cells t <= pos[s]: q [S][n_heads][rank +
+ * rope_dims] and out [S][n_heads][rank] in the cache's type, 16-byte aligned, not overlapping.  Sums and the softmax in 32 bits, its weights
+ * rounded to the cache's type before the second product, the output once.  Free places, rows without a cell, cells that are no numbers,
+ * repeated calls and scratch as for lag_hip_attn_paged.  n_heads up to 1024.  0 = ok */
+int    lag_hip_attn_latent(const LagHipLatentCache *c, const LagHipKvRows *r, const void *q, int n_heads, float scale, void *out, int S);
 /* x[i] += t[i] for n values: the residual after an output projection.  t may be x, or does
  * not overlap it.  0 = ok */
 int    lag_hip_add(float *x, const float *t, size_t n);

@@ -32,6 +32,7 @@ EXPORTS = [
     "lag_hip_last_groups", "lag_hip_rmsnorm", "lag_hip_moe_forward_rmsnorm", "lag_hip_head_argmax", "lag_hip_argmax", "lag_hip_set_grouped_kernel",
     "lag_hip_qk_rope_append", "lag_hip_attn_paged", "lag_hip_kv_copy_pages", "lag_hip_add", "lag_hip_sample",
     "lag_hip_attn_tree", "lag_hip_qk_rope_append_at", "lag_hip_tree_commit",
+    "lag_hip_latent_append", "lag_hip_latent_heads", "lag_hip_attn_latent",
     "lag_hip_set_q4_mode",
     "lag_hip_alloc", "lag_hip_h2d", "lag_hip_d2h", "lag_hip_d2d", "lag_hip_memset",
     "lag_hip_graph_begin", "lag_hip_graph_end", "lag_hip_graph_launch", "lag_hip_graph_destroy", "lag_hip_sync",
@@ -80,6 +81,15 @@ class LagHipKvRows(C.Structure):
 class LagHipTrees(C.Structure):
     _fields_ = [("first", VP), ("base", VP), ("seq", VP), ("pos", VP), ("table", VP), ("sees", VP), ("n_trees", C.c_int),
                 ("n_seqs", C.c_int), ("max_pages", C.c_int), ("max_nodes", C.c_int)]
+
+
+class LagHipLatentCache(C.Structure):
+    _fields_ = [("c", VP), ("type", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int), ("rank", C.c_int), ("rope_dims", C.c_int),
+                ("page_stride", C.c_int64), ("token_stride", C.c_int64)]
+
+
+class LagHipHeads(C.Structure):
+    _fields_ = [("p", VP), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
 
 
 class LagHipRope(C.Structure):
@@ -147,6 +157,11 @@ def load_library(path=None):
     L.lag_hip_attn_tree.argtypes = [KP, TP, VP, C.c_int, C.c_float, C.c_int, VP, C.c_int]
     L.lag_hip_qk_rope_append_at.argtypes = [KP, RP, VP, C.POINTER(LagHipRope), VP, C.c_int64, VP, VP, C.c_float, C.c_int, VP, C.c_int]
     L.lag_hip_tree_commit.argtypes = [KP, C.c_int, TP, VP, VP, VP, VP, VP, VP, C.c_int]
+    LP, HP = C.POINTER(LagHipLatentCache), C.POINTER(LagHipHeads)
+    L.lag_hip_latent_append.argtypes = [LP, RP, C.POINTER(LagHipRope), VP, C.c_int64, VP, C.c_float, VP, C.c_int64, C.c_int, C.c_int, HP, HP,
+                                        C.c_int]
+    L.lag_hip_latent_heads.argtypes = [C.c_int, HP, VP, C.c_int, C.c_int, C.c_int, HP, C.c_int, C.c_int]
+    L.lag_hip_attn_latent.argtypes = [LP, RP, VP, C.c_int, C.c_float, VP, C.c_int]
     L.lag_hip_kv_copy_pages.argtypes = [KP, C.c_int, VP, VP, C.c_int]
     L.lag_hip_add.argtypes = [VP, VP, C.c_size_t]
     L.lag_hip_sample.argtypes = [VP, C.c_int, C.c_int, C.POINTER(LagHipSample), VP, VP]
@@ -362,6 +377,17 @@ class Backend:
                            max_pages, max_nodes)
 
     @staticmethod
+    def latent_cache(c, type, n_pages, page_size, rank, rope_dims, strides=None):
+        """one layer's cache of latents; strides: (page, token) in elements, default [page][token][value]"""
+        ps, ts = strides or (page_size * (rank + rope_dims), rank + rope_dims)
+        return LagHipLatentCache(int(c), KV_TYPES[type], n_pages, page_size, rank, rope_dims, ps, ts)
+
+    @staticmethod
+    def heads(p, row_stride, head_stride):
+        """rows of heads: row s's head h begins at element s * row_stride + h * head_stride"""
+        return LagHipHeads(int(p), row_stride, head_stride)
+
+    @staticmethod
     def rope(freq_dev, dims, interleaved=False, factor=1.0):
         return LagHipRope(_ptr(freq_dev), dims, int(interleaved), factor)
 
@@ -394,6 +420,21 @@ class Backend:
         kv_caches)"""
         self.check(self.lib.lag_hip_tree_commit(caches, len(caches), trees, int(parent_dev), int(draft_dev), int(tok_dev), int(path_dev),
                                                 int(count_dev), int(next_dev), S), "lag_hip_tree_commit")
+
+    # latent attention: latent_append, then latent_heads (into the latent space), attn_latent, latent_heads (out of it), or
+    # attn_latent_prompt
+    def latent_append(self, cache, rows, rope, ckv_dev, ld_c, norm, eps, q_dev, ld_q, n_heads, nope, q_nope, q_rope, S):
+        """new tokens' latents normalised, rotary parts turned, into the rows' cells; query heads (Backend.heads) in the cache's type"""
+        self.check(self.lib.lag_hip_latent_append(cache, rows, rope, int(ckv_dev), ld_c, _ptr(norm), eps, _ptr(q_dev), ld_q, n_heads, nope,
+                                                  q_nope, q_rope, S), "lag_hip_latent_append")
+
+    def latent_heads(self, type, x, W_dev, n_heads, n_in, n_out, y, y_f32, S):
+        """y[s, h] = W[h] x[s, h] (x, y: Backend.heads; type: of x, W and, unless y_f32, y)"""
+        self.check(self.lib.lag_hip_latent_heads(KV_TYPES[type], x, int(W_dev), n_heads, n_in, n_out, y, int(y_f32), S), "lag_hip_latent_heads")
+
+    def attn_latent(self, cache, rows, q_dev, n_heads, scale, out_dev, S):
+        """one new token of each row against its sequence's latents, queries [S, n_heads, rank + rope_dims]"""
+        self.check(self.lib.lag_hip_attn_latent(cache, rows, int(q_dev), n_heads, scale, int(out_dev), S), "lag_hip_attn_latent")
 
     def kv_copy_pages(self, caches, src, dst):
         """pages src[i] -> dst[i] of every layer (caches from kv_caches; host indices)"""

@@ -1153,6 +1153,124 @@ extern "C" int lag_hip_kv_copy_pages(const LagHipKvCache *layers, int n_layers, 
     return 0;
 }
 
+// ---- latent attention ----
+static const char *latent_of(const LagHipLatentCache *c, SwLatent &o) {
+    if (!c || !c->c) return "no pool";
+    if (c->type != LAG_HIP_KV_BF16 && c->type != LAG_HIP_KV_F16) return "element type (bf16 or f16)";
+    if (c->n_pages < 1) return "page count";
+    if (c->page_size < 8 || c->page_size > 4096 || (c->page_size & (c->page_size - 1))) return "page_size (a power of two, 8 to 4096)";
+    if (c->rank < 128 || c->rank > 512 || c->rank % 128) return "rank (128, 256, 384 or 512)";
+    if (c->rope_dims < 0 || c->rope_dims > 64 || c->rope_dims % 16) return "rope_dims (a multiple of 16, at most 64)";
+    if ((uintptr_t)c->c % 16 || c->page_stride % 8 || c->token_stride % 8) return "pool and strides must be multiples of 16 bytes";
+    const int64_t cell = c->rank + c->rope_dims, most = (int64_t)1 << 60;
+    const bool tokens_first = c->token_stride <= c->page_stride;        // (pages apart, or the tokens of all pages interleaved)
+    const int64_t s0 = tokens_first ? c->token_stride : c->page_stride, n0 = tokens_first ? c->page_size : c->n_pages,
+                  s1 = tokens_first ? c->page_stride : c->token_stride, n1 = tokens_first ? c->n_pages : c->page_size;
+    int64_t extent = cell;
+    if (n0 > 1) {
+        if (s0 < extent || s0 > most / n0) return "strides that overlap";
+        extent += s0 * (n0 - 1);
+    }
+    if (n1 > 1 && (s1 < extent || s1 > most / n1)) return "strides that overlap";
+    o = {c->c, c->type, c->n_pages, __builtin_ctz((unsigned)c->page_size), c->rank, c->rope_dims, c->page_stride, c->token_stride};
+    return nullptr;
+}
+// rows of heads as the kernels take them, and the elements from p to their end
+static const char *heads_of(const LagHipHeads *h, int n_heads, int n, int S, SwHeads &o, size_t &extent) {
+    if (!h || !h->p) return "no heads";
+    if ((uintptr_t)h->p % 16 || h->row_stride % 8 || h->head_stride % 8) return "heads must begin on 16 bytes";
+    if (h->row_stride < 0 || h->head_stride < 0 || h->row_stride > (int64_t)1 << 40 || h->head_stride > (int64_t)1 << 40) return "strides of heads";
+    o = {h->p, h->row_stride, h->head_stride};
+    extent = (size_t)(S - 1) * h->row_stride + (size_t)(n_heads - 1) * h->head_stride + n;
+    return nullptr;
+}
+// written heads lie side by side or apart
+static bool heads_apart(const SwHeads &h, int n_heads, int n, int S) {
+    if (h.hs <= h.rs || S == 1) return (n_heads == 1 || h.hs >= n) && (S == 1 || h.rs >= (int64_t)(n_heads - 1) * h.hs + n);
+    return h.rs >= n && (n_heads == 1 || h.hs >= (int64_t)(S - 1) * h.rs + n);
+}
+// two sets of heads that share memory do so as parts of the same heads: same strides, and parts that do not meet
+static bool parts_of_heads(const SwHeads &a, int na, size_t ea, const SwHeads &b, int nb, size_t eb, int n_heads, int S) {
+    if (apart(a.p, ea * 2, b.p, eb * 2)) return true;
+    if ((S > 1 && a.rs != b.rs) || (n_heads > 1 && a.hs != b.hs)) return false;
+    const bool first = (uintptr_t)a.p < (uintptr_t)b.p;
+    const int64_t d = (int64_t)((uintptr_t)(first ? b.p : a.p) - (uintptr_t)(first ? a.p : b.p)) / 2;
+    const SwHeads both = {first ? a.p : b.p, a.rs, a.hs};
+    return d >= (first ? na : nb) && d < (int64_t)1 << 30 && heads_apart(both, n_heads, (int)d + (first ? nb : na), S);
+}
+extern "C" int lag_hip_latent_append(const LagHipLatentCache *c, const LagHipKvRows *r, const LagHipRope *rope, const float *ckv, int64_t ld_c,
+                                     const float *norm, float eps, const float *q, int64_t ld_q, int n_heads, int nope, const LagHipHeads *q_nope,
+                                     const LagHipHeads *q_rope, int S) {
+    static const char *me = "latent_append";
+    SwLatent lc;
+    SwRows rows;
+    if (const char *why = latent_of(c, lc)) return refuse(me, why);
+    if (const char *why = rows_of(r, c->page_size, S, rows)) return refuse(me, why);
+    if (!ckv || (uintptr_t)ckv % 16 || ld_c % 4) return refuse(me, "ckv must be 16-byte aligned rows");
+    if (ld_c < c->rank + c->rope_dims || ld_c > (int64_t)1 << 31) return refuse(me, "ld_c shorter than a row");
+    if (rope && (rope->dims != c->rope_dims || (rope->dims && !rope->freq))) return refuse(me, "rope dims (the cache's rope_dims)");
+    if (n_heads < 0 || n_heads > 1024) return refuse(me, "n_heads");
+    SwHeads hn = {}, hr = {};
+    if (n_heads) {
+        size_t en = 0, er = 0;
+        if (nope < 16 || nope > 256 || nope % 16) return refuse(me, "nope (a multiple of 16, at most 256)");
+        if (!q || (uintptr_t)q % 16 || ld_q % 4) return refuse(me, "q must be 16-byte aligned rows");
+        if (ld_q < (int64_t)n_heads * (nope + c->rope_dims) || ld_q > (int64_t)1 << 31) return refuse(me, "ld_q shorter than a row");
+        if (const char *why = heads_of(q_nope, n_heads, nope, S, hn, en)) return refuse(me, why);
+        if (!heads_apart(hn, n_heads, nope, S)) return refuse(me, "heads that overlap");
+        if (c->rope_dims) {
+            if (const char *why = heads_of(q_rope, n_heads, c->rope_dims, S, hr, er)) return refuse(me, why);
+            if (!heads_apart(hr, n_heads, c->rope_dims, S) || !parts_of_heads(hn, nope, en, hr, c->rope_dims, er, n_heads, S))
+                return refuse(me, "heads that overlap");
+        }
+        const size_t nc = ((size_t)(S - 1) * ld_c + c->rank + c->rope_dims) * 4, nq = ((size_t)(S - 1) * ld_q + (size_t)n_heads * (nope + c->rope_dims)) * 4;
+        if (!apart(hn.p, en * 2, ckv, nc) || !apart(hn.p, en * 2, q, nq) ||
+            (c->rope_dims && (!apart(hr.p, er * 2, ckv, nc) || !apart(hr.p, er * 2, q, nq))))
+            return refuse(me, "results that overlap what is read");
+    }
+    const SwRope ro = {rope && rope->dims ? rope->freq : nullptr, rope ? rope->dims / 2 : 0, rope ? rope->interleaved != 0 : 0, rope ? rope->factor : 1.f};
+    if (not_ready(me)) return -1;
+    PROF("latent_append");
+    if (sw_launch_latent_append(g_st, lc, rows, ro, ckv, ld_c, norm, eps, q, ld_q, n_heads, n_heads ? nope : 16, hn, hr, S)) return fail_msg("latent_append launch");
+    return 0;
+}
+extern "C" int lag_hip_latent_heads(int type, const LagHipHeads *x, const void *W, int n_heads, int n_in, int n_out, const LagHipHeads *y, int y_f32,
+                                    int S) {
+    static const char *me = "latent_heads";
+    SwHeads hx, hy;
+    size_t ex, ey;
+    if (type != LAG_HIP_KV_BF16 && type != LAG_HIP_KV_F16) return refuse(me, "element type (bf16 or f16)");
+    if (S < 1 || n_heads < 1 || n_heads > 1024) return refuse(me, "row or head count");
+    if (n_in < 32 || n_in > 1024 || n_in % 32 || n_out < 32 || n_out > 1024 || n_out % 32) return refuse(me, "n_in and n_out (multiples of 32, at most 1024)");
+    if (!W || (uintptr_t)W % 16) return refuse(me, "W must be 16-byte aligned");
+    if (const char *why = heads_of(x, n_heads, n_in, S, hx, ex)) return refuse(me, why);
+    if (const char *why = heads_of(y, n_heads, n_out, S, hy, ey)) return refuse(me, why);
+    if (!heads_apart(hy, n_heads, n_out, S)) return refuse(me, "heads that overlap");
+    if (!apart(hx.p, ex * 2, hy.p, ey * (y_f32 ? 4 : 2)) || !apart(hy.p, ey * (y_f32 ? 4 : 2), W, (size_t)n_heads * n_in * n_out * 2))
+        return refuse(me, "results that overlap what is read");
+    if (not_ready(me)) return -1;
+    PROF("latent_heads");
+    if (sw_launch_latent_heads(g_st, type, hx, W, n_heads, n_in, n_out, hy, y_f32, S)) return fail_msg("latent_heads launch");
+    return 0;
+}
+extern "C" int lag_hip_attn_latent(const LagHipLatentCache *c, const LagHipKvRows *r, const void *q, int n_heads, float scale, void *out, int S) {
+    static const char *me = "attn_latent";
+    SwLatent lc;
+    SwRows rows;
+    if (const char *why = latent_of(c, lc)) return refuse(me, why);
+    if (const char *why = rows_of(r, c->page_size, S, rows)) return refuse(me, why);
+    if (!q || !out || ((uintptr_t)q | (uintptr_t)out) % 16) return refuse(me, "q and out must be 16-byte aligned");
+    if (n_heads < 1 || n_heads > 1024) return refuse(me, "n_heads (1 to 1024)");
+    if ((int64_t)S * n_heads >= (int64_t)1 << 31) return refuse(me, "row or head count");
+    if (!apart(q, (size_t)S * n_heads * (c->rank + c->rope_dims) * 2, out, (size_t)S * n_heads * c->rank * 2)) return refuse(me, "q and out overlap");
+    if (not_ready(me)) return -1;
+    const int64_t np = sw_latent_part_floats(lc, rows, n_heads, S);
+    if (np && take_arena((size_t)np * 4)) return -1;
+    PROF("attn_latent");
+    if (sw_launch_latent(g_st, lc, rows, q, n_heads, scale, out, S, np ? (float *)g_arena.p : nullptr)) return fail_msg("attn_latent launch");
+    return 0;
+}
+
 extern "C" int lag_hip_add(float *x, const float *t, size_t n) {
     static const char *me = "add";
     if (!x || !t || !n) return refuse(me, "no values");

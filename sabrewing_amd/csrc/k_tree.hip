@@ -41,10 +41,12 @@ __global__ __launch_bounds__(FL_NT, (tr_occ<TYPE, DH>())) void k_tree(SwKv c, Sw
     using F = TrFl<TYPE, DH>;
     constexpr int CW = 32 * WC, NS = tr_ns<TYPE, DH, WC>(), WT = FL_NW / WC, ES = F::ES;
     constexpr int LK = (F::NCK / 2 + WC - 1) / WC, LV = (F::NCV / 2 + WC - 1) / WC;                    // loads of a wave
-    constexpr int SHT = WT * NS * F::TB, SHB = SHT > fl_end_bytes<F, DH>() ? SHT : fl_end_bytes<F, DH>();
+    constexpr int SHT = WT * NS * F::TB, SHB = SHT > fl_end_bytes<F, FL_NW>() ? SHT : fl_end_bytes<F, FL_NW>();
     static_assert(SHB <= 158 * 1024 && (NS < 3 ? 0 : NS - 2) * (LK + LV) < 64, "LDS, and loads that a wave can count");
     __shared__ __align__(16) char sh[SHB];
     __shared__ float s_m[FL_NW][32], s_l[FL_NW][32];
+    __shared__ uint32_t s_bad[2 * FL_NW];
+    __shared__ int s_lo;
     const int tid = threadIdx.x, lane = tid & 63, wave = fl_uni(tid >> 6), wc = wave % WC, cl = lane & 31, h = lane >> 5;
     const int G = Hq / c.Hkv, ncg = (t.max_nodes * G + CW - 1) / CW, per = c.Hkv * ncg;
     const int hg = blockIdx.x % per, b = blockIdx.x / per, hk = hg / ncg, c0 = hg % ncg * CW;
@@ -142,19 +144,26 @@ __global__ __launch_bounds__(FL_NT, (tr_occ<TYPE, DH>())) void k_tree(SwKv c, Sw
             from_pool(vp, F::NCV, F::MV == 7, LV, lds + 32 * F::RBK);
             return g.ok;
         };
-        auto whole = [&](int tile) {                                   // (the lanes' windows begin at different cells)
-            return tile * 32 + 31 < x.base && (window == 0 || __all(!mine || lo <= tile * 32));
-        };
+        int lo_all = 0;                                                // the last cell at which a column's window begins
+        if (window > 0) {
+            __syncthreads();
+            if (tid == 0) s_lo = 0;
+            __syncthreads();
+            if (mine) atomicMax(&s_lo, lo);
+            __syncthreads();
+            lo_all = fl_uni(s_lo);
+        }
+        auto whole = [&](int tile) { return tile * 32 + 31 < x.base && tile * 32 >= lo_all; };
         auto seen = [&](int tile, int k) {
             const int tok = tile * 32 + k, j = tok - x.base;
             const int pg = tok >> c.psh;
             const int page = pg < t.max_pages ? table[pg] : -1;
             return tok <= x.last && page >= 0 && page < c.n_pages && (j < 0 ? tok >= lo : j < x.n && ((sees >> j) & 1));
         };
-        fl_run<WC, NS, LK + LV>(f, sh, ta, ta + len, wave, columns, issue, whole, seen);
+        fl_run<WC, WT, 1, NS, LK + LV>(f, sh, nullptr, s_bad, ta, ta + len, wave, columns, issue, whole, seen);
         const bool all = len == tiles;
         float *pp = all ? nullptr : part + ((int64_t)hg * (B + t.n_trees) + b + i) * CW * (DH + 4);
-        fl_end<WC, F, DH>(f, sh, s_m, s_l, wave, [&](int col, int d, sw_f32x4 a, float mx, float sum) {
+        fl_end<WC, WT, 1>(f, sh, s_m, s_l, wave, [&](int col, int d, sw_f32x4 a, float mx, float sum) {
             const int ck = c0 + col;
             if (ck >= x.n * G) return;
             if (all) {

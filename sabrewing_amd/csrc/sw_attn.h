@@ -27,13 +27,26 @@ struct SwTrees {
     int n_trees, n_seqs, max_pages, max_nodes;
 };
 
+// One layer's pool of latents: cell (page, slot) holds `rank` values and `rope` turned ones at page * ps + slot * ts (16-bit elements).
+struct SwLatent {
+    void *p;
+    int type, n_pages, psh, rank, rope;
+    int64_t ps, ts;
+};
+// heads of rows: row s's head h at s * rs + h * hs (elements)
+struct SwHeads {
+    void *p;
+    int64_t rs, hs;
+};
+
 // the page of token t of sequence q, or -1 where the table or its entry leads nowhere
-__device__ __forceinline__ int sw_page(const SwKv &c, const SwRows &r, int q, int t) {
-    const int i = t >> c.psh;
+__device__ __forceinline__ int sw_page_of(const SwRows &r, int n_pages, int psh, int q, int t) {
+    const int i = t >> psh;
     if (q < 0 || q >= r.n_seqs || t < 0 || i >= r.max_pages) return -1;
     const int p = r.table[(int64_t)q * r.max_pages + i];
-    return p >= 0 && p < c.n_pages ? p : -1;
+    return p >= 0 && p < n_pages ? p : -1;
 }
+__device__ __forceinline__ int sw_page(const SwKv &c, const SwRows &r, int q, int t) { return sw_page_of(r, c.n_pages, c.psh, q, t); }
 
 // f32 to the cache's type, to nearest even (a NaN stays one)
 __device__ __forceinline__ uint16_t sw_bf16_rne(float f) {
@@ -114,6 +127,14 @@ int sw_launch_attn_tree(hipStream_t st, const SwKv &c, const SwTrees &t, const f
 // (k_cache.hip) the accepted path of each tree and its cells moved together in n_layers <= SW_COPY_LAYERS caches
 int sw_launch_tree_commit(hipStream_t st, const SwKv *layers, int n_layers, const SwTrees &t, const int *parent, const int *draft,
                           const int *tok, int *path, int *count, int *next, int S);
+// (k_latent.hip) cells of new tokens (norm null: not normalised) and their query heads, nope values and a rotary part each,
+// rounded to the cache's type; a product for each head, W [H][n_out][n_in]; the absorbed form, q [S][H][rank + rope], out [S][H][rank], part:
+// scratch of sw_latent_part_floats floats (0: none)
+int sw_launch_latent_append(hipStream_t st, const SwLatent &c, const SwRows &r, const SwRope &rope, const float *ckv, int64_t ldc, const float *norm,
+                            float eps, const float *q, int64_t ldq, int H, int nope, const SwHeads &qn, const SwHeads &qr, int S);
+int sw_launch_latent_heads(hipStream_t st, int type, const SwHeads &x, const void *W, int H, int n_in, int n_out, const SwHeads &y, int y_f32, int S);
+int64_t sw_latent_part_floats(const SwLatent &c, const SwRows &r, int H, int S);
+int sw_launch_latent(hipStream_t st, const SwLatent &c, const SwRows &r, const void *q, int H, float scale, void *out, int S, float *part);
 // (k_sample.hip) a pick of each row of logits; each setting may be null
 struct SwSample { const float *temp; const int *top_k; const float *top_p, *min_p; };
 int sw_launch_sample(hipStream_t st, const float *logits, int S, int V, const SwSample &p, const float *u, int *tok);

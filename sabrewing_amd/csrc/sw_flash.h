@@ -11,8 +11,10 @@
 // loading lanes pick their source address accordingly.  An output's operand wants 8 tokens of a value
 // where memory has 8 values of a token: a lane reads 8 x 8 and transposes them by byte permutations.
 //
-// The waves of a block share columns or tokens: WC of them have 32 columns each and read
-// the same tile, and 4 / WC groups of them take every (4 / WC)-th tile.
+// The waves of a block share columns, tokens or values: WC of them have 32 columns each and read
+// the same tile, and 4 / WC groups of them take every (4 / WC)-th tile.  Or (SPLIT > 1, where queries and outputs of a cell's width
+// do not fit a wave's registers) SPLIT waves have the same columns: each takes a share of the scores' sums, which they exchange
+// through LDS, and of the outputs' values.
 #ifndef SW_FLASH_H
 #define SW_FLASH_H
 #include "sw_attn.h"
@@ -125,14 +127,17 @@ __device__ __forceinline__ void fl_split(const float (&x)[8], sw_u32x4 (&o)[NP])
 
 // A wave's 32 columns.  NP: parts that a 32-bit q and the weights are split into (1: 16-bit queries, one
 // rounding of the weights).  DK: values of a query, a multiple of 32; DV: of an output; INK: a cell's
-// first DV values of k are its v.
-template <int TYPE, int NP, int DK, int DV, bool INK>
+// first DV values of k are its v.  AHEAD: dwords of a row that a lane reads at once (8 rows of them), and twice the scores' steps read
+// ahead: registers for it.
+template <int TYPE, int NP, int DK, int DV, bool INK, int SPLIT = 1, int AHEAD = 4>
 struct Fl {
     static constexpr bool F32 = TYPE == SW_KV_F32;
-    static constexpr int ES = F32 ? 4 : 2, RBK = DK * ES, RBV = INK ? RBK : DV * ES, VB = DV * ES;     // bytes of a row of k, of v, of v's values
-    static constexpr int NCK = RBK / 16, NCV = VB / 16;
-    static constexpr int TB = 32 * RBK + (INK ? 0 : 32 * VB);                                          // bytes of a tile
-    static constexpr int DKS = RBK / 32, NO = DV / 32;
+    static constexpr int ES = F32 ? 4 : 2, RBK = DK * ES, RBV = INK ? RBK : DV * ES;                   // bytes of a row of k, of v
+    static constexpr int NCK = RBK / 16, NCV = DV * ES / 16;
+    static constexpr int TB = 32 * RBK + (INK ? 0 : 32 * RBV);                                         // bytes of a tile
+    static constexpr int DKS = RBK / 32 / SPLIT, DVW = DV / SPLIT, NO = DVW / 32, VB = DVW * ES;       // a wave's share: steps of the scores, values
+    static_assert(RBK / 32 % SPLIT == 0 && (SPLIT == 1 || (DVW % 64 == 0 && RBK % 128 == 0)), "whole shares");
+    static constexpr int XB = SPLIT > 1 ? 4096 : 0;                                                    // bytes of a wave in the exchange
     // where a piece of a row lies: its low bits turned by the token
     static constexpr int MK = NCK % 8 == 0 ? 7 : 3, MV = INK ? MK : NCV % 8 == 0 ? 7 : 3;
     template <int M> static __device__ __forceinline__ int turn(int t) { return M == 7 ? t & 7 : (t >> 1) & 3; }
@@ -144,9 +149,10 @@ struct Fl {
     sw_u32x4 Q[F32 ? 1 : NP][DKS];
     fl_f32x16 O[NO];
     float m, l, sc;
-    int kb[MK == 7 ? 4 : 2];                                           // this lane's places in a tile
+    static constexpr int KB = MK == 3 ? 2 : 4 / SPLIT;                 // this lane's places in a tile's row of k: they repeat
+    int kb[KB], share;                                                 // after KB steps (every SPLIT-th is the wave's)
 
-    __device__ __forceinline__ void begin(float scale) {
+    __device__ __forceinline__ void begin(float scale, int share_ = 0) {
         const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
         m = -INFINITY;
         l = 0.f;
@@ -156,7 +162,8 @@ struct Fl {
 #pragma unroll
             for (int j = 0; j < 16; j++) O[i][j] = 0.f;
 #pragma unroll
-        for (int i = 0; i < (MK == 7 ? 4 : 2); i++) kb[i] = c * RBK + (((2 * i + h) ^ turn<MK>(c)) * 16);
+        for (int i = 0; i < KB; i++) kb[i] = c * RBK + (((2 * (SPLIT * i + share_) + h) ^ turn<MK>(c)) * 16);
+        share = share_;
     }
     // 8 values 16 i + 8 h .. of a 32-bit query (f32 cells: 4 of them, 8 i + 4 h ..); f16 in parts: called after scale_up
     __device__ __forceinline__ void query(int i, const float (&x)[8]) {
@@ -169,11 +176,11 @@ struct Fl {
     }
 
     // the scores of the tile at `t`, times the scale
-    __device__ __forceinline__ void scores(const char *t, float (&x)[16]) const {
+    __device__ __forceinline__ void scores(const char *t, float (&x)[16], char *xch, int wave) const {
         fl_f32x16 s = {};
 #pragma unroll
         for (int i = 0; i < DKS; i++) {
-            const sw_u32x4 a = *(const sw_u32x4 *)(t + kb[i & (MK == 7 ? 3 : 1)] + (MK == 7 ? (i >> 2) * 128 : (i >> 1) * 64));
+            const sw_u32x4 a = *(const sw_u32x4 *)(t + kb[i % KB] + i / KB * (KB * SPLIT * 32));
             if constexpr (F32) {
                 const sw_f32x4 y = __builtin_bit_cast(sw_f32x4, a), z = __builtin_bit_cast(sw_f32x4, Q[0][i]);
 #pragma unroll
@@ -182,7 +189,26 @@ struct Fl {
 #pragma unroll
                 for (int u = 0; u < NP; u++) s = fl_mfma<TYPE>(a, Q[u][i], s);
             }
-            if (i % 8 == 7) __builtin_amdgcn_sched_barrier(0);         // (reads of the whole row ahead would spill)
+            if (i % (2 * AHEAD) == 2 * AHEAD - 1) __builtin_amdgcn_sched_barrier(0);     // (reads of the whole row ahead would spill)
+        }
+        if constexpr (SPLIT > 1) {                                     // the shares in their order: the same sum in every wave
+            sw_f32x4 *to = (sw_f32x4 *)xch + (threadIdx.x & 63);
+#pragma unroll
+            for (int j = 0; j < 4; j++) to[(wave * 4 + j) * 64] = sw_f32x4{s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]};
+            __syncthreads();
+            const int w0 = wave - share;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                sw_f32x4 y = to[(w0 * 4 + j) * 64];
+#pragma unroll
+                for (int k = 1; k < SPLIT; k++) {
+                    const sw_f32x4 z = to[((w0 + k) * 4 + j) * 64];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[e] = y[e] + z[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[4 * j + e] = y[e];
+            }
         }
 #pragma unroll
         for (int j = 0; j < 16; j++) x[j] = s[j] * sc;
@@ -217,10 +243,8 @@ struct Fl {
         return ((w & E) == E ? 0xFFFFu : 0u) | ((w & (E << 16)) == E << 16 ? 0xFFFF0000u : 0u);
     }
 
-    // O += V^T P.  CLEAN: infinities and NaN of v are taken for 0 (a weight of 0 times one of them is none), bit j of `bad`: this lane
-    // met one in its token j.
-    template <bool CLEAN>
-    __device__ __forceinline__ void outputs(const char *t, const float (&p)[16], uint32_t &bad) {
+    // O += V^T P
+    __device__ __forceinline__ void outputs(const char *t, const float (&p)[16]) {
         int lane = threadIdx.x & 63;
         asm volatile("" : "+v"(lane));                                 // (the places are taken anew for each tile, not kept)
         const int c = lane & 31, h = lane >> 5;
@@ -228,7 +252,7 @@ struct Fl {
 #pragma unroll
             for (int j = 0; j < 16; j++) {
                 const int x = MV == 7 ? 4 * h + j % 4 : 2 * h + ((j % 4) >> 1);
-                group_f32<CLEAN, 4, 0, 0>(t + (8 * (j / 4) + j % 4 + 4 * h) * RBV, x, c, p[j], j, bad);
+                group_f32<AHEAD, 0, 0>(t + (8 * (j / 4) + j % 4 + 4 * h) * RBV, x, c, p[j]);
                 if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
         } else {
@@ -239,20 +263,34 @@ struct Fl {
                 for (int j = 0; j < 8; j++) p8[j] = p[8 * mm + j];
                 sw_u32x4 P[NP];
                 fl_split<TYPE, NP>(p8, P);
-                group<CLEAN, 4, 0, 0>(t + 16 * mm * RBV + 4 * h * RBV, c, h, P, 8 * mm, bad);
+                group<AHEAD, 0, 0>(t + 16 * mm * RBV + 4 * h * RBV, c, h, P);
             }
         }
     }
-    template <bool CLEAN>
-    static __device__ __forceinline__ uint32_t clean(uint32_t v, int j, uint32_t &bad) {
-        if constexpr (!CLEAN) return v;
-        const uint32_t n = infinite(v);
-        bad |= n ? 1u << j : 0u;
-        return v & ~n;
+    // Infinities and NaN among the values of a tile's v, in wave w of n's share, become 0 (a weight of 0 times one of them is none);
+    // the tokens that had one are marked in `bad`.
+    static __device__ __forceinline__ void clean(char *t, int w, int n, uint32_t *bad) {
+        char *v = INK ? t : t + 32 * RBK;
+        uint32_t met = 0;
+#pragma unroll 1
+        for (int i = w * 64 + (threadIdx.x & 63); i < 32 * NCV; i += n * 64) {
+            const int tok = i / NCV;
+            sw_u32x4 *a = (sw_u32x4 *)(v + tok * RBV + (i - tok * NCV) * 16);
+            sw_u32x4 y = *a;
+            uint32_t any = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t x = infinite(y[e]);
+                any |= x;
+                y[e] = y[e] & ~x;
+            }
+            if (any) { *a = y; met |= 1u << tok; }
+        }
+        if (met) atomicOr(bad, met);
     }
     // the values from byte B0 on (output tiles from O0 on), W dwords of a row a lane
-    template <bool CLEAN, int W, int B0, int O0>
-    __device__ __forceinline__ void group(const char *t, int c, int h, const sw_u32x4 (&P)[NP], int j0, uint32_t &bad) {
+    template <int W, int B0, int O0>
+    __device__ __forceinline__ void group(const char *t, int c, int h, const sw_u32x4 (&P)[NP]) {
         if constexpr (B0 + 32 * 4 * W <= VB) {
             uint32_t v[8][W];
 #pragma unroll
@@ -267,8 +305,6 @@ struct Fl {
                     const uint2 y = *(const uint2 *)a;
                     v[k][0] = y.x; v[k][1] = y.y;
                 } else v[k][0] = *(const uint32_t *)a;
-#pragma unroll
-                for (int e = 0; e < W; e++) v[k][e] = clean<CLEAN>(v[k][e], j0 + k, bad);
             }
 #pragma unroll
             for (int e = 0; e < 2 * W; e++) {
@@ -279,16 +315,15 @@ struct Fl {
                 for (int u = 0; u < NP; u++) O[O0 + e] = fl_mfma<TYPE>(a, P[u], O[O0 + e]);
             }
             __builtin_amdgcn_sched_barrier(0);
-            group<CLEAN, W, B0 + 128 * W, O0 + 2 * W>(t, c, h, P, j0, bad);
+            group<W, B0 + 128 * W, O0 + 2 * W>(t, c, h, P);
         } else if constexpr (W > 1) {
-            group<CLEAN, W / 2, B0, O0>(t, c, h, P, j0, bad);
+            group<W / 2, B0, O0>(t, c, h, P);
         } else if constexpr (B0 < VB) {                                // 32 values left: two bytes a lane
             uint32_t v[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) {
                 const int x = MV == 7 ? 4 * h + k % 4 : 2 * h + ((k % 4) >> 1);
                 v[k] = *(const uint16_t *)(t + (8 * (k / 4) + k % 4) * RBV + B0 + (((c / 8) ^ x) * 16 + c % 8 * 2));
-                v[k] = clean<CLEAN>(v[k], j0 + k, bad);
             }
             sw_u32x4 a;
 #pragma unroll
@@ -297,8 +332,8 @@ struct Fl {
             for (int u = 0; u < NP; u++) O[O0] = fl_mfma<TYPE>(a, P[u], O[O0]);
         }
     }
-    template <bool CLEAN, int W, int B0, int O0>
-    __device__ __forceinline__ void group_f32(const char *row, int x, int c, float p, int j, uint32_t &bad) {
+    template <int W, int B0, int O0>
+    __device__ __forceinline__ void group_f32(const char *row, int x, int c, float p) {
         if constexpr (B0 + 32 * 4 * W <= VB) {
             uint32_t v[W];
             const char *a = row + B0 + (((c * W / 4) ^ x) * 16 + (c * W % 4) * 4);
@@ -312,40 +347,31 @@ struct Fl {
             } else v[0] = *(const uint32_t *)a;
 #pragma unroll
             for (int e = 0; e < W; e++)
-                O[O0 + e] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, clean<CLEAN>(v[e], j, bad)), p, O[O0 + e], 0, 0, 0);
-            group_f32<CLEAN, W, B0 + 128 * W, O0 + W>(row, x, c, p, j, bad);
-        } else if constexpr (W > 1) group_f32<CLEAN, W / 2, B0, O0>(row, x, c, p, j, bad);
+                O[O0 + e] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, v[e]), p, O[O0 + e], 0, 0, 0);
+            group_f32<W, B0 + 128 * W, O0 + W>(row, x, c, p);
+        } else if constexpr (W > 1) group_f32<W / 2, B0, O0>(row, x, c, p);
     }
 
-    // One tile.  whole: every column attends to all of its tokens, else seen(token of the tile) says it for this lane's column.
+    // One tile.  whole: every column attends to all of its tokens, else seen(token of the tile) says it for this lane's column, and bit k of
+    // bad that token k's v is no number: whoever attends to it has no meaningful output.
     template <class Seen>
-    __device__ __forceinline__ void tile(const char *t, bool whole, Seen seen) {
-        const int h = (threadIdx.x & 63) >> 5;
-        const char *v = INK ? t : t + 32 * RBK;
+    __device__ __forceinline__ void tile(const char *t, bool whole, uint32_t bad, Seen seen, char *xch, int wave) {
         float x[16];
-        uint32_t bad = 0;
-        scores(t, x);
-        uint32_t in = 0;                                               // the tokens that this lane's column attends to
+        scores(t, x, xch, wave);
         if (!whole) {
+            const int h4 = (threadIdx.x & 32) >> 3;
+            uint32_t met = 0;
 #pragma unroll
             for (int j = 0; j < 16; j++) {
-                const bool s = seen(8 * (j / 4) + 4 * h + j % 4);
-                in |= s ? 1u << j : 0u;
+                const int k = 8 * (j / 4) + h4 + j % 4;
+                const bool s = seen(k);
                 if (!s) x[j] = -INFINITY;
+                else met |= bad >> k & 1;
             }
+            if (met) l = NAN;
         }
         weights(x);
-        if (whole) {
-            outputs<false>(v, x, bad);
-            return;
-        }
-        outputs<true>(v, x, bad);
-        if (__any(bad != 0)) {                                         // whoever attends to such a token has no meaningful output
-            uint32_t all = 0;
-#pragma unroll 1
-            for (int j = 0; j < 16; j++) all |= (uint32_t)(__ballot(bad >> j & 1) >> (32 * h)) ? 1u << j : 0u;
-            if (all & in) l = NAN;
-        }
+        outputs((INK ? t : t + 32 * RBK) + (SPLIT > 1 ? share * VB : 0), x);
     }
 
     // Where an output's values lie: tile o's row r is value d0 + T r + e of a group of values that T tiles share (groups of 256
@@ -353,9 +379,9 @@ struct Fl {
     struct Map { int d0[NO], tiles[NO], e[NO]; };
     static constexpr Map map() {
         Map m = {};
-        int d = 0, w = F32 ? 4 : 8;
+        int d = 0, w = F32 ? AHEAD : 2 * AHEAD;
         for (int at = 0; at < NO; at += w) {
-            while (d + 32 * w > DV) w /= 2;
+            while (d + 32 * w > DVW) w /= 2;
             for (int e = 0; e < w; e++) { m.d0[at + e] = d; m.tiles[at + e] = w; m.e[at + e] = e; }
             d += 32 * w;
         }
@@ -363,59 +389,79 @@ struct Fl {
     }
 };
 
-// A block's work on one item: tiles ta .. tb - 1, dealt to its 4 / WC groups of waves in turn; NS tiles of a group in LDS.
+// A block's work on one item: tiles ta .. tb - 1, dealt to its WT groups of waves in turn; NS tiles of a group in LDS (`sh`).
 // issue(tile, LDS address): the wave's share of a tile's loads, NL of them, and whether every page of it is there;
-// whole(tile), seen(tile, token): the mask.
-template <int WC, int NS, int NL, class F, class Issue, class Whole, class Seen>
-__device__ __forceinline__ void fl_run(F &f, const char *sh, int ta, int tb, int wave, bool columns, Issue issue, Whole whole, Seen seen) {
-    constexpr int WT = FL_NW / WC, TB = F::TB;
-    const int wt = wave / WC, all = (tb - ta + WT - 1) / WT, n = (tb - ta - wt + WT - 1) / WT;       // tiles of the longest group, of this one
-    const char *mine = sh + wt * NS * TB;
+// whole(tile) (alike in the waves that share a tile), seen(tile, token): the mask; columns: this wave has some (with SPLIT every
+// wave takes part); xch: LDS of the exchange; s_bad: two words a group.
+template <int WC, int WT, int SPLIT, int NS, int NL, class F, class Issue, class Whole, class Seen>
+__device__ __forceinline__ void fl_run(F &f, char *sh, char *xch, uint32_t *s_bad, int ta, int tb, int wave, bool columns, Issue issue, Whole whole, Seen seen) {
+    static_assert(WT == 1 || SPLIT == 1, "groups of waves do not exchange");
+    constexpr int TB = F::TB;
+    constexpr bool shared = WC * SPLIT > 1;
+    const int wt = WT == 1 ? 0 : wave / WC, all = (tb - ta + WT - 1) / WT, n = (tb - ta - wt + WT - 1) / WT;     // tiles of the longest group, of this one
+    char *mine = sh + wt * NS * TB;
+    s_bad += 2 * wt;
     const uint32_t lds = fl_lds_addr(mine);
+    const bool first = (threadIdx.x & 63) == 0 && (WT > 1 && WC == 1 ? true : wave % (WC * SPLIT) == 0);       // of its group
+    if (first) s_bad[0] = 0;                                           // (the item before is done with it)
     uint32_t there = 0;                                                // bit s: all pages of the tile in place s are there
-    auto load = [&](int i) {
-        const int s = i % NS;
+    auto load = [&](int i, int s) {
         const bool ok = issue(ta + wt + i * WT, lds + s * TB);
         there = ok ? there | 1u << s : there & ~(1u << s);
     };
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < NS - 1; i++)
-        if (i < n) load(i);
+        if (i < n) load(i, i);
+    int s = 0;                                                         // the place of tile i
+#pragma unroll 1
     for (int i = 0; i < all; i++) {
         if (NS == 1) {
-            if (WC > 1) __syncthreads();                               // (every wave of the group has read the tile before)
+            if (shared) __syncthreads();                               // (every wave of the group has read the tile before)
             else fl_wait_lds();
-            if (i < n) load(i);
+            if (i < n) load(i, 0);
         }
         if (NS < 3 || i + NS - 2 >= n) fl_wait<0>();
         else fl_wait<(NS < 3 ? 0 : NS - 2) * NL>();
-        if (WC > 1) __syncthreads();
-        else fl_wait_lds();
-        if (NS > 1 && i + NS - 1 < n) load(i + NS - 1);
-        if (i < n && columns) {
-            const int t = ta + wt + i * WT;
-            f.tile(mine + (i % NS) * TB, ((there >> (i % NS)) & 1) && whole(t), [&](int k) { return seen(t, k); });
+        const int t = ta + wt + i * WT;
+        const bool whl = i >= n || (((there >> s) & 1) && whole(t));
+        bool all_whole = whl;
+        if (!shared) fl_wait_lds();
+        else if (WT > 1) all_whole = __syncthreads_and(whl);
+        else __syncthreads();
+        if (NS > 1 && i + NS - 1 < n) load(i + NS - 1, s == 0 ? NS - 1 : s - 1);
+        if (first) s_bad[(i + 1) & 1] = 0;
+        uint32_t bad = 0;
+        if (!all_whole) {
+            if (!whl) f.clean(mine + s * TB, WT == 1 ? wave : wave % WC, WC * SPLIT, s_bad + (i & 1));
+            if (shared) __syncthreads();
+            else fl_wait_lds();
+            bad = s_bad[i & 1];
         }
+        if (SPLIT > 1 || (i < n && columns)) f.tile(mine + s * TB, whl, bad, [&](int k) { return seen(t, k); }, xch, wave);
+        s = s + 1 == NS ? 0 : s + 1;
     }
 }
 
 // The end of an item: the groups' outputs of a column joined in their order and given to put(column, value, four
 // outputs, maximum, sum).  sh: LDS of fl_end_bytes, free.
-template <class F, int DV>
-constexpr int fl_end_bytes() { return FL_NW * 32 * (DV / 4 + 4) * 4; }
-template <int WC, class F, int DV, class Put>
+template <class F, int NW>
+constexpr int fl_end_bytes() { return NW * 32 * (F::DVW / 4 + 4) * 4; }
+template <int WC, int WT, int SPLIT, class F, class Put>
 __device__ __forceinline__ void fl_end(F &f, char *sh, float (*s_m)[32], float (*s_l)[32], int wave, Put put) {
-    constexpr int WT = FL_NW / WC, LD = DV / 4 + 4, NO = F::NO;
+    constexpr int DVW = F::DVW, LD = DVW / 4 + 4, NO = F::NO, NT = WC * WT * SPLIT * 64;
     constexpr auto map = F::map();
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
     const float l = fl_sum2(f.l);
     __syncthreads();                                                   // the tiles are done with
     if (h == 0) { s_m[wave][c] = f.m; s_l[wave][c] = l; }
     __syncthreads();
-    float M = f.m;
+    float g = 1.f;
+    if constexpr (WT > 1) {
+        float M = f.m;
 #pragma unroll
-    for (int i = 0; i < WT; i++) M = fmaxf(M, s_m[i * WC + wave % WC][c]);
-    const float g = f.m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(f.m - M);
+        for (int i = 0; i < WT; i++) M = fmaxf(M, s_m[i * WC + wave % WC][c]);
+        g = f.m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(f.m - M);
+    }
     float *so = (float *)sh + (wave * 32 + c) * LD;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
@@ -423,32 +469,37 @@ __device__ __forceinline__ void fl_end(F &f, char *sh, float (*s_m)[32], float (
         for (int o = 0; o < NO; o++) {
             const int T = map.tiles[o], at = map.d0[o] / 4 + map.e[o];
 #pragma unroll
-            for (int j = 0; j < 4; j++) so[at + T * (4 * h + j)] = f.O[o][4 * q + j] * g;
+            for (int j = 0; j < 4; j++) so[at + T * (4 * h + j)] = WT > 1 ? f.O[o][4 * q + j] * g : f.O[o][4 * q + j];
         }
         __syncthreads();
-        for (int i = tid; i < WC * 32 * (DV / 16); i += FL_NT) {
-            const int col = i / (DV / 16), d = i % (DV / 16) * 4, w = col >> 5;
+        // (column, share, four values): the shares of a column are waves side by side
+#pragma unroll 1
+        for (int i = tid; i < WC * 32 * SPLIT * (DVW / 16); i += NT) {
+            const int v = i % (SPLIT * (DVW / 16)), col = i / (SPLIT * (DVW / 16)), sp = v / (DVW / 16), d = v % (DVW / 16) * 4;
+            const int w = (col >> 5) * SPLIT + sp;
             sw_f32x4 a = *(const sw_f32x4 *)((const float *)sh + (w * 32 + (col & 31)) * LD + d);
-            float mx = s_m[w][col & 31];
+            float mx = s_m[w][col & 31], sum = s_l[w][col & 31];
+            if constexpr (WT > 1) {
 #pragma unroll
-            for (int k = 1; k < WT; k++) {
-                const sw_f32x4 y = *(const sw_f32x4 *)((const float *)sh + ((w + k * WC) * 32 + (col & 31)) * LD + d);
+                for (int k = 1; k < WT; k++) {
+                    const sw_f32x4 y = *(const sw_f32x4 *)((const float *)sh + ((w + k * WC) * 32 + (col & 31)) * LD + d);
 #pragma unroll
-                for (int e = 0; e < 4; e++) a[e] = a[e] + y[e];
-                mx = fmaxf(mx, s_m[w + k * WC][col & 31]);
-            }
-            float sum = 0.f;
+                    for (int e = 0; e < 4; e++) a[e] = a[e] + y[e];
+                    mx = fmaxf(mx, s_m[w + k * WC][col & 31]);
+                }
+                sum = 0.f;
 #pragma unroll
-            for (int k = 0; k < WT; k++) {
-                const float x = s_m[w + k * WC][col & 31];
-                sum = __builtin_fmaf(s_l[w + k * WC][col & 31], x == -INFINITY ? (mx == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(x - mx), sum);
+                for (int k = 0; k < WT; k++) {
+                    const float x = s_m[w + k * WC][col & 31];
+                    sum = __builtin_fmaf(s_l[w + k * WC][col & 31], x == -INFINITY ? (mx == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(x - mx), sum);
+                }
             }
             // the quarter's value d: which group of values it is in
             int d0 = 0, T8 = 0;
 #pragma unroll
             for (int o = 0; o < NO; o++)
                 if (map.e[o] == 0 && map.d0[o] / 4 <= d) { d0 = map.d0[o]; T8 = map.tiles[o] * 8; }
-            put(col, d0 + T8 * q + d - d0 / 4, a, mx, sum);
+            put(col, sp * DVW + d0 + T8 * q + d - d0 / 4, a, mx, sum);
         }
         __syncthreads();
     }
