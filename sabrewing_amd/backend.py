@@ -32,7 +32,7 @@ EXPORTS = [
     "lag_hip_last_groups", "lag_hip_rmsnorm", "lag_hip_moe_forward_rmsnorm", "lag_hip_head_argmax", "lag_hip_argmax", "lag_hip_set_grouped_kernel",
     "lag_hip_qk_rope_append", "lag_hip_attn_paged", "lag_hip_kv_copy_pages", "lag_hip_add", "lag_hip_sample",
     "lag_hip_attn_tree", "lag_hip_qk_rope_append_at", "lag_hip_tree_commit",
-    "lag_hip_latent_append", "lag_hip_latent_heads", "lag_hip_attn_latent",
+    "lag_hip_latent_append", "lag_hip_latent_heads", "lag_hip_attn_latent", "lag_hip_attn_latent_prompt",
     "lag_hip_set_q4_mode",
     "lag_hip_alloc", "lag_hip_h2d", "lag_hip_d2h", "lag_hip_d2d", "lag_hip_memset",
     "lag_hip_graph_begin", "lag_hip_graph_end", "lag_hip_graph_launch", "lag_hip_graph_destroy", "lag_hip_sync",
@@ -162,6 +162,7 @@ def load_library(path=None):
                                         C.c_int]
     L.lag_hip_latent_heads.argtypes = [C.c_int, HP, VP, C.c_int, C.c_int, C.c_int, HP, C.c_int, C.c_int]
     L.lag_hip_attn_latent.argtypes = [LP, RP, VP, C.c_int, C.c_float, VP, C.c_int]
+    L.lag_hip_attn_latent_prompt.argtypes = [LP, VP, C.c_int, C.c_int, VP, VP, C.c_int, C.c_int, VP, C.c_int, C.c_float, VP, C.c_int, C.c_int]
     L.lag_hip_kv_copy_pages.argtypes = [KP, C.c_int, VP, VP, C.c_int]
     L.lag_hip_add.argtypes = [VP, VP, C.c_size_t]
     L.lag_hip_sample.argtypes = [VP, C.c_int, C.c_int, C.POINTER(LagHipSample), VP, VP]
@@ -435,6 +436,11 @@ class Backend:
     def attn_latent(self, cache, rows, q_dev, n_heads, scale, out_dev, S):
         """one new token of each row against its sequence's latents, queries [S, n_heads, rank + rope_dims]"""
         self.check(self.lib.lag_hip_attn_latent(cache, rows, int(q_dev), n_heads, scale, int(out_dev), S), "lag_hip_attn_latent")
+
+    def attn_latent_prompt(self, cache, pages_dev, n_seq_pages, start, wk_dev, wv_dev, nope, v_dim, q_dev, n_heads, scale, out_dev, out_f32, S):
+        """S tokens of one sequence from position `start` on against keys and values expanded from its latents"""
+        self.check(self.lib.lag_hip_attn_latent_prompt(cache, int(pages_dev), n_seq_pages, start, int(wk_dev), int(wv_dev), nope, v_dim, int(q_dev),
+                                                       n_heads, scale, int(out_dev), int(out_f32), S), "lag_hip_attn_latent_prompt")
 
     def kv_copy_pages(self, caches, src, dst):
         """pages src[i] -> dst[i] of every layer (caches from kv_caches; host indices)"""

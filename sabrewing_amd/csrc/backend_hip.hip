@@ -1271,6 +1271,28 @@ extern "C" int lag_hip_attn_latent(const LagHipLatentCache *c, const LagHipKvRow
     return 0;
 }
 
+extern "C" int lag_hip_attn_latent_prompt(const LagHipLatentCache *c, const int *pages, int n_seq_pages, int start, const void *wk, const void *wv, int nope,
+                                          int v_dim, const void *q, int n_heads, float scale, void *out, int out_f32, int S) {
+    static const char *me = "attn_latent_prompt";
+    SwLatent lc;
+    if (const char *why = latent_of(c, lc)) return refuse(me, why);
+    if (!pages || n_seq_pages < 1) return refuse(me, "no pages");
+    if (S < 1 || start < 0 || (int64_t)start + S > 1 << 22) return refuse(me, "tokens (start + S at most 2^22)");
+    if (n_heads < 1 || n_heads > 1024) return refuse(me, "n_heads (1 to 1024)");
+    if (nope < 32 || nope > 256 || nope % 32 || v_dim < 32 || v_dim > 256 || v_dim % 32) return refuse(me, "nope and v_dim (multiples of 32, at most 256)");
+    if (!wk || !wv || ((uintptr_t)wk | (uintptr_t)wv) % 16) return refuse(me, "wk and wv must be 16-byte aligned");
+    if (!q || !out || ((uintptr_t)q | (uintptr_t)out) % 16) return refuse(me, "q and out must be 16-byte aligned");
+    const size_t no = (size_t)S * n_heads * v_dim * (out_f32 ? 4 : 2), w = (size_t)n_heads * c->rank * 2;
+    if (!apart(out, no, q, (size_t)S * n_heads * (nope + c->rope_dims) * 2) || !apart(out, no, wk, w * nope) || !apart(out, no, wv, w * v_dim))
+        return refuse(me, "out overlaps what is read");
+    if (not_ready(me)) return -1;
+    if (take_arena((size_t)sw_latent_prompt_bytes(lc, n_heads, nope, v_dim, (int64_t)start + S))) return -1;
+    PROF("attn_latent_prompt");
+    if (sw_launch_latent_prompt(g_st, lc, pages, n_seq_pages, start, wk, wv, nope, v_dim, q, n_heads, scale, out, out_f32 != 0, S, g_arena.p))
+        return fail_msg("attn_latent_prompt launch");
+    return 0;
+}
+
 extern "C" int lag_hip_add(float *x, const float *t, size_t n) {
     static const char *me = "add";
     if (!x || !t || !n) return refuse(me, "no values");

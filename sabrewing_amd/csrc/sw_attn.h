@@ -135,6 +135,11 @@ int sw_launch_latent_append(hipStream_t st, const SwLatent &c, const SwRows &r, 
 int sw_launch_latent_heads(hipStream_t st, int type, const SwHeads &x, const void *W, int H, int n_in, int n_out, const SwHeads &y, int y_f32, int S);
 int64_t sw_latent_part_floats(const SwLatent &c, const SwRows &r, int H, int S);
 int sw_launch_latent(hipStream_t st, const SwLatent &c, const SwRows &r, const void *q, int H, float scale, void *out, int S, float *part);
+// (k_prompt.hip) the expanded form: S tokens from position `start` of one sequence (its pages), wk [H][nope][rank], wv [H][vd][rank], q
+// [S][H][nope + rope], out [S][H][vd]; scratch of sw_latent_prompt_bytes bytes (T = start + S), 256-byte aligned
+int64_t sw_latent_prompt_bytes(const SwLatent &c, int H, int nope, int vd, int64_t T);
+int sw_launch_latent_prompt(hipStream_t st, const SwLatent &c, const int *pages, int max_pages, int start, const void *wk, const void *wv, int nope, int vd,
+                            const void *q, int H, float scale, void *out, int out_f32, int S, void *scratch);
 // (k_sample.hip) a pick of each row of logits; each setting may be null
 struct SwSample { const float *temp; const int *top_k; const float *top_p, *min_p; };
 int sw_launch_sample(hipStream_t st, const float *logits, int S, int V, const SwSample &p, const float *u, int *tok);
