@@ -214,9 +214,10 @@ int sw_launch_latent_heads(hipStream_t st, int type, const SwHeads &x, const voi
 #define LN_SPLIT 256                                                   // beyond so many rows none is split
 // waves that share 32 heads, their groups a block, and tiles in LDS
 template <int R, int WC> constexpr int ln_split() { return WC < 4 && R % 256 == 0 ? 4 : 2; }
-template <int TYPE, int R, int WC> using LnFl = Fl<TYPE, 1, R + LN_ROPE, R, true, ln_split<R, WC>(), (R > 256 && WC == 4 ? 2 : 4)>;
+template <int R, int WC> constexpr int ln_ql() { return R > 384 && WC == 4 ? 4 : 0; }
+template <int TYPE, int R, int WC> using LnFl = Fl<TYPE, 1, R + LN_ROPE, R, true, ln_split<R, WC>(), ln_ql<R, WC>()>;
 template <int R, int WC> constexpr int ln_ns() {
-    constexpr int n = (156 * 1024 - WC * ln_split<R, WC>() * 4096) / (32 * (R + LN_ROPE) * 2);
+    constexpr int n = (156 * 1024 - WC * ln_split<R, WC>() * (4 + ln_ql<R, WC>()) * 1024) / (32 * (R + LN_ROPE) * 2);
     return n > 4 ? 4 : n;
 }
 struct LnRow { int seq, last; };
@@ -230,9 +231,9 @@ template <int TYPE, int R, int WC>
 __global__ __launch_bounds__((64 * WC * ln_split<R, WC>())) void k_latent(SwLatent c, SwRows r, const uint16_t *__restrict__ q, int S, int H, float sc,
                                                                 uint16_t *__restrict__ out, float *__restrict__ part, int B) {
     using F = LnFl<TYPE, R, WC>;
-    constexpr int SPLIT = ln_split<R, WC>(), NW = WC * SPLIT, NT = 64 * NW;
+    constexpr int SPLIT = ln_split<R, WC>(), QL = ln_ql<R, WC>(), NW = WC * SPLIT, NT = 64 * NW;
     constexpr int CW = 32 * WC, NS = ln_ns<R, WC>(), NL = (F::NCK / 2 + NW - 1) / NW;
-    constexpr int SHT = NS * F::TB + NW * F::XB, SHB = SHT > fl_end_bytes<F, NW>() ? SHT : fl_end_bytes<F, NW>();
+    constexpr int SHT = NS * F::TB + NW * (F::XB + F::QLB), SHB = SHT > fl_end_bytes<F, NW>() ? SHT : fl_end_bytes<F, NW>();
     static_assert(SHB <= 157 * 1024 && (NS < 3 ? 0 : NS - 2) * NL < 64, "LDS, and loads that a wave can count");
     __shared__ __align__(16) char sh[SHB];
     __shared__ float s_m[NW][32], s_l[NW][32];
@@ -267,11 +268,17 @@ __global__ __launch_bounds__((64 * WC * ln_split<R, WC>())) void k_latent(SwLate
         const int head = c0 + wc * 32 + cl;
         const uint16_t *qp = q + ((int64_t)s * H + head) * width;
         f.begin(sc, share);
+        f.ql = (sw_u32x4 *)(sh + NS * F::TB + NW * F::XB + wave * F::QLB) + lane;
+        if (QL) __syncthreads();                                       // (the item before is done with its LDS)
 #pragma unroll
         for (int k = 0; k < F::DKS; k++) {
-            f.Q[0][k] = sw_u32x4{0, 0, 0, 0};
+            sw_u32x4 y = {0, 0, 0, 0};
             const int d = 16 * (SPLIT * k + share) + 8 * h2;
-            if (head < H && d < width) f.Q[0][k] = *(const sw_u32x4 *)(qp + d);
+            if (head < H && d < width) y = *(const sw_u32x4 *)(qp + d);
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = F::signed_by(y[e], sc);
+            if (k < QL) f.ql[k * 64] = y;
+            else f.Q[0][k < QL ? 0 : k - QL] = y;
         }
         const int *table = r.table + (int64_t)x.seq * r.max_pages;
         auto issue = [&](int tile, uint32_t lds) {
@@ -279,14 +286,11 @@ __global__ __launch_bounds__((64 * WC * ln_split<R, WC>())) void k_latent(SwLate
             int lane_ = lane;
             asm volatile("" : "+v"(lane_));                            // (the pieces' places are taken anew, not kept in registers)
             const FlPages g = fl_pages(table, r.max_pages, c.n_pages, c.psh, t0);
-#pragma unroll
-            for (int k = 0; k < NL; k++) {
-                const int kk = min(k * NW + wave, F::NCK / 2 - 1), p = kk * 64 + lane_, tok = p / F::NCK;
-                const int ch = (p - tok * F::NCK) ^ F::template turn<F::MK>(tok);
-                const int g01 = tok & 8 ? g.p[1] : g.p[0], g23 = tok & 8 ? g.p[3] : g.p[2], page = tok & 16 ? g23 : g01;
-                const char *a = (const char *)c.p + ((int64_t)max(page, 0) * c.ps + (int64_t)((t0 + tok) & pmask) * c.ts) * 2 + ch * 16;
-                fl_load16(8 * ch < width ? a : (const char *)&g_fl_zero, lds + kk * 1024);
-            }
+            if (c.psh >= 5 && width == R + LN_ROPE && c.ts < 1 << 25)  // one page, whole rows, not far apart
+                fl_rows<F::NCK, F::MK, NW, NL>((const char *)c.p + ((int64_t)max(g.p[0], 0) * c.ps + (int64_t)(t0 & pmask) * c.ts) * 2, (uint32_t)c.ts * 2,
+                                               wave, lane_, lds);
+            else
+                fl_rows_any<F::NCK, F::MK, NW, NL>((const char *)c.p, g, c.ps * 2, c.ts * 2, t0, pmask, width / 8, wave, lane_, lds);
             return g.ok;
         };
         auto whole = [&](int tile) { return tile * 32 + 31 <= x.last; };
@@ -349,7 +353,7 @@ __global__ __launch_bounds__(FL_NT) void k_latent_join(SwLatent c, SwRows r, int
 struct LnPlan { int wc, groups, B; };
 static LnPlan ln_plan(const SwLatent &c, const SwRows &r, int H, int S) {
     LnPlan p;
-    p.wc = H <= 32 ? 1 : H <= 64 ? 2 : 4;
+    p.wc = H <= 32 ? 1 : 2;
     p.groups = (H + 32 * p.wc - 1) / (32 * p.wc);
     const int64_t tiles = ((((int64_t)r.max_pages << c.psh) + 31) / 32) * S, most = (tiles + LN_LEAST - 1) / LN_LEAST;
     const int n = 256 / p.groups;

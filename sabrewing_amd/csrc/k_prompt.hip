@@ -25,125 +25,173 @@ __device__ __forceinline__ int lp_exp(float x2) {
 }
 
 // Blocks 0 .. tiles - 1: 32 cells side by side in xl [tokens][rank] and xr [tokens][64] (zeros where there is no cell or no value), te: the
-// exponent of the tile's largest norm, vm: which tokens have a cell.  Blocks behind them: we[2 h + kv], the exponent of a head's
-// largest row norm of Wk or Wv.  Values that are no numbers do not count in a norm.
+// exponent of the tile's largest norm, vm: which tokens have a cell.  Blocks behind them, LP_PARTS for a head's keys and as many for its
+// values: we, the exponent of the largest norm of a share of the rows of Wk or Wv.  Values that are no numbers do not count in a
+// norm.  A wave takes its 8 rows at once: one wait.
+#define LP_PARTS 8
 template <int TYPE>
 __global__ __launch_bounds__(LP_NT) void k_prompt_gather(SwLatent c, const int *__restrict__ pages, int max_pages, int T, const uint16_t *__restrict__ wk,
                                                          const uint16_t *__restrict__ wv, int nope, int vd, uint16_t *__restrict__ xl,
                                                          uint16_t *__restrict__ xr, int *__restrict__ te, uint32_t *__restrict__ vm, int *__restrict__ we) {
-    __shared__ float s_n[LP_NT / 64];
-    __shared__ uint32_t s_v;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, tiles = (T + 31) / 32;
+    constexpr int NW = LP_NT / 64, N = 32 / NW;
+    __shared__ float s_n[NW];
+    __shared__ uint32_t s_v[NW];
+    const int tid = threadIdx.x, lane = tid & 63, wave = fl_uni(tid >> 6), tiles = (T + 31) / 32;
     float best = 0.f;
-    auto square = [](sw_u32x4 y) {
+    uint32_t there = 0;
+    // (every lane reads, those behind a row's end its last values, which do not count)
+    const bool in = 8 * lane < c.rank;
+    const int at = min(8 * lane, c.rank - 8), rat = c.rank + max(0, min(8 * lane, c.rope - 8));
+    sw_u32x4 a[N];
+    auto norm = [&](sw_u32x4 y, bool count) {
         float ss = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; e++)
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float f = lp_float<TYPE>(y[e], i), g = fabsf(f) < INFINITY ? f : 0.f;
+            for (int k = 0; k < 2; k++) {
+                const float f = lp_float<TYPE>(y[e], k), g = fabsf(f) < INFINITY ? f : 0.f;
                 ss = __builtin_fmaf(g, g, ss);
             }
-        return ss;
+        ss = count && in ? ss : 0.f;
+#pragma unroll
+        for (int o = 32; o; o >>= 1) ss = ss + __shfl_xor(ss, o);
+        best = fmaxf(best, ss);
     };
     if ((int)blockIdx.x < tiles) {
-        if (tid == 0) s_v = 0;
-        __syncthreads();
-#pragma unroll 2
-        for (int i = wave; i < 32; i += LP_NT / 64) {
-            const int t = blockIdx.x * 32 + i, pg = t >> c.psh;
-            int page = -1;
-            if (t < T && pg < max_pages) page = pages[pg];
-            if (page >= c.n_pages) page = -1;
-            const uint16_t *cell = (const uint16_t *)c.p + (int64_t)max(page, 0) * c.ps + (int64_t)(t & ((1 << c.psh) - 1)) * c.ts;
-            sw_u32x4 a = {0, 0, 0, 0}, b = a;
-            if (page >= 0 && 8 * lane < c.rank) a = *(const sw_u32x4 *)(cell + 8 * lane);
-            if (page >= 0 && 8 * lane < c.rope) b = *(const sw_u32x4 *)(cell + c.rank + 8 * lane);
-            if (8 * lane < c.rank) *(sw_u32x4 *)(xl + (int64_t)t * c.rank + 8 * lane) = a;
-            if (lane < LP_ROPE / 8) *(sw_u32x4 *)(xr + (int64_t)t * LP_ROPE + 8 * lane) = b;
-            float ss = square(a);
-            for (int o = 32; o; o >>= 1) ss = ss + __shfl_xor(ss, o);
-            best = fmaxf(best, ss);
-            if (lane == 0 && page >= 0) atomicOr(&s_v, 1u << i);
+        const int t0 = blockIdx.x * 32 + wave * N, pmask = (1 << c.psh) - 1;
+        const int pg = min(t0 + (lane & (N - 1)), T - 1) >> c.psh;
+        int page = pages[min(pg, max_pages - 1)];
+        if (t0 + (lane & (N - 1)) >= T || pg >= max_pages || page >= c.n_pages) page = -1;
+        there = (uint32_t)__ballot(lane < N && page >= 0);
+        sw_u32x4 b[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int p = max(__builtin_amdgcn_readlane(page, i), 0);
+            const uint16_t *cell = (const uint16_t *)c.p + (int64_t)p * c.ps + (int64_t)((t0 + i) & pmask) * c.ts;
+            a[i] = *(const sw_u32x4 *)(cell + at);
+            b[i] = *(const sw_u32x4 *)(cell + (c.rope ? rat : 0));
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const bool cell = there >> i & 1;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                a[i][e] = cell ? a[i][e] : 0u;
+                b[i][e] = cell && 8 * lane < c.rope ? b[i][e] : 0u;
+            }
+            if (in) *(sw_u32x4 *)(xl + (int64_t)(t0 + i) * c.rank + 8 * lane) = a[i];
+            if (lane < LP_ROPE / 8) *(sw_u32x4 *)(xr + (int64_t)(t0 + i) * LP_ROPE + 8 * lane) = b[i];
+            norm(a[i], true);
         }
     } else {
-        const int k = blockIdx.x - tiles, h = k >> 1, n = k & 1 ? vd : nope;
+        const int k = (blockIdx.x - tiles) / LP_PARTS, part = (blockIdx.x - tiles) % LP_PARTS, h = k >> 1, n = k & 1 ? vd : nope;
         const uint16_t *w = (k & 1 ? wv : wk) + (int64_t)h * n * c.rank;
-#pragma unroll 4
-        for (int i = wave; i < n; i += LP_NT / 64) {
-            float ss = 8 * lane < c.rank ? square(*(const sw_u32x4 *)(w + (int64_t)i * c.rank + 8 * lane)) : 0.f;
-            for (int o = 32; o; o >>= 1) ss = ss + __shfl_xor(ss, o);
-            best = fmaxf(best, ss);
-        }
+        const int i0 = part * (n / LP_PARTS) + wave * N, end = (part + 1) * (n / LP_PARTS);           // (n: a multiple of 32, at most 256)
+#pragma unroll
+        for (int i = 0; i < N; i++) a[i] = *(const sw_u32x4 *)(w + (int64_t)min(i0 + i, n - 1) * c.rank + at);
+#pragma unroll
+        for (int i = 0; i < N; i++) norm(a[i], i0 + i < end);
     }
-    if (lane == 0) s_n[wave] = best;
+    if (lane == 0) { s_n[wave] = best; s_v[wave] = there << (wave * N); }
     __syncthreads();
     if (tid == 0) {
 #pragma unroll
-        for (int i = 1; i < LP_NT / 64; i++) best = fmaxf(best, s_n[i]);
-        if ((int)blockIdx.x < tiles) { te[blockIdx.x] = lp_exp(best); vm[blockIdx.x] = s_v; }
+        for (int i = 1; i < NW; i++) best = fmaxf(best, s_n[i]);
+        if ((int)blockIdx.x < tiles) { te[blockIdx.x] = lp_exp(best); vm[blockIdx.x] = s_v[0] | s_v[1] | s_v[2] | s_v[3]; }
         else we[blockIdx.x - tiles] = lp_exp(best);
     }
 }
 
-// Keys and values of heads h0 ..: [head][tokens][n] in f16, times 2^eh.  A wave takes 64 outputs by 64 tokens, its
-// operands straight from memory; a block 128 by 128.
+// Keys and values of heads h0 ..: [head][tokens][np or vp] in f16, times 2^eh, the values behind nope or vd zeros.  A block takes 128 outputs
+// by 128 tokens, both in LDS by 64 of the summed values, two lots ahead; a wave 64 by 64 of them.  A die's blocks share
+// a range of tokens (they stay in its cache) and go through all heads.
+#define LE_K 64
+#define LE_TILE (128 * LE_K * 2)
 template <int TYPE>
-__global__ __launch_bounds__(LP_NT) void k_prompt_expand(const uint16_t *__restrict__ xl, const int *__restrict__ te, const int *__restrict__ we, int T32,
-                                                         int rank, const uint16_t *__restrict__ wk, const uint16_t *__restrict__ wv, int nope, int vd,
-                                                         int h0, uint16_t *__restrict__ kb, uint16_t *__restrict__ vb, int *__restrict__ eh) {
+__global__ __launch_bounds__(LP_NT, 2) void k_prompt_expand(const uint16_t *__restrict__ xl, const int *__restrict__ te, const int *__restrict__ we, int T32,
+                                                            int rank, const uint16_t *__restrict__ wk, const uint16_t *__restrict__ wv, int nope, int vd,
+                                                            int np, int vp, int heads, int h0, uint16_t *__restrict__ kb, uint16_t *__restrict__ vb,
+                                                            int *__restrict__ eh) {
+    __shared__ __align__(16) char sh[2 * 2 * LE_TILE];
     __shared__ int s_e[LP_NT / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = fl_uni(tid >> 6), c = lane & 31, g = lane >> 5;
-    const int tk = (nope + 127) / 128, tv = (vd + 127) / 128, hl = blockIdx.y / (tk + tv), by = blockIdx.y % (tk + tv), h = h0 + hl;
-    const int kv = by >= tk, n = kv ? vd : nope;
+    const int tk = (np + 127) / 128, tv = (vp + 127) / 128, nt = (T32 + 127) / 128, per = (nt + 7) / 8;
+    const int die = blockIdx.x & 7, j0 = blockIdx.x >> 3, tt = die * per + j0 % per, y0 = j0 / per;
+    if (tt >= nt || y0 >= heads * (tk + tv)) return;
+    const int hl = y0 / (tk + tv), by = y0 % (tk + tv), h = h0 + hl, kv = by >= tk, n = kv ? vd : nope, pad = kv ? vp : np;
+    const int o0 = (kv ? by - tk : by) * 128, s0 = tt * 128;
+    const uint16_t *W = (kv ? wv : wk) + (int64_t)h * n * rank;
+    // rows o0 .. of W and s0 .. of xl (the last in the place of those behind), 8 pieces of 16 bytes each, turned by the row
+    uint32_t wo[4], xo[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int r = (k * 4 + wave) * 8 + (lane >> 3), p = (lane & 7) ^ (r & 7);
+        wo[k] = (uint32_t)min(o0 + r, n - 1) * rank * 2 + p * 16;
+        xo[k] = (uint32_t)min(r, T32 - 1 - s0) * rank * 2 + p * 16;
+    }
+    const char *xb = (const char *)(xl + (int64_t)s0 * rank);
+    const uint32_t lds = fl_lds_addr(sh);
+    auto load = [&](int i) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) fl_load16((const char *)W + i * (LE_K * 2), wo[k], lds + (i & 1) * 2 * LE_TILE + (k * 4 + wave) * 1024);
+#pragma unroll
+        for (int k = 0; k < 4; k++) fl_load16(xb + i * (LE_K * 2), xo[k], lds + (i & 1) * 2 * LE_TILE + LE_TILE + (k * 4 + wave) * 1024);
+    };
+    load(0);
     int e = -100;
     for (int i = tid; i < T32 / 32; i += LP_NT) e = max(e, te[i]);
     for (int o = 32; o; o >>= 1) e = max(e, __shfl_xor(e, o));
     if (lane == 0) s_e[wave] = e;
     __syncthreads();
+    int w = -100;
 #pragma unroll
     for (int i = 0; i < LP_NT / 64; i++) e = max(e, s_e[i]);
-    e = min(max(15 - e - we[2 * h + kv], -120), 120);
-    if (tid == 0 && blockIdx.x == 0) eh[2 * h + kv] = e;
-    const int o0 = (kv ? by - tk : by) * 128 + (wave & 1) * 64, s0 = blockIdx.x * 128 + (wave >> 1) * 64;
-    if (o0 >= n || s0 >= T32) return;
-    const uint16_t *wp[2], *xp[2];
 #pragma unroll
-    for (int i = 0; i < 2; i++) wp[i] = (kv ? wv : wk) + ((int64_t)h * n + min(o0 + 32 * i + c, n - 1)) * rank + 8 * g;
-#pragma unroll
-    for (int i = 0; i < 2; i++) xp[i] = xl + (int64_t)min(s0 + 32 * i + c, T32 - 1) * rank + 8 * g;
+    for (int i = 0; i < LP_PARTS; i++) w = max(w, we[(2 * h + kv) * LP_PARTS + i]);
+    e = min(max(15 - e - w, -120), 120);
+    if (tid == 0 && tt == 0) eh[2 * h + kv] = e;
     fl_f32x16 acc[2][2];
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
         for (int j = 0; j < 2; j++) acc[i][j] = fl_f32x16{};
-#pragma unroll 2
-    for (int k = 0; k < rank; k += 16) {
-        sw_u32x4 a[2], b[2];
+    const int wo0 = (wave & 1) * 64, ws0 = (wave >> 1) * 64, steps = rank / LE_K;
+#pragma unroll 1
+    for (int i = 0; i < steps; i++) {
+        fl_wait<0>();
+        __syncthreads();                                               // lot i is there, lot i - 1 read
+        if (i + 1 < steps) load(i + 1);
+        const char *A = sh + (i & 1) * 2 * LE_TILE, *B = A + LE_TILE;
 #pragma unroll
-        for (int i = 0; i < 2; i++) a[i] = *(const sw_u32x4 *)(wp[i] + k);
+        for (int k = 0; k < LE_K / 16; k++) {
+            sw_u32x4 a[2], b[2];
 #pragma unroll
-        for (int i = 0; i < 2; i++) b[i] = *(const sw_u32x4 *)(xp[i] + k);
+            for (int u = 0; u < 2; u++) {
+                a[u] = *(const sw_u32x4 *)(A + (wo0 + 32 * u + c) * (LE_K * 2) + (((2 * k + g) ^ (c & 7)) * 16));
+                b[u] = *(const sw_u32x4 *)(B + (ws0 + 32 * u + c) * (LE_K * 2) + (((2 * k + g) ^ (c & 7)) * 16));
+            }
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+            for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int j = 0; j < 2; j++) acc[i][j] = fl_mfma<TYPE>(a[i], b[j], acc[i][j]);
+                for (int v = 0; v < 2; v++) acc[u][v] = fl_mfma<TYPE>(a[u], b[v], acc[u][v]);
+        }
     }
     const float f = ldexpf(1.f, e);
-    uint16_t *y = (kv ? vb : kb) + (int64_t)hl * T32 * n;
+    uint16_t *y = (kv ? vb : kb) + (int64_t)hl * T32 * pad;
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-        const int s = s0 + 32 * j + c;
+        const int s = s0 + ws0 + 32 * j + c;
         if (s >= T32) continue;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            if (o0 + 32 * i >= n) break;
+            const int o = o0 + wo0 + 32 * i;
+            if (o >= pad) break;
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 uint32_t p[4];
 #pragma unroll
-                for (int q = 0; q < 4; q++) p[q] = __builtin_bit_cast(uint16_t, (_Float16)(acc[i][j][r + q] * f));
-                *(uint2 *)(y + (int64_t)s * n + o0 + 32 * i + 2 * r + 4 * g) = make_uint2(p[0] | (p[1] << 16), p[2] | (p[3] << 16));
+                for (int q = 0; q < 4; q++) p[q] = o < n ? (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(acc[i][j][r + q] * f)) : 0u;
+                *(uint2 *)(y + (int64_t)s * pad + o + 2 * r + 4 * g) = make_uint2(p[0] | (p[1] << 16), p[2] | (p[3] << 16));
             }
         }
     }
@@ -154,32 +202,18 @@ template <int TYPE, int NOPE, int DV>
 struct LpFl : Fl<SW_KV_F16, 1, NOPE, DV, false> {
     using Base = Fl<SW_KV_F16, 1, NOPE, DV, false>;
     static constexpr int ROPE_AT = Base::TB, TB = Base::TB + 32 * LP_ROPE * 2;
-    sw_u32x4 R[LP_ROPE / 16];
-    float scr;
+    sw_u32x4 R[LP_ROPE / 16];                                          // the queries' rotary part, scaled as the other is with its keys
     template <class Seen>
     __device__ __forceinline__ void tile(const char *t, bool whole, uint32_t bad, Seen seen, char *, int) {
-        const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+        const int lane = fl_lane<Base::KEEP>(), c = lane & 31, h = lane >> 5;
         fl_f32x16 s = {};
+        sw_u32x4 r[LP_ROPE / 16];
 #pragma unroll
-        for (int i = 0; i < LP_ROPE / 16; i++)
-            s = fl_mfma<TYPE>(*(const sw_u32x4 *)(t + ROPE_AT + c * (LP_ROPE * 2) + (((2 * i + h) ^ (c & 7)) * 16)), R[i], s);
-        float x[16];
-        this->scores(t, x, nullptr, 0);
+        for (int i = 0; i < LP_ROPE / 16; i++) r[i] = *(const sw_u32x4 *)(t + ROPE_AT + c * (LP_ROPE * 2) + (((2 * i + h) ^ (c & 7)) * 16));
+        this->dot(t, s);
 #pragma unroll
-        for (int j = 0; j < 16; j++) x[j] = __builtin_fmaf(s[j], scr, x[j]);
-        if (!whole) {
-            uint32_t met = 0;
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const int k = 8 * (j / 4) + 4 * h + j % 4;
-                const bool in = seen(k);
-                if (!in) x[j] = -INFINITY;
-                else met |= bad >> k & 1;
-            }
-            if (met) this->l = NAN;
-        }
-        this->weights(x);
-        this->outputs(t + 32 * Base::RBK, x);
+        for (int i = 0; i < LP_ROPE / 16; i++) s = fl_mfma<TYPE>(r[i], R[i], s);
+        this->rest(t, whole, bad, seen, s);
     }
 };
 template <int NOPE, int DV> constexpr int lp_occ() { return NOPE / 4 + DV / 2 <= 112 ? 2 : 1; }
@@ -217,42 +251,55 @@ __global__ __launch_bounds__(FL_NT, (lp_occ<NOPE, DV>())) void k_prompt(const ui
 #pragma unroll
         for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(lp_float<TYPE>(raw[k][e / 2], e & 1)));
     }
+    sw_u32x4 rr[LP_ROPE / 16];
+    float mr = 0.f;
+#pragma unroll
+    for (int k = 0; k < LP_ROPE / 16; k++) {
+        rr[k] = sw_u32x4{0, 0, 0, 0};
+        if (16 * k + 8 * h2 < rope) rr[k] = *(const sw_u32x4 *)(qp + nope + 16 * k + 8 * h2);
+#pragma unroll
+        for (int e = 0; e < 8; e++) mr = fmaxf(mr, fabsf(lp_float<TYPE>(rr[k][e / 2], e & 1)));
+    }
     mx = fl_max2(mx);
-    const int up = mx > 0.f && mx < INFINITY ? 13 - ilogbf(mx) : 0;
+    mr = fl_max2(mr);
+    // The scores are to be 2^E times as large, of both parts: the keys are 2^ek times, the queries 2^(E - ek) -- up to 2^13 -- and the
+    // rotary queries, whose keys are as they were, 2^E, up to 2^15 in f16 (2^100 in bf16).  Where those bind, the first part is the
+    // smaller one by as much, and what its queries lose below f16's range is as small beside the other.
     const int ek = eh[2 * h], ev = eh[2 * h + 1];
-    f.begin(ldexpf(sc0, -up - ek));
-    f.scr = sc0;
+    const bool nx = mx > 0.f && mx < INFINITY, nr = mr > 0.f && mr < INFINITY;
+    int E = nx ? 13 - ilogbf(mx) + ek : ek;
+    if (nr) E = min(E, (TYPE == SW_KV_BF16 ? 100 : 14) - ilogbf(mr));
+    E = min(max(E, -120), 120);
+    const float sg = sc0 < 0.f ? -1.f : sc0 == 0.f ? 0.f : 1.f;       // (the scale's sign, or none: see Fl::begin)
+    f.begin(ldexpf(sc0, -E));
 #pragma unroll
     for (int k = 0; k < F::DKS; k++) {
         float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = ldexpf(lp_float<TYPE>(raw[k][e / 2], e & 1), up);
+        for (int e = 0; e < 8; e++) y[e] = sg * ldexpf(lp_float<TYPE>(raw[k][e / 2], e & 1), E - ek);
         f.query(k, y);
     }
 #pragma unroll
     for (int k = 0; k < LP_ROPE / 16; k++) {
-        f.R[k] = sw_u32x4{0, 0, 0, 0};
-        if (16 * k + 8 * h2 < rope) f.R[k] = *(const sw_u32x4 *)(qp + nope + 16 * k + 8 * h2);
-    }
-    const char *kp = (const char *)(kb + (int64_t)hl * T32 * nope), *vp = (const char *)(vb + (int64_t)hl * T32 * vd);
-    auto issue = [&](int tile, uint32_t lds) {
-        int lane_ = lane;
-        asm volatile("" : "+v"(lane_));                                // (the pieces' places are taken anew, not kept in registers)
-        auto rows = [&](const char *src, int nch, int real, bool turn7, int loads, uint32_t to) {
-            src += (int64_t)tile * 32 * real * 16;
+        float y[8];
 #pragma unroll
-            for (int k = 0; k < loads; k++) {
-                const int kk = min(k * WC + wc, nch / 2 - 1), p = kk * 64 + lane_, tok = p / nch;
-                const int ch = (p - tok * nch) ^ (turn7 ? tok & 7 : (tok >> 1) & 3);
-                fl_load16(ch < real ? src + (tok * real + ch) * 16 : (const char *)&g_fl_zero, to + kk * 1024);
-            }
-        };
-        rows(kp, F::NCK, nope / 8, F::MK == 7, LK, lds);
-        rows(vp, F::NCV, vd / 8, F::MV == 7, LV, lds + 32 * F::RBK);
-        rows((const char *)xr, LP_ROPE / 8, LP_ROPE / 8, true, LR, lds + F::ROPE_AT);
-        return fl_entry((const int *)vm, tile) == -1;
+        for (int e = 0; e < 8; e++) y[e] = sg * ldexpf(lp_float<TYPE>(rr[k][e / 2], e & 1), E);
+        sw_u32x4 o[1];
+        fl_split<TYPE, 1>(y, o);
+        f.R[k] = o[0];
+    }
+    bool every = true;                                                 // no token without a cell before the last tile
+    for (int i = tid; i < tiles - 1; i += FL_NT) every = every && vm[i] == 0xFFFFFFFFu;
+    every = __syncthreads_and(every);
+    const char *kp = (const char *)(kb + (int64_t)hl * T32 * NOPE), *vp = (const char *)(vb + (int64_t)hl * T32 * DV);
+    auto issue = [&](int tile, uint32_t lds) {
+        const int lane_ = fl_lane<F::KEEP>();
+        fl_rows<F::NCK, F::MK, WC, LK>(kp + (int64_t)tile * (32 * NOPE * 2), NOPE * 2, wc, lane_, lds);
+        fl_rows<F::NCV, F::MV, WC, LV>(vp + (int64_t)tile * (32 * DV * 2), DV * 2, wc, lane_, lds + 32 * F::RBK);
+        fl_rows<LP_ROPE / 8, 7, WC, LR>((const char *)xr + (int64_t)tile * (32 * LP_ROPE * 2), LP_ROPE * 2, wc, lane_, lds + F::ROPE_AT);
+        return every || fl_entry((const int *)vm, tile) == -1;
     };
-    auto whole = [&](int tile) { return tile * 32 + 31 <= start + r0; };
+    auto whole = [&](int tile) { return tile * 32 + 31 <= start + r0 && tile < tiles - 1; };
     auto seen = [&](int tile, int k) { return tile * 32 + k <= start + row && ((vm[tile] >> k) & 1); };
     fl_run<WC, WT, 1, NS, NL>(f, sh, nullptr, s_bad, 0, tiles, wave, true, issue, whole, seen);
     fl_end<WC, WT, 1>(f, sh, s_m, s_l, wave, [&](int col, int d, sw_f32x4 a, float, float sum) {
@@ -273,11 +320,13 @@ __global__ __launch_bounds__(FL_NT, (lp_occ<NOPE, DV>())) void k_prompt(const ui
 
 // ------------------------------------------------------------------ scratch and launches ----
 // heads expanded at a time: what they take stays about a GiB
-struct LpPlan { int64_t T32, xl, xr, te, vm, we, eh, kb, vb, total; int heads; };
+struct LpPlan { int64_t T32, xl, xr, te, vm, we, eh, kb, vb, total; int heads, np, vp; };
 static LpPlan lp_plan(const SwLatent &c, int H, int nope, int vd, int64_t T) {
     LpPlan p;
     p.T32 = (T + 31) / 32 * 32;
-    const int64_t one = p.T32 * (nope + vd) * 2, most = ((int64_t)1 << 30) / one;
+    p.np = nope <= 64 ? 64 : nope <= 128 ? 128 : 256;
+    p.vp = vd <= 64 ? 64 : vd <= 128 ? 128 : 256;
+    const int64_t one = p.T32 * (p.np + p.vp) * 2, most = ((int64_t)1 << 30) / one;
     p.heads = (int)(most < 1 ? 1 : most < H ? most : H);
     int64_t at = 0;
     auto take = [&](int64_t n) { const int64_t x = at; at += (n + 255) / 256 * 256; return x; };
@@ -285,10 +334,10 @@ static LpPlan lp_plan(const SwLatent &c, int H, int nope, int vd, int64_t T) {
     p.xr = take(p.T32 * LP_ROPE * 2);
     p.te = take(p.T32 / 8);
     p.vm = take(p.T32 / 8);
-    p.we = take((int64_t)H * 8);
+    p.we = take((int64_t)H * 8 * LP_PARTS);
     p.eh = take((int64_t)H * 8);
-    p.kb = take(p.heads * p.T32 * nope * 2);
-    p.vb = take(p.heads * p.T32 * vd * 2);
+    p.kb = take(p.heads * p.T32 * p.np * 2);
+    p.vb = take(p.heads * p.T32 * p.vp * 2);
     p.total = at;
     return p;
 }
@@ -322,12 +371,13 @@ static int lp_run(hipStream_t st, const SwLatent &c, const int *pages, int max_p
     uint16_t *xl = (uint16_t *)(A + p.xl), *xr = (uint16_t *)(A + p.xr), *kb = (uint16_t *)(A + p.kb), *vb = (uint16_t *)(A + p.vb);
     int *te = (int *)(A + p.te), *we = (int *)(A + p.we), *eh = (int *)(A + p.eh);
     uint32_t *vm = (uint32_t *)(A + p.vm);
-    SW_LAUNCH(k_prompt_gather<TYPE>, dim3((unsigned)(p.T32 / 32 + 2 * H)), dim3(LP_NT), 0, st, c, pages, max_pages, T, (const uint16_t *)wk, (const uint16_t *)wv,
+    SW_LAUNCH(k_prompt_gather<TYPE>, dim3((unsigned)(p.T32 / 32 + 2 * H * LP_PARTS)), dim3(LP_NT), 0, st, c, pages, max_pages, T, (const uint16_t *)wk, (const uint16_t *)wv,
               nope, vd, xl, xr, te, vm, we);
     for (int h0 = 0; h0 < H; h0 += p.heads) {
-        const int heads = H - h0 < p.heads ? H - h0 : p.heads, blocks = (nope + 127) / 128 + (vd + 127) / 128;
-        SW_LAUNCH(k_prompt_expand<TYPE>, dim3((unsigned)((p.T32 + 127) / 128), (unsigned)(heads * blocks)), dim3(LP_NT), 0, st, xl, te, we, (int)p.T32, c.rank,
-                  (const uint16_t *)wk, (const uint16_t *)wv, nope, vd, h0, kb, vb, eh);
+        const int heads = H - h0 < p.heads ? H - h0 : p.heads, blocks = (p.np + 127) / 128 + (p.vp + 127) / 128;
+        const int64_t per = (p.T32 / 32 + 31) / 32;                     // lots of 128 tokens of a die
+        SW_LAUNCH(k_prompt_expand<TYPE>, dim3((unsigned)(8 * per * heads * blocks)), dim3(LP_NT), 0, st, xl, te, we, (int)p.T32, c.rank,
+                  (const uint16_t *)wk, (const uint16_t *)wv, nope, vd, p.np, p.vp, heads, h0, kb, vb, eh);
         const LpArgs a = {kb, vb, xr, vm, eh, (int)p.T32, start, S, nope, vd, c.rope, (const uint16_t *)q, H, h0, heads, sc, out, out_f32};
         if (nope <= 64) lp_values<TYPE, 64>(st, a);
         else if (nope <= 128) lp_values<TYPE, 128>(st, a);

@@ -67,6 +67,7 @@ __global__ __launch_bounds__(FL_NT, (tr_occ<TYPE, DH>())) void k_tree(SwKv c, Sw
     const int pmask = (1 << c.psh) - 1;
     const char *kp = (const char *)c.k + (int64_t)hk * c.hs * ES, *vp = (const char *)c.v + (int64_t)hk * c.hs * ES;
     const int64_t psb = c.ps * ES, tsb = c.ts * ES;
+    const bool near = tsb < (int64_t)1 << 26;
     F f;
     for (; at < end; i++) {
         TrTree x = tr_tree(c, t, i, S, window);
@@ -111,7 +112,8 @@ __global__ __launch_bounds__(FL_NT, (tr_occ<TYPE, DH>())) void k_tree(SwKv c, Sw
             if constexpr (F::F32) {
                 sw_f32x4 y = {0.f, 0.f, 0.f, 0.f};
                 if (mine) y = *(const sw_f32x4 *)(qp + 8 * k + 4 * h);
-                f.Q[0][k] = __builtin_bit_cast(sw_u32x4, y);
+#pragma unroll
+                for (int e = 0; e < 4; e++) f.Q[0][k][e] = F::signed_by(__builtin_bit_cast(uint32_t, (float)y[e]), sc);
             } else {
                 float y[8];
 #pragma unroll
@@ -120,6 +122,8 @@ __global__ __launch_bounds__(FL_NT, (tr_occ<TYPE, DH>())) void k_tree(SwKv c, Sw
                     if (mine) z = *(const sw_f32x4 *)(qp + 16 * k + 8 * h + 4 * j);
 #pragma unroll
                     for (int e = 0; e < 4; e++) y[4 * j + e] = TYPE == SW_KV_F16 ? ldexpf(z[e], up) : z[e];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[4 * j + e] = sc == 0.f ? 0.f : sc < 0.f ? -y[4 * j + e] : y[4 * j + e];
                 }
                 f.query(k, y);
             }
@@ -131,17 +135,14 @@ __global__ __launch_bounds__(FL_NT, (tr_occ<TYPE, DH>())) void k_tree(SwKv c, Sw
             int lane_ = lane;
             asm volatile("" : "+v"(lane_));                            // (the pieces' places are taken anew, not kept in registers)
             const FlPages g = fl_pages(table, t.max_pages, c.n_pages, c.psh, t0);
-            auto from_pool = [&](const char *pool, int nch, int turn7, int loads, uint32_t to) {
-#pragma unroll
-                for (int k = 0; k < loads; k++) {
-                    const int kk = min(k * WC + wc, nch / 2 - 1), p = kk * 64 + lane_, tok = p / nch;
-                    const int ch = (p - tok * nch) ^ (turn7 ? tok & 7 : (tok >> 1) & 3);
-                    const int g01 = tok & 8 ? g.p[1] : g.p[0], g23 = tok & 8 ? g.p[3] : g.p[2], page = tok & 16 ? g23 : g01;
-                    fl_load16(pool + (int64_t)max(page, 0) * psb + (int64_t)((t0 + tok) & pmask) * tsb + ch * 16, to + kk * 1024);
-                }
-            };
-            from_pool(kp, F::NCK, F::MK == 7, LK, lds);
-            from_pool(vp, F::NCV, F::MV == 7, LV, lds + 32 * F::RBK);
+            if (near && c.psh >= 5) {                                  // one page, rows not far apart
+                const int64_t at = (int64_t)max(g.p[0], 0) * psb + (int64_t)(t0 & pmask) * tsb;
+                fl_rows<F::NCK, F::MK, WC, LK>(kp + at, (uint32_t)tsb, wc, lane_, lds);
+                fl_rows<F::NCV, F::MV, WC, LV>(vp + at, (uint32_t)tsb, wc, lane_, lds + 32 * F::RBK);
+            } else {
+                fl_rows_any<F::NCK, F::MK, WC, LK>(kp, g, psb, tsb, t0, pmask, F::NCK, wc, lane_, lds);
+                fl_rows_any<F::NCV, F::MV, WC, LV>(vp, g, psb, tsb, t0, pmask, F::NCV, wc, lane_, lds + 32 * F::RBK);
+            }
             return g.ok;
         };
         int lo_all = 0;                                                // the last cell at which a column's window begins

@@ -9,7 +9,7 @@
 // one in work.  Of a row's 16-byte pieces, piece i of token t lies at i ^ x(t), so that neither the scores'
 // reads (one piece of 32 tokens) nor the outputs' (32 pieces of a token) meet on a bank; the
 // loading lanes pick their source address accordingly.  An output's operand wants 8 tokens of a value
-// where memory has 8 values of a token: a lane reads 8 x 8 and transposes them by byte permutations.
+// where memory has 8 values of a token: transposing reads bring them so.
 //
 // The waves of a block share columns, tokens or values: WC of them have 32 columns each and read
 // the same tile, and 4 / WC groups of them take every (4 / WC)-th tile.  Or (SPLIT > 1, where queries and outputs of a cell's width
@@ -27,6 +27,13 @@ typedef float fl_f32x16 __attribute__((ext_vector_type(16)));
 __device__ __forceinline__ int fl_uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int64_t fl_uni(int64_t x) {
     return (int64_t)(((uint64_t)(uint32_t)fl_uni((int)(x >> 32)) << 32) | (uint32_t)fl_uni((int)x));
+}
+// the lane, for places in LDS that are taken anew for each tile: kept, they would take the registers that the queries need
+template <bool KEEP = false>
+__device__ __forceinline__ int fl_lane() {
+    int lane = threadIdx.x & 63;
+    if (!KEEP) asm volatile("" : "+v"(lane));
+    return lane;
 }
 __device__ __forceinline__ float fl_max2(float x) {                    // over the two lanes of a column
     const uint2 a = sw_pair<32>(__builtin_bit_cast(uint32_t, x));
@@ -48,6 +55,10 @@ __device__ __forceinline__ fl_f32x16 fl_mfma(sw_u32x4 a, sw_u32x4 b, fl_f32x16 c
 // with its others (vmcnt); fl_wait waits for all but the last N.
 __device__ __forceinline__ void fl_load16(const void *g, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(lds), "v"(g) : "memory");
+}
+// the same from a scalar base and a lane's 32-bit offset
+__device__ __forceinline__ void fl_load16(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(off), "s"(base) : "memory");
 }
 template <int N> __device__ __forceinline__ void fl_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 __device__ __forceinline__ void fl_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -83,6 +94,47 @@ __device__ __forceinline__ FlPages fl_pages(const int *table, int max_pages, int
     return g;
 }
 
+// By how much (an exclusive or) a row's pieces are turned in LDS: M 7 and 3 for the scores' reads, one piece of 32 tokens (rows of whole 128 bytes, or
+// of odd 64); 6 and 0 for the outputs', two pieces of four tokens.
+template <int M> __device__ __forceinline__ int fl_turn(int t) { return M == 7 ? t & 7 : M == 3 ? (t >> 1) & 3 : M == 6 ? 2 * (t & 3) : 0; }
+// Rows of NCH 16-byte pieces from `base` on, `step` bytes apart (below 2^26), into a tile at `to`: wave w of W's share, N loads of it.
+// M: the pieces' turn by token.
+template <int NCH, int M, int W, int N>
+__device__ __forceinline__ void fl_rows(const char *base, uint32_t step, int w, int lane, uint32_t to) {
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const int kk = (N * W > NCH / 2) ? min(k * W + w, NCH / 2 - 1) : k * W + w;
+        if constexpr (64 % NCH == 0 && 64 / NCH <= 8 && M != 3) {      // a load is some whole rows: a part of the turn is the wave's
+            constexpr int RP = 64 / NCH;
+            const uint32_t off = lane / NCH * step + ((lane % NCH ^ fl_turn<M>(lane / NCH) ^ fl_turn<M>(kk * RP)) * 16);
+            fl_load16(base + (int64_t)kk * RP * step, off, to + kk * 1024);
+        } else {
+            const int p = kk * 64 + lane, tok = p / NCH, ch = (p - tok * NCH) ^ fl_turn<M>(tok);
+            fl_load16(base, tok * step + ch * 16, to + kk * 1024);
+        }
+    }
+}
+// The same from pages that end inside the tile, or rows far apart or shorter than the tile's (real pieces of them, then zeros): cell
+// of token t0 + k in page g.p[k / 8].
+template <int NCH, int M, int W, int N>
+__device__ __forceinline__ void fl_rows_any(const char *pool, const FlPages &g, int64_t page, int64_t step, int t0, int pmask, int real, int w, int lane,
+                                            uint32_t to) {
+#pragma unroll 1
+    for (int k = 0; k < N; k++) {
+        const int kk = min(k * W + w, NCH / 2 - 1), p = kk * 64 + lane, tok = p / NCH, ch = (p - tok * NCH) ^ fl_turn<M>(tok);
+        const int g01 = tok & 8 ? g.p[1] : g.p[0], g23 = tok & 8 ? g.p[3] : g.p[2], x = tok & 16 ? g23 : g01;
+        const char *a = pool + (int64_t)max(x, 0) * page + (int64_t)((t0 + tok) & pmask) * step + ch * 16;
+        fl_load16(ch < real ? a : (const char *)&g_fl_zero, to + kk * 1024);
+    }
+}
+
+// x plus two 16-bit values
+template <int TYPE>
+__device__ __forceinline__ float fl_sum(uint32_t w, float x) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    if constexpr (TYPE == SW_KV_BF16) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), b2{(__bf16)1.f, (__bf16)1.f}, x, false);
+    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(sw_half2, w), sw_half2{(_Float16)1.f, (_Float16)1.f}, x, false);
+}
 // parts of 8 values: one (to nearest), three bf16 (by truncation, each takes the next 8 bits: exact) or two f16
 template <int TYPE, int NP>
 __device__ __forceinline__ void fl_split(const float (&x)[8], sw_u32x4 (&o)[NP]) {
@@ -98,6 +150,15 @@ __device__ __forceinline__ void fl_split(const float (&x)[8], sw_u32x4 (&o)[NP])
             for (int i = 0; i < 8; i++) h[i] = (_Float16)x[i];
             o[0] = __builtin_bit_cast(sw_u32x4, h);
         }
+    } else if constexpr (TYPE == SW_KV_BF16 && NP == 2) {
+        sw_bf16x8 hi, lo;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            hi[i] = (__bf16)x[i];
+            lo[i] = (__bf16)(x[i] - (float)hi[i]);
+        }
+        o[0] = __builtin_bit_cast(sw_u32x4, hi);
+        o[1] = __builtin_bit_cast(sw_u32x4, lo);
     } else if constexpr (TYPE == SW_KV_BF16) {
         uint32_t b[8], m[8], z[8];
 #pragma unroll
@@ -127,9 +188,10 @@ __device__ __forceinline__ void fl_split(const float (&x)[8], sw_u32x4 (&o)[NP])
 
 // A wave's 32 columns.  NP: parts that a 32-bit q and the weights are split into (1: 16-bit queries, one
 // rounding of the weights).  DK: values of a query, a multiple of 32; DV: of an output; INK: a cell's
-// first DV values of k are its v.  AHEAD: dwords of a row that a lane reads at once (8 rows of them), and twice the scores' steps read
-// ahead: registers for it.
-template <int TYPE, int NP, int DK, int DV, bool INK, int SPLIT = 1, int AHEAD = 4>
+// first DV values of k are its v.  QL: steps of the scores whose queries wait in LDS, where registers would not hold them.  AHEAD: dwords of a row that a lane reads at once, 8 rows of them.  How
+// much is read ahead of the products goes by the registers that queries and outputs leave: a spilled one would be a load in the loop, and
+// waiting for it would wait for every tile on its way.
+template <int TYPE, int NP, int DK, int DV, bool INK, int SPLIT = 1, int QL = 0, int AHEAD = 2>
 struct Fl {
     static constexpr bool F32 = TYPE == SW_KV_F32;
     static constexpr int ES = F32 ? 4 : 2, RBK = DK * ES, RBV = INK ? RBK : DV * ES;                   // bytes of a row of k, of v
@@ -137,33 +199,41 @@ struct Fl {
     static constexpr int TB = 32 * RBK + (INK ? 0 : 32 * RBV);                                         // bytes of a tile
     static constexpr int DKS = RBK / 32 / SPLIT, DVW = DV / SPLIT, NO = DVW / 32, VB = DVW * ES;       // a wave's share: steps of the scores, values
     static_assert(RBK / 32 % SPLIT == 0 && (SPLIT == 1 || (DVW % 64 == 0 && RBK % 128 == 0)), "whole shares");
+    static_assert(SPLIT == 1 || SPLIT == 2 || SPLIT == 4, "pairs");
+    static constexpr int HELD = (F32 ? 1 : NP) * (DKS - QL) * 4 + NO * 16;
+    static constexpr bool KEEP = HELD <= 128;                          // room for places in LDS
+    static constexpr int PIPE = HELD <= 144 ? 2 : 1, QB = HELD <= 144 && NP == 1 && !F32 ? 4 : 2, VT = HELD <= 144 ? 4 : 2;
     static constexpr int XB = SPLIT > 1 ? 4096 : 0;                                                    // bytes of a wave in the exchange
-    // where a piece of a row lies: its low bits turned by the token
-    static constexpr int MK = NCK % 8 == 0 ? 7 : 3, MV = INK ? MK : NCV % 8 == 0 ? 7 : 3;
-    template <int M> static __device__ __forceinline__ int turn(int t) { return M == 7 ? t & 7 : (t >> 1) & 3; }
+    // how a row's pieces are turned
+    static constexpr int MK = NCK % 8 == 0 ? 7 : 3, MV = INK ? MK : F32 ? (NCV % 8 == 0 ? 7 : 3) : NCV % 8 == 0 ? 6 : 0;
     // weights are kept below 2^OFF; a maximum may lag behind by LAG powers of two (a running maximum that grows costs a pass
     // over the outputs; 16-bit weights hold 2^8 as well as 1, in parts they may not)
+    static constexpr int PP = NP > 2 ? 2 : NP;                         // parts of a weight
     static constexpr float LAG = NP == 1 && !F32 ? 8.f : 0.f;
     static constexpr float OFF = TYPE != SW_KV_F16 ? 0.f : NP == 1 ? 7.f : 13.f;
 
-    sw_u32x4 Q[F32 ? 1 : NP][DKS];
+    static_assert(QL == 0 || (NP == 1 && !F32), "16-bit queries");
+    static constexpr int QLB = QL * 1024;                              // their bytes of a wave
+    sw_u32x4 Q[F32 ? 1 : NP][DKS - QL];
+    sw_u32x4 *ql;                                                      // this lane's of them, 64 apart
     fl_f32x16 O[NO];
     float m, l, sc;
-    static constexpr int KB = MK == 3 ? 2 : 4 / SPLIT;                 // this lane's places in a tile's row of k: they repeat
-    int kb[KB], share;                                                 // after KB steps (every SPLIT-th is the wave's)
+    static constexpr int KB = MK == 3 ? 2 : 4 / SPLIT;                 // a lane's places in a tile's row of k repeat after KB steps
+    int share;                                                         // (every SPLIT-th step is the wave's)
 
+    // scale: of the scores, in powers of two.  Its sign (and a scale of 0) goes into the queries, see query().
     __device__ __forceinline__ void begin(float scale, int share_ = 0) {
-        const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
         m = -INFINITY;
         l = 0.f;
-        sc = scale;
+        sc = scale == 0.f ? 1.f : fabsf(scale);
 #pragma unroll
         for (int i = 0; i < NO; i++)
 #pragma unroll
             for (int j = 0; j < 16; j++) O[i][j] = 0.f;
-#pragma unroll
-        for (int i = 0; i < KB; i++) kb[i] = c * RBK + (((2 * (SPLIT * i + share_) + h) ^ turn<MK>(c)) * 16);
         share = share_;
+    }
+    static __device__ __forceinline__ uint32_t signed_by(uint32_t w, float scale) {   // two 16-bit values (or one of 32) times the scale's sign
+        return scale == 0.f ? 0u : scale < 0.f ? w ^ (F32 ? 0x80000000u : 0x80008000u) : w;
     }
     // 8 values 16 i + 8 h .. of a 32-bit query (f32 cells: 4 of them, 8 i + 4 h ..); f16 in parts: called after scale_up
     __device__ __forceinline__ void query(int i, const float (&x)[8]) {
@@ -171,57 +241,82 @@ struct Fl {
             sw_u32x4 o[NP];
             fl_split<TYPE, NP>(x, o);
 #pragma unroll
-            for (int u = 0; u < NP; u++) Q[u][i] = o[u];
+            for (int u = 0; u < NP; u++) Q[u][i - QL] = o[u];
         }
     }
 
-    // the scores of the tile at `t`, times the scale
-    __device__ __forceinline__ void scores(const char *t, float (&x)[16], char *xch, int wave) const {
-        fl_f32x16 s = {};
+    // the scores of the tile at `t`, not yet times the scale: a wave's share of their sums added to s, and all of them
+    __device__ __forceinline__ void dot(const char *t, fl_f32x16 &s) const {
+        // QB steps' operands are read while the QB before are multiplied
+        constexpr int NB = (DKS + QB - 1) / QB;
+        const int lane = fl_lane<KEEP>(), c = lane & 31, h = lane >> 5;
+        int kb[KB];
 #pragma unroll
-        for (int i = 0; i < DKS; i++) {
-            const sw_u32x4 a = *(const sw_u32x4 *)(t + kb[i % KB] + i / KB * (KB * SPLIT * 32));
-            if constexpr (F32) {
-                const sw_f32x4 y = __builtin_bit_cast(sw_f32x4, a), z = __builtin_bit_cast(sw_f32x4, Q[0][i]);
+        for (int i = 0; i < KB; i++) kb[i] = c * RBK + (((2 * (SPLIT * i + share) + h) ^ fl_turn<MK>(c)) * 16);
+        sw_u32x4 a[2][QB], w[2][QL ? QB : 1];
+        auto read = [&](int b) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_32x32x2f32(y[e], z[e], s, 0, 0, 0);
-            } else {
+            for (int k = 0; k < QB; k++)
+                if (b * QB + k < QL) w[b & 1][QL ? k : 0] = ql[(b * QB + k) * 64];
 #pragma unroll
-                for (int u = 0; u < NP; u++) s = fl_mfma<TYPE>(a, Q[u][i], s);
+            for (int k = 0; k < QB; k++)
+                if (b * QB + k < DKS) a[b & 1][k] = *(const sw_u32x4 *)(t + kb[(b * QB + k) % KB] + (b * QB + k) / KB * (KB * SPLIT * 32));
+        };
+        read(0);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            if (b + 1 < NB) read(b + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < QB; k++) {
+                const int i = b * QB + k;
+                if (i >= DKS) break;
+                if constexpr (F32) {
+                    const sw_f32x4 y = __builtin_bit_cast(sw_f32x4, a[b & 1][k]), z = __builtin_bit_cast(sw_f32x4, Q[0][i]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_32x32x2f32(y[e], z[e], s, 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < NP; u++) s = fl_mfma<TYPE>(a[b & 1][k], i < QL ? w[b & 1][QL ? k : 0] : Q[u][i < QL ? 0 : i - QL], s);
+                }
             }
-            if (i % (2 * AHEAD) == 2 * AHEAD - 1) __builtin_amdgcn_sched_barrier(0);     // (reads of the whole row ahead would spill)
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (SPLIT > 1) {                                     // the shares in their order: the same sum in every wave
-            sw_f32x4 *to = (sw_f32x4 *)xch + (threadIdx.x & 63);
+        __builtin_amdgcn_s_setprio(0);
+    }
+    __device__ __forceinline__ void scores(const char *t, fl_f32x16 &s, char *xch, int wave) const {
+        s = fl_f32x16{};
+        dot(t, s);
+        if constexpr (SPLIT > 1) {                                     // pairs, then pairs of them: the same sum in every wave
+            sw_f32x4 *to = (sw_f32x4 *)xch + fl_lane();
 #pragma unroll
             for (int j = 0; j < 4; j++) to[(wave * 4 + j) * 64] = sw_f32x4{s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]};
             __syncthreads();
-            const int w0 = wave - share;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                sw_f32x4 y = to[(w0 * 4 + j) * 64];
+                sw_f32x4 y = to[((wave ^ 1) * 4 + j) * 64];
 #pragma unroll
-                for (int k = 1; k < SPLIT; k++) {
-                    const sw_f32x4 z = to[((w0 + k) * 4 + j) * 64];
+                for (int e = 0; e < 4; e++) s[4 * j + e] = s[4 * j + e] + y[e];
+                if constexpr (SPLIT == 4) {
+                    y = to[((wave ^ 2) * 4 + j) * 64];
+                    const sw_f32x4 z = to[((wave ^ 3) * 4 + j) * 64];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) y[e] = y[e] + z[e];
+                    for (int e = 0; e < 4; e++) s[4 * j + e] = s[4 * j + e] + (y[e] + z[e]);
                 }
-#pragma unroll
-                for (int e = 0; e < 4; e++) s[4 * j + e] = y[e];
             }
         }
-#pragma unroll
-        for (int j = 0; j < 16; j++) x[j] = s[j] * sc;
     }
 
-    // scores (masked ones -INFINITY) to weights; the outputs follow a maximum that grew
-    __device__ __forceinline__ void weights(float (&x)[16]) {
-        float mx = x[0];
+    // scores (masked ones -INFINITY) to weights; the outputs follow a maximum that grew.  (16-bit weights are summed as they are rounded, in outputs().)
+    static constexpr bool SUMS = !F32 && PP == 1;
+    __device__ __forceinline__ void weights(const fl_f32x16 &s, float (&x)[16]) {
+        float mx = s[0];
 #pragma unroll
-        for (int j = 1; j < 16; j++) mx = fmaxf(mx, x[j]);
+        for (int j = 1; j < 16; j++) mx = fmaxf(mx, s[j]);
         const float nm = fl_max2(mx);
-        if (__any(nm > m + LAG)) {
-            const float n = fmaxf(m, nm), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - n);
+        if (__any(LAG == 0.f ? nm > m : (nm - m) * sc > LAG)) {
+            const float n = fmaxf(m, nm), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - n) * sc);
             l = l * f;
 #pragma unroll
             for (int i = 0; i < NO; i++)
@@ -229,11 +324,11 @@ struct Fl {
                 for (int j = 0; j < 16; j++) O[i][j] = O[i][j] * f;
             m = n;
         }
-        const float base = m == -INFINITY ? 0.f : m - OFF;
+        const float base = m == -INFINITY ? 0.f : OFF - m * sc;
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-            x[j] = __builtin_amdgcn_exp2f(x[j] - base);
-            l = l + x[j];
+            x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], sc, base));
+            if constexpr (!SUMS) l = l + x[j];
         }
     }
 
@@ -243,29 +338,99 @@ struct Fl {
         return ((w & E) == E ? 0xFFFFu : 0u) | ((w & (E << 16)) == E << 16 ? 0xFFFF0000u : 0u);
     }
 
-    // O += V^T P
-    __device__ __forceinline__ void outputs(const char *t, const float (&p)[16]) {
-        int lane = threadIdx.x & 63;
-        asm volatile("" : "+v"(lane));                                 // (the places are taken anew for each tile, not kept)
-        const int c = lane & 31, h = lane >> 5;
+    // O += V^T P.  Operands are read while those before are multiplied; the first are in `first`.
+    // 16-bit cells: an operand is 32 values of 16 tokens, 8 of a lane, where memory has the values side by side: two transposing reads, by which 16
+    // lanes fetch 4 tokens' 16 values and each gets one value of the four.  VT operands at a time, output tile o values 32 o ...
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    // f32 cells: a lane's piece of a row (AHEAD values) is an operand of as many tiles; four tokens at a time, groups of values by rising width
+    static constexpr int NG = NO + 1;
+    struct Steps { int n, b0[NG], w[NG], o0[NG]; };
+    static constexpr Steps steps() {
+        Steps s = {};
+        int b = 0, o = 0, w = AHEAD;
+        while (b < VB) {
+            while (b + 128 * w > VB) w /= 2;
+            s.b0[s.n] = b; s.w[s.n] = w; s.o0[s.n] = o; s.n++;
+            b += 128 * w;
+            o += w;
+        }
+        return s;
+    }
+    static constexpr int NST = F32 ? 4 * steps().n : (2 * NO + VT - 1) / VT;
+    struct Piece { uint32_t v[F32 ? 4 * AHEAD : 4 * VT]; };
+    static __device__ __forceinline__ void read(const char *t, int step, Piece &p) {
+        const int lane = fl_lane<KEEP>();
         if constexpr (F32) {
+            constexpr Steps S = steps();
+            const int lot = step / S.n, g = step % S.n, w = S.w[g], c = lane & 31, h = lane >> 5;
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const int x = MV == 7 ? 4 * h + j % 4 : 2 * h + ((j % 4) >> 1);
-                group_f32<AHEAD, 0, 0>(t + (8 * (j / 4) + j % 4 + 4 * h) * RBV, x, c, p[j]);
-                if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            for (int k = 0; k < 4; k++) {
+                const int x = MV == 7 ? 4 * h + k : 2 * h + (k >> 1);
+                const char *row = t + (8 * lot + k + 4 * h) * RBV + S.b0[g];
+                if (w == 2) {
+                    const uint2 y = *(const uint2 *)(row + ((c >> 1) ^ x) * 16 + (c & 1) * 8);
+                    p.v[AHEAD * k] = y.x; p.v[AHEAD * k + 1] = y.y;
+                } else p.v[AHEAD * k] = *(const uint32_t *)(row + ((c >> 2) ^ x) * 16 + (c & 3) * 4);
             }
         } else {
+            const int k = 4 * (lane >> 5) + ((lane & 15) >> 2), d = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), x = fl_turn<MV>(k);
+            const char *row = t + k * RBV + (lane & 1) * 8;
 #pragma unroll
-            for (int mm = 0; mm < 2; mm++) {
-                float p8[8];
+            for (int i = 0; i < VT; i++) {
+                const int at = step * VT + i, lot = at / NO, o = at % NO;
+                if (at >= 2 * NO) break;
 #pragma unroll
-                for (int j = 0; j < 8; j++) p8[j] = p[8 * mm + j];
-                sw_u32x4 P[NP];
-                fl_split<TYPE, NP>(p8, P);
-                group<AHEAD, 0, 0>(t + 16 * mm * RBV + 4 * h * RBV, c, h, P);
+                for (int b = 0; b < 2; b++) {
+                    const int piece = MV == 7 || MV == 6 ? ((4 * (o & 1) + d) ^ x) + 8 * (o >> 1) : (d ^ x) + 4 * o;
+                    const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(row + (16 * lot + 8 * b) * RBV + piece * 16));
+                    const uint2 z = __builtin_bit_cast(uint2, y);
+                    p.v[4 * i + 2 * b] = z.x; p.v[4 * i + 2 * b + 1] = z.y;
+                }
             }
         }
+    }
+    __device__ __forceinline__ void outputs(const char *t, const float (&p)[16], Piece &first) {
+        Piece v[PIPE];
+        v[0] = first;
+        sw_u32x4 P[2][F32 ? 1 : PP];
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int s = 0; s < NST; s++) {
+            if (PIPE == 1 && s > 0) read(t, s, v[0]);
+            if (PIPE == 2 && s + 1 < NST) read(t, s + 1, v[(s + 1) % PIPE]);
+            __builtin_amdgcn_sched_barrier(0);
+            Piece &y = v[s % PIPE];
+            if constexpr (F32) {
+                constexpr Steps S = steps();
+                const int lot = s / S.n, g = s % S.n;
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int e = 0; e < S.w[g]; e++)
+                        O[S.o0[g] + e] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, y.v[AHEAD * k + e]), p[4 * lot + k], O[S.o0[g] + e], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VT; i++) {
+                    const int at = s * VT + i, lot = at / NO, o = at % NO;
+                    if (at >= 2 * NO) break;
+                    if (o == 0) {
+                        float p8[8];
+#pragma unroll
+                        for (int j = 0; j < 8; j++) p8[j] = p[8 * lot + j];
+                        fl_split<TYPE, PP>(p8, P[lot]);
+                        if constexpr (SUMS)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) l = fl_sum<TYPE>(P[lot][0][j], l);
+                    }
+                    const sw_u32x4 a = {y.v[4 * i], y.v[4 * i + 1], y.v[4 * i + 2], y.v[4 * i + 3]};
+#pragma unroll
+                    for (int u = 0; u < PP; u++) O[o] = fl_mfma<TYPE>(a, P[lot][u], O[o]);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
     }
     // Infinities and NaN among the values of a tile's v, in wave w of n's share, become 0 (a weight of 0 times one of them is none);
     // the tokens that had one are marked in `bad`.
@@ -288,98 +453,43 @@ struct Fl {
         }
         if (met) atomicOr(bad, met);
     }
-    // the values from byte B0 on (output tiles from O0 on), W dwords of a row a lane
-    template <int W, int B0, int O0>
-    __device__ __forceinline__ void group(const char *t, int c, int h, const sw_u32x4 (&P)[NP]) {
-        if constexpr (B0 + 32 * 4 * W <= VB) {
-            uint32_t v[8][W];
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const int x = MV == 7 ? 4 * h + k % 4 : 2 * h + ((k % 4) >> 1);
-                const char *a = t + (8 * (k / 4) + k % 4) * RBV + B0 + (((c * W / 4) ^ x) * 16 + (c * W % 4) * 4);
-                if constexpr (W == 4) {
-                    const sw_u32x4 y = *(const sw_u32x4 *)a;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[k][e] = y[e];
-                } else if constexpr (W == 2) {
-                    const uint2 y = *(const uint2 *)a;
-                    v[k][0] = y.x; v[k][1] = y.y;
-                } else v[k][0] = *(const uint32_t *)a;
-            }
-#pragma unroll
-            for (int e = 0; e < 2 * W; e++) {
-                sw_u32x4 a;
-#pragma unroll
-                for (int i = 0; i < 4; i++) a[i] = __builtin_amdgcn_perm(v[2 * i + 1][e / 2], v[2 * i][e / 2], e & 1 ? 0x07060302 : 0x05040100);
-#pragma unroll
-                for (int u = 0; u < NP; u++) O[O0 + e] = fl_mfma<TYPE>(a, P[u], O[O0 + e]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            group<W, B0 + 128 * W, O0 + 2 * W>(t, c, h, P);
-        } else if constexpr (W > 1) {
-            group<W / 2, B0, O0>(t, c, h, P);
-        } else if constexpr (B0 < VB) {                                // 32 values left: two bytes a lane
-            uint32_t v[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const int x = MV == 7 ? 4 * h + k % 4 : 2 * h + ((k % 4) >> 1);
-                v[k] = *(const uint16_t *)(t + (8 * (k / 4) + k % 4) * RBV + B0 + (((c / 8) ^ x) * 16 + c % 8 * 2));
-            }
-            sw_u32x4 a;
-#pragma unroll
-            for (int i = 0; i < 4; i++) a[i] = v[2 * i] | (v[2 * i + 1] << 16);
-#pragma unroll
-            for (int u = 0; u < NP; u++) O[O0] = fl_mfma<TYPE>(a, P[u], O[O0]);
-        }
-    }
-    template <int W, int B0, int O0>
-    __device__ __forceinline__ void group_f32(const char *row, int x, int c, float p) {
-        if constexpr (B0 + 32 * 4 * W <= VB) {
-            uint32_t v[W];
-            const char *a = row + B0 + (((c * W / 4) ^ x) * 16 + (c * W % 4) * 4);
-            if constexpr (W == 4) {
-                const sw_u32x4 y = *(const sw_u32x4 *)a;
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = y[e];
-            } else if constexpr (W == 2) {
-                const uint2 y = *(const uint2 *)a;
-                v[0] = y.x; v[1] = y.y;
-            } else v[0] = *(const uint32_t *)a;
-#pragma unroll
-            for (int e = 0; e < W; e++)
-                O[O0 + e] = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, v[e]), p, O[O0 + e], 0, 0, 0);
-            group_f32<W, B0 + 128 * W, O0 + W>(row, x, c, p);
-        } else if constexpr (W > 1) group_f32<W / 2, B0, O0>(row, x, c, p);
-    }
-
     // One tile.  whole: every column attends to all of its tokens, else seen(token of the tile) says it for this lane's column, and bit k of
     // bad that token k's v is no number: whoever attends to it has no meaningful output.
     template <class Seen>
     __device__ __forceinline__ void tile(const char *t, bool whole, uint32_t bad, Seen seen, char *xch, int wave) {
-        float x[16];
-        scores(t, x, xch, wave);
+        fl_f32x16 s;
+        scores(t, s, xch, wave);
+        rest(t, whole, bad, seen, s);
+    }
+    template <class Seen>
+    __device__ __forceinline__ void rest(const char *t, bool whole, uint32_t bad, Seen seen, fl_f32x16 &s) {
+        const char *v = (INK ? t : t + 32 * RBK) + (SPLIT > 1 ? share * VB : 0);
         if (!whole) {
             const int h4 = (threadIdx.x & 32) >> 3;
             uint32_t met = 0;
 #pragma unroll
             for (int j = 0; j < 16; j++) {
                 const int k = 8 * (j / 4) + h4 + j % 4;
-                const bool s = seen(k);
-                if (!s) x[j] = -INFINITY;
-                else met |= bad >> k & 1;
+                const bool in = seen(k);
+                s[j] = in ? s[j] : -INFINITY;
+                met |= in ? bad >> k & 1 : 0u;
             }
             if (met) l = NAN;
         }
-        weights(x);
-        outputs((INK ? t : t + 32 * RBK) + (SPLIT > 1 ? share * VB : 0), x);
+        Piece first;
+        read(v, 0, first);
+        __builtin_amdgcn_sched_barrier(0);
+        float x[16];
+        weights(s, x);
+        outputs(v, x, first);
     }
 
-    // Where an output's values lie: tile o's row r is value d0 + T r + e of a group of values that T tiles share (groups of 256
-    // values (f32: 128), 128, 64 and 32), tile o being its e-th.
+    // Where an output's values lie: tile o's row r is value d0 + T r + e of a group of values that T tiles share (f32: groups of 64 and 32
+    // values; else T is 1), tile o being its e-th.
     struct Map { int d0[NO], tiles[NO], e[NO]; };
     static constexpr Map map() {
         Map m = {};
-        int d = 0, w = F32 ? AHEAD : 2 * AHEAD;
+        int d = 0, w = F32 ? AHEAD : 1;
         for (int at = 0; at < NO; at += w) {
             while (d + 32 * w > DVW) w /= 2;
             for (int e = 0; e < w; e++) { m.d0[at + e] = d; m.tiles[at + e] = w; m.e[at + e] = e; }
@@ -451,16 +561,16 @@ __device__ __forceinline__ void fl_end(F &f, char *sh, float (*s_m)[32], float (
     constexpr int DVW = F::DVW, LD = DVW / 4 + 4, NO = F::NO, NT = WC * WT * SPLIT * 64;
     constexpr auto map = F::map();
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
-    const float l = fl_sum2(f.l);
+    const float l = fl_sum2(f.l), m = f.m * f.sc;                      // (from here on the maximum is times the scale)
     __syncthreads();                                                   // the tiles are done with
-    if (h == 0) { s_m[wave][c] = f.m; s_l[wave][c] = l; }
+    if (h == 0) { s_m[wave][c] = m; s_l[wave][c] = l; }
     __syncthreads();
     float g = 1.f;
     if constexpr (WT > 1) {
-        float M = f.m;
+        float M = m;
 #pragma unroll
         for (int i = 0; i < WT; i++) M = fmaxf(M, s_m[i * WC + wave % WC][c]);
-        g = f.m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(f.m - M);
+        g = m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m - M);
     }
     float *so = (float *)sh + (wave * 32 + c) * LD;
 #pragma unroll
