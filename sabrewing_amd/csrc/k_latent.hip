@@ -210,14 +210,12 @@ int sw_launch_latent_heads(hipStream_t st, int type, const SwHeads &x, const voi
 
 // ------------------------------------------------------------------ the absorbed form ----
 #define LN_ROPE 64                                                     // a cell's rotary part in LDS: the rest of it zeros
-#define LN_LEAST 4
 #define LN_SPLIT 256                                                   // beyond so many rows none is split
-// waves that share 32 heads, their groups a block, and tiles in LDS
-template <int R, int WC> constexpr int ln_split() { return WC < 4 && R % 256 == 0 ? 4 : 2; }
-template <int R, int WC> constexpr int ln_ql() { return R > 384 && WC == 4 ? 4 : 0; }
-template <int TYPE, int R, int WC> using LnFl = Fl<TYPE, 1, R + LN_ROPE, R, true, ln_split<R, WC>(), ln_ql<R, WC>()>;
+// waves that share 32 heads (a share of the outputs is whole pairs of 32 values), and tiles in LDS
+template <int R> constexpr int ln_split() { return R % 256 == 0 ? 4 : 2; }
+template <int TYPE, int R> using LnFl = Fl<TYPE, 1, R + LN_ROPE, R, true, ln_split<R>()>;
 template <int R, int WC> constexpr int ln_ns() {
-    constexpr int n = (156 * 1024 - WC * ln_split<R, WC>() * (4 + ln_ql<R, WC>()) * 1024) / (32 * (R + LN_ROPE) * 2);
+    constexpr int n = (156 * 1024 - WC * ln_split<R>() * 5 * 1024) / (32 * (R + LN_ROPE) * 2);
     return n > 4 ? 4 : n;
 }
 struct LnRow { int seq, last; };
@@ -228,12 +226,12 @@ __device__ __forceinline__ LnRow ln_row(const SwLatent &c, const SwRows &r, int 
     return x;
 }
 template <int TYPE, int R, int WC>
-__global__ __launch_bounds__((64 * WC * ln_split<R, WC>())) void k_latent(SwLatent c, SwRows r, const uint16_t *__restrict__ q, int S, int H, float sc,
+__global__ __launch_bounds__((64 * WC * ln_split<R>())) void k_latent(SwLatent c, SwRows r, const uint16_t *__restrict__ q, int S, int H, float sc,
                                                                 uint16_t *__restrict__ out, float *__restrict__ part, int B) {
-    using F = LnFl<TYPE, R, WC>;
-    constexpr int SPLIT = ln_split<R, WC>(), QL = ln_ql<R, WC>(), NW = WC * SPLIT, NT = 64 * NW;
+    using F = LnFl<TYPE, R>;
+    constexpr int SPLIT = ln_split<R>(), NW = WC * SPLIT, NT = 64 * NW;
     constexpr int CW = 32 * WC, NS = ln_ns<R, WC>(), NL = (F::NCK / 2 + NW - 1) / NW;
-    constexpr int SHT = NS * F::TB + NW * (F::XB + F::QLB), SHB = SHT > fl_end_bytes<F, NW>() ? SHT : fl_end_bytes<F, NW>();
+    constexpr int SHT = NS * F::TB + NW * F::XB, SHB = SHT > fl_end_bytes<F, NW>() ? SHT : fl_end_bytes<F, NW>();
     static_assert(SHB <= 157 * 1024 && (NS < 3 ? 0 : NS - 2) * NL < 64, "LDS, and loads that a wave can count");
     __shared__ __align__(16) char sh[SHB];
     __shared__ float s_m[NW][32], s_l[NW][32];
@@ -248,7 +246,7 @@ __global__ __launch_bounds__((64 * WC * ln_split<R, WC>())) void k_latent(SwLate
     int64_t at = 0, end = 1, before = 0;
     int s = b;
     if (B) {
-        const FlDeal deal = fl_deal(S, B, LN_LEAST, count);
+        const FlDeal deal = fl_deal(S, B, (int64_t)H * R, count);
         at = (int64_t)b * deal.q;
         end = at + deal.q < deal.N ? at + deal.q : deal.N;
         if (at >= end) return;
@@ -268,8 +266,6 @@ __global__ __launch_bounds__((64 * WC * ln_split<R, WC>())) void k_latent(SwLate
         const int head = c0 + wc * 32 + cl;
         const uint16_t *qp = q + ((int64_t)s * H + head) * width;
         f.begin(sc, share);
-        f.ql = (sw_u32x4 *)(sh + NS * F::TB + NW * F::XB + wave * F::QLB) + lane;
-        if (QL) __syncthreads();                                       // (the item before is done with its LDS)
 #pragma unroll
         for (int k = 0; k < F::DKS; k++) {
             sw_u32x4 y = {0, 0, 0, 0};
@@ -277,8 +273,7 @@ __global__ __launch_bounds__((64 * WC * ln_split<R, WC>())) void k_latent(SwLate
             if (head < H && d < width) y = *(const sw_u32x4 *)(qp + d);
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] = F::signed_by(y[e], sc);
-            if (k < QL) f.ql[k * 64] = y;
-            else f.Q[0][k < QL ? 0 : k - QL] = y;
+            f.Q[0][k] = y;
         }
         const int *table = r.table + (int64_t)x.seq * r.max_pages;
         auto issue = [&](int tile, uint32_t lds) {
@@ -306,7 +301,7 @@ __global__ __launch_bounds__((64 * WC * ln_split<R, WC>())) void k_latent(SwLate
             if (col >= nh) return;
             if (all) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) a[e] = sum == 0.f ? 0.f : a[e] / sum;
+                for (int e = 0; e < 4; e++) a[e] = sum == 0.f ? 0.f : a[e] * (1.f / sum);
                 *(uint2 *)(out + ((int64_t)s * H + c0 + col) * R + d) = make_uint2(lt_pack<TYPE>(a[0], a[1]), lt_pack<TYPE>(a[2], a[3]));
             } else {
                 float *o = pp + col * (R + 4);
@@ -318,35 +313,21 @@ __global__ __launch_bounds__((64 * WC * ln_split<R, WC>())) void k_latent(SwLate
     }
 }
 
-// The parts of a row's heads joined, in their order: R / 4 threads a head.
+// The parts of a row's heads joined: a wave 256 values of a head
 template <int TYPE, int R>
 __global__ __launch_bounds__(FL_NT) void k_latent_join(SwLatent c, SwRows r, int S, int H, const float *__restrict__ part, int B, int CW,
                                                        uint16_t *__restrict__ out) {
-    constexpr int ND = R / 4, NC = FL_NT / ND;
-    const int s = blockIdx.y, head = blockIdx.x * NC + threadIdx.x / ND, d = threadIdx.x % ND * 4;
-    auto count = [&](int k) { return (ln_row(c, r, k).last >> 5) + 1; };
+    constexpr int NV = (R + 255) / 256;
+    const int s = blockIdx.y, k = fl_uni((int)(blockIdx.x * FL_NW + (threadIdx.x >> 6))), head = k / NV, v0 = k % NV * 256, d = v0 + (threadIdx.x & 63) * 4;
+    auto count = [&](int i) { return (ln_row(c, r, i).last >> 5) + 1; };
     const int tiles = count(s);
-    if (tiles == 0) return;
-    const FlDeal deal = fl_deal(S, B, LN_LEAST, count);
+    if (tiles == 0 || head >= H) return;
+    const FlDeal deal = fl_deal(S, B, (int64_t)H * R, count);
     const int64_t before = fl_before(s, count);
     const int b0 = (int)(before / deal.q), parts = (int)((before + tiles - 1) / deal.q) - b0 + 1;
-    if (parts < 2 || threadIdx.x >= ND * NC || head >= H) return;
-    const int64_t step = (int64_t)CW * (R + 4);
-    const float *p = part + (((int64_t)(head / CW) * (B + S) + b0 + s) * CW + head % CW) * (R + 4);
-    float M = -INFINITY, L = 0.f;
-    for (int k = 0; k < parts; k++) M = fmaxf(M, p[k * step]);
-    sw_f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int k = 0; k < parts; k++) {
-        const float m = p[k * step], g = m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m - M);
-        const sw_f32x4 y = *(const sw_f32x4 *)(p + k * step + 4 + d);
-        L = __builtin_fmaf(p[k * step + 1], g, L);
-#pragma unroll
-        for (int e = 0; e < 4; e++) a[e] = __builtin_fmaf(y[e], g, a[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; e++) a[e] = L == 0.f ? 0.f : a[e] / L;
-    *(uint2 *)(out + ((int64_t)s * H + head) * R + d) = make_uint2(lt_pack<TYPE>(a[0], a[1]), lt_pack<TYPE>(a[2], a[3]));
+    if (parts < 2) return;
+    const sw_f32x4 a = fl_join<R>(part + (((int64_t)(head / CW) * (B + S) + b0 + s) * CW + head % CW) * (R + 4), (int64_t)CW * (R + 4), parts, v0);
+    if (d < R && (threadIdx.x & 63) * 4 < R) *(uint2 *)(out + ((int64_t)s * H + head) * R + d) = make_uint2(lt_pack<TYPE>(a[0], a[1]), lt_pack<TYPE>(a[2], a[3]));
 }
 
 // columns of a block (waves that have 32 each) and blocks of each group of heads; 0: a block a row
@@ -355,9 +336,9 @@ static LnPlan ln_plan(const SwLatent &c, const SwRows &r, int H, int S) {
     LnPlan p;
     p.wc = H <= 32 ? 1 : 2;
     p.groups = (H + 32 * p.wc - 1) / (32 * p.wc);
-    const int64_t tiles = ((((int64_t)r.max_pages << c.psh) + 31) / 32) * S, most = (tiles + LN_LEAST - 1) / LN_LEAST;
+    const int64_t tiles = ((((int64_t)r.max_pages << c.psh) + 31) / 32) * S;
     const int n = 256 / p.groups;
-    p.B = S > LN_SPLIT ? 0 : (int)(n < 1 ? 1 : n < most ? n : most);
+    p.B = S > LN_SPLIT ? 0 : (int)(n < 1 ? 1 : n < tiles ? n : tiles);
     return p;
 }
 int64_t sw_latent_part_floats(const SwLatent &c, const SwRows &r, int H, int S) {
@@ -369,12 +350,11 @@ static int ln_launch(hipStream_t st, const SwLatent &c, const SwRows &r, const u
     const LnPlan p = ln_plan(c, r, H, S);
     const int64_t grid = (int64_t)(p.B ? p.B : S) * p.groups;
     if (grid >= (int64_t)1 << 31 || (p.B > 1 && !part)) return -1;
-    if (p.wc == 1) SW_LAUNCH((k_latent<TYPE, R, 1>), dim3((unsigned)grid), dim3(64 * 1 * ln_split<R, 1>()), 0, st, c, r, q, S, H, sc, out, part, p.B);
-    else if (p.wc == 2) SW_LAUNCH((k_latent<TYPE, R, 2>), dim3((unsigned)grid), dim3(64 * 2 * ln_split<R, 2>()), 0, st, c, r, q, S, H, sc, out, part, p.B);
-    else SW_LAUNCH((k_latent<TYPE, R, 4>), dim3((unsigned)grid), dim3(64 * 4 * ln_split<R, 4>()), 0, st, c, r, q, S, H, sc, out, part, p.B);
+    if (p.wc == 1) SW_LAUNCH((k_latent<TYPE, R, 1>), dim3((unsigned)grid), dim3(64 * ln_split<R>()), 0, st, c, r, q, S, H, sc, out, part, p.B);
+    else SW_LAUNCH((k_latent<TYPE, R, 2>), dim3((unsigned)grid), dim3(128 * ln_split<R>()), 0, st, c, r, q, S, H, sc, out, part, p.B);
     if (p.B > 1) {
-        constexpr int NC = FL_NT / (R / 4);
-        SW_LAUNCH((k_latent_join<TYPE, R>), dim3((unsigned)((H + NC - 1) / NC), (unsigned)S), dim3(FL_NT), 0, st, c, r, S, H, part, p.B, 32 * p.wc, out);
+        constexpr int NV = (R + 255) / 256;
+        SW_LAUNCH((k_latent_join<TYPE, R>), dim3((unsigned)((H * NV + FL_NW - 1) / FL_NW), (unsigned)S), dim3(FL_NT), 0, st, c, r, S, H, part, p.B, 32 * p.wc, out);
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }

@@ -204,7 +204,7 @@ struct LpFl : Fl<SW_KV_F16, 1, NOPE, DV, false> {
     static constexpr int ROPE_AT = Base::TB, TB = Base::TB + 32 * LP_ROPE * 2;
     sw_u32x4 R[LP_ROPE / 16];                                          // the queries' rotary part, scaled as the other is with its keys
     template <class Seen>
-    __device__ __forceinline__ void tile(const char *t, bool whole, uint32_t bad, Seen seen, char *, int) {
+    __device__ __forceinline__ void tile(const char *t, bool whole, uint32_t bad, Seen seen, char *, int, int) {
         const int lane = fl_lane<Base::KEEP>(), c = lane & 31, h = lane >> 5;
         fl_f32x16 s = {};
         sw_u32x4 r[LP_ROPE / 16];
@@ -213,7 +213,7 @@ struct LpFl : Fl<SW_KV_F16, 1, NOPE, DV, false> {
         this->dot(t, s);
 #pragma unroll
         for (int i = 0; i < LP_ROPE / 16; i++) s = fl_mfma<TYPE>(r[i], R[i], s);
-        this->rest(t, whole, bad, seen, s);
+        this->alone(t, whole, bad, seen, s);
     }
 };
 template <int NOPE, int DV> constexpr int lp_occ() { return NOPE / 4 + DV / 2 <= 112 ? 2 : 1; }
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(FL_NT, (lp_occ<NOPE, DV>())) void k_prompt(const ui
         const int s = r0 + col;
         if (s >= S || d >= vd) return;
 #pragma unroll
-        for (int e = 0; e < 4; e++) a[e] = sum == 0.f ? 0.f : ldexpf(a[e] / sum, -ev);
+        for (int e = 0; e < 4; e++) a[e] = sum == 0.f ? 0.f : ldexpf(a[e] * (1.f / sum), -ev);
         const int64_t at = ((int64_t)s * H + h) * vd + d;
         if (of32) *(sw_f32x4 *)((float *)out + at) = a;
         else {

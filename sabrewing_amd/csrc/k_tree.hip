@@ -22,7 +22,8 @@ __device__ __forceinline__ int tr_tiles(const TrTree &x, int G, int c0) {
     return x.last < x.first || x.n * G <= c0 ? 0 : (x.last >> 5) - (x.first >> 5) + 1;
 }
 
-#define TR_LEAST 4
+// outputs of a tree with all its nodes
+__host__ __device__ inline int64_t tr_values(const SwTrees &t, int Hq, int dh) { return (int64_t)t.max_nodes * Hq * dh; }
 template <int TYPE> constexpr int tr_np() { return TYPE == SW_KV_F32 ? 1 : TYPE == SW_KV_BF16 ? 3 : 2; }
 template <int TYPE, int DH> using TrFl = Fl<TYPE, tr_np<TYPE>(), DH, DH, false>;
 template <int TYPE, int DH> constexpr int tr_occ() {
@@ -59,7 +60,7 @@ __global__ __launch_bounds__(FL_NT, (tr_occ<TYPE, DH>())) void k_tree(SwKv c, Sw
                 *(sw_f32x4 *)(out + ((int64_t)(x.row + ci / G) * Hq + hk * G + ci % G) * DH + k % (DH / 4) * 4) = sw_f32x4{0.f, 0.f, 0.f, 0.f};
             }
     }
-    const FlDeal deal = fl_deal(t.n_trees, B, TR_LEAST, count);
+    const FlDeal deal = fl_deal(t.n_trees, B, tr_values(t, Hq, c.dh), count);
     int64_t at = (int64_t)b * deal.q, before = 0;
     const int64_t end = at + deal.q < deal.N ? at + deal.q : deal.N;
     if (at >= end) return;
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(FL_NT, (tr_occ<TYPE, DH>())) void k_tree(SwKv c, Sw
             if (ck >= x.n * G) return;
             if (all) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) a[e] = sum == 0.f ? 0.f : a[e] / sum;
+                for (int e = 0; e < 4; e++) a[e] = sum == 0.f ? 0.f : a[e] * (1.f / sum);
                 *(sw_f32x4 *)(out + ((int64_t)(x.row + ck / G) * Hq + hk * G + ck % G) * DH + d) = a;
             } else {
                 float *o = pp + col * (DH + 4);
@@ -180,39 +181,23 @@ __global__ __launch_bounds__(FL_NT, (tr_occ<TYPE, DH>())) void k_tree(SwKv c, Sw
     }
 }
 
-// The parts of a tree's columns joined, in their order: DH / 4 threads a column.
+// The parts of a tree's columns joined: a wave a column
 template <int DH>
 __global__ __launch_bounds__(FL_NT) void k_tree_join(SwKv c, SwTrees t, int S, int Hq, int window, const float *__restrict__ part, int B,
                                                      int CW, float *__restrict__ out) {
-    constexpr int ND = DH / 4, NC = FL_NT / ND;
-    const int G = Hq / c.Hkv, ncg = (t.max_nodes * G + CW - 1) / CW, nb = (CW + NC - 1) / NC;
-    const int hg = blockIdx.x / nb, i = blockIdx.y, hk = hg / ncg, c0 = hg % ncg * CW;
-    const int col = blockIdx.x % nb * NC + threadIdx.x / ND, d = threadIdx.x % ND * 4;
+    const int G = Hq / c.Hkv, ncg = (t.max_nodes * G + CW - 1) / CW, nb = CW / FL_NW, lane = threadIdx.x & 63;
+    const int hg = blockIdx.x / nb, i = blockIdx.y, hk = hg / ncg, c0 = hg % ncg * CW, col = fl_uni((int)(blockIdx.x % nb * FL_NW + (threadIdx.x >> 6)));
     auto count = [&](int k) { return tr_tiles(tr_tree(c, t, k, S, window), G, c0); };
     const TrTree x = tr_tree(c, t, i, S, window);
     const int tiles = tr_tiles(x, G, c0);
-    if (tiles == 0) return;
-    const FlDeal deal = fl_deal(t.n_trees, B, TR_LEAST, count);
+    if (tiles == 0 || c0 + col >= x.n * G) return;
+    const FlDeal deal = fl_deal(t.n_trees, B, tr_values(t, Hq, c.dh), count);
     const int64_t before = fl_before(i, count);
     const int b0 = (int)(before / deal.q), parts = (int)((before + tiles - 1) / deal.q) - b0 + 1;
-    if (parts < 2 || threadIdx.x >= ND * NC || col >= CW || c0 + col >= x.n * G) return;
-    const int64_t step = (int64_t)CW * (DH + 4);
-    const float *p = part + (((int64_t)hg * (B + t.n_trees) + b0 + i) * CW + col) * (DH + 4);
-    float M = -INFINITY, L = 0.f;
-    for (int k = 0; k < parts; k++) M = fmaxf(M, p[k * step]);
-    sw_f32x4 a = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int k = 0; k < parts; k++) {
-        const float m = p[k * step], g = m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m - M);
-        const sw_f32x4 y = *(const sw_f32x4 *)(p + k * step + 4 + d);
-        L = __builtin_fmaf(p[k * step + 1], g, L);
-#pragma unroll
-        for (int e = 0; e < 4; e++) a[e] = __builtin_fmaf(y[e], g, a[e]);
-    }
+    if (parts < 2) return;
+    const sw_f32x4 a = fl_join<DH>(part + (((int64_t)hg * (B + t.n_trees) + b0 + i) * CW + col) * (DH + 4), (int64_t)CW * (DH + 4), parts, 0);
     const int ck = c0 + col;
-#pragma unroll
-    for (int e = 0; e < 4; e++) a[e] = L == 0.f ? 0.f : a[e] / L;
-    *(sw_f32x4 *)(out + ((int64_t)(x.row + ck / G) * Hq + hk * G + ck % G) * DH + d) = a;
+    if (lane < DH / 4) *(sw_f32x4 *)(out + ((int64_t)(x.row + ck / G) * Hq + hk * G + ck % G) * DH + lane * 4) = a;
 }
 
 // columns of a block and blocks of each of their groups
@@ -223,9 +208,9 @@ static TrPlan tr_plan(const SwKv &c, const SwTrees &t, int Hq) {
     const int cols = t.max_nodes * (Hq / c.Hkv);
     p.wc = cols <= 32 ? tr_wc<TYPE, DH>() : 4;
     p.groups = c.Hkv * ((cols + 32 * p.wc - 1) / (32 * p.wc));
-    const int64_t tiles = ((((int64_t)t.max_pages << c.psh) + 31) / 32 + 1) * t.n_trees, most = (tiles + TR_LEAST - 1) / TR_LEAST;
+    const int64_t tiles = ((((int64_t)t.max_pages << c.psh) + 31) / 32 + 1) * t.n_trees;
     const int n = 256 * tr_occ<TYPE, DH>() / p.groups;
-    p.B = (int)(n < 1 ? 1 : n < most ? n : most);
+    p.B = (int)(n < 1 ? 1 : n < tiles ? n : tiles);
     return p;
 }
 template <int TYPE, int DH>
@@ -241,8 +226,7 @@ static int tr_launch(hipStream_t st, const SwKv &c, const SwTrees &t, const floa
     if (p.wc == 4) SW_LAUNCH((k_tree<TYPE, DH, 4>), grid, dim3(FL_NT), 0, st, c, t, q, S, Hq, sc, window, out, part, p.B);
     else SW_LAUNCH((k_tree<TYPE, DH, tr_wc<TYPE, DH>()>), grid, dim3(FL_NT), 0, st, c, t, q, S, Hq, sc, window, out, part, p.B);
     if (p.B > 1) {
-        constexpr int NC = FL_NT / (DH / 4);
-        const int CW = 32 * p.wc, nb = (CW + NC - 1) / NC;
+        const int CW = 32 * p.wc, nb = CW / FL_NW;
         SW_LAUNCH((k_tree_join<DH>), dim3((unsigned)(p.groups * nb), (unsigned)t.n_trees), dim3(FL_NT), 0, st, c, t, S, Hq, window, part, p.B, CW, out);
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;

@@ -150,15 +150,6 @@ __device__ __forceinline__ void fl_split(const float (&x)[8], sw_u32x4 (&o)[NP])
             for (int i = 0; i < 8; i++) h[i] = (_Float16)x[i];
             o[0] = __builtin_bit_cast(sw_u32x4, h);
         }
-    } else if constexpr (TYPE == SW_KV_BF16 && NP == 2) {
-        sw_bf16x8 hi, lo;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            hi[i] = (__bf16)x[i];
-            lo[i] = (__bf16)(x[i] - (float)hi[i]);
-        }
-        o[0] = __builtin_bit_cast(sw_u32x4, hi);
-        o[1] = __builtin_bit_cast(sw_u32x4, lo);
     } else if constexpr (TYPE == SW_KV_BF16) {
         uint32_t b[8], m[8], z[8];
 #pragma unroll
@@ -188,34 +179,31 @@ __device__ __forceinline__ void fl_split(const float (&x)[8], sw_u32x4 (&o)[NP])
 
 // A wave's 32 columns.  NP: parts that a 32-bit q and the weights are split into (1: 16-bit queries, one
 // rounding of the weights).  DK: values of a query, a multiple of 32; DV: of an output; INK: a cell's
-// first DV values of k are its v.  QL: steps of the scores whose queries wait in LDS, where registers would not hold them.  AHEAD: dwords of a row that a lane reads at once, 8 rows of them.  How
-// much is read ahead of the products goes by the registers that queries and outputs leave: a spilled one would be a load in the loop, and
-// waiting for it would wait for every tile on its way.
-template <int TYPE, int NP, int DK, int DV, bool INK, int SPLIT = 1, int QL = 0, int AHEAD = 2>
+// first DV values of k are its v.  How much is read ahead of the products goes by the registers that queries and outputs leave: a
+// spilled one would be a load in the loop, and waiting for it would wait for every tile on its way.
+template <int TYPE, int NP, int DK, int DV, bool INK, int SPLIT = 1>
 struct Fl {
     static constexpr bool F32 = TYPE == SW_KV_F32;
+    static constexpr int AHEAD = 2;                                    // f32 cells: dwords of a row that a lane reads at once, 4 rows of them
     static constexpr int ES = F32 ? 4 : 2, RBK = DK * ES, RBV = INK ? RBK : DV * ES;                   // bytes of a row of k, of v
     static constexpr int NCK = RBK / 16, NCV = DV * ES / 16;
     static constexpr int TB = 32 * RBK + (INK ? 0 : 32 * RBV);                                         // bytes of a tile
     static constexpr int DKS = RBK / 32 / SPLIT, DVW = DV / SPLIT, NO = DVW / 32, VB = DVW * ES;       // a wave's share: steps of the scores, values
     static_assert(RBK / 32 % SPLIT == 0 && (SPLIT == 1 || (DVW % 64 == 0 && RBK % 128 == 0)), "whole shares");
     static_assert(SPLIT == 1 || SPLIT == 2 || SPLIT == 4, "pairs");
-    static constexpr int HELD = (F32 ? 1 : NP) * (DKS - QL) * 4 + NO * 16;
+    static constexpr int HELD = (F32 ? 1 : NP) * DKS * 4 + NO * 16;
     static constexpr bool KEEP = HELD <= 128;                          // room for places in LDS
     static constexpr int PIPE = HELD <= 144 ? 2 : 1, QB = HELD <= 144 && NP == 1 && !F32 ? 4 : 2, VT = HELD <= 144 ? 4 : 2;
-    static constexpr int XB = SPLIT > 1 ? 4096 : 0;                                                    // bytes of a wave in the exchange
+    // bytes of a wave in the exchange, and of 32 columns: a share's sums of scores; the columns' weights and maxima
+    static constexpr int XB = SPLIT > 1 ? 4096 + (2048 + SPLIT * 128) / SPLIT + 16 : 0;
     // how a row's pieces are turned
     static constexpr int MK = NCK % 8 == 0 ? 7 : 3, MV = INK ? MK : F32 ? (NCV % 8 == 0 ? 7 : 3) : NCV % 8 == 0 ? 6 : 0;
     // weights are kept below 2^OFF; a maximum may lag behind by LAG powers of two (a running maximum that grows costs a pass
     // over the outputs; 16-bit weights hold 2^8 as well as 1, in parts they may not)
-    static constexpr int PP = NP > 2 ? 2 : NP;                         // parts of a weight
     static constexpr float LAG = NP == 1 && !F32 ? 8.f : 0.f;
     static constexpr float OFF = TYPE != SW_KV_F16 ? 0.f : NP == 1 ? 7.f : 13.f;
 
-    static_assert(QL == 0 || (NP == 1 && !F32), "16-bit queries");
-    static constexpr int QLB = QL * 1024;                              // their bytes of a wave
-    sw_u32x4 Q[F32 ? 1 : NP][DKS - QL];
-    sw_u32x4 *ql;                                                      // this lane's of them, 64 apart
+    sw_u32x4 Q[F32 ? 1 : NP][DKS];
     fl_f32x16 O[NO];
     float m, l, sc;
     static constexpr int KB = MK == 3 ? 2 : 4 / SPLIT;                 // a lane's places in a tile's row of k repeat after KB steps
@@ -241,11 +229,11 @@ struct Fl {
             sw_u32x4 o[NP];
             fl_split<TYPE, NP>(x, o);
 #pragma unroll
-            for (int u = 0; u < NP; u++) Q[u][i - QL] = o[u];
+            for (int u = 0; u < NP; u++) Q[u][i] = o[u];
         }
     }
 
-    // the scores of the tile at `t`, not yet times the scale: a wave's share of their sums added to s, and all of them
+    // the scores of the tile at `t` (a wave's share of their sums), not yet times the scale, added to s
     __device__ __forceinline__ void dot(const char *t, fl_f32x16 &s) const {
         // QB steps' operands are read while the QB before are multiplied
         constexpr int NB = (DKS + QB - 1) / QB;
@@ -253,11 +241,8 @@ struct Fl {
         int kb[KB];
 #pragma unroll
         for (int i = 0; i < KB; i++) kb[i] = c * RBK + (((2 * (SPLIT * i + share) + h) ^ fl_turn<MK>(c)) * 16);
-        sw_u32x4 a[2][QB], w[2][QL ? QB : 1];
+        sw_u32x4 a[2][QB];
         auto read = [&](int b) {
-#pragma unroll
-            for (int k = 0; k < QB; k++)
-                if (b * QB + k < QL) w[b & 1][QL ? k : 0] = ql[(b * QB + k) * 64];
 #pragma unroll
             for (int k = 0; k < QB; k++)
                 if (b * QB + k < DKS) a[b & 1][k] = *(const sw_u32x4 *)(t + kb[(b * QB + k) % KB] + (b * QB + k) / KB * (KB * SPLIT * 32));
@@ -278,38 +263,15 @@ struct Fl {
                     for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_32x32x2f32(y[e], z[e], s, 0, 0, 0);
                 } else {
 #pragma unroll
-                    for (int u = 0; u < NP; u++) s = fl_mfma<TYPE>(a[b & 1][k], i < QL ? w[b & 1][QL ? k : 0] : Q[u][i < QL ? 0 : i - QL], s);
+                    for (int u = 0; u < NP; u++) s = fl_mfma<TYPE>(a[b & 1][k], Q[u][i], s);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_s_setprio(0);
     }
-    __device__ __forceinline__ void scores(const char *t, fl_f32x16 &s, char *xch, int wave) const {
-        s = fl_f32x16{};
-        dot(t, s);
-        if constexpr (SPLIT > 1) {                                     // pairs, then pairs of them: the same sum in every wave
-            sw_f32x4 *to = (sw_f32x4 *)xch + fl_lane();
-#pragma unroll
-            for (int j = 0; j < 4; j++) to[(wave * 4 + j) * 64] = sw_f32x4{s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]};
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                sw_f32x4 y = to[((wave ^ 1) * 4 + j) * 64];
-#pragma unroll
-                for (int e = 0; e < 4; e++) s[4 * j + e] = s[4 * j + e] + y[e];
-                if constexpr (SPLIT == 4) {
-                    y = to[((wave ^ 2) * 4 + j) * 64];
-                    const sw_f32x4 z = to[((wave ^ 3) * 4 + j) * 64];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) s[4 * j + e] = s[4 * j + e] + (y[e] + z[e]);
-                }
-            }
-        }
-    }
-
     // scores (masked ones -INFINITY) to weights; the outputs follow a maximum that grew.  (16-bit weights are summed as they are rounded, in outputs().)
-    static constexpr bool SUMS = !F32 && PP == 1;
+    static constexpr bool SUMS = !F32 && NP == 1;
     __device__ __forceinline__ void weights(const fl_f32x16 &s, float (&x)[16]) {
         float mx = s[0];
 #pragma unroll
@@ -390,10 +352,11 @@ struct Fl {
             }
         }
     }
-    __device__ __forceinline__ void outputs(const char *t, const float (&p)[16], Piece &first) {
+    // (p, or where they are operands already, P)
+    typedef sw_u32x4 Weights[2][F32 ? 1 : NP];
+    __device__ __forceinline__ void outputs(const char *t, const float (&p)[16], Weights &P, Piece &first) {
         Piece v[PIPE];
         v[0] = first;
-        sw_u32x4 P[2][F32 ? 1 : PP];
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int s = 0; s < NST; s++) {
@@ -414,18 +377,18 @@ struct Fl {
                 for (int i = 0; i < VT; i++) {
                     const int at = s * VT + i, lot = at / NO, o = at % NO;
                     if (at >= 2 * NO) break;
-                    if (o == 0) {
+                    if (o == 0 && SPLIT == 1) {
                         float p8[8];
 #pragma unroll
                         for (int j = 0; j < 8; j++) p8[j] = p[8 * lot + j];
-                        fl_split<TYPE, PP>(p8, P[lot]);
+                        fl_split<TYPE, NP>(p8, P[lot]);
                         if constexpr (SUMS)
 #pragma unroll
                             for (int j = 0; j < 4; j++) l = fl_sum<TYPE>(P[lot][0][j], l);
                     }
                     const sw_u32x4 a = {y.v[4 * i], y.v[4 * i + 1], y.v[4 * i + 2], y.v[4 * i + 3]};
 #pragma unroll
-                    for (int u = 0; u < PP; u++) O[o] = fl_mfma<TYPE>(a, P[lot][u], O[o]);
+                    for (int u = 0; u < NP; u++) O[o] = fl_mfma<TYPE>(a, P[lot][u], O[o]);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -456,14 +419,15 @@ struct Fl {
     // One tile.  whole: every column attends to all of its tokens, else seen(token of the tile) says it for this lane's column, and bit k of
     // bad that token k's v is no number: whoever attends to it has no meaningful output.
     template <class Seen>
-    __device__ __forceinline__ void tile(const char *t, bool whole, uint32_t bad, Seen seen, char *xch, int wave) {
-        fl_f32x16 s;
-        scores(t, s, xch, wave);
-        rest(t, whole, bad, seen, s);
+    __device__ __forceinline__ void tile(const char *t, bool whole, uint32_t bad, Seen seen, char *xch, int wave, int odd) {
+        fl_f32x16 s = {};
+        dot(t, s);
+        if constexpr (SPLIT > 1) shared(t, whole, bad, seen, s, xch, wave, odd);
+        else alone(t, whole, bad, seen, s);
     }
     template <class Seen>
-    __device__ __forceinline__ void rest(const char *t, bool whole, uint32_t bad, Seen seen, fl_f32x16 &s) {
-        const char *v = (INK ? t : t + 32 * RBK) + (SPLIT > 1 ? share * VB : 0);
+    __device__ __forceinline__ void alone(const char *t, bool whole, uint32_t bad, Seen seen, fl_f32x16 &s) {
+        const char *v = INK ? t : t + 32 * RBK;
         if (!whole) {
             const int h4 = (threadIdx.x & 32) >> 3;
             uint32_t met = 0;
@@ -480,8 +444,98 @@ struct Fl {
         read(v, 0, first);
         __builtin_amdgcn_sched_barrier(0);
         float x[16];
+        Weights P;
         weights(s, x);
-        outputs(v, x, first);
+        outputs(v, x, P, first);
+    }
+    // Columns that SPLIT waves share: each wave has a share of the scores' sums of all 32 tokens.  They put them into LDS; each takes all sums of its
+    // own tokens (QT quads of a lane), makes their weights and puts those into LDS as the outputs' operand, which all read.  A maximum that
+    // grew too far (the waves' lags alike) is rare: then the waves put their maxima there too and make the weights again.
+    static constexpr int QT = 4 / SPLIT;
+    template <class Seen>
+    __device__ __forceinline__ void shared(const char *t, bool whole, uint32_t bad, Seen seen, fl_f32x16 &s, char *xch, int wave, int odd) {
+        static_assert(SPLIT == 1 || SUMS, "16-bit weights");
+        const int lane = fl_lane<KEEP>(), c = lane & 31, h4 = (lane & 32) >> 3;
+        const char *v = (INK ? t : t + 32 * RBK) + share * VB;
+        char *mine = xch + (wave - share) * XB;                        // of the columns: the shares' sums, the weights, the maxima, two flags
+        sw_f32x4 *sums = (sw_f32x4 *)mine + lane;
+        uint2 *w = (uint2 *)(mine + SPLIT * 4096) + lane * 2;
+        float *top = (float *)(mine + SPLIT * 4096 + 2048) + c;
+        int *grew = (int *)(xch + SPLIT * 4096 + 2048 + SPLIT * 128);  // (of all columns: the block's first)
+#pragma unroll
+        for (int j = 0; j < 4; j++) sums[(share * 4 + j) * 64] = sw_f32x4{s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]};
+        __syncthreads();
+        float x[4 * QT], mx = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < QT; q++) {
+            sw_f32x4 y = sums[(share * QT + q) * 64];
+#pragma unroll
+            for (int k = 1; k < SPLIT; k++) {
+                const sw_f32x4 z = sums[(k * 4 + share * QT + q) * 64];
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = y[e] + z[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[4 * q + e] = y[e];
+        }
+        if (!whole) {
+            uint32_t met = 0;
+#pragma unroll
+            for (int j = 0; j < 4 * QT; j++) {
+                const int k = 8 * (share * QT + j / 4) + h4 + j % 4;
+                const bool in = seen(k);
+                x[j] = in ? x[j] : -INFINITY;
+                met |= in ? bad >> k & 1 : 0u;
+            }
+            if (met) l = NAN;
+        }
+#pragma unroll
+        for (int j = 0; j < 4 * QT; j++) mx = fmaxf(mx, x[j]);
+        mx = fl_max2(mx);
+        auto put = [&](float &add) {                                   // this wave's tokens' weights and their sum
+            const float base = m == -INFINITY ? 0.f : OFF - m * sc;
+            add = 0.f;
+#pragma unroll
+            for (int q = 0; q < QT; q++) {
+                float p8[8] = {};
+#pragma unroll
+                for (int e = 0; e < 4; e++) p8[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[4 * q + e], sc, base));
+                sw_u32x4 o[1];
+                fl_split<TYPE, 1>(p8, o);
+                add = fl_sum<TYPE>(o[0][0], fl_sum<TYPE>(o[0][1], add));
+                const int quad = share * QT + q;
+                w[(quad >> 1) * 128 + (quad & 1)] = make_uint2(o[0][0], o[0][1]);
+            }
+        };
+        float add;
+        if (__any((mx - m) * sc > LAG) && lane == 0) grew[odd] = 1;
+        if (wave == 0 && lane == 0) grew[odd ^ 1] = 0;                 // (read last before the barrier above)
+        put(add);
+        Piece first;
+        read(v, 0, first);
+        __syncthreads();
+        if (__builtin_expect(grew[odd], 0)) {
+            if (lane < 32) top[share * 32] = mx;
+            __syncthreads();
+            float n = m;
+#pragma unroll
+            for (int k = 0; k < SPLIT; k++) n = fmaxf(n, top[k * 32]);
+            const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - n) * sc);
+            l = l * f;
+#pragma unroll
+            for (int i = 0; i < NO; i++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) O[i][j] = O[i][j] * f;
+            m = n;
+            put(add);
+            __syncthreads();
+        }
+        l = l + add;
+        Weights P;
+#pragma unroll
+        for (int i = 0; i < 2; i++) P[i][0] = *(const sw_u32x4 *)(w + i * 128);
+        const float none[16] = {};
+        outputs(v, none, P, first);
     }
 
     // Where an output's values lie: tile o's row r is value d0 + T r + e of a group of values that T tiles share (f32: groups of 64 and 32
@@ -514,6 +568,10 @@ __device__ __forceinline__ void fl_run(F &f, char *sh, char *xch, uint32_t *s_ba
     const uint32_t lds = fl_lds_addr(mine);
     const bool first = (threadIdx.x & 63) == 0 && (WT > 1 && WC == 1 ? true : wave % (WC * SPLIT) == 0);       // of its group
     if (first) s_bad[0] = 0;                                           // (the item before is done with it)
+    if (SPLIT > 1 && threadIdx.x == 0) {
+        int *grew = (int *)(xch + SPLIT * 4096 + 2048 + SPLIT * 128);
+        grew[0] = grew[1] = 0;
+    }
     uint32_t there = 0;                                                // bit s: all pages of the tile in place s are there
     auto load = [&](int i, int s) {
         const bool ok = issue(ta + wt + i * WT, lds + s * TB);
@@ -547,21 +605,22 @@ __device__ __forceinline__ void fl_run(F &f, char *sh, char *xch, uint32_t *s_ba
             else fl_wait_lds();
             bad = s_bad[i & 1];
         }
-        if (SPLIT > 1 || (i < n && columns)) f.tile(mine + s * TB, whl, bad, [&](int k) { return seen(t, k); }, xch, wave);
+        if (SPLIT > 1 || (i < n && columns)) f.tile(mine + s * TB, whl, bad, [&](int k) { return seen(t, k); }, xch, wave, i & 1);
         s = s + 1 == NS ? 0 : s + 1;
     }
 }
 
 // The end of an item: the groups' outputs of a column joined in their order and given to put(column, value, four
-// outputs, maximum, sum).  sh: LDS of fl_end_bytes, free.
+// outputs, maximum, sum), rows of 32 values or more at a time, so that they are written as whole lines.  sh: LDS of fl_end_bytes, free.
+template <class F> constexpr int fl_end_row() { return 32 * (F::F32 ? 2 : 1) + 4; }
 template <class F, int NW>
-constexpr int fl_end_bytes() { return NW * 32 * (F::DVW / 4 + 4) * 4; }
+constexpr int fl_end_bytes() { return NW * 32 * fl_end_row<F>() * 4; }
 template <int WC, int WT, int SPLIT, class F, class Put>
 __device__ __forceinline__ void fl_end(F &f, char *sh, float (*s_m)[32], float (*s_l)[32], int wave, Put put) {
-    constexpr int DVW = F::DVW, LD = DVW / 4 + 4, NO = F::NO, NT = WC * WT * SPLIT * 64;
+    constexpr int LD = fl_end_row<F>(), NO = F::NO;
     constexpr auto map = F::map();
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
-    const float l = fl_sum2(f.l), m = f.m * f.sc;                      // (from here on the maximum is times the scale)
+    const float l = fl_sum2(f.l), m = f.m * f.sc;                      // (from here on the maximum is times the scale; with SPLIT the sums are of shares)
     __syncthreads();                                                   // the tiles are done with
     if (h == 0) { s_m[wave][c] = m; s_l[wave][c] = l; }
     __syncthreads();
@@ -572,60 +631,128 @@ __device__ __forceinline__ void fl_end(F &f, char *sh, float (*s_m)[32], float (
         for (int i = 0; i < WT; i++) M = fmaxf(M, s_m[i * WC + wave % WC][c]);
         g = m == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m - M);
     }
+    const float *all = (const float *)sh;
     float *so = (float *)sh + (wave * 32 + c) * LD;
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
+    for (int o0 = 0; o0 < NO; o0++) {                                  // T tiles share a row of 32 T values
+        if (map.e[o0]) continue;
+        const int T = map.tiles[o0], d0 = map.d0[o0];
 #pragma unroll
-        for (int o = 0; o < NO; o++) {
-            const int T = map.tiles[o], at = map.d0[o] / 4 + map.e[o];
+        for (int e = 0; e < T; e++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) so[at + T * (4 * h + j)] = WT > 1 ? f.O[o][4 * q + j] * g : f.O[o][4 * q + j];
-        }
-        __syncthreads();
-        // (column, share, four values): the shares of a column are waves side by side
+            for (int j = 0; j < 16; j++) so[T * (8 * (j / 4) + 4 * h + j % 4) + e] = WT > 1 ? f.O[o0 + e][j] * g : f.O[o0 + e][j];
+        if constexpr (WT == 1) {                                       // a wave's own columns
+            fl_wait_lds();
 #pragma unroll 1
-        for (int i = tid; i < WC * 32 * SPLIT * (DVW / 16); i += NT) {
-            const int v = i % (SPLIT * (DVW / 16)), col = i / (SPLIT * (DVW / 16)), sp = v / (DVW / 16), d = v % (DVW / 16) * 4;
-            const int w = (col >> 5) * SPLIT + sp;
-            sw_f32x4 a = *(const sw_f32x4 *)((const float *)sh + (w * 32 + (col & 31)) * LD + d);
-            float mx = s_m[w][col & 31], sum = s_l[w][col & 31];
-            if constexpr (WT > 1) {
+            for (int i = 0; i < 4 * T; i++) {
+                const int k = i * 64 + lane, col = k / (8 * T), d = k % (8 * T) * 4, wc = wave / SPLIT;
+                const sw_f32x4 a = *(const sw_f32x4 *)(all + (wave * 32 + col) * LD + d);
+                float sum = s_l[wc * SPLIT][col];
+#pragma unroll
+                for (int k2 = 1; k2 < SPLIT; k2++) sum = sum + s_l[wc * SPLIT + k2][col];
+                put(wc * 32 + col, (wave % SPLIT) * F::DVW + d0 + d, a, s_m[wave][col], sum);
+            }
+            fl_wait_lds();
+        } else {
+            __syncthreads();
+#pragma unroll 1
+            for (int i = tid; i < WC * 32 * 8 * T; i += WC * WT * 64) {
+                const int col = i / (8 * T), d = i % (8 * T) * 4, w = col >> 5;
+                sw_f32x4 a = *(const sw_f32x4 *)(all + (w * 32 + (col & 31)) * LD + d);
+                float mx = s_m[w][col & 31], sum = 0.f;
 #pragma unroll
                 for (int k = 1; k < WT; k++) {
-                    const sw_f32x4 y = *(const sw_f32x4 *)((const float *)sh + ((w + k * WC) * 32 + (col & 31)) * LD + d);
+                    const sw_f32x4 y = *(const sw_f32x4 *)(all + ((w + k * WC) * 32 + (col & 31)) * LD + d);
 #pragma unroll
                     for (int e = 0; e < 4; e++) a[e] = a[e] + y[e];
                     mx = fmaxf(mx, s_m[w + k * WC][col & 31]);
                 }
-                sum = 0.f;
 #pragma unroll
                 for (int k = 0; k < WT; k++) {
                     const float x = s_m[w + k * WC][col & 31];
                     sum = __builtin_fmaf(s_l[w + k * WC][col & 31], x == -INFINITY ? (mx == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(x - mx), sum);
                 }
+                put(col, d0 + d, a, mx, sum);
             }
-            // the quarter's value d: which group of values it is in
-            int d0 = 0, T8 = 0;
-#pragma unroll
-            for (int o = 0; o < NO; o++)
-                if (map.e[o] == 0 && map.d0[o] / 4 <= d) { d0 = map.d0[o]; T8 = map.tiles[o] * 8; }
-            put(col, sp * DVW + d0 + T8 * q + d - d0 / 4, a, mx, sum);
+            __syncthreads();
         }
-        __syncthreads();
     }
+    if (WT == 1) __syncthreads();                                      // (the next item's tiles take the same LDS)
+}
+
+// Parts of one column joined, in their order: part k at p + k * step holds its maximum and sum, then (behind 4) DV outputs.  A wave
+// takes 256 values from v0 on, 4 a lane; where DV / 4 lanes are a part of a wave, its parts take turns.  Weights are a lane's each, 64
+// parts at a time.  Returns the outputs divided by the sum (0 where there is none).
+template <int DV>
+__device__ __forceinline__ sw_f32x4 fl_join(const float *p, int64_t step, int parts, int v0) {
+    constexpr int ND = DV / 4, SUB = ND <= 32 && (ND & (ND - 1)) == 0 ? 64 / ND : 1;
+    const int lane = threadIdx.x & 63, sub = SUB > 1 ? lane / ND : 0, d = v0 + (SUB > 1 ? lane % ND : lane) * 4;
+    const bool mine = d < DV;
+    sw_f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    float M = -INFINITY, L = 0.f;
+    for (int k0 = 0; k0 < parts; k0 += 64) {
+        float m = -INFINITY, l = 0.f;
+        if (k0 + lane < parts) {
+            const float2 y = *(const float2 *)(p + (k0 + lane) * step);
+            m = y.x; l = y.y;
+        }
+        float n = fmaxf(M, m);
+#pragma unroll
+        for (int o = 32; o; o >>= 1) n = fmaxf(n, __shfl_xor(n, o));
+        const float g = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M - n);                          // (nothing summed before: any factor)
+        const float w = m == -INFINITY ? (n == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(m - n);
+        float s = l * w;
+#pragma unroll
+        for (int o = 32; o; o >>= 1) s = s + __shfl_xor(s, o);
+        L = __builtin_fmaf(L, g, s);
+        M = n;
+#pragma unroll
+        for (int e = 0; e < 4; e++) a[e] = a[e] * g;
+        const int top = min(64, parts - k0);
+        for (int k = 0; k < top; k += 8 * SUB) {
+            sw_f32x4 y[8];
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int at = k + i * SUB + sub;
+                y[i] = sw_f32x4{0.f, 0.f, 0.f, 0.f};
+                if (mine && at < top) y[i] = *(const sw_f32x4 *)(p + (k0 + at) * step + 4 + d);
+                f[i] = __shfl(w, at & 63);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) a[e] = k + i * SUB + sub < top ? __builtin_fmaf(y[i][e], f[i], a[e]) : a[e];
+        }
+    }
+#pragma unroll
+    for (int o = ND; o < 64 && SUB > 1; o <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; e++) a[e] = a[e] + __shfl_xor(a[e], o);
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int e = 0; e < 4; e++) a[e] = L == 0.f ? 0.f : a[e] * inv;
+    return a;
+}
+
+// The least tiles of a block: a tile takes it some 2 us, and the outputs of a part (cols columns of all blocks that share its tokens) are written and
+// read again at some 4 TB/s, so with N tiles in all the two are least together where q^2 = N cols values 8 bytes / 8 MB.
+__device__ __forceinline__ int fl_least(int64_t N, int64_t values) {
+    const int q = (int)sqrtf((float)N * (float)values * 1e-6f);
+    return q < 1 ? 1 : q;
 }
 
 // How items' tiles are dealt to B blocks: laid end to end they are N, and block b takes those from b q to (b + 1) q, whatever
-// items they fall in.  count(i): the tiles of item i (evaluated 64 items at a time, a lane each).  `least`: no fewer
-// tiles a block.
+// items they fall in.  count(i): the tiles of item i (evaluated 64 items at a time, a lane each).  `values`: outputs of an item (fl_least).
 struct FlDeal { int64_t N, q; };
 template <class Count>
-__device__ __forceinline__ FlDeal fl_deal(int items, int B, int least, Count count) {
+__device__ __forceinline__ FlDeal fl_deal(int items, int B, int64_t values, Count count) {
     const int lane = threadIdx.x & 63;
     FlDeal d = {0, 0};
     for (int i0 = 0; i0 < items; i0 += 64)
         d.N += (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)sw_wave_scan(i0 + lane < items ? (uint32_t)count(i0 + lane) : 0u), 63);
     d.q = (d.N + B - 1) / B;
+    const int least = fl_uni(fl_least(d.N, values));
     if (d.q < least) d.q = least;
     return d;
 }

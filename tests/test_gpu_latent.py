@@ -104,6 +104,12 @@ def test_long(be, kind, H, lens):
     one(be, 1, kind, H, 512, 64, 64, lens, poison=False)
 
 
+@pytest.mark.parametrize("H", [16, 100])
+def test_blocks_that_take_several_rows(be, H):
+    rng = np.random.default_rng(H)
+    one(be, H, "bf16", H, 512, 64, 64, list(rng.integers(500, 3000, 60)), poison=False)
+
+
 @pytest.mark.parametrize("S", [100, 256, 257, 400])
 def test_many_rows(be, S):
     rng = np.random.default_rng(S)

@@ -133,6 +133,13 @@ def test_long(be, kind, Hq, Hkv, dh, P, base, sizes):
     one(be, 1, kind, Hq, Hkv, dh, P, base, sizes, poison=False)
 
 
+@pytest.mark.parametrize("top", [8, 30])
+def test_blocks_that_take_several_trees(be, top):
+    """more tiles than blocks: a block ends one tree and begins the next"""
+    rng = np.random.default_rng(top)
+    one(be, 5, "bf16", 8, 2, 64, 64, list(rng.integers(1500, 6000, 40)), list(rng.integers(1, top + 1, 40)), poison=False)
+
+
 def test_many_trees(be):
     rng = np.random.default_rng(3)
     one(be, 2, "bf16", 4, 2, 64, 16, list(rng.integers(0, 200, 150)), list(rng.integers(1, 9, 150)))
