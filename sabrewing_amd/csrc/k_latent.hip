@@ -296,7 +296,7 @@ __global__ __launch_bounds__((64 * WC * ln_split<R>())) void k_latent(SwLatent c
         };
         fl_run<WC, 1, SPLIT, NS, NL>(f, sh, sh + NS * F::TB, s_bad, from, from + len, wave, true, issue, whole, seen);
         const bool all = len == tiles;
-        float *pp = all ? nullptr : part + ((int64_t)hg * (B + S) + b + s) * CW * (R + 4);
+        float *pp = all ? nullptr : part + ((int64_t)hg * 2 * B + fl_slot(b, from)) * CW * (R + 4);
         fl_end<WC, 1, SPLIT>(f, sh, s_m, s_l, wave, [&](int col, int d, sw_f32x4 a, float mx, float sum) {
             if (col >= nh) return;
             if (all) {
@@ -313,21 +313,24 @@ __global__ __launch_bounds__((64 * WC * ln_split<R>())) void k_latent(SwLatent c
     }
 }
 
-// The parts of a row's heads joined: a wave 256 values of a head
+// The parts of a row's heads joined: a wave 256 values of a head at a time
 template <int TYPE, int R>
 __global__ __launch_bounds__(FL_NT) void k_latent_join(SwLatent c, SwRows r, int S, int H, const float *__restrict__ part, int B, int CW,
                                                        uint16_t *__restrict__ out) {
     constexpr int NV = (R + 255) / 256;
-    const int s = blockIdx.y, k = fl_uni((int)(blockIdx.x * FL_NW + (threadIdx.x >> 6))), head = k / NV, v0 = k % NV * 256, d = v0 + (threadIdx.x & 63) * 4;
+    const int s = blockIdx.y, k0 = fl_uni((int)(blockIdx.x * FL_NW + (threadIdx.x >> 6)));
     auto count = [&](int i) { return (ln_row(c, r, i).last >> 5) + 1; };
     const int tiles = count(s);
-    if (tiles == 0 || head >= H) return;
+    if (tiles == 0 || k0 >= H * NV) return;
     const FlDeal deal = fl_deal(S, B, (int64_t)H * R, count);
     const int64_t before = fl_before(s, count);
     const int b0 = (int)(before / deal.q), parts = (int)((before + tiles - 1) / deal.q) - b0 + 1;
     if (parts < 2) return;
-    const sw_f32x4 a = fl_join<R>(part + (((int64_t)(head / CW) * (B + S) + b0 + s) * CW + head % CW) * (R + 4), (int64_t)CW * (R + 4), parts, v0);
-    if (d < R && (threadIdx.x & 63) * 4 < R) *(uint2 *)(out + ((int64_t)s * H + head) * R + d) = make_uint2(lt_pack<TYPE>(a[0], a[1]), lt_pack<TYPE>(a[2], a[3]));
+    for (int k = k0; k < H * NV; k += gridDim.x * FL_NW) {
+        const int head = k / NV, v0 = k % NV * 256, d = v0 + (threadIdx.x & 63) * 4;
+        const sw_f32x4 a = fl_join<R>(part + (((int64_t)(head / CW) * 2 * B + fl_slot(b0, 0)) * CW + head % CW) * (R + 4), (int64_t)CW * (R + 4), parts, v0);
+        if (d < R && (threadIdx.x & 63) * 4 < R) *(uint2 *)(out + ((int64_t)s * H + head) * R + d) = make_uint2(lt_pack<TYPE>(a[0], a[1]), lt_pack<TYPE>(a[2], a[3]));
+    }
 }
 
 // columns of a block (waves that have 32 each) and blocks of each group of heads; 0: a block a row
@@ -343,7 +346,7 @@ static LnPlan ln_plan(const SwLatent &c, const SwRows &r, int H, int S) {
 }
 int64_t sw_latent_part_floats(const SwLatent &c, const SwRows &r, int H, int S) {
     const LnPlan p = ln_plan(c, r, H, S);
-    return p.B > 1 ? (int64_t)p.groups * (p.B + S) * 32 * p.wc * (c.rank + 4) : 0;
+    return p.B > 1 ? (int64_t)p.groups * 2 * p.B * 32 * p.wc * (c.rank + 4) : 0;
 }
 template <int TYPE, int R>
 static int ln_launch(hipStream_t st, const SwLatent &c, const SwRows &r, const uint16_t *q, int H, float sc, uint16_t *out, int S, float *part) {
@@ -354,7 +357,7 @@ static int ln_launch(hipStream_t st, const SwLatent &c, const SwRows &r, const u
     else SW_LAUNCH((k_latent<TYPE, R, 2>), dim3((unsigned)grid), dim3(128 * ln_split<R>()), 0, st, c, r, q, S, H, sc, out, part, p.B);
     if (p.B > 1) {
         constexpr int NV = (R + 255) / 256;
-        SW_LAUNCH((k_latent_join<TYPE, R>), dim3((unsigned)((H * NV + FL_NW - 1) / FL_NW), (unsigned)S), dim3(FL_NT), 0, st, c, r, S, H, part, p.B, 32 * p.wc, out);
+        SW_LAUNCH((k_latent_join<TYPE, R>), dim3((unsigned)fl_join_blocks((H * NV + FL_NW - 1) / FL_NW, S), (unsigned)S), dim3(FL_NT), 0, st, c, r, S, H, part, p.B, 32 * p.wc, out);
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }

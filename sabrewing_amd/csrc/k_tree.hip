@@ -164,7 +164,7 @@ __global__ __launch_bounds__(FL_NT, (tr_occ<TYPE, DH>())) void k_tree(SwKv c, Sw
         };
         fl_run<WC, WT, 1, NS, LK + LV>(f, sh, nullptr, s_bad, ta, ta + len, wave, columns, issue, whole, seen);
         const bool all = len == tiles;
-        float *pp = all ? nullptr : part + ((int64_t)hg * (B + t.n_trees) + b + i) * CW * (DH + 4);
+        float *pp = all ? nullptr : part + ((int64_t)hg * 2 * B + fl_slot(b, from)) * CW * (DH + 4);
         fl_end<WC, WT, 1>(f, sh, s_m, s_l, wave, [&](int col, int d, sw_f32x4 a, float mx, float sum) {
             const int ck = c0 + col;
             if (ck >= x.n * G) return;
@@ -181,23 +181,25 @@ __global__ __launch_bounds__(FL_NT, (tr_occ<TYPE, DH>())) void k_tree(SwKv c, Sw
     }
 }
 
-// The parts of a tree's columns joined: a wave a column
+// The parts of a tree's columns joined: a wave a column at a time
 template <int DH>
 __global__ __launch_bounds__(FL_NT) void k_tree_join(SwKv c, SwTrees t, int S, int Hq, int window, const float *__restrict__ part, int B,
-                                                     int CW, float *__restrict__ out) {
-    const int G = Hq / c.Hkv, ncg = (t.max_nodes * G + CW - 1) / CW, nb = CW / FL_NW, lane = threadIdx.x & 63;
-    const int hg = blockIdx.x / nb, i = blockIdx.y, hk = hg / ncg, c0 = hg % ncg * CW, col = fl_uni((int)(blockIdx.x % nb * FL_NW + (threadIdx.x >> 6)));
+                                                     int CW, int nb, float *__restrict__ out) {
+    const int G = Hq / c.Hkv, ncg = (t.max_nodes * G + CW - 1) / CW, lane = threadIdx.x & 63;
+    const int hg = blockIdx.x / nb, i = blockIdx.y, hk = hg / ncg, c0 = hg % ncg * CW, col0 = fl_uni((int)(blockIdx.x % nb * FL_NW + (threadIdx.x >> 6)));
     auto count = [&](int k) { return tr_tiles(tr_tree(c, t, k, S, window), G, c0); };
     const TrTree x = tr_tree(c, t, i, S, window);
     const int tiles = tr_tiles(x, G, c0);
-    if (tiles == 0 || c0 + col >= x.n * G) return;
+    if (tiles == 0 || c0 + col0 >= x.n * G) return;
     const FlDeal deal = fl_deal(t.n_trees, B, tr_values(t, Hq, c.dh), count);
     const int64_t before = fl_before(i, count);
     const int b0 = (int)(before / deal.q), parts = (int)((before + tiles - 1) / deal.q) - b0 + 1;
     if (parts < 2) return;
-    const sw_f32x4 a = fl_join<DH>(part + (((int64_t)hg * (B + t.n_trees) + b0 + i) * CW + col) * (DH + 4), (int64_t)CW * (DH + 4), parts, 0);
-    const int ck = c0 + col;
-    if (lane < DH / 4) *(sw_f32x4 *)(out + ((int64_t)(x.row + ck / G) * Hq + hk * G + ck % G) * DH + lane * 4) = a;
+    for (int col = col0; col < min(CW, x.n * G - c0); col += nb * FL_NW) {
+        const sw_f32x4 a = fl_join<DH>(part + (((int64_t)hg * 2 * B + fl_slot(b0, 0)) * CW + col) * (DH + 4), (int64_t)CW * (DH + 4), parts, 0);
+        const int ck = c0 + col;
+        if (lane < DH / 4) *(sw_f32x4 *)(out + ((int64_t)(x.row + ck / G) * Hq + hk * G + ck % G) * DH + lane * 4) = a;
+    }
 }
 
 // columns of a block and blocks of each of their groups
@@ -216,7 +218,7 @@ static TrPlan tr_plan(const SwKv &c, const SwTrees &t, int Hq) {
 template <int TYPE, int DH>
 static int64_t tr_part(const SwKv &c, const SwTrees &t, int Hq) {
     const TrPlan p = tr_plan<TYPE, DH>(c, t, Hq);
-    return p.B > 1 ? (int64_t)p.groups * (p.B + t.n_trees) * 32 * p.wc * (DH + 4) : 0;
+    return p.B > 1 ? (int64_t)p.groups * 2 * p.B * 32 * p.wc * (DH + 4) : 0;
 }
 template <int TYPE, int DH>
 static int tr_launch(hipStream_t st, const SwKv &c, const SwTrees &t, const float *q, int S, int Hq, float sc, int window, float *out, float *part) {
@@ -226,8 +228,8 @@ static int tr_launch(hipStream_t st, const SwKv &c, const SwTrees &t, const floa
     if (p.wc == 4) SW_LAUNCH((k_tree<TYPE, DH, 4>), grid, dim3(FL_NT), 0, st, c, t, q, S, Hq, sc, window, out, part, p.B);
     else SW_LAUNCH((k_tree<TYPE, DH, tr_wc<TYPE, DH>()>), grid, dim3(FL_NT), 0, st, c, t, q, S, Hq, sc, window, out, part, p.B);
     if (p.B > 1) {
-        const int CW = 32 * p.wc, nb = CW / FL_NW;
-        SW_LAUNCH((k_tree_join<DH>), dim3((unsigned)(p.groups * nb), (unsigned)t.n_trees), dim3(FL_NT), 0, st, c, t, S, Hq, window, part, p.B, CW, out);
+        const int CW = 32 * p.wc, nb = fl_join_blocks(CW / FL_NW, (int64_t)p.groups * t.n_trees);
+        SW_LAUNCH((k_tree_join<DH>), dim3((unsigned)(p.groups * nb), (unsigned)t.n_trees), dim3(FL_NT), 0, st, c, t, S, Hq, window, part, p.B, CW, nb, out);
     }
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }

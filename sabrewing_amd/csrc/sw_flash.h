@@ -680,7 +680,10 @@ __device__ __forceinline__ void fl_end(F &f, char *sh, float (*s_m)[32], float (
     if (WT == 1) __syncthreads();                                      // (the next item's tiles take the same LDS)
 }
 
-// Parts of one column joined, in their order: part k at p + k * step holds its maximum and sum, then (behind 4) DV outputs.  A wave
+// A block's parts: of the item that it goes on with, and of the one that it begins and does not end (an item's tiles from `from` on).  An
+// item's part k is then 2 k - 1 places behind its first.
+__device__ __forceinline__ int64_t fl_slot(int b, int from) { return 2 * (int64_t)b + (from == 0); }
+// Parts of one column joined, in their order: part k at p + max(0, 2 k - 1) * step holds its maximum and sum, then (behind 4) DV outputs.  A wave
 // takes 256 values from v0 on, 4 a lane; where DV / 4 lanes are a part of a wave, its parts take turns.  Weights are a lane's each, 64
 // parts at a time.  Returns the outputs divided by the sum (0 where there is none).
 template <int DV>
@@ -693,7 +696,7 @@ __device__ __forceinline__ sw_f32x4 fl_join(const float *p, int64_t step, int pa
     for (int k0 = 0; k0 < parts; k0 += 64) {
         float m = -INFINITY, l = 0.f;
         if (k0 + lane < parts) {
-            const float2 y = *(const float2 *)(p + (k0 + lane) * step);
+            const float2 y = *(const float2 *)(p + max(0, 2 * (k0 + lane) - 1) * step);
             m = y.x; l = y.y;
         }
         float n = fmaxf(M, m);
@@ -716,7 +719,7 @@ __device__ __forceinline__ sw_f32x4 fl_join(const float *p, int64_t step, int pa
             for (int i = 0; i < 8; i++) {
                 const int at = k + i * SUB + sub;
                 y[i] = sw_f32x4{0.f, 0.f, 0.f, 0.f};
-                if (mine && at < top) y[i] = *(const sw_f32x4 *)(p + (k0 + at) * step + 4 + d);
+                if (mine && at < top) y[i] = *(const sw_f32x4 *)(p + max(0, 2 * (k0 + at) - 1) * step + 4 + d);
                 f[i] = __shfl(w, at & 63);
             }
 #pragma unroll
@@ -733,6 +736,13 @@ __device__ __forceinline__ sw_f32x4 fl_join(const float *p, int64_t step, int pa
 #pragma unroll
     for (int e = 0; e < 4; e++) a[e] = L == 0.f ? 0.f : a[e] * inv;
     return a;
+}
+
+// Blocks of a join of `of` such groups of columns, `all` of one: waves take several columns where they would not all run at once, and
+// find their place among the items once (16 trees' join 27 -> 16 us, and as much with half or twice the blocks).
+inline int fl_join_blocks(int all, int64_t of) {
+    const int64_t n = 1024 / (of < 1 ? 1 : of);
+    return n < 1 ? 1 : n < all ? (int)n : all;
 }
 
 // The least tiles of a block: a tile takes it some 2 us, and the outputs of a part (cols columns of all blocks that share its tokens) are written and
