@@ -58,22 +58,30 @@ class PagedCache:
     so that a recorded step replays over what the next rows() put there."""
 
     def __init__(self, be, n_layers, n_pages, page_size, n_heads, head_dim, kind="bf16", max_seqs=64, max_len=None, max_rows=None):
-        self.be, self.n_layers, self.n_pages, self.page_size = be, n_layers, n_pages, page_size
         self.n_heads, self.head_dim, self.kind = n_heads, head_dim, kind
         if min(n_layers, n_pages, page_size, n_heads, head_dim, max_seqs) < 1 or page_size & (page_size - 1):
             raise ValueError("PagedCache: sizes must be positive, page_size a power of two")
         if not 8 <= page_size <= 4096 or head_dim % 32 or head_dim > 256 or n_heads > 1024 or kind not in KV_TYPES:
             raise ValueError("PagedCache: page_size 8 to 4096, head_dim a multiple of 32 up to 256, at most 1024 heads, f32, bf16 or f16")
+        self._sizes(be, n_layers, n_pages, page_size, max_seqs, max_len, max_rows)
         item = 4 if KV_TYPES[kind] == 0 else 2
-        self.max_seqs, self.max_rows = max_seqs, max_rows or max_seqs
-        self.max_pages = -(-(max_len or n_pages * page_size) // page_size)
-        if self.max_pages * page_size > 1 << 30:
-            raise ValueError("PagedCache: sequences of more than 2^30 tokens (max_len)")
         one = n_pages * n_heads * page_size * head_dim * item              # one layer's keys or values
         self.pool = be.alloc(2 * n_layers * one)
         base = int(self.pool)
         self.layers = be.kv_caches([be.kv_cache(base + 2 * l * one, base + (2 * l + 1) * one, kind, n_pages, page_size, n_heads,
                                                 head_dim) for l in range(n_layers)])
+        self.copied = self.layers                                          # (as kv_copy_pages sees the pages)
+        self._sequences()
+
+    def _sizes(self, be, n_layers, n_pages, page_size, max_seqs, max_len, max_rows):
+        self.be, self.n_layers, self.n_pages, self.page_size = be, n_layers, n_pages, page_size
+        self.max_seqs, self.max_rows = max_seqs, max_rows or max_seqs
+        self.max_pages = -(-(max_len or n_pages * page_size) // page_size)
+        if self.max_pages * page_size > 1 << 30:
+            raise ValueError("PagedCache: sequences of more than 2^30 tokens (max_len)")
+
+    def _sequences(self):
+        be, n_pages, max_seqs = self.be, self.n_pages, self.max_seqs
         self._users = np.zeros(n_pages, np.int32)
         self._free = list(range(n_pages - 1, -1, -1))                      # the lowest last
         self._pages = [None] * max_seqs
@@ -191,7 +199,7 @@ class PagedCache:
                     of[s] = self._take(took)
                     self._users[src[-1]] -= 1
             if src:
-                self.be.kv_copy_pages(self.layers, src, list(of.values()))
+                self.be.kv_copy_pages(self.copied, src, list(of.values()))
             at = 0
             for s, n in batch:
                 if s is None:
@@ -242,7 +250,7 @@ class PagedCache:
         src = used[used >= n]
         dst = np.flatnonzero(self._users[:n] == 0)
         if src.size:
-            self.be.kv_copy_pages(self.layers, src, dst)
+            self.be.kv_copy_pages(self.copied, src, dst)
             to = np.arange(self.n_pages)
             to[src] = dst
             for s, pages in enumerate(self._pages):
@@ -324,8 +332,9 @@ class DeviceAttention:
         return cls(be, acfg, D, ones(D, T_ATTN_NORM), matrix(acfg.qkv_rows, D, T_QKV),
                    matrix(D, acfg.n_q * acfg.head_dim, T_O), qn, kn, rope)
 
-    def forward(self, h, xn, S, cache_layer, rows, scratch):
-        """h [S, D] += attention of its normalised rows (device; xn [S, D] scratch)"""
+    def forward(self, h, xn, S, cache_layer, rows, scratch, trees=None):
+        """h [S, D] += attention of its normalised rows (device; xn [S, D] scratch); trees: the DraftTrees
+        whose nodes the rows are"""
         be, a, D = self.be, self.acfg, self.D
         if (cache_layer.n_heads, cache_layer.head_dim) != (a.n_kv, a.head_dim):
             raise ValueError("DeviceAttention: a cache of other heads")
@@ -333,9 +342,15 @@ class DeviceAttention:
             raise ValueError("DeviceAttention: scratch for fewer rows or other heads")
         be.rmsnorm(h, self.norm, xn, S, D, a.eps)
         be.head_argmax(self.wqkv, True, xn, S, D, a.qkv_rows, scratch.qkv)
-        be.qk_rope_append(cache_layer, rows, self.rope.desc, scratch.qkv, a.qkv_rows, self.q_norm, self.k_norm, a.eps, a.n_q,
-                          scratch.q, S)
-        be.attn_paged(cache_layer, rows, scratch.q, a.n_q, 1.0 / math.sqrt(a.head_dim), a.window, scratch.ctx, S)
+        scale = 1.0 / math.sqrt(a.head_dim)
+        if trees is None:
+            be.qk_rope_append(cache_layer, rows, self.rope.desc, scratch.qkv, a.qkv_rows, self.q_norm, self.k_norm, a.eps, a.n_q,
+                              scratch.q, S)
+            be.attn_paged(cache_layer, rows, scratch.q, a.n_q, scale, a.window, scratch.ctx, S)
+        else:
+            be.qk_rope_append_at(cache_layer, rows, trees.at, self.rope.desc, scratch.qkv, a.qkv_rows, self.q_norm, self.k_norm,
+                                 a.eps, a.n_q, scratch.q, S)
+            be.attn_tree(cache_layer, trees.desc, scratch.q, a.n_q, scale, a.window, scratch.ctx, S)
         be.head_argmax(self.wo, True, scratch.ctx, S, a.n_q * a.head_dim, D, scratch.out)
         be.add(h, scratch.out, S * D)
 

@@ -1,0 +1,125 @@
+"""Drafted tokens verified in one step: a tree of them for each sequence, its nodes the rows of a step over a
+PagedCache (attention.py).
+
+    rows, S = trees.place([(seq, parents, tokens), ...])
+    stack.step(h, xn, logits, tok, S, cache=cache, rows=rows, trees=trees)
+    accepted = trees.commit(tok)
+
+Node 0 is the sequence's next token (the pick that the last step ended in), every other node a drafted token
+behind its parent.  A step gives each node the pick that follows it; commit() keeps the longest path from node 0 on whose
+drafted tokens are those picks, and the sequence goes on behind it.  No counterpart in the reference, whose engines take one
+token of a sequence at a time.
+"""
+from operator import index
+
+import numpy as np
+
+
+def tree_of(parents, max_nodes=64):
+    """(depths [n], sees [n] u64) of a tree given by its nodes' parents: -1 for node 0, of every other an
+    earlier node.  Bit j of sees[i]: node i attends to node j (itself and its ancestors)."""
+    parents = [index(p) for p in parents]
+    if not 1 <= len(parents) <= max_nodes or parents[0] != -1 or any(not 0 <= p < i for i, p in enumerate(parents[1:], 1)):
+        raise ValueError(f"a tree: 1 to {max_nodes} nodes, -1 and then an earlier node of each as its parent")
+    depth, sees = [0], [1]
+    for i, p in enumerate(parents[1:], 1):
+        depth.append(depth[p] + 1)
+        sees.append(sees[p] | 1 << i)
+    return np.array(depth, np.int32), np.array(sees, np.uint64)
+
+
+class DraftTrees:
+    """Trees of at most max_nodes nodes, up to max_trees of them in a step, over `cache`.  Its arrays stay where they are, so
+    that a recorded step replays over what the next place() puts there."""
+
+    def __init__(self, cache, max_trees=None, max_nodes=32):
+        self.cache, self.be = cache, cache.be
+        self.max_trees, self.max_nodes = max_trees or cache.max_seqs, max_nodes
+        if not 1 <= self.max_trees <= 65535 or not 1 <= max_nodes <= 64:
+            raise ValueError("DraftTrees: 1 to 65535 trees of 1 to 64 nodes")
+        T, R = self.max_trees, cache.max_rows
+        self._host = np.zeros(2 * R + (T + 1) + 2 * T + 3 * R, np.int32)   # sees, first, base, seq, at, parent, draft
+        self.dev = self.be.upload(self._host)
+        at, self._parts, self._addr = 0, [], []
+        for n in (2 * R, T + 1, T, T, R, R, R):
+            self._parts.append(self._host[at:at + n])
+            self._addr.append(int(self.dev) + 4 * at)
+            at += n
+        sees, first, base, seq, self.at, self._parent, self._draft = self._addr
+        self.dev_out = self.be.alloc(4 * T * (max_nodes + 2))              # count, next, path
+        self.desc = self.be.trees(first, base, sees, int(cache.dev_table), T, cache.max_seqs, cache.max_pages, max_nodes, seq, self.at)
+        self._placed = None
+
+    def place(self, batch, rows=None):
+        """The nodes of a batch's trees get the next cells of their sequences: entries are (sequence, parents, tokens), tokens[0]
+        the sequence's next token.  Returns (rows descriptor, number of rows), the trees' nodes in order; with `rows`
+        the step has so many, free places behind the last tree's (as many as trees without a sequence have room for).
+        CacheFull, or an upload that fails, leaves the sequences as they were."""
+        cache, T = self.cache, self.max_trees
+        if self._placed is not None:
+            raise ValueError("DraftTrees.place: the trees before are neither committed nor dropped")
+        batch = [(index(s), tree_of(parents, self.max_nodes), [index(p) for p in parents], [index(t) for t in tokens]) for s, parents, tokens in batch]
+        used = sum(len(p) for _, _, p, _ in batch)
+        rest = (rows or used) - used
+        if not 1 <= len(batch) <= T or any(len(p) != len(t) for _, _, p, t in batch):
+            raise ValueError(f"DraftTrees.place: 1 to {T} trees, a token of each node")
+        if not 0 <= rest <= (T - len(batch)) * self.max_nodes:
+            raise ValueError("DraftTrees.place: rows for fewer than the nodes, or more free places than trees without a sequence have room for")
+        placed = [(s, cache.length(s), len(p)) for s, _, p, _ in batch]
+        desc, total = cache.rows([(s, n) for s, _, n in placed] + ([(None, rest)] if rest else []))
+        sees, first, base, seq, at, parent, draft = self._parts
+        sees = sees.view(np.uint64)
+        base[:], seq[:], at[:], parent[:], draft[:] = -1, -1, -1, -1, -1
+        sees[:] = 0
+        row = 0
+        for i, ((s, start, n), (_, (depth, see), p, tokens)) in enumerate(zip(placed, batch)):
+            first[i], base[i], seq[i] = row, start, s
+            sees[row:row + n], at[row:row + n], parent[row:row + n], draft[row:row + n] = see, start + depth, p, tokens
+            row += n
+        for i in range(len(batch), T + 1):                                 # free places share the rest
+            first[i] = row
+            row = min(row + self.max_nodes, total)
+        try:
+            self.be.h2d(self.dev, self._host)
+        except BaseException:
+            for s, start, _ in placed:
+                cache.truncate(s, start)
+            raise
+        self._placed = placed
+        self._rows = total
+        return desc, total
+
+    def _open(self, what):
+        if self._placed is None:
+            raise ValueError(f"DraftTrees.{what}: no trees are placed")
+        for s, start, n in self._placed:
+            if self.cache.length(s) != start + n or any(self.cache._users[p] > 1 for p in self.cache._pages[s][start // self.cache.page_size:]):
+                raise ValueError(f"DraftTrees.{what}: sequence {s} went on, or was forked, with its tree in it")
+
+    def commit(self, tok):
+        """Keep each tree's accepted path: its cells move to the sequence's next places in every layer, and the sequence
+        ends behind them.  tok: the picks of the step's rows (device).  Returns for each tree (the path's nodes, the token
+        that follows): the next tree's node 0."""
+        self._open("commit")
+        T, N = self.max_trees, self.max_nodes
+        count, nxt, path = (int(self.dev_out) + 4 * n for n in (0, T, 2 * T))
+        self.be.tree_commit(self.cache.layers, self.desc, self._parent, self._draft, tok, path, count, nxt, self._rows)
+        out = self.be.d2h(self.dev_out, (T * (N + 2),), np.int32)
+        count, nxt, path = out[:T], out[T:2 * T], out[2 * T:].reshape(T, N)
+        kept = []
+        for i, (s, start, _) in enumerate(self._placed):
+            self.cache.truncate(s, start + int(count[i]))
+            kept.append((path[i, :count[i]].tolist(), int(nxt[i])))
+        self._placed = None
+        return kept
+
+    def drop(self):
+        """forget the placed trees: their sequences are as before place()"""
+        self._open("drop")
+        for s, start, _ in self._placed:
+            self.cache.truncate(s, start)
+        self._placed = None
+
+    def free(self):
+        for b in (self.dev, self.dev_out):
+            b.free()

@@ -4,7 +4,8 @@ the bf16 head and a greedy pick (c/laguna.c forward_span / argmax_logits,
 c/laguna.c:1156-1160; rmsnorm_row c/moe_math.h:58-62).
 
 With attention layers (attn=) a layer is h += attention(rmsnorm(h)), then the MoE half, over a
-PagedCache (attention.py); with draw= a step ends in a random pick (lag_hip_sample) in place of the
+PagedCache (attention.py) or, latent attention, a LatentCache (latent.py); with trees= the rows are
+nodes of trees of drafted tokens (drafts.py); with draw= a step ends in a random pick (lag_hip_sample) in place of the
 greedy one.
 
 Synthetic stacks are seeded like the layers: norm weights 1 + N(0, 0.02)
@@ -17,6 +18,7 @@ from . import synth
 from .attention import AttnScratch, DeviceAttention, Rope
 from .backend import DeviceLayer, desc_of
 from .configs import WEIGHT_SIGMA
+from .latent import DeviceLatentAttention, LatentCache, LatentConfig, LatentScratch
 
 NORM_EPS = 1e-6
 
@@ -29,8 +31,8 @@ class DeviceStack:
         self.attn, self.rope, self.scratch, self.kept = [], None, None, []
 
     def add_attention(self, acfg, layers=None, seed=0):
-        """attention layers in front of the MoE ones: DeviceAttention's (sharing self.rope), or seeded
-        ones made on the device; once per stack"""
+        """attention layers in front of the MoE ones: DeviceAttention's (with a LatentConfig
+        DeviceLatentAttention's), sharing self.rope, or seeded ones made on the device; once per stack"""
         if self.attn:
             raise ValueError("add_attention: the stack has its attention layers")
         if layers is not None and len(layers) != len(self.layers):
@@ -39,7 +41,8 @@ class DeviceStack:
             raise ValueError("add_attention: layers of one width and of the same heads")
         self.rope = self.rope or Rope(self.be, acfg)
         self.attn = list(layers) if layers is not None else [
-            DeviceAttention.generate(self.be, acfg, self.cfg.D, seed, l, self.rope) for l in range(len(self.layers))]
+            (DeviceLatentAttention if isinstance(acfg, LatentConfig) else DeviceAttention).generate(
+                self.be, acfg, self.cfg.D, seed, l, self.rope) for l in range(len(self.layers))]
         return self
 
     def reserve(self, S):
@@ -48,7 +51,8 @@ class DeviceStack:
         if self.attn and (self.scratch is None or self.scratch.S < S):
             if self.scratch:
                 self.kept.append(self.scratch)
-            self.scratch = AttnScratch(self.be, self.attn[0].acfg, self.cfg.D, S)
+            acfg = self.attn[0].acfg
+            self.scratch = (LatentScratch if isinstance(acfg, LatentConfig) else AttnScratch)(self.be, acfg, self.cfg.D, S)
 
     @classmethod
     def from_host(cls, be, cfg, host_layers, norms, final_norm, head_bf16):
@@ -88,11 +92,12 @@ class DeviceStack:
         self.bufs.append(b)
         return b
 
-    def step(self, h, xn, logits, tok, S, fused=True, cache=None, rows=None, draw=None):
+    def step(self, h, xn, logits, tok, S, fused=True, cache=None, rows=None, draw=None, trees=None):
         """h [S, D] (device, updated in place), xn [S, D] scratch, logits [S, V], tok [S] int32;
         fused: each layer's RMSNorm inside its routing launch (lag_hip_moe_forward_rmsnorm,
         the same bits as the separate rmsnorm + forward); cache, rows: the PagedCache and the
-        descriptor of its rows() for the S tokens (a stack with attention layers); draw: (settings
+        descriptor of its rows() for the S tokens (a stack with attention layers), or of a LatentCache's
+        prompt(); trees: the DraftTrees over that cache whose place() gave the rows; draw: (settings
         from Backend.sample_params or None, random numbers [S] on the device)"""
         be, D = self.be, self.cfg.D
         desc = desc_of(self.cfg)
@@ -101,10 +106,17 @@ class DeviceStack:
                 raise ValueError("step: a stack with attention needs a cache of its layers, and rows")
             if rows is cache.desc and S > cache.max_rows:
                 raise ValueError("step: more rows than the cache has places for")
+            if isinstance(self.attn[0].acfg, LatentConfig) != isinstance(cache, LatentCache):
+                raise ValueError("step: latent attention and no other needs a LatentCache")
+            if trees is not None and (trees.cache is not cache or isinstance(cache, LatentCache)):
+                raise ValueError("step: trees over another cache, or over latents")
             self.reserve(S)
         for l, dl in enumerate(self.layers):
             if self.attn:
-                self.attn[l].forward(h, xn, S, cache.layers[l], rows, self.scratch)
+                if trees is None:
+                    self.attn[l].forward(h, xn, S, cache.layers[l], rows, self.scratch)
+                else:
+                    self.attn[l].forward(h, xn, S, cache.layers[l], rows, self.scratch, trees)
             if fused:
                 be.moe_forward_rmsnorm(desc, dl.weights(), self.norms[l], NORM_EPS, xn, h, S)
             else:
