@@ -158,17 +158,38 @@ __global__ __launch_bounds__(LH_NT) void k_latent_heads(const uint16_t *__restri
     for (int i = 0; i < OT; i++)
 #pragma unroll
         for (int j = 0; j < TT; j++) acc[i][j] = fl_f32x16{};
-#pragma unroll 2
-    for (int k = 0; k < n_in; k += 16) {
-        sw_u32x4 a[OT], b[TT];
+    // KC steps' operands are fetched while those before are multiplied: a wave has 16 loads or more on their way
+    constexpr int KC = 8 / OT;
+    const int steps = n_in / 16;
+    sw_u32x4 a[2][KC][OT], b[2][KC][TT];
+    auto fetch = [&](int k0, int to) {
 #pragma unroll
-        for (int i = 0; i < OT; i++) a[i] = *(const sw_u32x4 *)(wp[i] + k);
+        for (int u = 0; u < KC; u++) {
+            const int k = min(k0 + u, steps - 1) * 16;
 #pragma unroll
-        for (int i = 0; i < TT; i++) b[i] = *(const sw_u32x4 *)(xp[i] + k);
+            for (int i = 0; i < OT; i++) a[to][u][i] = *(const sw_u32x4 *)(wp[i] + k);
 #pragma unroll
-        for (int i = 0; i < OT; i++)
+            for (int i = 0; i < TT; i++) b[to][u][i] = *(const sw_u32x4 *)(xp[i] + k);
+        }
+    };
+    auto multiply = [&](int k0, int from) {
 #pragma unroll
-            for (int j = 0; j < TT; j++) acc[i][j] = fl_mfma<TYPE>(a[i], b[j], acc[i][j]);
+        for (int u = 0; u < KC; u++) {
+            if (k0 + u >= steps) break;
+#pragma unroll
+            for (int i = 0; i < OT; i++)
+#pragma unroll
+                for (int j = 0; j < TT; j++) acc[i][j] = fl_mfma<TYPE>(a[from][u][i], b[from][u][j], acc[i][j]);
+        }
+    };
+    fetch(0, 0);
+#pragma unroll 1
+    for (int k = 0; k < steps; k += 2 * KC) {
+        if (k + KC < steps) fetch(k + KC, 1);
+        multiply(k, 0);
+        if (k + KC >= steps) break;
+        if (k + 2 * KC < steps) fetch(k + 2 * KC, 0);
+        multiply(k + KC, 1);
     }
 #pragma unroll
     for (int j = 0; j < TT; j++) {
