@@ -315,7 +315,7 @@ __global__ __launch_bounds__((64 * WC * ln_split<R>())) void k_latent(SwLatent c
             const int page = pg < r.max_pages ? table[pg] : -1;
             return tok <= x.last && page >= 0 && page < c.n_pages;
         };
-        fl_run<WC, 1, SPLIT, NS, NL>(f, sh, sh + NS * F::TB, s_bad, from, from + len, wave, true, issue, whole, seen);
+        fl_run_split<WC, SPLIT, NS, NL>(f, sh, sh + NS * F::TB, s_bad, from, from + len, wave, issue, whole, seen);
         const bool all = len == tiles;
         float *pp = all ? nullptr : part + ((int64_t)hg * 2 * B + fl_slot(b, from)) * CW * (R + 4);
         fl_end<WC, 1, SPLIT>(f, sh, s_m, s_l, wave, [&](int col, int d, sw_f32x4 a, float mx, float sum) {

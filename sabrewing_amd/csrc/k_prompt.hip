@@ -204,7 +204,7 @@ struct LpFl : Fl<SW_KV_F16, 1, NOPE, DV, false> {
     static constexpr int ROPE_AT = Base::TB, TB = Base::TB + 32 * LP_ROPE * 2;
     sw_u32x4 R[LP_ROPE / 16];                                          // the queries' rotary part, scaled as the other is with its keys
     template <class Seen>
-    __device__ __forceinline__ void tile(const char *t, bool whole, uint32_t bad, Seen seen, char *, int, int) {
+    __device__ __forceinline__ void tile(const char *t, bool whole, uint32_t bad, Seen seen) {
         const int lane = fl_lane<Base::KEEP>(), c = lane & 31, h = lane >> 5;
         fl_f32x16 s = {};
         sw_u32x4 r[LP_ROPE / 16];
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(FL_NT, (lp_occ<NOPE, DV>())) void k_prompt(const ui
     };
     auto whole = [&](int tile) { return tile * 32 + 31 <= start + r0 && tile < tiles - 1; };
     auto seen = [&](int tile, int k) { return tile * 32 + k <= start + row && ((vm[tile] >> k) & 1); };
-    fl_run<WC, WT, 1, NS, NL>(f, sh, nullptr, s_bad, 0, tiles, wave, true, issue, whole, seen);
+    fl_run<WC, WT, NS, NL>(f, sh, s_bad, 0, tiles, wave, true, issue, whole, seen);
     fl_end<WC, WT, 1>(f, sh, s_m, s_l, wave, [&](int col, int d, sw_f32x4 a, float, float sum) {
         const int s = r0 + col;
         if (s >= S || d >= vd) return;

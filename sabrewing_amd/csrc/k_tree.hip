@@ -162,7 +162,7 @@ __global__ __launch_bounds__(FL_NT, (tr_occ<TYPE, DH>())) void k_tree(SwKv c, Sw
             const int page = pg < t.max_pages ? table[pg] : -1;
             return tok <= x.last && page >= 0 && page < c.n_pages && (j < 0 ? tok >= lo : j < x.n && ((sees >> j) & 1));
         };
-        fl_run<WC, WT, 1, NS, LK + LV>(f, sh, nullptr, s_bad, ta, ta + len, wave, columns, issue, whole, seen);
+        fl_run<WC, WT, NS, LK + LV>(f, sh, s_bad, ta, ta + len, wave, columns, issue, whole, seen);
         const bool all = len == tiles;
         float *pp = all ? nullptr : part + ((int64_t)hg * 2 * B + fl_slot(b, from)) * CW * (DH + 4);
         fl_end<WC, WT, 1>(f, sh, s_m, s_l, wave, [&](int col, int d, sw_f32x4 a, float mx, float sum) {

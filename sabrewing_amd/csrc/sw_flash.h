@@ -419,11 +419,10 @@ struct Fl {
     // One tile.  whole: every column attends to all of its tokens, else seen(token of the tile) says it for this lane's column, and bit k of
     // bad that token k's v is no number: whoever attends to it has no meaningful output.
     template <class Seen>
-    __device__ __forceinline__ void tile(const char *t, bool whole, uint32_t bad, Seen seen, char *xch, int wave, int odd) {
+    __device__ __forceinline__ void tile(const char *t, bool whole, uint32_t bad, Seen seen) {
         fl_f32x16 s = {};
         dot(t, s);
-        if constexpr (SPLIT > 1) shared(t, whole, bad, seen, s, xch, wave, odd);
-        else alone(t, whole, bad, seen, s);
+        alone(t, whole, bad, seen, s);
     }
     template <class Seen>
     __device__ __forceinline__ void alone(const char *t, bool whole, uint32_t bad, Seen seen, fl_f32x16 &s) {
@@ -448,30 +447,35 @@ struct Fl {
         weights(s, x);
         outputs(v, x, P, first);
     }
-    // Columns that SPLIT waves share: each wave has a share of the scores' sums of all 32 tokens.  They put them into LDS; each takes all sums of its
-    // own tokens (QT quads of a lane), makes their weights and puts those into LDS as the outputs' operand, which all read.  A maximum that
-    // grew too far (the waves' lags alike) is rare: then the waves put their maxima there too and make the weights again.
+    // Columns that SPLIT waves share: each wave has a share of the scores' sums of all 32 tokens, which it puts into LDS (sums).  Behind a
+    // barrier each takes all sums of its own tokens (QT quads of a lane), makes their weights and puts those into LDS as the outputs'
+    // operand, which all read behind another (weigh).  A maximum that grew too far (the waves' lags alike) is rare: then the waves
+    // put their maxima there too and make the weights again.
     static constexpr int QT = 4 / SPLIT;
+    __device__ __forceinline__ void sums(const char *t, char *xch, int wave) const {
+        fl_f32x16 s = {};
+        dot(t, s);
+        sw_f32x4 *to = (sw_f32x4 *)(xch + (wave - share) * XB) + fl_lane<KEEP>();
+#pragma unroll
+        for (int j = 0; j < 4; j++) to[(share * 4 + j) * 64] = sw_f32x4{s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]};
+    }
     template <class Seen>
-    __device__ __forceinline__ void shared(const char *t, bool whole, uint32_t bad, Seen seen, fl_f32x16 &s, char *xch, int wave, int odd) {
+    __device__ __forceinline__ void weigh(const char *t, bool whole, uint32_t bad, Seen seen, char *xch, int wave, int odd) {
         static_assert(SPLIT == 1 || SUMS, "16-bit weights");
         const int lane = fl_lane<KEEP>(), c = lane & 31, h4 = (lane & 32) >> 3;
         const char *v = (INK ? t : t + 32 * RBK) + share * VB;
         char *mine = xch + (wave - share) * XB;                        // of the columns: the shares' sums, the weights, the maxima, two flags
-        sw_f32x4 *sums = (sw_f32x4 *)mine + lane;
+        const sw_f32x4 *all = (const sw_f32x4 *)mine + lane;
         uint2 *w = (uint2 *)(mine + SPLIT * 4096) + lane * 2;
         float *top = (float *)(mine + SPLIT * 4096 + 2048) + c;
         int *grew = (int *)(xch + SPLIT * 4096 + 2048 + SPLIT * 128);  // (of all columns: the block's first)
-#pragma unroll
-        for (int j = 0; j < 4; j++) sums[(share * 4 + j) * 64] = sw_f32x4{s[4 * j], s[4 * j + 1], s[4 * j + 2], s[4 * j + 3]};
-        __syncthreads();
         float x[4 * QT], mx = -INFINITY;
 #pragma unroll
         for (int q = 0; q < QT; q++) {
-            sw_f32x4 y = sums[(share * QT + q) * 64];
+            sw_f32x4 y = all[(share * QT + q) * 64];
 #pragma unroll
             for (int k = 1; k < SPLIT; k++) {
-                const sw_f32x4 z = sums[(k * 4 + share * QT + q) * 64];
+                const sw_f32x4 z = all[(k * 4 + share * QT + q) * 64];
 #pragma unroll
                 for (int e = 0; e < 4; e++) y[e] = y[e] + z[e];
             }
@@ -509,7 +513,7 @@ struct Fl {
         };
         float add;
         if (__any((mx - m) * sc > LAG) && lane == 0) grew[odd] = 1;
-        if (wave == 0 && lane == 0) grew[odd ^ 1] = 0;                 // (read last before the barrier above)
+        if (wave == 0 && lane == 0) grew[odd ^ 1] = 0;                 // (read last before the barrier before)
         put(add);
         Piece first;
         read(v, 0, first);
@@ -555,23 +559,17 @@ struct Fl {
 
 // A block's work on one item: tiles ta .. tb - 1, dealt to its WT groups of waves in turn; NS tiles of a group in LDS (`sh`).
 // issue(tile, LDS address): the wave's share of a tile's loads, NL of them, and whether every page of it is there;
-// whole(tile) (alike in the waves that share a tile), seen(tile, token): the mask; columns: this wave has some (with SPLIT every
-// wave takes part); xch: LDS of the exchange; s_bad: two words a group.
-template <int WC, int WT, int SPLIT, int NS, int NL, class F, class Issue, class Whole, class Seen>
-__device__ __forceinline__ void fl_run(F &f, char *sh, char *xch, uint32_t *s_bad, int ta, int tb, int wave, bool columns, Issue issue, Whole whole, Seen seen) {
-    static_assert(WT == 1 || SPLIT == 1, "groups of waves do not exchange");
+// whole(tile) (alike in the waves that share a tile), seen(tile, token): the mask; columns: this wave has some; s_bad: two words a group.
+template <int WC, int WT, int NS, int NL, class F, class Issue, class Whole, class Seen>
+__device__ __forceinline__ void fl_run(F &f, char *sh, uint32_t *s_bad, int ta, int tb, int wave, bool columns, Issue issue, Whole whole, Seen seen) {
     constexpr int TB = F::TB;
-    constexpr bool shared = WC * SPLIT > 1;
+    constexpr bool shared = WC > 1;
     const int wt = WT == 1 ? 0 : wave / WC, all = (tb - ta + WT - 1) / WT, n = (tb - ta - wt + WT - 1) / WT;     // tiles of the longest group, of this one
     char *mine = sh + wt * NS * TB;
     s_bad += 2 * wt;
     const uint32_t lds = fl_lds_addr(mine);
-    const bool first = (threadIdx.x & 63) == 0 && (WT > 1 && WC == 1 ? true : wave % (WC * SPLIT) == 0);       // of its group
+    const bool first = (threadIdx.x & 63) == 0 && (WT > 1 && WC == 1 ? true : wave % WC == 0);       // of its group
     if (first) s_bad[0] = 0;                                           // (the item before is done with it)
-    if (SPLIT > 1 && threadIdx.x == 0) {
-        int *grew = (int *)(xch + SPLIT * 4096 + 2048 + SPLIT * 128);
-        grew[0] = grew[1] = 0;
-    }
     uint32_t there = 0;                                                // bit s: all pages of the tile in place s are there
     auto load = [&](int i, int s) {
         const bool ok = issue(ta + wt + i * WT, lds + s * TB);
@@ -600,13 +598,61 @@ __device__ __forceinline__ void fl_run(F &f, char *sh, char *xch, uint32_t *s_ba
         if (first) s_bad[(i + 1) & 1] = 0;
         uint32_t bad = 0;
         if (!all_whole) {
-            if (!whl) f.clean(mine + s * TB, WT == 1 ? wave : wave % WC, WC * SPLIT, s_bad + (i & 1));
+            if (!whl) f.clean(mine + s * TB, WT == 1 ? wave : wave % WC, WC, s_bad + (i & 1));
             if (shared) __syncthreads();
             else fl_wait_lds();
             bad = s_bad[i & 1];
         }
-        if (SPLIT > 1 || (i < n && columns)) f.tile(mine + s * TB, whl, bad, [&](int k) { return seen(t, k); }, xch, wave, i & 1);
+        if (i < n && columns) f.tile(mine + s * TB, whl, bad, [&](int k) { return seen(t, k); });
         s = s + 1 == NS ? 0 : s + 1;
+    }
+}
+
+// The same for WC groups of SPLIT waves that share columns, all of one tile; xch: LDS of the exchange.  Two barriers a tile: the outputs of one and the
+// sums of the next lie between the same two, where the waves' products fill each other's waits.
+template <int WC, int SPLIT, int NS, int NL, class F, class Issue, class Whole, class Seen>
+__device__ __forceinline__ void fl_run_split(F &f, char *sh, char *xch, uint32_t *s_bad, int ta, int tb, int wave, Issue issue, Whole whole, Seen seen) {
+    static_assert(NS >= 3, "a tile in the outputs, one in the sums, one on its way");
+    constexpr int TB = F::TB;
+    const int n = tb - ta;
+    const uint32_t lds = fl_lds_addr(sh);
+    const bool first = threadIdx.x == 0;
+    if (first) {
+        int *grew = (int *)(xch + SPLIT * 4096 + 2048 + SPLIT * 128);
+        grew[0] = grew[1] = 0;
+        s_bad[0] = 0;                                                  // (the item before is done with them)
+    }
+    uint32_t there = 0;                                                // bit s: all pages of the tile in place s are there
+    auto load = [&](int i, int s) {
+        const bool ok = issue(ta + i, lds + s * TB);
+        there = ok ? there | 1u << s : there & ~(1u << s);
+    };
+#pragma unroll 1
+    for (int i = 0; i < NS - 1; i++)
+        if (i < n) load(i, i);
+    if (NS - 2 >= n) fl_wait<0>();
+    else fl_wait<(NS - 2) * NL>();
+    __syncthreads();                                                   // the first tile is there
+    f.sums(sh, xch, wave);
+    int s = 0;                                                         // the place of tile i
+#pragma unroll 1
+    for (int i = 0; i < n; i++) {
+        if (i + NS - 2 >= n) fl_wait<0>();
+        else fl_wait<(NS - 3) * NL>();
+        __syncthreads();                                               // tile i + 1 and the sums of i are there, tile i - 1 is read
+        if (i + NS - 1 < n) load(i + NS - 1, s == 0 ? NS - 1 : s - 1);
+        if (first) s_bad[(i + 1) & 1] = 0;
+        char *t = sh + s * TB;
+        const bool whl = ((there >> s) & 1) && whole(ta + i);
+        uint32_t bad = 0;
+        if (!whl) {
+            f.clean(t, wave, WC * SPLIT, s_bad + (i & 1));
+            __syncthreads();
+            bad = s_bad[i & 1];
+        }
+        f.weigh(t, whl, bad, [&](int k) { return seen(ta + i, k); }, xch, wave, i & 1);
+        s = s + 1 == NS ? 0 : s + 1;
+        if (i + 1 < n) f.sums(sh + s * TB, xch, wave);
     }
 }
 
