@@ -254,7 +254,7 @@ __global__ __launch_bounds__((64 * WC * ln_split<R>())) void k_latent(SwLatent c
     constexpr int CW = 32 * WC, NS = ln_ns<R, WC>(), NL = (F::NCK / 2 + NW - 1) / NW;
     constexpr int SHT = NS * F::TB + NW * F::XB, SHB = SHT > fl_end_bytes<F, NW>() ? SHT : fl_end_bytes<F, NW>();
     static_assert(SHB <= 157 * 1024 && (NS < 3 ? 0 : NS - 2) * NL < 64, "LDS, and loads that a wave can count");
-    __shared__ __align__(16) char sh[SHB];
+    __shared__ __align__(256) char sh[SHB];
     __shared__ float s_m[NW][32], s_l[NW][32];
     __shared__ uint32_t s_bad[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = fl_uni(tid >> 6), wc = wave / SPLIT, share = wave % SPLIT, cl = lane & 31, h2 = lane >> 5;
@@ -299,14 +299,12 @@ __global__ __launch_bounds__((64 * WC * ln_split<R>())) void k_latent(SwLatent c
         const int *table = r.table + (int64_t)x.seq * r.max_pages;
         auto issue = [&](int tile, uint32_t lds) {
             const int t0 = tile * 32;
-            int lane_ = lane;
-            asm volatile("" : "+v"(lane_));                            // (the pieces' places are taken anew, not kept in registers)
             const FlPages g = fl_pages(table, r.max_pages, c.n_pages, c.psh, t0);
             if (c.psh >= 5 && width == R + LN_ROPE && c.ts < 1 << 25)  // one page, whole rows, not far apart
                 fl_rows<F::NCK, F::MK, NW, NL>((const char *)c.p + ((int64_t)max(g.p[0], 0) * c.ps + (int64_t)(t0 & pmask) * c.ts) * 2, (uint32_t)c.ts * 2,
-                                               wave, lane_, lds);
+                                               wave, lane, lds);
             else
-                fl_rows_any<F::NCK, F::MK, NW, NL>((const char *)c.p, g, c.ps * 2, c.ts * 2, t0, pmask, width / 8, wave, lane_, lds);
+                fl_rows_any<F::NCK, F::MK, NW, NL>((const char *)c.p, g, c.ps * 2, c.ts * 2, t0, pmask, width / 8, wave, lane, lds);
             return g.ok;
         };
         auto whole = [&](int tile) { return tile * 32 + 31 <= x.last; };

@@ -125,7 +125,7 @@ __global__ __launch_bounds__(LP_NT, 2) void k_prompt_expand(const uint16_t *__re
     uint32_t wo[4], xo[4];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        const int r = (k * 4 + wave) * 8 + (lane >> 3), p = (lane & 7) ^ (r & 7);
+        const int r = (k * 4 + wave) * 8 + (lane >> 3), p = (lane & 7) ^ fl_turn<7>(r);
         wo[k] = (uint32_t)min(o0 + r, n - 1) * rank * 2 + p * 16;
         xo[k] = (uint32_t)min(r, T32 - 1 - s0) * rank * 2 + p * 16;
     }
@@ -167,8 +167,8 @@ __global__ __launch_bounds__(LP_NT, 2) void k_prompt_expand(const uint16_t *__re
             sw_u32x4 a[2], b[2];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                a[u] = *(const sw_u32x4 *)(A + (wo0 + 32 * u + c) * (LE_K * 2) + (((2 * k + g) ^ (c & 7)) * 16));
-                b[u] = *(const sw_u32x4 *)(B + (ws0 + 32 * u + c) * (LE_K * 2) + (((2 * k + g) ^ (c & 7)) * 16));
+                a[u] = *(const sw_u32x4 *)(A + (wo0 + 32 * u + c) * (LE_K * 2) + (((2 * k + g) ^ fl_turn<7>(c)) * 16));
+                b[u] = *(const sw_u32x4 *)(B + (ws0 + 32 * u + c) * (LE_K * 2) + (((2 * k + g) ^ fl_turn<7>(c)) * 16));
             }
 #pragma unroll
             for (int u = 0; u < 2; u++)
@@ -209,7 +209,7 @@ struct LpFl : Fl<SW_KV_F16, 1, NOPE, DV, false> {
         fl_f32x16 s = {};
         sw_u32x4 r[LP_ROPE / 16];
 #pragma unroll
-        for (int i = 0; i < LP_ROPE / 16; i++) r[i] = *(const sw_u32x4 *)(t + ROPE_AT + c * (LP_ROPE * 2) + (((2 * i + h) ^ (c & 7)) * 16));
+        for (int i = 0; i < LP_ROPE / 16; i++) r[i] = *(const sw_u32x4 *)(t + ROPE_AT + c * (LP_ROPE * 2) + (((2 * i + h) ^ fl_turn<7>(c)) * 16));
         this->dot(t, s);
 #pragma unroll
         for (int i = 0; i < LP_ROPE / 16; i++) s = fl_mfma<TYPE>(r[i], R[i], s);
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(FL_NT, (lp_occ<NOPE, DV>())) void k_prompt(const ui
     constexpr int LK = (F::NCK / 2 + WC - 1) / WC, LV = (F::NCV / 2 + WC - 1) / WC, LR = (LP_ROPE / 16 + WC - 1) / WC, NL = LK + LV + LR;
     constexpr int SHT = WT * NS * F::TB, SHB = SHT > fl_end_bytes<F, FL_NW>() ? SHT : fl_end_bytes<F, FL_NW>();
     static_assert(SHB <= 157 * 1024 && (NS < 3 ? 0 : NS - 2) * NL < 64, "LDS, and loads that a wave can count");
-    __shared__ __align__(16) char sh[SHB];
+    __shared__ __align__(256) char sh[SHB];
     __shared__ float s_m[FL_NW][32], s_l[FL_NW][32];
     __shared__ uint32_t s_bad[2 * FL_NW];
     const int tid = threadIdx.x, lane = tid & 63, wave = fl_uni(tid >> 6), wc = wave % WC, cl = lane & 31, h2 = lane >> 5;

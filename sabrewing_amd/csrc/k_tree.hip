@@ -44,7 +44,7 @@ __global__ __launch_bounds__(FL_NT, (tr_occ<TYPE, DH>())) void k_tree(SwKv c, Sw
     constexpr int LK = (F::NCK / 2 + WC - 1) / WC, LV = (F::NCV / 2 + WC - 1) / WC;                    // loads of a wave
     constexpr int SHT = WT * NS * F::TB, SHB = SHT > fl_end_bytes<F, FL_NW>() ? SHT : fl_end_bytes<F, FL_NW>();
     static_assert(SHB <= 158 * 1024 && (NS < 3 ? 0 : NS - 2) * (LK + LV) < 64, "LDS, and loads that a wave can count");
-    __shared__ __align__(16) char sh[SHB];
+    __shared__ __align__(256) char sh[SHB];
     __shared__ float s_m[FL_NW][32], s_l[FL_NW][32];
     __shared__ uint32_t s_bad[2 * FL_NW];
     __shared__ int s_lo;
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(FL_NT, (tr_occ<TYPE, DH>())) void k_tree(SwKv c, Sw
         auto issue = [&](int tile, uint32_t lds) {
             const int t0 = tile * 32;
             int lane_ = lane;
-            asm volatile("" : "+v"(lane_));                            // (the pieces' places are taken anew, not kept in registers)
+            if constexpr (WC < 4) asm volatile("" : "+v"(lane_));      // (the pieces' places are taken anew, not kept in registers)
             const FlPages g = fl_pages(table, t.max_pages, c.n_pages, c.psh, t0);
             if (near && c.psh >= 5) {                                  // one page, rows not far apart
                 const int64_t at = (int64_t)max(g.p[0], 0) * psb + (int64_t)(t0 & pmask) * tsb;

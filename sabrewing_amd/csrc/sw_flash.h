@@ -65,6 +65,8 @@ __device__ __forceinline__ void fl_wait_lds() { asm volatile("s_waitcnt lgkmcnt(
 __device__ __forceinline__ uint32_t fl_lds_addr(const void *p) {
     return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p;
 }
+// LDS at an address (tiles begin on 256 bytes, so that a piece's turn is an exclusive or of the whole address)
+template <class T> __device__ __forceinline__ T fl_lds(uint32_t a) { return *(const __attribute__((address_space(3))) T *)(uintptr_t)a; }
 static __device__ const sw_u32x4 g_fl_zero = {0, 0, 0, 0};             // the source of pieces that a cell does not have
 
 // A token's page: entries of the table are read through the scalar cache (a vector load would wait for every
@@ -94,9 +96,13 @@ __device__ __forceinline__ FlPages fl_pages(const int *table, int max_pages, int
     return g;
 }
 
-// By how much (an exclusive or) a row's pieces are turned in LDS: M 7 and 3 for the scores' reads, one piece of 32 tokens (rows of whole 128 bytes, or
-// of odd 64); 6 and 0 for the outputs', two pieces of four tokens.
-template <int M> __device__ __forceinline__ int fl_turn(int t) { return M == 7 ? t & 7 : M == 3 ? (t >> 1) & 3 : M == 6 ? 2 * (t & 3) : 0; }
+// By how much (an exclusive or) a row's pieces are turned in LDS, whose 64 banks are 16 pieces.  The scores read one piece of 16 tokens at a time: M 15, 7
+// and 3 for rows of whole 256 bytes, odd 128 and odd 64 (where 1, 2 and 4 rows begin on different banks by themselves).  The outputs read four pieces
+// of four tokens: 12, 4 and 0 for the same rows; 7 does for them too, where one row serves both.  Each is linear in t's bits.
+template <int M>
+__device__ __forceinline__ constexpr int fl_turn(int t) {
+    return M == 15 ? t & 15 : M == 7 ? (t & 2) << 1 | (t & 4) >> 1 | (t & 8) >> 3 : M == 3 ? (t >> 2) & 3 : M == 12 ? 4 * (t & 3) : M == 4 ? 2 * (t & 2) : 0;
+}
 // Rows of NCH 16-byte pieces from `base` on, `step` bytes apart (below 2^26), into a tile at `to`: wave w of W's share, N loads of it.
 // M: the pieces' turn by token.
 template <int NCH, int M, int W, int N>
@@ -104,7 +110,7 @@ __device__ __forceinline__ void fl_rows(const char *base, uint32_t step, int w, 
 #pragma unroll
     for (int k = 0; k < N; k++) {
         const int kk = (N * W > NCH / 2) ? min(k * W + w, NCH / 2 - 1) : k * W + w;
-        if constexpr (64 % NCH == 0 && 64 / NCH <= 8 && M != 3) {      // a load is some whole rows: a part of the turn is the wave's
+        if constexpr (64 % NCH == 0) {                                 // a load is some whole rows: a part of the turn is the wave's
             constexpr int RP = 64 / NCH;
             const uint32_t off = lane / NCH * step + ((lane % NCH ^ fl_turn<M>(lane / NCH) ^ fl_turn<M>(kk * RP)) * 16);
             fl_load16(base + (int64_t)kk * RP * step, off, to + kk * 1024);
@@ -197,7 +203,9 @@ struct Fl {
     // bytes of a wave in the exchange, and of 32 columns: a share's sums of scores; the columns' weights and maxima
     static constexpr int XB = SPLIT > 1 ? 4096 + (2048 + SPLIT * 128) / SPLIT + 16 : 0;
     // how a row's pieces are turned
-    static constexpr int MK = NCK % 8 == 0 ? 7 : 3, MV = INK ? MK : F32 ? (NCV % 8 == 0 ? 7 : 3) : NCV % 8 == 0 ? 6 : 0;
+    static constexpr int MK = NCK % 16 == 0 ? 15 : NCK % 8 == 0 ? 7 : 3;
+    static constexpr int MV = INK ? MK : F32 ? (NCV % 16 == 0 ? 15 : NCV % 8 == 0 ? 7 : 3) : NCV % 16 == 0 ? 12 : NCV % 8 == 0 ? 4 : 0;
+    static_assert(!INK || MK == 7, "a turn that serves both reads");
     // weights are kept below 2^OFF; a maximum may lag behind by LAG powers of two (a running maximum that grows costs a pass
     // over the outputs; 16-bit weights hold 2^8 as well as 1, in parts they may not)
     static constexpr float LAG = NP == 1 && !F32 ? 8.f : 0.f;
@@ -206,7 +214,7 @@ struct Fl {
     sw_u32x4 Q[F32 ? 1 : NP][DKS];
     fl_f32x16 O[NO];
     float m, l, sc;
-    static constexpr int KB = MK == 3 ? 2 : 4 / SPLIT;                 // a lane's places in a tile's row of k repeat after KB steps
+    static constexpr int KB = MK == 3 ? 2 : (MK == 15 ? 8 : 4) / SPLIT;// a lane's places in a tile's row of k repeat after KB steps
     int share;                                                         // (every SPLIT-th step is the wave's)
 
     // scale: of the scores, in powers of two.  Its sign (and a scale of 0) goes into the queries, see query().
@@ -238,14 +246,15 @@ struct Fl {
         // QB steps' operands are read while the QB before are multiplied
         constexpr int NB = (DKS + QB - 1) / QB;
         const int lane = fl_lane<KEEP>(), c = lane & 31, h = lane >> 5;
-        int kb[KB];
+        const uint32_t row = fl_lds_addr(t) + c * RBK + (((2 * share + h) ^ fl_turn<MK>(c)) * 16);
+        uint32_t kb[KB];
 #pragma unroll
-        for (int i = 0; i < KB; i++) kb[i] = c * RBK + (((2 * (SPLIT * i + share) + h) ^ fl_turn<MK>(c)) * 16);
+        for (int i = 0; i < KB; i++) kb[i] = row ^ (32 * SPLIT * i);
         sw_u32x4 a[2][QB];
         auto read = [&](int b) {
 #pragma unroll
             for (int k = 0; k < QB; k++)
-                if (b * QB + k < DKS) a[b & 1][k] = *(const sw_u32x4 *)(t + kb[(b * QB + k) % KB] + (b * QB + k) / KB * (KB * SPLIT * 32));
+                if (b * QB + k < DKS) a[b & 1][k] = fl_lds<sw_u32x4>(kb[(b * QB + k) % KB] + (b * QB + k) / KB * (KB * SPLIT * 32));
         };
         read(0);
         __builtin_amdgcn_s_setprio(1);
@@ -328,7 +337,7 @@ struct Fl {
             const int lot = step / S.n, g = step % S.n, w = S.w[g], c = lane & 31, h = lane >> 5;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const int x = MV == 7 ? 4 * h + k : 2 * h + (k >> 1);
+                const int x = fl_turn<MV>(8 * lot + k) ^ fl_turn<MV>(4 * h);
                 const char *row = t + (8 * lot + k + 4 * h) * RBV + S.b0[g];
                 if (w == 2) {
                     const uint2 y = *(const uint2 *)(row + ((c >> 1) ^ x) * 16 + (c & 1) * 8);
@@ -337,15 +346,16 @@ struct Fl {
             }
         } else {
             const int k = 4 * (lane >> 5) + ((lane & 15) >> 2), d = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), x = fl_turn<MV>(k);
-            const char *row = t + k * RBV + (lane & 1) * 8;
+            const uint32_t row = fl_lds_addr(t) + k * RBV + (lane & 1) * 8 + (d ^ x) * 16;
 #pragma unroll
             for (int i = 0; i < VT; i++) {
                 const int at = step * VT + i, lot = at / NO, o = at % NO;
                 if (at >= 2 * NO) break;
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
-                    const int piece = MV == 7 || MV == 6 ? ((4 * (o & 1) + d) ^ x) + 8 * (o >> 1) : (d ^ x) + 4 * o;
-                    const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(row + (16 * lot + 8 * b) * RBV + piece * 16));
+                    constexpr int W = MV == 12 ? 4 : MV == 0 ? 1 : 2;  // (operands of the pieces that are turned among themselves)
+                    const uint32_t a = (row ^ (64 * (o % W) ^ 16 * fl_turn<MV>(8 * b))) + (16 * lot + 8 * b) * RBV + 64 * W * (o / W);
+                    const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(uintptr_t)a);
                     const uint2 z = __builtin_bit_cast(uint2, y);
                     p.v[4 * i + 2 * b] = z.x; p.v[4 * i + 2 * b + 1] = z.y;
                 }
