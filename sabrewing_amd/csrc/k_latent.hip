@@ -145,7 +145,9 @@ __global__ __launch_bounds__(LH_NT) void k_latent_heads(const uint16_t *__restri
                                                         int n_in, int n_out, void *__restrict__ y, int64_t yrs, int64_t yhs, int S) {
     const int lane = threadIdx.x & 63, c = lane & 31, g = lane >> 5;
     const int to = (n_out / 32 + OT - 1) / OT, ts = (S + 32 * TT - 1) / (32 * TT);
-    const int64_t w = (int64_t)blockIdx.x * (LH_NT / 64) + fl_uni((int)(threadIdx.x >> 6));
+    // a die takes neighbouring blocks: those of a head's other rows find its W in their cache
+    const unsigned n8 = gridDim.x & ~7u, block = blockIdx.x < n8 ? (blockIdx.x & 7) * (n8 >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+    const int64_t w = (int64_t)block * (LH_NT / 64) + fl_uni((int)(threadIdx.x >> 6));
     if (w >= (int64_t)H * to * ts) return;
     const int o0 = (int)(w % to) * OT * 32, s0 = (int)(w / to % ts) * TT * 32, h = (int)(w / to / ts);
     const uint16_t *wp[OT], *xp[TT];
