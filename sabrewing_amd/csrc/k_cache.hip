@@ -269,6 +269,7 @@ int sw_launch_kv_copy(hipStream_t st, const SwKv *layers, int n_layers, const in
 // A tree's accepted path and its cells.  The walk takes a ballot a step (a node a lane) and is taken by every wave of every
 // layer's block: nothing to wait for.  A path's nodes rise, so node path[i]'s cell lies at or behind its place i and is
 // nobody's place before i: a thread moves one piece of 16 bytes of all cells in turn, eight reads and then their writes.
+// Bound by the launch and a chain of waits: 48 layers of 8 heads of 128, one tree of 16 nodes 5.4 us, 32 of 64 nodes 5.8.
 #define TC_NT 256
 struct SwCommit { void *pool[2 * SW_COPY_LAYERS]; };
 __global__ __launch_bounds__(TC_NT) void k_tree_commit(SwCommit a, SwKv c, SwTrees t, const int *__restrict__ parent, const int *__restrict__ draft,

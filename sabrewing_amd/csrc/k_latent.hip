@@ -44,7 +44,8 @@ __device__ __forceinline__ void lt_turn(LtPairs p, int u, int dims, bool inter, 
         *(uint2 *)(to + dims / 2 + 4 * u) = make_uint2(lt_pack<TYPE>(w[0], w[1]), lt_pack<TYPE>(w[2], w[3]));
     }
 }
-// Blocks (row, y): y = 0 the row's cell, others LA_UNITS units of eight values a thread of its query heads.
+// Blocks (row, y): y = 0 the row's cell, others UNITS units of eight values a thread of its query heads; the row's angles are taken once a block, in 64
+// bits.  Bound by bytes: 1,024 rows of 128 heads (128 + 64), 151 MB, 36 us or 4.2 TB/s; one row of 16 heads 4.9 us, a launch.
 #define LA_NT 256
 template <int TYPE, int UNITS>
 __global__ __launch_bounds__(LA_NT) void k_latent_append(SwLatent c, SwRows r, SwRope rope, const float *__restrict__ ckv, int64_t ldc,
@@ -138,7 +139,9 @@ int sw_launch_latent_append(hipStream_t st, const SwLatent &c, const SwRows &r, 
 
 // ------------------------------------------------------------------ a product for each head ----
 // y[s, h] = W[h] x[s, h]: a wave takes OT x 32 outputs of a head and TT x 32 rows on the 32 x 32 matrix instructions, operands
-// straight from memory (a row of W is read by one wave, or from the caches by the few that share its outputs).
+// straight from memory (a row of W is read by one wave, or from the caches by the few that share its outputs).  Up to 64 rows a wave takes 32 by 32,
+// as there are few waves; beyond 64 by 64, half the reads.  Bound by W's bytes: 128 heads of 512 x 128, one row 6.0 us (16.8 MB, 2.8 TB/s with the
+// launch), 64 rows of 128 x 512 with 32-bit outputs 11.0 us (29 MB).  Two steps' operands at a time instead of eight: 6.6 and 12.7.
 #define LH_NT 256
 template <int TYPE, bool YF32, int OT, int TT>
 __global__ __launch_bounds__(LH_NT) void k_latent_heads(const uint16_t *__restrict__ x, int64_t xrs, int64_t xhs, const uint16_t *__restrict__ W, int H,
@@ -232,8 +235,13 @@ int sw_launch_latent_heads(hipStream_t st, int type, const SwHeads &x, const voi
 }
 
 // ------------------------------------------------------------------ the absorbed form ----
+// Heads are the columns, a cell is key and value of all of them: 2 (2 rank + rope) operations a head for 2 (rank + rope) bytes.  Queries and outputs of 512
+// values by 32 columns are more than a wave's registers, so that waves share columns (sw_flash.h).  Rows' tiles are laid end to end and dealt to
+// 256 blocks as trees' are.  Bf16, rank 512 + 64: 32 rows of 128 heads over 100 to 16,384 cells 151 us: matrix instructions a
+// quarter of the cycles, vector ones 16 %, LDS 27 %, the rest waits at two barriers a tile of eight waves on a CU; the join's 10 us within.  One row
+// of 16 heads over 1,500 cells 19 us: a chain of waits, and the join's launch.
 #define LN_ROPE 64                                                     // a cell's rotary part in LDS: the rest of it zeros
-#define LN_SPLIT 256                                                   // beyond so many rows none is split
+#define LN_SPLIT 256                                                   // beyond so many rows none is split: they fill the chip by themselves
 // waves that share 32 heads (a share of the outputs is whole pairs of 32 values), and tiles in LDS
 template <int R> constexpr int ln_split() { return R % 256 == 0 ? 4 : 2; }
 template <int TYPE, int R> using LnFl = Fl<TYPE, 1, R + LN_ROPE, R, true, ln_split<R>()>;
@@ -354,7 +362,8 @@ __global__ __launch_bounds__(FL_NT) void k_latent_join(SwLatent c, SwRows r, int
     }
 }
 
-// columns of a block (waves that have 32 each) and blocks of each group of heads; 0: a block a row
+// Columns of a block (32 times wc) and blocks of each group of heads; 0: a block a row.  64 columns a block where there are more than 32: 128 heads 151 us,
+// in blocks of 128 columns (half the reads of cells, queries in LDS for want of registers) 20 more, with two waves to share 64 columns 40 more.
 struct LnPlan { int wc, groups, B; };
 static LnPlan ln_plan(const SwLatent &c, const SwRows &r, int H, int S) {
     LnPlan p;
