@@ -48,7 +48,7 @@ class DraftTrees:
         sees, first, base, seq, self.at, self._parent, self._draft = self._addr
         self.dev_out = self.be.alloc(4 * T * (max_nodes + 2))              # count, next, path
         self.desc = self.be.trees(first, base, sees, int(cache.dev_table), T, cache.max_seqs, cache.max_pages, max_nodes, seq, self.at)
-        self._placed = None
+        self._placed, self.rows = None, 0                                  # (rows: of the placed trees' step)
 
     def place(self, batch, rows=None):
         """The nodes of a batch's trees get the next cells of their sequences: entries are (sequence, parents, tokens), tokens[0]
@@ -58,7 +58,7 @@ class DraftTrees:
         cache, T = self.cache, self.max_trees
         if self._placed is not None:
             raise ValueError("DraftTrees.place: the trees before are neither committed nor dropped")
-        batch = [(index(s), tree_of(parents, self.max_nodes), [index(p) for p in parents], [index(t) for t in tokens]) for s, parents, tokens in batch]
+        batch = [(index(s), tree_of(parents, self.max_nodes), [index(p) for p in parents], np.array([index(t) for t in tokens], np.int32)) for s, parents, tokens in batch]
         used = sum(len(p) for _, _, p, _ in batch)
         rest = (rows or used) - used
         if not 1 <= len(batch) <= T or any(len(p) != len(t) for _, _, p, t in batch):
@@ -85,40 +85,37 @@ class DraftTrees:
             for s, start, _ in placed:
                 cache.truncate(s, start)
             raise
-        self._placed = placed
-        self._rows = total
+        self._placed, self.rows = placed, total
         return desc, total
-
-    def _open(self, what):
-        if self._placed is None:
-            raise ValueError(f"DraftTrees.{what}: no trees are placed")
-        for s, start, n in self._placed:
-            if self.cache.length(s) != start + n or any(self.cache._users[p] > 1 for p in self.cache._pages[s][start // self.cache.page_size:]):
-                raise ValueError(f"DraftTrees.{what}: sequence {s} went on, or was forked, with its tree in it")
 
     def commit(self, tok):
         """Keep each tree's accepted path: its cells move to the sequence's next places in every layer, and the sequence
         ends behind them.  tok: the picks of the step's rows (device).  Returns for each tree (the path's nodes, the token
-        that follows): the next tree's node 0."""
-        self._open("commit")
+        that follows): the next tree's node 0.  Refused, with the trees as they were, where a sequence was closed, went on or was forked
+        since; drop() is the way out."""
+        if self._placed is None:
+            raise ValueError("DraftTrees.commit: no trees are placed")
+        for s, start, n in self._placed:
+            if self.cache.length(s) != start + n or any(self.cache._users[p] > 1 for p in self.cache._pages[s][start // self.cache.page_size:]):
+                raise ValueError(f"DraftTrees.commit: sequence {s} went on, or was forked, with its tree in it")
         T, N = self.max_trees, self.max_nodes
         count, nxt, path = (int(self.dev_out) + 4 * n for n in (0, T, 2 * T))
-        self.be.tree_commit(self.cache.layers, self.desc, self._parent, self._draft, tok, path, count, nxt, self._rows)
+        self.be.tree_commit(self.cache.layers, self.desc, self._parent, self._draft, tok, path, count, nxt, self.rows)
         out = self.be.d2h(self.dev_out, (T * (N + 2),), np.int32)
         count, nxt, path = out[:T], out[T:2 * T], out[2 * T:].reshape(T, N)
         kept = []
         for i, (s, start, _) in enumerate(self._placed):
             self.cache.truncate(s, start + int(count[i]))
             kept.append((path[i, :count[i]].tolist(), int(nxt[i])))
-        self._placed = None
+        self._placed, self.rows = None, 0
         return kept
 
     def drop(self):
-        """forget the placed trees: their sequences are as before place()"""
-        self._open("drop")
-        for s, start, _ in self._placed:
-            self.cache.truncate(s, start)
-        self._placed = None
+        """forget the placed trees: their sequences are as before place(), but those that were closed or went on since"""
+        for s, start, n in self._placed or ():
+            if self.cache._pages[s] is not None and self.cache.length(s) == start + n:
+                self.cache.truncate(s, start)
+        self._placed, self.rows = None, 0
 
     def free(self):
         for b in (self.dev, self.dev_out):

@@ -46,10 +46,10 @@ class LatentConfig:
 
 
 class LatentPrompt:
-    """the rows of a prompt: `rows` for appending, where its sequence's pages are listed, its first position"""
+    """the n rows of a prompt: `rows` for appending, where its sequence's pages are listed, its first position"""
 
-    def __init__(self, rows, pages, n_pages, start):
-        self.rows, self.pages, self.n_pages, self.start = rows, pages, n_pages, start
+    def __init__(self, rows, pages, n_pages, start, n):
+        self.rows, self.pages, self.n_pages, self.start, self.n = rows, pages, n_pages, start, n
 
 
 class LatentCache(PagedCache):
@@ -77,7 +77,7 @@ class LatentCache(PagedCache):
         """rows((seq, n)) for a step that takes a prompt's keys and values from its latents once: (LatentPrompt, n)"""
         start = self.length(seq)
         rows, total = self.rows([(seq, n)])
-        return LatentPrompt(rows, int(self.dev_table) + 4 * seq * self.max_pages, len(self._pages[seq]), start), total
+        return LatentPrompt(rows, int(self.dev_table) + 4 * seq * self.max_pages, len(self._pages[seq]), start, n), total
 
 
 class DeviceLatentAttention:
@@ -132,6 +132,8 @@ class DeviceLatentAttention:
             raise ValueError("DeviceLatentAttention: a cache of other latents")
         if S > t.S or t.shape != self.shape:
             raise ValueError("DeviceLatentAttention: scratch for fewer rows or other heads")
+        if isinstance(rows, LatentPrompt) and S != rows.n:
+            raise ValueError("DeviceLatentAttention: a prompt of another number of rows")
         be.rmsnorm(h, self.norm, xn, S, D, a.eps)
         be.head_argmax(self.wkv, True, xn, S, D, a.cell, t.ckv)
         if a.q_rank:

@@ -110,6 +110,8 @@ class DeviceStack:
                 raise ValueError("step: latent attention and no other needs a LatentCache")
             if trees is not None and (trees.cache is not cache or isinstance(cache, LatentCache)):
                 raise ValueError("step: trees over another cache, or over latents")
+            if trees is not None and S != trees.rows:
+                raise ValueError("step: another number of rows than the placed trees have")
             self.reserve(S)
         for l, dl in enumerate(self.layers):
             if self.attn:

@@ -108,13 +108,26 @@ def test_what_place_refuses_changes_nothing():
     c.fork(a)
     with pytest.raises(ValueError):
         t.commit(0)                                    # the fork holds the tree's cells
-    c2 = PagedCache(be, 1, 4, 8, 2, 32, max_seqs=2)
+    c2 = PagedCache(be, 1, 4, 8, 2, 32, max_seqs=2, max_rows=8)
     t2 = DraftTrees(c2)
     s = c2.open()
     t2.place([(s, [-1], [1])])
     c2.rows([s])
     with pytest.raises(ValueError):
         t2.commit(0)
+    t2.drop()
+    assert c2.length(s) == 2                           # (it went on: left as it is)
+    r = c2.open()
+    t2.place([(s, [-1], [1]), (r, [-1, 0], [1, 2])])
+    c2.close(r)
+    with pytest.raises(ValueError):
+        t2.commit(0)
+    t2.drop()
+    assert c2.length(s) == 2
+    with pytest.raises(OverflowError):
+        t2.place([(s, [-1], [1 << 31])])
+    assert c2.length(s) == 2 and t2._placed is None
+    invariants(c2)
     for kw in (dict(max_nodes=0), dict(max_nodes=65), dict(max_trees=65536)):
         with pytest.raises(ValueError):
             DraftTrees(c, **kw)
@@ -157,9 +170,12 @@ def test_stacks_of_latents_and_trees_refuse_each_other():
     def step(s, c, rows, trees=None):
         be.calls.clear()
         s.step(be.alloc(4), be.alloc(4), be.alloc(4), be.alloc(4), 2, cache=c, rows=rows, trees=trees)
+    t.place([(cache.open(), [-1, 0], [3, 4])])
     step(st, cache, cache.desc, t)
     assert "attn_tree" in be.calls and "attn_paged" not in be.calls and "qk_rope_append_at" in be.calls
-    for c, tr in ((lat, None), (other, t)):
+    one = DraftTrees(cache, 1)
+    one.place([(cache.open(), [-1], [3])])
+    for c, tr in ((lat, None), (other, t), (cache, one), (cache, DraftTrees(cache))):
         with pytest.raises(ValueError):
             step(st, c, c.desc, tr)
         assert not be.calls
@@ -173,8 +189,12 @@ def test_stacks_of_latents_and_trees_refuse_each_other():
     ls.add_attention(L, [make(L)])
     step(ls, lat, lat.desc)
     assert isinstance(ls.scratch, LatentScratch) and be.calls.count("latent_heads") == 2 and "attn_latent" in be.calls
-    step(ls, lat, LatentPrompt(lat.desc, 4096, 2, 0))
+    step(ls, lat, LatentPrompt(lat.desc, 4096, 2, 0, 2))
     assert "latent_heads" not in be.calls and "attn_latent" not in be.calls and "attn_latent_prompt" in be.calls
+    for n in (1, 3):
+        with pytest.raises(ValueError):
+            step(ls, lat, LatentPrompt(lat.desc, 4096, 2, 0, n))
+        assert not be.calls
     for c, tr in ((cache, None), (LatentCache(be, 1, 8, 8, 256, 16, max_seqs=3), None), (LatentCache(be, 1, 8, 8, 128, 16, "f16", max_seqs=3), None), (lat, t)):
         with pytest.raises(ValueError):
             step(ls, c, c.desc, tr)
