@@ -239,7 +239,7 @@ int sw_launch_latent_heads(hipStream_t st, int type, const SwHeads &x, const voi
 // values by 32 columns are more than a wave's registers, so that waves share columns (sw_flash.h).  Rows' tiles are laid end to end and dealt to
 // 256 blocks as trees' are.  Bf16, rank 512 + 64: 32 rows of 128 heads over 100 to 16,384 cells 151 us: matrix instructions a
 // quarter of the cycles, vector ones 16 %, LDS 27 %, the rest waits at two barriers a tile of eight waves on a CU; the join's 10 us within.  One row
-// of 16 heads over 1,500 cells 19 us: a chain of waits, and the join's launch.
+// of 16 heads over 1,500 cells 18 us: a chain of waits, and the join's launch.
 #define LN_ROPE 64                                                     // a cell's rotary part in LDS: the rest of it zeros
 #define LN_SPLIT 256                                                   // beyond so many rows none is split: they fill the chip by themselves
 // waves that share 32 heads (a share of the outputs is whole pairs of 32 values), and tiles in LDS

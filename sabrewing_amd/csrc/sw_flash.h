@@ -749,12 +749,22 @@ __device__ __forceinline__ sw_f32x4 fl_join(const float *p, int64_t step, int pa
     const bool mine = d < DV;
     sw_f32x4 a = {0.f, 0.f, 0.f, 0.f};
     float M = -INFINITY, L = 0.f;
+    parts = fl_uni(parts);
     for (int k0 = 0; k0 < parts; k0 += 64) {
+        const int top = min(64, parts - k0);
+        constexpr int LOT = 8;                                         // outputs on their way, the first while the weights are made (16: 2 us more for many columns)
+        sw_f32x4 y[LOT];
+        auto fetch = [&](int k) {
+#pragma unroll
+            for (int i = 0; i < LOT; i++)
+                if (k + i * SUB < top) y[i] = *(const sw_f32x4 *)(p + max(0, 2 * (k0 + min(k + i * SUB + sub, top - 1)) - 1) * step + 4 + (mine ? d : 0));
+        };
         float m = -INFINITY, l = 0.f;
         if (k0 + lane < parts) {
-            const float2 y = *(const float2 *)(p + max(0, 2 * (k0 + lane) - 1) * step);
-            m = y.x; l = y.y;
+            const float2 z = *(const float2 *)(p + max(0, 2 * (k0 + lane) - 1) * step);
+            m = z.x; l = z.y;
         }
+        fetch(0);
         float n = fmaxf(M, m);
 #pragma unroll
         for (int o = 32; o; o >>= 1) n = fmaxf(n, __shfl_xor(n, o));
@@ -767,21 +777,18 @@ __device__ __forceinline__ sw_f32x4 fl_join(const float *p, int64_t step, int pa
         M = n;
 #pragma unroll
         for (int e = 0; e < 4; e++) a[e] = a[e] * g;
-        const int top = min(64, parts - k0);
-        for (int k = 0; k < top; k += 8 * SUB) {
-            sw_f32x4 y[8];
-            float f[8];
+        for (int k = 0;;) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < LOT; i++) {
+                if (k + i * SUB >= top) break;
                 const int at = k + i * SUB + sub;
-                y[i] = sw_f32x4{0.f, 0.f, 0.f, 0.f};
-                if (mine && at < top) y[i] = *(const sw_f32x4 *)(p + max(0, 2 * (k0 + at) - 1) * step + 4 + d);
-                f[i] = __shfl(w, at & 63);
+                const float f = __shfl(w, at & 63);
+#pragma unroll
+                for (int e = 0; e < 4; e++) a[e] = at < top ? __builtin_fmaf(y[i][e], f, a[e]) : a[e];
             }
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) a[e] = k + i * SUB + sub < top ? __builtin_fmaf(y[i][e], f[i], a[e]) : a[e];
+            k += LOT * SUB;
+            if (k >= top) break;
+            fetch(k);
         }
     }
 #pragma unroll
