@@ -7,8 +7,7 @@ PagedCache (attention.py).
 
 Node 0 is the sequence's next token (the pick that the last step ended in), every other node a drafted token
 behind its parent.  A step gives each node the pick that follows it; commit() keeps the longest path from node 0 on whose
-drafted tokens are those picks, and the sequence goes on behind it.  No counterpart in the reference, whose engines take one
-token of a sequence at a time.
+drafted tokens are those picks, and the sequence goes on behind it.  The reference's tables have no slot for it.
 """
 from operator import index
 
