@@ -249,11 +249,11 @@ template <int R, int WC> constexpr int ln_ns() {
     constexpr int n = (156 * 1024 - WC * ln_split<R>() * 5 * 1024) / (32 * (R + LN_ROPE) * 2);
     return n > 4 ? 4 : n;
 }
-struct LnRow { int seq, last; };
+struct LnRow { int seq, last; };                                       // (last: -1 for every free place, so that it has no tiles)
 __device__ __forceinline__ LnRow ln_row(const SwLatent &c, const SwRows &r, int s) {
     LnRow x;
     x.seq = r.seq ? r.seq[s] : s;
-    x.last = x.seq < 0 || x.seq >= r.n_seqs ? -1 : min(r.pos[s], (r.max_pages << c.psh) - 1);
+    x.last = x.seq < 0 || x.seq >= r.n_seqs ? -1 : max(-1, min(r.pos[s], (r.max_pages << c.psh) - 1));
     return x;
 }
 template <int TYPE, int R, int WC>
