@@ -86,6 +86,7 @@ class PagedCache:
         self._free = list(range(n_pages - 1, -1, -1))                      # the lowest last
         self._pages = [None] * max_seqs
         self._len = [0] * max_seqs
+        self._marks, self._changes = [0] * max_seqs, 0                     # (no two states of a place share a mark)
         self._table = np.full((max_seqs, self.max_pages), -1, np.int32)
         self._dirty = set()
         self._rows = np.full((2, self.max_rows), -1, np.int32)             # positions, sequences
@@ -103,10 +104,20 @@ class PagedCache:
                 return i
         raise CacheFull(f"all {self.max_seqs} sequences are in use")
 
+    def _changed(self, seq):
+        self._changes += 1
+        self._marks[seq] = self._changes
+
+    def mark(self, seq):
+        """a number that the sequence keeps until it grows, is truncated or closed, and that no other has had"""
+        self._check(seq)
+        return self._marks[seq]
+
     def open(self):
         """a new, empty sequence"""
         seq = self._slot()
         self._pages[seq], self._len[seq] = [], 0
+        self._changed(seq)
         return seq
 
     def fork(self, seq):
@@ -115,6 +126,7 @@ class PagedCache:
         new = self._slot()
         self._pages[new], self._len[new] = list(self._pages[seq]), self._len[seq]
         self._users[self._pages[new]] += 1
+        self._changed(new)
         self._table[new] = self._table[seq]
         self._dirty.add(new)
         return new
@@ -133,6 +145,8 @@ class PagedCache:
         if not 0 <= length <= self._len[seq]:
             raise ValueError(f"PagedCache: sequence {seq} has {self._len[seq]} tokens, not {length}")
         keep = -(-length // self.page_size)
+        if length < self._len[seq]:
+            self._changed(seq)
         gone, self._pages[seq], self._len[seq] = self._pages[seq][keep:], self._pages[seq][:keep], length
         if gone:
             self._drop(gone)
@@ -236,6 +250,8 @@ class PagedCache:
                 self._users[p] = 0
                 self._free.append(p)
             raise
+        for s in old:
+            self._changed(s)
         return self.desc, total
 
     def _upload(self):

@@ -47,7 +47,7 @@ class DraftTrees:
         sees, first, base, seq, self.at, self._parent, self._draft = self._addr
         self.dev_out = self.be.alloc(4 * T * (max_nodes + 2))              # count, next, path
         self.desc = self.be.trees(first, base, sees, int(cache.dev_table), T, cache.max_seqs, cache.max_pages, max_nodes, seq, self.at)
-        self._placed, self.rows = None, 0                                  # (rows: of the placed trees' step)
+        self._placed, self._marks, self.rows = None, (), 0                 # (rows: of the placed trees' step)
 
     def place(self, batch, rows=None):
         """The nodes of a batch's trees get the next cells of their sequences: entries are (sequence, parents, tokens), tokens[0]
@@ -66,6 +66,7 @@ class DraftTrees:
             raise ValueError("DraftTrees.place: rows for fewer than the nodes, or more free places than trees without a sequence have room for")
         placed = [(s, cache.length(s), len(p)) for s, _, p, _ in batch]
         desc, total = cache.rows([(s, n) for s, _, n in placed] + ([(None, rest)] if rest else []))
+        marks = [cache.mark(s) for s, _, _ in placed]
         sees, first, base, seq, at, parent, draft = self._parts
         sees = sees.view(np.uint64)
         base[:], seq[:], at[:], parent[:], draft[:] = -1, -1, -1, -1, -1
@@ -84,19 +85,19 @@ class DraftTrees:
             for s, start, _ in placed:
                 cache.truncate(s, start)
             raise
-        self._placed, self.rows = placed, total
+        self._placed, self._marks, self.rows = placed, marks, total
         return desc, total
 
     def commit(self, tok):
         """Keep each tree's accepted path: its cells move to the sequence's next places in every layer, and the sequence
         ends behind them.  tok: the picks of the step's rows (device).  Returns for each tree (the path's nodes, the token
-        that follows): the next tree's node 0.  Refused, with the trees as they were, where a sequence was closed, went on or was forked
-        since; drop() is the way out."""
+        that follows): the next tree's node 0.  Refused, with the trees as they were, where a sequence was closed (its place may be another's
+        by now), went on, was truncated or forked since; drop() is the way out."""
         if self._placed is None:
             raise ValueError("DraftTrees.commit: no trees are placed")
-        for s, start, n in self._placed:
-            if self.cache.length(s) != start + n or any(self.cache._users[p] > 1 for p in self.cache._pages[s][start // self.cache.page_size:]):
-                raise ValueError(f"DraftTrees.commit: sequence {s} went on, or was forked, with its tree in it")
+        for (s, start, n), mark in zip(self._placed, self._marks):
+            if self.cache.mark(s) != mark or any(self.cache._users[p] > 1 for p in self.cache._pages[s][start // self.cache.page_size:]):
+                raise ValueError(f"DraftTrees.commit: sequence {s} is another, went on, was truncated or forked, with its tree in it")
         T, N = self.max_trees, self.max_nodes
         count, nxt, path = (int(self.dev_out) + 4 * n for n in (0, T, 2 * T))
         self.be.tree_commit(self.cache.layers, self.desc, self._parent, self._draft, tok, path, count, nxt, self.rows)
@@ -110,9 +111,9 @@ class DraftTrees:
         return kept
 
     def drop(self):
-        """forget the placed trees: their sequences are as before place(), but those that were closed or went on since"""
-        for s, start, n in self._placed or ():
-            if self.cache._pages[s] is not None and self.cache.length(s) == start + n:
+        """forget the placed trees: their sequences are as before place(), but those that were closed, truncated or went on since"""
+        for (s, start, _), mark in zip(self._placed or (), self._marks):
+            if self.cache._pages[s] is not None and self.cache.mark(s) == mark:
                 self.cache.truncate(s, start)
         self._placed, self.rows = None, 0
 
