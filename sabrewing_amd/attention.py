@@ -356,6 +356,8 @@ class DeviceAttention:
             raise ValueError("DeviceAttention: a cache of other heads")
         if S > scratch.S or scratch.shape != self.shape:
             raise ValueError("DeviceAttention: scratch for fewer rows or other heads")
+        if trees is not None:
+            trees.within(a.window)
         be.rmsnorm(h, self.norm, xn, S, D, a.eps)
         be.head_argmax(self.wqkv, True, xn, S, D, a.qkv_rows, scratch.qkv)
         scale = 1.0 / math.sqrt(a.head_dim)

@@ -47,13 +47,23 @@ class DraftTrees:
         sees, first, base, seq, self.at, self._parent, self._draft = self._addr
         self.dev_out = self.be.alloc(4 * T * (max_nodes + 2))              # count, next, path
         self.desc = self.be.trees(first, base, sees, int(cache.dev_table), T, cache.max_seqs, cache.max_pages, max_nodes, seq, self.at)
+        self.window = 0                                                    # the narrowest of the layers that were run over the trees
+        self._depth = 0                                                    # of the placed trees' deepest node
         self._placed, self._marks, self.rows = None, (), 0                 # (rows: of the placed trees' step)
+
+    def within(self, window):
+        """A layer with such a window (0: none) is to run over the trees.  A node attends to all of its ancestors, so that a tree as deep as
+        the window is refused: here, and by every later place(), whose trees a recorded step takes without asking."""
+        if window and self._placed is not None and self._depth >= window:
+            raise ValueError(f"DraftTrees: a tree {self._depth} deep, and a layer whose window is {window}")
+        self.window = min(self.window or window, window or self.window)
 
     def place(self, batch, rows=None):
         """The nodes of a batch's trees get the next cells of their sequences: entries are (sequence, parents, tokens), tokens[0]
         the sequence's next token.  Returns (rows descriptor, number of rows), the trees' nodes in order; with `rows`
         the step has so many, free places behind the last tree's (as many as trees without a sequence have room for).
-        CacheFull, or an upload that fails, leaves the sequences as they were."""
+        Trees as deep as a layer's window are refused (see within).  CacheFull, or an upload that fails, leaves the sequences as
+        they were."""
         cache, T = self.cache, self.max_trees
         if self._placed is not None:
             raise ValueError("DraftTrees.place: the trees before are neither committed nor dropped")
@@ -64,6 +74,9 @@ class DraftTrees:
             raise ValueError(f"DraftTrees.place: 1 to {T} trees, a token of each node")
         if not 0 <= rest <= (T - len(batch)) * self.max_nodes:
             raise ValueError("DraftTrees.place: rows for fewer than the nodes, or more free places than trees without a sequence have room for")
+        deepest = max(int(depth.max()) for _, (depth, _), _, _ in batch)
+        if self.window and deepest >= self.window:
+            raise ValueError(f"DraftTrees.place: a tree {deepest} deep, and a layer whose window is {self.window}")
         placed = [(s, cache.length(s), len(p)) for s, _, p, _ in batch]
         desc, total = cache.rows([(s, n) for s, _, n in placed] + ([(None, rest)] if rest else []))
         marks = [cache.mark(s) for s, _, _ in placed]
@@ -85,7 +98,7 @@ class DraftTrees:
             for s, start, _ in placed:
                 cache.truncate(s, start)
             raise
-        self._placed, self._marks, self.rows = placed, marks, total
+        self._placed, self._marks, self._depth, self.rows = placed, marks, deepest, total
         return desc, total
 
     def commit(self, tok):

@@ -112,6 +112,9 @@ class DeviceStack:
                 raise ValueError("step: trees over another cache, or over latents")
             if trees is not None and S != trees.rows:
                 raise ValueError("step: another number of rows than the placed trees have")
+            if trees is not None:
+                for a in self.attn:
+                    trees.within(a.acfg.window)
             self.reserve(S)
         for l, dl in enumerate(self.layers):
             if self.attn:
