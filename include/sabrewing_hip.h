@@ -350,7 +350,7 @@ int    lag_hip_attn_latent(const LagHipLatentCache *c, const LagHipKvRows *r, co
  * [n_seq_pages]) are the sequence's pages as its table row names them; wk [n_heads][nope][rank] and wv [n_heads][v_dim][rank] in the cache's
  * type; q [S][n_heads][nope + rope_dims] in the cache's type; out [S][n_heads][v_dim] in f32 (out_f32) or the cache's type: row s
  * attends to the tokens t <= start + s.  nope and v_dim: multiples of 32 up to 256.  Keys and values are made once a call, rounded to 11 bits
- * (f16, scaled by a power of two for each head: what is more than 2^20 below a head's largest loses bits); sums and the softmax in 32 bits,
+ * (f16, scaled by a power of two for each head: what is more than 2^20 below the largest of a head's, over all of the call's tokens, loses bits); sums and the softmax in 32 bits,
  * its weights in 11.  Cells that lead nowhere are not attended to; cells that are no numbers reach the rows that attend to them.  Everything
  * is 16-byte aligned; out overlaps nothing that is read.  start + S <= 2^22.  Its scratch (2 (rank + 64) bytes a token, and a GiB at most of keys and values) is the arena's.  0 = ok */
 int    lag_hip_attn_latent_prompt(const LagHipLatentCache *c, const int *pages, int n_seq_pages, int start, const void *wk, const void *wv, int nope,

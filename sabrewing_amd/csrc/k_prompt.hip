@@ -11,8 +11,8 @@
 // Keys and values are held in f16, whatever the cache's type: 11 bits, where bf16's 8 would add errors as large as the
 // output's own rounding three times over.  f16's range is met by powers of two: |k_d| <= |Wk_d| |c_t| (their 2-norms), so each
 // head's keys are scaled by 2^(15 - a - b), a and b the exponents of the largest |Wk_d| and |c_t|, which keeps them
-// below 2^15; a sum of many terms stays some 2^8 below that bound, and what is more than 2^20 smaller than the largest loses bits.
-// Values alike; queries are scaled to 2^13.  The rotary part stays as the cache has it.
+// below 2^15; a sum of many terms stays some 2^8 below that bound, and what is more than 2^20 smaller than the largest, of whichever
+// token, loses bits.  Values alike; queries are scaled to 2^13.  The rotary part stays as the cache has it.
 #include "sw_flash.h"
 
 #define LP_NT 256
@@ -22,44 +22,44 @@ template <int TYPE> __device__ __forceinline__ float lp_float(uint32_t w, int hi
     if constexpr (TYPE == SW_KV_BF16) return __builtin_bit_cast(float, hi ? w & 0xFFFF0000u : w << 16);
     else return (float)__builtin_bit_cast(_Float16, (uint16_t)(hi ? w >> 16 : w));
 }
-// e with x < 2^e for a finite sum of squares x^2; far from the ends of f32
-__device__ __forceinline__ int lp_exp(float x2) {
-    const float x = sqrtf(x2);
-    return x > 0.f ? min(max(ilogbf(x) + 1, -100), 100) : -100;
-}
+// e with x < 2^e for a sum of squares x^2, in 64 bits: whatever finite values of 16 bits are squared, it is finite, and 0 where they all are
+#define LP_LEAST -140
+__device__ __forceinline__ int lp_exp(double x2) { return x2 > 0.0 ? (ilogb(x2) + 2) >> 1 : LP_LEAST; }
 
 // Blocks 0 .. tiles - 1: 32 cells side by side in xl [tokens][rank] and xr [tokens][64] (zeros where there is no cell or no value), te: the
-// exponent of the tile's largest norm, vm: which tokens have a cell.  Blocks behind them, LP_PARTS for a head's keys and as many for its
+// exponent of the tile's largest norm, re: of its largest rotary value, vm: which tokens have a cell.  Blocks behind them, LP_PARTS for a head's keys and as many for its
 // values: we, the exponent of the largest norm of a share of the rows of Wk or Wv.  Values that are no numbers do not count in a
 // norm.  A wave takes its 8 rows at once: one wait.
 #define LP_PARTS 8
 template <int TYPE>
 __global__ __launch_bounds__(LP_NT) void k_prompt_gather(SwLatent c, const int *__restrict__ pages, int max_pages, int T, const uint16_t *__restrict__ wk,
                                                          const uint16_t *__restrict__ wv, int nope, int vd, uint16_t *__restrict__ xl,
-                                                         uint16_t *__restrict__ xr, int *__restrict__ te, uint32_t *__restrict__ vm, int *__restrict__ we) {
+                                                         uint16_t *__restrict__ xr, int *__restrict__ te, int *__restrict__ re, uint32_t *__restrict__ vm,
+                                                         int *__restrict__ we) {
     constexpr int NW = LP_NT / 64, N = 32 / NW;
-    __shared__ float s_n[NW];
+    __shared__ int s_n[NW];
+    __shared__ float s_r[NW];
     __shared__ uint32_t s_v[NW];
     const int tid = threadIdx.x, lane = tid & 63, wave = fl_uni(tid >> 6), tiles = (T + 31) / 32;
-    float best = 0.f;
+    double ss[N];                                                      // of each row
+    float turned = 0.f;
     uint32_t there = 0;
     // (every lane reads, those behind a row's end its last values, which do not count)
     const bool in = 8 * lane < c.rank;
     const int at = min(8 * lane, c.rank - 8), rat = c.rank + max(0, min(8 * lane, c.rope - 8));
     sw_u32x4 a[N];
-    auto norm = [&](sw_u32x4 y, bool count) {
-        float ss = 0.f;
+    auto finite = [](uint32_t y, int k) {
+        const float f = lp_float<TYPE>(y, k);
+        return fabsf(f) < INFINITY ? f : 0.f;
+    };
+    auto squares = [&](sw_u32x4 y, bool count) {
+        double x = 0.0;
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const float f = lp_float<TYPE>(y[e], k), g = fabsf(f) < INFINITY ? f : 0.f;
-                ss = __builtin_fmaf(g, g, ss);
-            }
-        ss = count && in ? ss : 0.f;
-#pragma unroll
-        for (int o = 32; o; o >>= 1) ss = ss + __shfl_xor(ss, o);
-        best = fmaxf(best, ss);
+        for (int e = 0; e < 8; e++) {
+            const double g = finite(y[e / 2], e & 1);
+            x = __builtin_fma(g, g, x);
+        }
+        return count && in ? x : 0.0;
     };
     if ((int)blockIdx.x < tiles) {
         const int t0 = blockIdx.x * 32 + wave * N, pmask = (1 << c.psh) - 1;
@@ -85,8 +85,12 @@ __global__ __launch_bounds__(LP_NT) void k_prompt_gather(SwLatent c, const int *
             }
             if (in) *(sw_u32x4 *)(xl + (int64_t)(t0 + i) * c.rank + 8 * lane) = a[i];
             if (lane < LP_ROPE / 8) *(sw_u32x4 *)(xr + (int64_t)(t0 + i) * LP_ROPE + 8 * lane) = b[i];
-            norm(a[i], true);
+            ss[i] = squares(a[i], true);
+#pragma unroll
+            for (int e = 0; e < 8; e++) turned = fmaxf(turned, fabsf(finite(b[i][e / 2], e & 1)));
         }
+#pragma unroll
+        for (int o = LP_ROPE / 16; o; o >>= 1) turned = fmaxf(turned, __shfl_xor(turned, o));
     } else {
         const int k = (blockIdx.x - tiles) / LP_PARTS, part = (blockIdx.x - tiles) % LP_PARTS, h = k >> 1, n = k & 1 ? vd : nope;
         const uint16_t *w = (k & 1 ? wv : wk) + (int64_t)h * n * c.rank;
@@ -94,30 +98,48 @@ __global__ __launch_bounds__(LP_NT) void k_prompt_gather(SwLatent c, const int *
 #pragma unroll
         for (int i = 0; i < N; i++) a[i] = *(const sw_u32x4 *)(w + (int64_t)min(i0 + i, n - 1) * c.rank + at);
 #pragma unroll
-        for (int i = 0; i < N; i++) norm(a[i], i0 + i < end);
+        for (int i = 0; i < N; i++) ss[i] = squares(a[i], i0 + i < end);
     }
-    if (lane == 0) { s_n[wave] = best; s_v[wave] = there << (wave * N); }
+    // the rows' sums, half of the rows with each half of the lanes: 10 exchanges instead of 48
+    static_assert(N == 8, "rows of a wave");
+#pragma unroll
+    for (int o = 32, n = N / 2; n; o >>= 1, n >>= 1)
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+            const double give = lane & o ? ss[i] : ss[i + n], keep = lane & o ? ss[i + n] : ss[i];
+            ss[i] = keep + __shfl_xor(give, o);
+        }
+#pragma unroll
+    for (int o = 4; o; o >>= 1) ss[0] = ss[0] + __shfl_xor(ss[0], o);
+    int best = lp_exp(ss[0]);
+#pragma unroll
+    for (int o = 32; o >= 8; o >>= 1) best = max(best, __shfl_xor(best, o));
+    if (lane == 0) { s_n[wave] = best; s_r[wave] = turned; s_v[wave] = there << (wave * N); }
     __syncthreads();
     if (tid == 0) {
 #pragma unroll
-        for (int i = 1; i < NW; i++) best = fmaxf(best, s_n[i]);
-        if ((int)blockIdx.x < tiles) { te[blockIdx.x] = lp_exp(best); vm[blockIdx.x] = s_v[0] | s_v[1] | s_v[2] | s_v[3]; }
-        else we[blockIdx.x - tiles] = lp_exp(best);
+        for (int i = 1; i < NW; i++) { best = max(best, s_n[i]); turned = fmaxf(turned, s_r[i]); }
+        if ((int)blockIdx.x < tiles) {
+            te[blockIdx.x] = best;
+            re[blockIdx.x] = turned > 0.f ? ilogbf(turned) + 1 : LP_LEAST;
+            vm[blockIdx.x] = s_v[0] | s_v[1] | s_v[2] | s_v[3];
+        }
+        else we[blockIdx.x - tiles] = best;
     }
 }
 
-// Keys and values of heads h0 ..: [head][tokens][np or vp] in f16, times 2^eh, the values behind nope or vd zeros.  A block takes 128 outputs
-// by 128 tokens, both in LDS by 64 of the summed values, two lots ahead; a wave 64 by 64 of them.  A die's blocks share
+// Keys and values of heads h0 .. of H: [head][tokens][np or vp] in f16, times 2^eh, the values behind nope or vd zeros (eh[2 H]: the
+// exponent of the largest rotary value of all tokens).  A block takes 128 outputs by 128 tokens, both in LDS by 64 of the summed values, two lots ahead; a wave 64 by 64 of them.  A die's blocks share
 // a range of tokens (they stay in its cache) and go through all heads.
 #define LE_K 64
 #define LE_TILE (128 * LE_K * 2)
 template <int TYPE>
-__global__ __launch_bounds__(LP_NT, 2) void k_prompt_expand(const uint16_t *__restrict__ xl, const int *__restrict__ te, const int *__restrict__ we, int T32,
-                                                            int rank, const uint16_t *__restrict__ wk, const uint16_t *__restrict__ wv, int nope, int vd,
+__global__ __launch_bounds__(LP_NT, 2) void k_prompt_expand(const uint16_t *__restrict__ xl, const int *__restrict__ te, const int *__restrict__ re,
+                                                            const int *__restrict__ we, int T32, int H, int rank, const uint16_t *__restrict__ wk, const uint16_t *__restrict__ wv, int nope, int vd,
                                                             int np, int vp, int heads, int h0, uint16_t *__restrict__ kb, uint16_t *__restrict__ vb,
                                                             int *__restrict__ eh) {
     __shared__ __align__(16) char sh[2 * 2 * LE_TILE];
-    __shared__ int s_e[LP_NT / 64];
+    __shared__ int s_e[LP_NT / 64], s_r[LP_NT / 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = fl_uni(tid >> 6), c = lane & 31, g = lane >> 5;
     const int tk = (np + 127) / 128, tv = (vp + 127) / 128, nt = (T32 + 127) / 128, per = (nt + 7) / 8;
     const int die = blockIdx.x & 7, j0 = blockIdx.x >> 3, tt = die * per + j0 % per, y0 = j0 / per;
@@ -142,18 +164,18 @@ __global__ __launch_bounds__(LP_NT, 2) void k_prompt_expand(const uint16_t *__re
         for (int k = 0; k < 4; k++) fl_load16(xb + i * (LE_K * 2), xo[k], lds + (i & 1) * 2 * LE_TILE + LE_TILE + (k * 4 + wave) * 1024);
     };
     load(0);
-    int e = -100;
-    for (int i = tid; i < T32 / 32; i += LP_NT) e = max(e, te[i]);
-    for (int o = 32; o; o >>= 1) e = max(e, __shfl_xor(e, o));
-    if (lane == 0) s_e[wave] = e;
+    int e = LP_LEAST, r = LP_LEAST;
+    for (int i = tid; i < T32 / 32; i += LP_NT) { e = max(e, te[i]); r = max(r, re[i]); }
+    for (int o = 32; o; o >>= 1) { e = max(e, __shfl_xor(e, o)); r = max(r, __shfl_xor(r, o)); }
+    if (lane == 0) { s_e[wave] = e; s_r[wave] = r; }
     __syncthreads();
-    int w = -100;
+    int w = LP_LEAST;
 #pragma unroll
-    for (int i = 0; i < LP_NT / 64; i++) e = max(e, s_e[i]);
+    for (int i = 0; i < LP_NT / 64; i++) { e = max(e, s_e[i]); r = max(r, s_r[i]); }
 #pragma unroll
     for (int i = 0; i < LP_PARTS; i++) w = max(w, we[(2 * h + kv) * LP_PARTS + i]);
     e = min(max(15 - e - w, -120), 120);
-    if (tid == 0 && tt == 0) eh[2 * h + kv] = e;
+    if (tid == 0 && tt == 0) { eh[2 * h + kv] = e; eh[2 * H] = r; }    // (every block the same)
     fl_f32x16 acc[2][2];
 #pragma unroll
     for (int i = 0; i < 2; i++)
@@ -207,6 +229,8 @@ struct LpFl : Fl<SW_KV_F16, 1, NOPE, DV, false> {
     using Base = Fl<SW_KV_F16, 1, NOPE, DV, false>;
     static constexpr int ROPE_AT = Base::TB, TB = Base::TB + 32 * LP_ROPE * 2;
     sw_u32x4 R[LP_ROPE / 16];                                          // the queries' rotary part, scaled as the other is with its keys
+    int lift;                                                          // or 2^lift less (lifts: in any of the wave's columns)
+    bool lifts;
     template <class Seen>
     __device__ __forceinline__ void tile(const char *t, bool whole, uint32_t bad, Seen seen) {
         const int lane = fl_lane<Base::KEEP>(), c = lane & 31, h = lane >> 5;
@@ -215,8 +239,14 @@ struct LpFl : Fl<SW_KV_F16, 1, NOPE, DV, false> {
 #pragma unroll
         for (int i = 0; i < LP_ROPE / 16; i++) r[i] = *(const sw_u32x4 *)(t + ROPE_AT + c * (LP_ROPE * 2) + (((2 * i + h) ^ fl_turn<7>(c)) * 16));
         this->dot(t, s);
+        if (__builtin_expect(lifts, 0))
+#pragma unroll
+            for (int j = 0; j < 16; j++) s[j] = ldexpf(s[j], -lift);
 #pragma unroll
         for (int i = 0; i < LP_ROPE / 16; i++) s = fl_mfma<TYPE>(r[i], R[i], s);
+        if (__builtin_expect(lifts, 0))
+#pragma unroll
+            for (int j = 0; j < 16; j++) s[j] = ldexpf(s[j], lift);
         this->alone(t, whole, bad, seen, s);
     }
 };
@@ -267,13 +297,19 @@ __global__ __launch_bounds__(FL_NT, (lp_occ<NOPE, DV>())) void k_prompt(const ui
     mx = fl_max2(mx);
     mr = fl_max2(mr);
     // The scores are to be 2^E times as large, of both parts: the keys are 2^ek times, the queries 2^(E - ek) -- up to 2^13 -- and the
-    // rotary queries, whose keys are as they were, 2^E, up to 2^15 in f16 (2^100 in bf16).  Where those bind, the first part is the
-    // smaller one by as much, and what its queries lose below f16's range is as small beside the other.
-    const int ek = eh[2 * h], ev = eh[2 * h + 1];
+    // rotary queries, whose keys are as they were, 2^E, where the sum of their products then stays far below f32's largest (er).  But they are
+    // 2^15 at most in f16 (2^120 in bf16).  Where that binds, E follows while the first part's queries keep their bits (2^1 and
+    // what is 2^15 below it); else the rotary scores are made 2^lift smaller and lifted.
+    const int ek = eh[2 * h], ev = eh[2 * h + 1], er = eh[2 * H];
     const bool nx = mx > 0.f && mx < INFINITY, nr = mr > 0.f && mr < INFINITY;
-    int E = nx ? 13 - ilogbf(mx) + ek : ek;
-    if (nr) E = min(E, (TYPE == SW_KV_BF16 ? 100 : 14) - ilogbf(mr));
-    E = min(max(E, -120), 120);
+    int E = min(max(nx ? 13 - ilogbf(mx) + ek : ek, -120), 120), Er = E;
+    if (nr) {
+        E = max(min(E, 99 - ilogbf(mr) - er), -120);
+        Er = min(E, (TYPE == SW_KV_BF16 ? 120 : 14) - ilogbf(mr));
+        if (E - Er <= 12) E = Er;
+    }
+    f.lift = E - Er;
+    f.lifts = __any(f.lift != 0);
     const float sg = sc0 < 0.f ? -1.f : sc0 == 0.f ? 0.f : 1.f;       // (the scale's sign, or none: see Fl::begin)
     f.begin(ldexpf(sc0, -E));
 #pragma unroll
@@ -287,7 +323,7 @@ __global__ __launch_bounds__(FL_NT, (lp_occ<NOPE, DV>())) void k_prompt(const ui
     for (int k = 0; k < LP_ROPE / 16; k++) {
         float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = sg * ldexpf(lp_float<TYPE>(rr[k][e / 2], e & 1), E);
+        for (int e = 0; e < 8; e++) y[e] = sg * ldexpf(lp_float<TYPE>(rr[k][e / 2], e & 1), Er);
         sw_u32x4 o[1];
         fl_split<TYPE, 1>(y, o);
         f.R[k] = o[0];
@@ -324,7 +360,7 @@ __global__ __launch_bounds__(FL_NT, (lp_occ<NOPE, DV>())) void k_prompt(const ui
 
 // ------------------------------------------------------------------ scratch and launches ----
 // heads expanded at a time: what they take stays about a GiB
-struct LpPlan { int64_t T32, xl, xr, te, vm, we, eh, kb, vb, total; int heads, np, vp; };
+struct LpPlan { int64_t T32, xl, xr, te, re, vm, we, eh, kb, vb, total; int heads, np, vp; };
 static LpPlan lp_plan(const SwLatent &c, int H, int nope, int vd, int64_t T) {
     LpPlan p;
     p.T32 = (T + 31) / 32 * 32;
@@ -337,9 +373,10 @@ static LpPlan lp_plan(const SwLatent &c, int H, int nope, int vd, int64_t T) {
     p.xl = take(p.T32 * c.rank * 2);
     p.xr = take(p.T32 * LP_ROPE * 2);
     p.te = take(p.T32 / 8);
+    p.re = take(p.T32 / 8);
     p.vm = take(p.T32 / 8);
     p.we = take((int64_t)H * 8 * LP_PARTS);
-    p.eh = take((int64_t)H * 8);
+    p.eh = take((int64_t)H * 8 + 4);
     p.kb = take(p.heads * p.T32 * p.np * 2);
     p.vb = take(p.heads * p.T32 * p.vp * 2);
     p.total = at;
@@ -373,14 +410,14 @@ static int lp_run(hipStream_t st, const SwLatent &c, const int *pages, int max_p
     const int T = start + S;
     const LpPlan p = lp_plan(c, H, nope, vd, T);
     uint16_t *xl = (uint16_t *)(A + p.xl), *xr = (uint16_t *)(A + p.xr), *kb = (uint16_t *)(A + p.kb), *vb = (uint16_t *)(A + p.vb);
-    int *te = (int *)(A + p.te), *we = (int *)(A + p.we), *eh = (int *)(A + p.eh);
+    int *te = (int *)(A + p.te), *re = (int *)(A + p.re), *we = (int *)(A + p.we), *eh = (int *)(A + p.eh);
     uint32_t *vm = (uint32_t *)(A + p.vm);
     SW_LAUNCH(k_prompt_gather<TYPE>, dim3((unsigned)(p.T32 / 32 + 2 * H * LP_PARTS)), dim3(LP_NT), 0, st, c, pages, max_pages, T, (const uint16_t *)wk, (const uint16_t *)wv,
-              nope, vd, xl, xr, te, vm, we);
+              nope, vd, xl, xr, te, re, vm, we);
     for (int h0 = 0; h0 < H; h0 += p.heads) {
         const int heads = H - h0 < p.heads ? H - h0 : p.heads, blocks = (p.np + 127) / 128 + (p.vp + 127) / 128;
         const int64_t per = (p.T32 / 32 + 31) / 32;                     // lots of 128 tokens of a die
-        SW_LAUNCH(k_prompt_expand<TYPE>, dim3((unsigned)(8 * per * heads * blocks)), dim3(LP_NT), 0, st, xl, te, we, (int)p.T32, c.rank,
+        SW_LAUNCH(k_prompt_expand<TYPE>, dim3((unsigned)(8 * per * heads * blocks)), dim3(LP_NT), 0, st, xl, te, re, we, (int)p.T32, H, c.rank,
                   (const uint16_t *)wk, (const uint16_t *)wv, nope, vd, p.np, p.vp, heads, h0, kb, vb, eh);
         const LpArgs a = {kb, vb, xr, vm, eh, (int)p.T32, start, S, nope, vd, c.rope, (const uint16_t *)q, H, h0, heads, sc, out, out_f32};
         if (nope <= 64) lp_values<TYPE, 64>(st, a);

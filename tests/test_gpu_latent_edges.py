@@ -2,7 +2,10 @@
 import numpy as np
 import pytest
 
+from latents import Latents, NAN, normal
+from paged import from_bits, to_type
 from test_gpu_latent import Case
+from test_gpu_prompt import Case as Prompt
 
 pytestmark = pytest.mark.gpu
 
@@ -22,4 +25,53 @@ def test_every_negative_position_is_a_free_place(be, free, named, S, at):
     be.h2d(c.bufs[1], c.pos)
     got = c.check()
     assert not np.any(got[at])
+    c.free()
+
+
+# ------------------------------------------------------------------ the expanded form's range ----
+
+@pytest.mark.parametrize("kind,wsigma,csigma", [("bf16", 1.0, 1e-30), ("bf16", 1e-30, 1.0), ("bf16", 1e10, 1e-33), ("bf16", 1.0, 1e25), ("bf16", 1e25, 1.0), ("bf16", 1e-15, 1e33),
+                                                ("bf16", 1e-33, 1e33), ("f16", 1.0, 1e-6), ("f16", 1.0, 1e4)])
+@pytest.mark.parametrize("rope", [0, 32])
+def test_norms_whose_squares_pass_32_bits(be, kind, wsigma, csigma, rope):
+    """latents and matrices whose squares' sum is 0 or infinite in 32 bits"""
+    c = Prompt(be, 3, kind, 2, 128, rope, 64, 64, 16, 40, 60, wsigma=wsigma, csigma=csigma, f32=True)
+    if rope:                                                           # (rotary keys of a size with the others)
+        rng = np.random.default_rng(4)
+        stored, _ = normal(rng, kind, *c.cells.shape[:2], rope, sigma=min(wsigma * csigma, 1e4))
+        live = np.isfinite(from_bits(c.cells[..., :1]))
+        c.cells[..., 128:] = np.where(live, stored, NAN[kind])
+        c.cache.free()
+        c.cache = Latents(be, kind, c.cells, 128)
+    c.check()
+    c.free()
+
+
+@pytest.mark.parametrize("size", [1.0, 1e12, 1e30])
+def test_rotary_keys_beside_none(be, size):
+    """Wk of zeros: the scores are the rotary part's alone, of any size"""
+    c = Prompt(be, 5, "bf16", 2, 128, 32, 64, 64, 16, 40, 60, f32=True)
+    c.wk[...], c.wk64[...] = 0, 0.0
+    live = np.isfinite(from_bits(c.cells[..., :1]))
+    c.cells[..., 128:] = np.where(live, normal(np.random.default_rng(6), "bf16", *c.cells.shape[:2], 32, sigma=size)[0], NAN["bf16"])
+    c.scale = float(np.float32(c.scale / size))
+    c.cache.free()
+    c.cache = Latents(be, "bf16", c.cells, 128)
+    be.h2d(c.bufs[1], c.wk)
+    c.check()
+    c.free()
+
+
+@pytest.mark.parametrize("by", [2.0 ** 15, 1e20])
+def test_one_large_latent_behind(be, by):
+    """a token whose latent is so many times the others': rows before it stay within the bound (which counts 2^-31 of the largest key and value),
+    and finite"""
+    c = Prompt(be, 7, "bf16", 2, 128, 32, 64, 64, 16, 40, 60, f32=True)
+    at = c.pages[99 // 16], 99 % 16
+    c.cells[at[0], at[1], :128] = to_type(from_bits(c.cells[at[0], at[1], :128]) * by, "bf16")[0]
+    c.cache.free()
+    c.cache = Latents(be, "bf16", c.cells, 128)
+    got, (want, bound) = c.run(), c.want()
+    assert np.all(np.isfinite(got))
+    assert np.all(np.abs(got - want) <= bound)
     c.free()
