@@ -18,7 +18,7 @@ __device__ __forceinline__ uint32_t lt_pack(float a, float b) {
     else return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16);
 }
 // eight values of a rotary part whose pairs are 4 u .. 4 u + 3: read as its halves' values 4 u .. 4 u + 3 or
-// (interleaved) as 8 u .. 8 u + 7, turned, and written in the same places
+// (interleaved) as 8 u .. 8 u + 7, turned (np pairs of the part, all or none: none are written as they are), and written in the same places
 struct LtPairs { sw_f32x4 a, b; };
 __device__ __forceinline__ LtPairs lt_read(const float *x, int u, int dims, bool inter) {
     LtPairs p;
@@ -27,15 +27,15 @@ __device__ __forceinline__ LtPairs lt_read(const float *x, int u, int dims, bool
     return p;
 }
 template <int TYPE>
-__device__ __forceinline__ void lt_turn(LtPairs p, int u, int dims, bool inter, const float *s_cs, const float *s_sn, uint16_t *to) {
+__device__ __forceinline__ void lt_turn(LtPairs p, int u, int dims, int np, bool inter, const float *s_cs, const float *s_sn, uint16_t *to) {
     const sw_f32x4 cs = *(const sw_f32x4 *)(s_cs + 4 * u), sn = *(const sw_f32x4 *)(s_sn + 4 * u);
     float x[4], y[4], v[4], w[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         x[e] = inter ? (e < 2 ? p.a[2 * e] : p.b[2 * e - 4]) : p.a[e];
         y[e] = inter ? (e < 2 ? p.a[2 * e + 1] : p.b[2 * e - 3]) : p.b[e];
-        v[e] = __builtin_fmaf(x[e], cs[e], -(y[e] * sn[e]));
-        w[e] = __builtin_fmaf(y[e], cs[e], x[e] * sn[e]);
+        v[e] = np ? __builtin_fmaf(x[e], cs[e], -(y[e] * sn[e])) : x[e];
+        w[e] = np ? __builtin_fmaf(y[e], cs[e], x[e] * sn[e]) : y[e];
     }
     if (inter) {
         *(sw_u32x4 *)(to + 8 * u) = sw_u32x4{lt_pack<TYPE>(v[0], w[0]), lt_pack<TYPE>(v[1], w[1]), lt_pack<TYPE>(v[2], w[2]), lt_pack<TYPE>(v[3], w[3])};
@@ -58,11 +58,7 @@ __global__ __launch_bounds__(LA_NT) void k_latent_append(SwLatent c, SwRows r, S
     if (pos < 0) return;
     const bool inter = rope.interleaved;
     auto angles = [&] {
-        if (tid < dims / 2) {
-            s_cs[tid] = 1.f;
-            s_sn[tid] = 0.f;
-            if (tid < rope.np) lt_angle(rope.freq[tid], pos, rope.factor, s_cs[tid], s_sn[tid]);
-        }
+        if (tid < rope.np) lt_angle(rope.freq[tid], pos, rope.factor, s_cs[tid], s_sn[tid]);
         __syncthreads();
     };
     if (blockIdx.y == 0) {                                             // wave 0 the latent, wave 1 the rotary part
@@ -89,7 +85,7 @@ __global__ __launch_bounds__(LA_NT) void k_latent_append(SwLatent c, SwRows r, S
             if (page >= 0 && 8 * lane < c.rank)
                 *(sw_u32x4 *)(cell + 8 * lane) = sw_u32x4{lt_pack<TYPE>(a[0], a[1]), lt_pack<TYPE>(a[2], a[3]), lt_pack<TYPE>(b[0], b[1]), lt_pack<TYPE>(b[2], b[3])};
         } else if (page >= 0 && 8 * lane < dims) {
-            lt_turn<TYPE>(p, lane, dims, inter, s_cs, s_sn, cell + c.rank);
+            lt_turn<TYPE>(p, lane, dims, rope.np, inter, s_cs, s_sn, cell + c.rank);
         }
         return;
     }
@@ -112,7 +108,7 @@ __global__ __launch_bounds__(LA_NT) void k_latent_append(SwLatent c, SwRows r, S
         if (8 * k < nope)
             *(sw_u32x4 *)(qn + s * nrs + h * nhs + 8 * k) = sw_u32x4{lt_pack<TYPE>(p[i].a[0], p[i].a[1]), lt_pack<TYPE>(p[i].a[2], p[i].a[3]),
                                                                      lt_pack<TYPE>(p[i].b[0], p[i].b[1]), lt_pack<TYPE>(p[i].b[2], p[i].b[3])};
-        else lt_turn<TYPE>(p[i], k - nope / 8, dims, inter, s_cs, s_sn, qr + s * rrs + h * rhs);
+        else lt_turn<TYPE>(p[i], k - nope / 8, dims, rope.np, inter, s_cs, s_sn, qr + s * rrs + h * rhs);
     }
 }
 

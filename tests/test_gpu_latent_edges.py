@@ -75,3 +75,30 @@ def test_one_large_latent_behind(be, by):
     assert np.all(np.isfinite(got))
     assert np.all(np.abs(got - want) <= bound)
     c.free()
+
+
+# ------------------------------------------------------------------ appended without a turn ----
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("inter", [False, True])
+def test_what_is_not_turned_passes_as_it_is(be, kind, inter):
+    """without a rope a rotary part is rounded and no more: infinities and NaN stay beside their partners, -0 keeps its sign"""
+    S, H, rank, rope, nope, P = 3, 2, 128, 32, 16, 8
+    rng = np.random.default_rng(2)
+    ckv, q = rng.standard_normal((S, rank + rope)).astype(np.float32), rng.standard_normal((S, H, nope + rope)).astype(np.float32)
+    odd = np.array([np.inf, -0.0, np.nan, 0.0, -np.inf, -0.0], np.float32)
+    for x, at in ((ckv, rank), (q, nope)):
+        x[..., at:at + 6], x[..., at + rope // 2 + 3:at + rope // 2 + 9] = odd, odd[::-1]
+    cache = Latents(be, kind, normal(rng, kind, 1, P, rank + rope)[0], rank)
+    one = np.zeros(S * H * (nope + rope), np.uint16)
+    b = [be.upload(np.ascontiguousarray(a)) for a in (np.arange(S, dtype=np.int32), np.zeros(S, np.int32), np.zeros(1, np.int32), ckv, q, one)]
+    pd, sd, td, cd, qd, od = b
+    width = nope + rope
+    be.latent_append(cache.c, be.kv_rows(pd, td, 1, 1, sd), None, cd, rank + rope, None, 1e-6, qd, H * width, H, nope,
+                     be.heads(od, H * width, width), be.heads(int(od) + 2 * nope, H * width, width), S)
+    nan = lambda a: np.where(np.isnan(from_bits(a)), np.uint16(0xFFFF), np.uint16(0))              # (any NaN is one)
+    same = lambda a, f: np.array_equal(a.view(np.uint16) | nan(a), to_type(f, kind)[0].view(np.uint16) | nan(to_type(f, kind)[0]))
+    assert same(cache.read()[0, :S], ckv)
+    assert same(be.d2h(od, (S, H, width), np.float16 if kind == "f16" else np.uint16), q)
+    for x in b + [cache]:
+        x.free()
