@@ -101,6 +101,8 @@ class DeviceStack:
         from Backend.sample_params or None, random numbers [S] on the device)"""
         be, D = self.be, self.cfg.D
         desc = desc_of(self.cfg)
+        if trees is not None and not self.attn:
+            raise ValueError("step: trees need a stack with attention layers")
         if self.attn:
             if cache is None or rows is None or cache.n_layers != len(self.attn):
                 raise ValueError("step: a stack with attention needs a cache of its layers, and rows")
