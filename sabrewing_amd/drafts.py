@@ -69,7 +69,7 @@ class DraftTrees:
             raise ValueError("DraftTrees.place: the trees before are neither committed nor dropped")
         batch = [(index(s), tree_of(parents, self.max_nodes), [index(p) for p in parents], np.array([index(t) for t in tokens], np.int32)) for s, parents, tokens in batch]
         used = sum(len(p) for _, _, p, _ in batch)
-        rest = (rows or used) - used
+        rest = (used if rows is None else index(rows)) - used
         if not 1 <= len(batch) <= T or any(len(p) != len(t) for _, _, p, t in batch):
             raise ValueError(f"DraftTrees.place: 1 to {T} trees, a token of each node")
         if not 0 <= rest <= (T - len(batch)) * self.max_nodes:

@@ -32,3 +32,17 @@ def test_trees_and_a_stack_without_attention():
         step(be, st, cache, rows, S, t)
     assert not be.calls
     step(be, st, None, None, S)
+
+
+def test_places_for_no_rows():
+    be = R()
+    cache = PagedCache(be, 1, 8, 8, 2, 32, max_seqs=3)
+    t = DraftTrees(cache)
+    s = cache.open()
+    for rows in (0, 1, -1):
+        with pytest.raises(ValueError):
+            t.place([(s, [-1, 0], [1, 2])], rows=rows)
+    with pytest.raises(TypeError):
+        t.place([(s, [-1, 0], [1, 2])], rows=2.0)
+    assert cache.length(s) == 0
+    assert t.place([(s, [-1, 0], [1, 2])], rows=2)[1] == 2
