@@ -13,6 +13,8 @@ from operator import index
 
 import numpy as np
 
+from .latent import LatentCache
+
 
 def tree_of(parents, max_nodes=64):
     """(depths [n], sees [n] u64) of a tree given by its nodes' parents: -1 for node 0, of every other an
@@ -32,6 +34,8 @@ class DraftTrees:
     that a recorded step replays over what the next place() puts there."""
 
     def __init__(self, cache, max_trees=None, max_nodes=32):
+        if isinstance(cache, LatentCache):
+            raise ValueError("DraftTrees: over a PagedCache, not over latents")
         self.cache, self.be = cache, cache.be
         self.max_trees, self.max_nodes = max_trees or cache.max_seqs, max_nodes
         if not 1 <= self.max_trees <= 65535 or not 1 <= max_nodes <= 64:

@@ -4,6 +4,7 @@ import pytest
 from sabrewing_amd.attention import AttnConfig, PagedCache
 from sabrewing_amd.backend import Backend
 from sabrewing_amd.drafts import DraftTrees
+from sabrewing_amd.latent import LatentCache
 from sabrewing_amd.stack import DeviceStack
 from test_attention_stack_host import Recorder, stack
 
@@ -46,3 +47,10 @@ def test_places_for_no_rows():
         t.place([(s, [-1, 0], [1, 2])], rows=2.0)
     assert cache.length(s) == 0
     assert t.place([(s, [-1, 0], [1, 2])], rows=2)[1] == 2
+
+
+def test_trees_over_latents():
+    """at their making: place() would take cells that no step may fill and no commit can move"""
+    be = R()
+    with pytest.raises(ValueError):
+        DraftTrees(LatentCache(be, 1, 8, 8, 128, 16, max_seqs=3))
