@@ -90,6 +90,7 @@ class PagedCache:
         self._table = np.full((max_seqs, self.max_pages), -1, np.int32)
         self._dirty = set()
         self._rows = np.full((2, self.max_rows), -1, np.int32)             # positions, sequences
+        self.rows_made = 0                                                 # calls of rows() that were answered: the arrays hold the last one's
         self.dev_rows, self.dev_table = be.upload(self._rows), be.upload(self._table)
         self.desc = be.kv_rows(self.dev_rows, self.dev_table, max_seqs, self.max_pages, int(self.dev_rows) + 4 * self.max_rows)
 
@@ -252,6 +253,7 @@ class PagedCache:
             raise
         for s in old:
             self._changed(s)
+        self.rows_made += 1
         return self.desc, total
 
     def _upload(self):

@@ -53,6 +53,7 @@ class DraftTrees:
         self.desc = self.be.trees(first, base, sees, int(cache.dev_table), T, cache.max_seqs, cache.max_pages, max_nodes, seq, self.at)
         self.window = 0                                                    # the narrowest of the layers that were run over the trees
         self._depth = 0                                                    # of the placed trees' deepest node
+        self.rows_made = 0                                                 # the cache's when they were placed
         self._placed, self._marks, self.rows = None, (), 0                 # (rows: of the placed trees' step)
 
     def within(self, window):
@@ -102,7 +103,7 @@ class DraftTrees:
             for s, start, _ in placed:
                 cache.truncate(s, start)
             raise
-        self._placed, self._marks, self._depth, self.rows = placed, marks, deepest, total
+        self._placed, self._marks, self._depth, self.rows, self.rows_made = placed, marks, deepest, total, cache.rows_made
         return desc, total
 
     def commit(self, tok):

@@ -46,10 +46,12 @@ class LatentConfig:
 
 
 class LatentPrompt:
-    """the n rows of a prompt: `rows` for appending, where its sequence's pages are listed, its first position"""
+    """the n rows of a prompt: `rows` for appending, where its sequence's pages are listed, its first position; of a cache's
+    prompt(), the cache and its rows_made"""
 
-    def __init__(self, rows, pages, n_pages, start, n):
-        self.rows, self.pages, self.n_pages, self.start, self.n = rows, pages, n_pages, start, n
+    def __init__(self, rows, pages, n_pages, start, n, cache=None):
+        self.rows, self.pages, self.n_pages, self.start, self.n, self.cache = rows, pages, n_pages, start, n, cache
+        self.rows_made = cache.rows_made if cache is not None else 0
 
 
 class LatentCache(PagedCache):
@@ -77,7 +79,7 @@ class LatentCache(PagedCache):
         """rows((seq, n)) for a step that takes a prompt's keys and values from its latents once: (LatentPrompt, n)"""
         start = self.length(seq)
         rows, total = self.rows([(seq, n)])
-        return LatentPrompt(rows, int(self.dev_table) + 4 * seq * self.max_pages, len(self._pages[seq]), start, n), total
+        return LatentPrompt(rows, int(self.dev_table) + 4 * seq * self.max_pages, len(self._pages[seq]), start, n, self), total
 
 
 class DeviceLatentAttention:

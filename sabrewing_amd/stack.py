@@ -18,7 +18,7 @@ from . import synth
 from .attention import AttnScratch, DeviceAttention, Rope
 from .backend import DeviceLayer, desc_of
 from .configs import WEIGHT_SIGMA
-from .latent import DeviceLatentAttention, LatentCache, LatentConfig, LatentScratch
+from .latent import DeviceLatentAttention, LatentCache, LatentConfig, LatentPrompt, LatentScratch
 
 NORM_EPS = 1e-6
 
@@ -97,7 +97,8 @@ class DeviceStack:
         fused: each layer's RMSNorm inside its routing launch (lag_hip_moe_forward_rmsnorm,
         the same bits as the separate rmsnorm + forward); cache, rows: the PagedCache and the
         descriptor of its rows() for the S tokens (a stack with attention layers), or of a LatentCache's
-        prompt(); trees: the DraftTrees over that cache whose place() gave the rows; draw: (settings
+        prompt(); trees: the DraftTrees over that cache whose place() gave the rows (a cache has the rows of its last rows(), prompt() or
+        place() alone); draw: (settings
         from Backend.sample_params or None, random numbers [S] on the device)"""
         be, D = self.be, self.cfg.D
         desc = desc_of(self.cfg)
@@ -114,6 +115,11 @@ class DeviceStack:
                 raise ValueError("step: trees over another cache, or over latents")
             if trees is not None and S != trees.rows:
                 raise ValueError("step: another number of rows than the placed trees have")
+            if isinstance(rows, LatentPrompt) and rows.cache is not None and rows.cache is not cache:
+                raise ValueError("step: a prompt of another cache")
+            for made in (trees, rows if isinstance(rows, LatentPrompt) and rows.cache is not None else None):
+                if made is not None and made.rows_made != cache.rows_made:
+                    raise ValueError("step: the cache has made other rows since the trees or the prompt")
             if trees is not None:
                 for a in self.attn:
                     trees.within(a.acfg.window)
