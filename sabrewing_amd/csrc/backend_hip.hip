@@ -1104,10 +1104,11 @@ extern "C" int lag_hip_tree_commit(const LagHipKvCache *layers, int n_layers, co
     if (!parent || !draft || !tok) return refuse(me, "no parents, drafted tokens or picks");
     if (!path || !count || !next) return refuse(me, "no place for the paths, their lengths or the next tokens");
     const struct { const int *p; size_t n; } reads[] = {{parent, (size_t)S}, {draft, (size_t)S}, {tok, (size_t)S},
-                                                        {t->first, (size_t)t->n_trees + 1}, {t->base, (size_t)t->n_trees}},
+                                                        {t->first, (size_t)t->n_trees + 1}, {t->base, (size_t)t->n_trees},
+                                                        {t->seq, t->seq ? (size_t)t->n_trees : 0}, {t->table, (size_t)t->n_seqs * t->max_pages}},
         writes[] = {{path, (size_t)t->n_trees * t->max_nodes}, {count, (size_t)t->n_trees}, {next, (size_t)t->n_trees}};
     for (auto &w : writes) {
-        for (auto &r : reads) if (!apart(w.p, w.n * 4, r.p, r.n * 4)) return refuse(me, "results that overlap what is read");
+        for (auto &r : reads) if (r.n && !apart(w.p, w.n * 4, r.p, r.n * 4)) return refuse(me, "results that overlap what is read");
         for (auto &v : writes) if (&v != &w && !apart(w.p, w.n * 4, v.p, v.n * 4)) return refuse(me, "results that overlap");
     }
     if (not_ready(me)) return -1;
