@@ -122,6 +122,9 @@ static int grow_pinned(Buf &b, size_t need) {
     return 0;
 }
 static Buf g_arena, g_hin, g_hout;
+// A latent prompt's scratch, a GiB and more, is its own: steps recorded after one do not take as much with them.
+static Buf g_prompt;
+static bool g_prompt_recorded;          // in the open recording, which then takes it
 // The last forward's expert groups (lag_hip_last_groups): 1, their lists on the device, in the arena or the fixed
 // region; 0, a count alone.  What takes the arena next writes its first bytes, and frees it where it has to grow.
 static int g_last_G_dev = 0, g_last_ng = 0;
@@ -1287,9 +1290,10 @@ extern "C" int lag_hip_attn_latent_prompt(const LagHipLatentCache *c, const int 
     if (!apart(out, no, q, (size_t)S * n_heads * (nope + c->rope_dims) * 2) || !apart(out, no, wk, w * nope) || !apart(out, no, wv, w * v_dim))
         return refuse(me, "out overlaps what is read");
     if (not_ready(me)) return -1;
-    if (take_arena((size_t)sw_latent_prompt_bytes(lc, n_heads, nope, v_dim, (int64_t)start + S))) return -1;
+    if (grow_dev(g_prompt, (size_t)sw_latent_prompt_bytes(lc, n_heads, nope, v_dim, (int64_t)start + S))) return -1;
+    if (g_capturing) g_prompt_recorded = true;
     PROF("attn_latent_prompt");
-    if (sw_launch_latent_prompt(g_st, lc, pages, n_seq_pages, start, wk, wv, nope, v_dim, q, n_heads, scale, out, out_f32 != 0, S, g_arena.p))
+    if (sw_launch_latent_prompt(g_st, lc, pages, n_seq_pages, start, wk, wv, nope, v_dim, q, n_heads, scale, out, out_f32 != 0, S, g_prompt.p))
         return fail_msg("attn_latent_prompt launch");
     return 0;
 }
@@ -1424,16 +1428,18 @@ extern "C" const char *lag_hip_last_error(void) { return g_err; }
 // move memory that a live graph replays over.  A recording that starts with
 // no arena (the previous recording took it) first allocates one of the
 // capacity the last arena had, so graphs of the same shapes can be recorded
-// back to back; shapes beyond that capacity need an eager call first.
+// back to back; shapes beyond that capacity need an eager call first.  So with the
+// latent prompts' scratch, which only recordings that use it take.
 // Destroying a graph while another recording is open is deferred to the end
 // of that recording (a stream synchronisation would break the capture).
-struct GraphRec { hipGraphExec_t exec; Buf arena; };
-static size_t g_arena_last_cap = 0;
+struct GraphRec { hipGraphExec_t exec; Buf arena, prompt; };
+static size_t g_arena_last_cap = 0, g_prompt_last_cap = 0;
 static std::vector<GraphRec *> g_graph_deferred;
 static void graph_free(GraphRec *r) {
     (void)hipStreamSynchronize(g_st);   // no replay may still be reading the buffers
     (void)hipGraphExecDestroy(r->exec);
     if (r->arena.p) (void)hipFree(r->arena.p);
+    if (r->prompt.p) (void)hipFree(r->prompt.p);
     delete r;
 }
 extern "C" int lag_hip_graph_begin(void) {
@@ -1443,8 +1449,13 @@ extern "C" int lag_hip_graph_begin(void) {
         CK(hipMalloc(&g_arena.p, g_arena_last_cap), "device scratch allocation");
         g_arena.cap = g_arena_last_cap;
     }
+    if (!g_prompt.p && g_prompt_last_cap) {                             // (without it a recorded prompt is refused, no other call)
+        if (hipMalloc(&g_prompt.p, g_prompt_last_cap) == hipSuccess) g_prompt.cap = g_prompt_last_cap;
+        else { g_prompt.p = nullptr; (void)hipGetLastError(); }
+    }
     CK(hipStreamBeginCapture(g_st, hipStreamCaptureModeRelaxed), "begin capture");
     g_capturing = 1;
+    g_prompt_recorded = false;
     return 0;
 }
 extern "C" void *lag_hip_graph_end(void) {
@@ -1459,9 +1470,10 @@ extern "C" void *lag_hip_graph_end(void) {
     e = hipGraphInstantiate(&exec, graph, nullptr, nullptr, 0);
     (void)hipGraphDestroy(graph);
     if (e != hipSuccess) { fail("graph instantiate", e); return nullptr; }
-    GraphRec *r = new GraphRec{exec, g_arena};
+    GraphRec *r = new GraphRec{exec, g_arena, g_prompt_recorded ? g_prompt : Buf{}};
     if (g_arena.cap) g_arena_last_cap = g_arena.cap;
     g_arena = Buf{};
+    if (g_prompt_recorded) { g_prompt_last_cap = g_prompt.cap; g_prompt = Buf{}; }
     g_last_G_dev = 0;                   // the last groups now live in the graph's arena
     g_last_ng = 0;
     return (void *)r;
