@@ -352,7 +352,10 @@ int    lag_hip_attn_latent(const LagHipLatentCache *c, const LagHipKvRows *r, co
  * attends to the tokens t <= start + s.  nope and v_dim: multiples of 32 up to 256.  Keys and values are made once a call, rounded to 11 bits
  * (f16, scaled by a power of two for each head: what is more than 2^20 below the largest of a head's, over all of the call's tokens, loses bits); sums and the softmax in 32 bits,
  * its weights in 11.  Cells that lead nowhere are not attended to; cells that are no numbers reach the rows that attend to them.  Everything
- * is 16-byte aligned; out overlaps nothing that is read.  start + S <= 2^22.  Its scratch (2 (rank + 64) bytes a token, and a GiB at most of keys and values) is its own, which a recording of it takes.  0 = ok */
+ * is 16-byte aligned; out overlaps nothing that is read.  start + S <= 2^22.  Its scratch is its own, and a recording of it keeps it:
+ * 2 (rank + 64) bytes a token, and keys and values, 2 (nope + v_dim) bytes a token and head with each rounded up to 64, 128 or 256, of as many
+ * heads at a time as a GiB holds, but of one at least (4 GiB for 2^22 tokens of 256 + 256).  It is allocated twice as large as a call needs
+ * when it grows.  0 = ok */
 int    lag_hip_attn_latent_prompt(const LagHipLatentCache *c, const int *pages, int n_seq_pages, int start, const void *wk, const void *wv, int nope,
                                   int v_dim, const void *q, int n_heads, float scale, void *out, int out_f32, int S);
 /* x[i] += t[i] for n values: the residual after an output projection.  t may be x, or does

@@ -359,7 +359,7 @@ __global__ __launch_bounds__(FL_NT, (lp_occ<NOPE, DV>())) void k_prompt(const ui
 }
 
 // ------------------------------------------------------------------ scratch and launches ----
-// heads expanded at a time: what they take stays about a GiB
+// heads expanded at a time: as many as a GiB holds, and one at least (beyond 2^20 tokens of 256 + 256 that is more, up to 4 GiB)
 struct LpPlan { int64_t T32, xl, xr, te, re, vm, we, eh, kb, vb, total; int heads, np, vp; };
 static LpPlan lp_plan(const SwLatent &c, int H, int nope, int vd, int64_t T) {
     LpPlan p;
