@@ -283,8 +283,8 @@ typedef struct {
 } LagHipTrees;
 /* lag_hip_attn_paged for trees: out[s][h] = sum_t p_t v_t over the cells t < base of row s's tree (with window > 0 those with t >
  * max(pos[s], base) - window) and the cells base + j of the nodes that sees[s] names (whatever the window: a caller whose trees are
- * as deep as it clears the bits of ancestors that it leaves out).  A tree's cells are read once for all of its nodes.  q, out, scale and the accuracy as there; S rows in all.  A row that attends to nothing, or of a free
- * place, gives zeros; rows of no tree are left as they were.  An infinity or NaN in a cell reaches the rows that attend to it, as
+ * as deep as it clears the bits of ancestors that it leaves out).  A tree's cells are read once for all of its nodes.  q, out, scale and
+ * the accuracy as there; S rows in all.  A row that attends to nothing, or of a free place, gives zeros; rows of no tree are left as they were.  An infinity or NaN in a cell reaches the rows that attend to it, as
  * outputs without meaning, and no others.  max_pages * page_size <= 2^30.  0 = ok */
 int    lag_hip_attn_tree(const LagHipKvCache *c, const LagHipTrees *t, const float *q, int n_q_heads, float scale, int window,
                          float *out, int S);

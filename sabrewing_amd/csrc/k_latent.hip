@@ -137,7 +137,8 @@ int sw_launch_latent_append(hipStream_t st, const SwLatent &c, const SwRows &r, 
 // y[s, h] = W[h] x[s, h]: a wave takes OT x 32 outputs of a head and TT x 32 rows on the 32 x 32 matrix instructions, operands
 // straight from memory (a row of W is read by one wave, or from the caches by the few that share its outputs).  Up to 64 rows a wave takes 32 by 32,
 // as there are few waves; beyond 64 by 64, half the reads.  Bound by W's bytes: 128 heads of 512 x 128, one row 6.0 us (16.8 MB, 2.8 TB/s with the
-// launch), 64 rows of 128 x 512 with 32-bit outputs 11.0 us (29 MB).  Two steps' operands at a time instead of eight: 6.6 and 12.7.
+// launch), 64 rows of 128 x 512 with 32-bit outputs 11.0 us (29 MB), 256 rows 22 us
+// and of 512 x 128 27 us (67 and 59 MB, 195 and 156 TFLOP/s).  Two steps' operands at a time instead of eight: 6.6 and 12.7.
 #define LH_NT 256
 template <int TYPE, bool YF32, int OT, int TT>
 __global__ __launch_bounds__(LH_NT) void k_latent_heads(const uint16_t *__restrict__ x, int64_t xrs, int64_t xhs, const uint16_t *__restrict__ W, int H,
@@ -233,11 +234,15 @@ int sw_launch_latent_heads(hipStream_t st, int type, const SwHeads &x, const voi
 // ------------------------------------------------------------------ the absorbed form ----
 // Heads are the columns, a cell is key and value of all of them: 2 (2 rank + rope) operations a head for 2 (rank + rope) bytes.  Queries and outputs of 512
 // values by 32 columns are more than a wave's registers, so that waves share columns (sw_flash.h).  Rows' tiles are laid end to end and dealt to
-// 256 blocks as trees' are.  Bf16, rank 512 + 64: 32 rows of 128 heads over 100 to 16,384 cells 151 us: matrix instructions a
-// quarter of the cycles, vector ones 16 %, LDS 27 %, the rest waits at two barriers a tile of eight waves on a CU; the join's 10 us within.  One row
-// of 16 heads over 1,500 cells 18 us: a chain of waits, and the join's launch.
+// 256 blocks as trees' are.  Bf16, rank 512 + 64: 32 rows of 128 heads over 100 to 16,384 cells 139 to 158 us by the lengths drawn: matrix
+// instructions a quarter of the cycles, vector ones 16 %, LDS 27 %, the rest waits at two barriers a tile of eight waves on a CU; the join's 12 us
+// within.  One row of 16 heads over 1,500 cells 18 us: a chain of waits, and the join's launch.
+//
+// The softmax's weights are rounded once to the cells' type, 8 bits in bf16.  Weights in two parts double the second product, 13 us
+// more (158 -> 171) without what their exchange would add; they would bring the outputs' error, relative to 64 bits, from 0.0019 to the 0.0017 that
+// the outputs' own rounding to bf16 leaves.  attn_paged and attn_tree, whose outputs are of 32 bits, keep 24.
 #define LN_ROPE 64                                                     // a cell's rotary part in LDS: the rest of it zeros
-#define LN_SPLIT 256                                                   // beyond so many rows none is split: they fill the chip by themselves
+#define LN_SPLIT 256                                                   // beyond so many rows none is split: rows of like lengths fill the chip (of ragged ones the longest is waited for)
 // waves that share 32 heads (a share of the outputs is whole pairs of 32 values), and tiles in LDS
 template <int R> constexpr int ln_split() { return R % 256 == 0 ? 4 : 2; }
 template <int TYPE, int R> using LnFl = Fl<TYPE, 1, R + LN_ROPE, R, true, ln_split<R>()>;
@@ -358,8 +363,8 @@ __global__ __launch_bounds__(FL_NT) void k_latent_join(SwLatent c, SwRows r, int
     }
 }
 
-// Columns of a block (32 times wc) and blocks of each group of heads; 0: a block a row.  64 columns a block where there are more than 32: 128 heads 151 us,
-// in blocks of 128 columns (half the reads of cells, queries in LDS for want of registers) 20 more, with two waves to share 64 columns 40 more.
+// Columns of a block (32 times wc) and blocks of each group of heads; 0: a block a row.  64 columns a block where there are more than 32: 128 heads 151 us
+// at the time, in blocks of 128 columns (half the reads of cells, queries in LDS for want of registers) 20 more, with two waves to share 64 columns 40 more.
 struct LnPlan { int wc, groups, B; };
 static LnPlan ln_plan(const SwLatent &c, const SwRows &r, int H, int S) {
     LnPlan p;

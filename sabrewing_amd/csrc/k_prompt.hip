@@ -1,15 +1,16 @@
 // k_prompt.hip -- latent attention of a prompt's tokens, the expanded form: keys Wk[h] c_t and values Wv[h] c_t of every token
 // are made once, then out[s, h] = sum_t p_t v_t, p = softmax over t <= start + s of scale * q[s, h] . (k_t, r_t).
 //
-// Bf16, 32 heads of 128 + 64 and 128, rank 512: 2,048 tokens from position 6,000 on 431 us: the gathering 10, the expansion 110 (67 GFLOP, 610
-// TFLOP/s: eight lots of 64 values are few to fill the pipe), the attention 315 (295 GFLOP, 940 TFLOP/s: matrix instructions half of the cycles, vector
-// ones -- exponentials -- the rest).  300 tokens of 16 heads from the beginning 33 us, its three launches' begins and ends.
+// Bf16, 32 heads of 128 + 64 and 128, rank 512: 2,048 tokens from position 6,000 on 433 to 463 us by the card (362 GFLOP, 836 to 780 TFLOP/s).  Traced,
+// where the launches take longer than back to back: the gathering 10, the expansion 112 (67 GFLOP: eight lots of 64 values are few to fill the pipe),
+// the attention 358 (295 GFLOP: matrix instructions half of the cycles, vector ones -- exponentials -- the rest).  Heads of 192 and 256 are held as 256, one block
+// a CU: 747 us with 192 + 64 and 128, 1,108 with 256 + 64 and 256.  300 tokens of 16 heads from the beginning 34 us, its three launches' begins and ends.
 //
 // Three launches: cells gathered from their pages, keys and values of some heads expanded, their attention.  Against the
 // absorbed form a pair of tokens costs 2 (nope + rope + v) instead of 2 (2 rank + rope) operations, and a token 2 rank (nope + v) once.
 //
 // Keys and values are held in f16, whatever the cache's type: 11 bits, where bf16's 8 would add errors as large as the
-// output's own rounding three times over.  f16's range is met by powers of two: |k_d| <= |Wk_d| |c_t| (their 2-norms), so each
+// output's own rounding three times over.  (Outputs of 32 bits have no more: 24 would be three times the products.)  f16's range is met by powers of two: |k_d| <= |Wk_d| |c_t| (their 2-norms), so each
 // head's keys are scaled by 2^(15 - a - b), a and b the exponents of the largest |Wk_d| and |c_t|, which keeps them
 // below 2^15; a sum of many terms stays some 2^8 below that bound, and what is more than 2^20 smaller than the largest, of whichever
 // token, loses bits.  Values alike; queries are scaled to 2^13.  The rotary part stays as the cache has it.
@@ -129,7 +130,7 @@ __global__ __launch_bounds__(LP_NT) void k_prompt_gather(SwLatent c, const int *
 }
 
 // Keys and values of heads h0 .. of H: [head][tokens][np or vp] in f16, times 2^eh, the values behind nope or vd zeros (eh[2 H]: the
-// exponent of the largest rotary value of all tokens).  A block takes 128 outputs by 128 tokens, both in LDS by 64 of the summed values, two lots ahead; a wave 64 by 64 of them.  A die's blocks share
+// exponent of the largest rotary value of all tokens).  A block takes 128 outputs by 128 tokens, both in LDS by 64 of the summed values, one lot ahead; a wave 64 by 64 of them.  A die's blocks share
 // a range of tokens (they stay in its cache) and go through all heads.
 #define LE_K 64
 #define LE_TILE (128 * LE_K * 2)

@@ -6,9 +6,13 @@
 // meet 16-bit cells in parts of the cells' type, products exact in 32-bit sums (bf16 three parts, f16 two): that is what bounds a batch, each
 // cell costing three times the matrix instructions, and splitting the weights about as many cycles of vector instructions.
 // Trees' tiles are laid end to end and dealt to the blocks in equal shares, the parts of a tree joined by a second launch.  Bf16, 32 heads over 8
-// of 128: 16 trees of up to 26 nodes over 500 to 12,000 cells 148 us (matrix instructions 36 % of the cycles, vector 35 %); one tree of 8
-// nodes over 700 cells 24 us, 19 of them a chain of waits in 22 blocks of one tile a cache head, 6 the join.  Two parts of a weight
-// (16 bits) took 8 us less and doubled the error.
+// of 128: 16 trees of up to 26 nodes over 500 to 12,000 cells 147 to 164 us by the lengths drawn (matrix instructions 36 % of the cycles, vector
+// 35 %); one tree of 8 nodes over 700 cells 24 us, 19 of them a chain of waits in 22 blocks of one tile a cache head, 6 the join, over 60,000
+// cells 73 us (3.4 TB/s).  8 trees over up to 6,000 f32 cells 154 us.  Two parts of a weight (16 bits) took 8 us less and doubled the error.
+//
+// Registers: bf16 of 256 (both forms), and with up to 32 columns bf16 of 128 and 192 and f16 of 224, spill 14 to 43 of them, those of 256 within the
+// tiles' loop (a reload waits for the tiles on their way: time, not results).  f32 of 96, 128 and 160 and f16 of 160 with up to 32 columns run
+// one block a CU where tr_occ allows two, and have half of the blocks waiting.
 #include "sw_flash.h"
 
 // tree i: its rows, and the cells that any of them may attend to
@@ -210,7 +214,8 @@ __global__ __launch_bounds__(FL_NT) void k_tree_join(SwKv c, SwTrees t, int S, i
     }
 }
 
-// Columns of a block and blocks of each of their groups.  Up to 32 columns: a wave has them all and four take tiles in turn (one tile a wave
+// Columns of a block and blocks of each of their groups, by max_nodes and n_trees: what is placed is known on the device alone, so that 8 nodes in a
+// place for 32 take the form for more than 32 columns.  Up to 32 columns: a wave has them all and four take tiles in turn (one tile a wave
 // in flight costs less than three idle waves).  Beyond, four waves have 32 each and read one tile.  Two blocks a CU where registers allow.
 struct TrPlan { int wc, groups, B; };
 template <int TYPE, int DH>

@@ -184,9 +184,9 @@ __device__ __forceinline__ void fl_split(const float (&x)[8], sw_u32x4 (&o)[NP])
 }
 
 // A wave's 32 columns.  NP: parts that a 32-bit q and the weights are split into (1: 16-bit queries, one
-// rounding of the weights).  DK: values of a query, a multiple of 32; DV: of an output; INK: a cell's
+// rounding of the weights; k_latent.hip says what it costs and saves).  DK: values of a query, a multiple of 32; DV: of an output; INK: a cell's
 // first DV values of k are its v.  How much is read ahead of the products goes by the registers that queries and outputs leave: a
-// spilled one would be a load in the loop, and waiting for it would wait for every tile on its way.
+// spilled one is a load in the loop, and waiting for it waits for every tile on its way (k_tree.hip: where that is so).
 template <int TYPE, int NP, int DK, int DV, bool INK, int SPLIT = 1>
 struct Fl {
     static constexpr bool F32 = TYPE == SW_KV_F32;
