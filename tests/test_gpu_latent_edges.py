@@ -102,3 +102,18 @@ def test_what_is_not_turned_passes_as_it_is(be, kind, inter):
     assert same(be.d2h(od, (S, H, width), np.float16 if kind == "f16" else np.uint16), q)
     for x in b + [cache]:
         x.free()
+
+
+@pytest.mark.parametrize("H,start,S", [(3, 40, 60), (130, 0, 129)])
+@pytest.mark.parametrize("nope,vd", [(64, 64), (192, 96)])
+def test_rows_whose_rotary_part_outweighs_the_other(be, H, start, S, nope, vd):
+    """f16: every third row's other part is 2^-14 of the rotary one, so that its rotary scores are lifted, beside rows where they are not; and all cells at
+    1e-6, where every row's are"""
+    c = Prompt(be, 8, "f16", H, 128, 32, nope, vd, 16, start, S)
+    c.q[::3, :, :nope], c.q64[::3, :, :nope] = to_type(c.q64[::3, :, :nope] * 2.0 ** -14, "f16")
+    be.h2d(c.bufs[3], c.q)
+    c.check()
+    c.free()
+    c = Prompt(be, 9, "f16", H, 128, 32, nope, vd, 16, start, S, csigma=1e-6, f32=True)
+    c.check()
+    c.free()
