@@ -26,6 +26,27 @@ template <int TYPE> __device__ __forceinline__ float lp_float(uint32_t w, int hi
 // e with x < 2^e for a sum of squares x^2, in 64 bits: whatever finite values of 16 bits are squared, it is finite, and 0 where they all are
 #define LP_LEAST -140
 __device__ __forceinline__ int lp_exp(double x2) { return x2 > 0.0 ? (ilogb(x2) + 2) >> 1 : LP_LEAST; }
+// a + b of the lanes BY (16, 32) apart: of a in the lower of the two, of b in the upper
+template <int BY>
+__device__ __forceinline__ double lp_halves(double a, double b) {
+    const uint2 x = __builtin_bit_cast(uint2, a), y = __builtin_bit_cast(uint2, b);
+    if constexpr (BY == 16) {
+        const auto lo = __builtin_amdgcn_permlane16_swap(x.x, y.x, false, false), hi = __builtin_amdgcn_permlane16_swap(x.y, y.y, false, false);
+        return __builtin_bit_cast(double, make_uint2((uint32_t)lo[0], (uint32_t)hi[0])) + __builtin_bit_cast(double, make_uint2((uint32_t)lo[1], (uint32_t)hi[1]));
+    } else {
+        const auto lo = __builtin_amdgcn_permlane32_swap(x.x, y.x, false, false), hi = __builtin_amdgcn_permlane32_swap(x.y, y.y, false, false);
+        return __builtin_bit_cast(double, make_uint2((uint32_t)lo[0], (uint32_t)hi[0])) + __builtin_bit_cast(double, make_uint2((uint32_t)lo[1], (uint32_t)hi[1]));
+    }
+}
+// x plus the value of the lane that a rotation in rows of 16 lanes brings
+template <int DPP>
+__device__ __forceinline__ double lp_turned(double x) {
+    const uint2 u = __builtin_bit_cast(uint2, x);
+    return x + __builtin_bit_cast(double, make_uint2((uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.x, DPP, 0xF, 0xF, false),
+                                                     (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u.y, DPP, 0xF, 0xF, false)));
+}
+// a wave's largest exponent
+__device__ __forceinline__ int lp_max(int e) { return (int)sw_wave_max((uint32_t)(e + 1024)) - 1024; }
 
 // Blocks 0 .. tiles - 1: 32 cells side by side in xl [tokens][rank] and xr [tokens][64] (zeros where there is no cell or no value), te: the
 // exponent of the tile's largest norm, re: of its largest rotary value, vm: which tokens have a cell.  Blocks behind them, LP_PARTS for a head's keys and as many for its
@@ -90,8 +111,7 @@ __global__ __launch_bounds__(LP_NT) void k_prompt_gather(SwLatent c, const int *
 #pragma unroll
             for (int e = 0; e < 8; e++) turned = fmaxf(turned, fabsf(finite(b[i][e / 2], e & 1)));
         }
-#pragma unroll
-        for (int o = LP_ROPE / 16; o; o >>= 1) turned = fmaxf(turned, __shfl_xor(turned, o));
+        turned = __builtin_bit_cast(float, sw_wave_max(__builtin_bit_cast(uint32_t, turned)));         // (none is negative)
     } else {
         const int k = (blockIdx.x - tiles) / LP_PARTS, part = (blockIdx.x - tiles) % LP_PARTS, h = k >> 1, n = k & 1 ? vd : nope;
         const uint16_t *w = (k & 1 ? wv : wk) + (int64_t)h * n * c.rank;
@@ -101,20 +121,13 @@ __global__ __launch_bounds__(LP_NT) void k_prompt_gather(SwLatent c, const int *
 #pragma unroll
         for (int i = 0; i < N; i++) ss[i] = squares(a[i], i0 + i < end);
     }
-    // the rows' sums, half of the rows with each half of the lanes: 10 exchanges instead of 48
+    // the rows' sums: halves and quarters of the rows go to halves and quarters of the lanes, whose 16 lanes add up two rows each
     static_assert(N == 8, "rows of a wave");
 #pragma unroll
-    for (int o = 32, n = N / 2; n; o >>= 1, n >>= 1)
+    for (int i = 0; i < 4; i++) ss[i] = lp_halves<32>(ss[i], ss[i + 4]);
 #pragma unroll
-        for (int i = 0; i < n; i++) {
-            const double give = lane & o ? ss[i] : ss[i + n], keep = lane & o ? ss[i + n] : ss[i];
-            ss[i] = keep + __shfl_xor(give, o);
-        }
-#pragma unroll
-    for (int o = 4; o; o >>= 1) ss[0] = ss[0] + __shfl_xor(ss[0], o);
-    int best = lp_exp(ss[0]);
-#pragma unroll
-    for (int o = 32; o >= 8; o >>= 1) best = max(best, __shfl_xor(best, o));
+    for (int i = 0; i < 2; i++) ss[i] = lp_turned<0x121>(lp_turned<0x122>(lp_turned<0x124>(lp_turned<0x128>(lp_halves<16>(ss[i], ss[i + 2])))));
+    int best = lp_max(max(lp_exp(ss[0]), lp_exp(ss[1])));
     if (lane == 0) { s_n[wave] = best; s_r[wave] = turned; s_v[wave] = there << (wave * N); }
     __syncthreads();
     if (tid == 0) {
@@ -167,7 +180,8 @@ __global__ __launch_bounds__(LP_NT, 2) void k_prompt_expand(const uint16_t *__re
     load(0);
     int e = LP_LEAST, r = LP_LEAST;
     for (int i = tid; i < T32 / 32; i += LP_NT) { e = max(e, te[i]); r = max(r, re[i]); }
-    for (int o = 32; o; o >>= 1) { e = max(e, __shfl_xor(e, o)); r = max(r, __shfl_xor(r, o)); }
+    e = lp_max(e);
+    r = lp_max(r);
     if (lane == 0) { s_e[wave] = e; s_r[wave] = r; }
     __syncthreads();
     int w = LP_LEAST;
