@@ -1,10 +1,11 @@
 // k_prompt.hip -- latent attention of a prompt's tokens, the expanded form: keys Wk[h] c_t and values Wv[h] c_t of every token
 // are made once, then out[s, h] = sum_t p_t v_t, p = softmax over t <= start + s of scale * q[s, h] . (k_t, r_t).
 //
-// Bf16, 32 heads of 128 + 64 and 128, rank 512: 2,048 tokens from position 6,000 on 433 to 463 us by the card (362 GFLOP, 836 to 780 TFLOP/s).  Traced,
+// Bf16, 32 heads of 128 + 64 and 128, rank 512: 2,048 tokens from position 6,000 on 433 to 476 us by the card (362 GFLOP, 836 to 760 TFLOP/s).  Traced,
 // where the launches take longer than back to back: the gathering 10, the expansion 112 (67 GFLOP: eight lots of 64 values are few to fill the pipe),
 // the attention 358 (295 GFLOP: matrix instructions half of the cycles, vector ones -- exponentials -- the rest).  Heads of 192 and 256 are held as 256, one block
-// a CU: 747 us with 192 + 64 and 128, 1,108 with 256 + 64 and 256.  300 tokens of 16 heads from the beginning 34 us, its three launches' begins and ends.
+// a CU: 747 us with 192 + 64 and 128, 1,108 with 256 + 64 and 256.  300 tokens of 16 heads from the beginning 33 us, its three launches' begins
+// and ends.
 //
 // Three launches: cells gathered from their pages, keys and values of some heads expanded, their attention.  Against the
 // absorbed form a pair of tokens costs 2 (nope + rope + v) instead of 2 (2 rank + rope) operations, and a token 2 rank (nope + v) once.
@@ -265,6 +266,7 @@ struct LpFl : Fl<SW_KV_F16, 1, NOPE, DV, false> {
         this->alone(t, whole, bad, seen, s);
     }
 };
+// blocks a CU (with 32 rows a block, heads of 128 + 128 and of 256 + 64 take registers for one all the same)
 template <int NOPE, int DV> constexpr int lp_occ() { return NOPE / 4 + DV / 2 <= 112 ? 2 : 1; }
 template <int TYPE, int NOPE, int DV, int WC> constexpr int lp_ns() {
     constexpr int n = (lp_occ<NOPE, DV>() == 2 ? 78 : 156) * 1024 / (FL_NW / WC * LpFl<TYPE, NOPE, DV>::TB);
