@@ -298,7 +298,8 @@ int    lag_hip_qk_rope_append_at(const LagHipKvCache *c, const LagHipKvRows *r, 
  * path [n_trees][max_nodes] (indices of the path's nodes, then -1), count [n_trees] (its length; a free place or a tree without
  * nodes: 0) and next [n_trees] (the pick at its last node; -1 without one), and moves the cells of the path's nodes together: node
  * path[i]'s k and v to cell base + i, in every one of n_layers caches (one geometry and type).  Cells behind base + count
- * hold what they held.  Cells that lead nowhere are left out.  parent, draft, tok: [S].  sees and pos of t are not used.  0 = ok */
+ * hold what they held.  Cells that lead nowhere are left out.  A tree's cells are its own: no other tree of the call has a node or a path's
+ * place in them (one tree of a sequence, in pages that no other holds).  What is written overlaps nothing that is read.  parent, draft, tok: [S].  sees and pos of t are not used.  0 = ok */
 int    lag_hip_tree_commit(const LagHipKvCache *layers, int n_layers, const LagHipTrees *t, const int *parent, const int *draft,
                            const int *tok, int *path, int *count, int *next, int S);
 /* Page src[i] of every one of n_layers caches (one geometry and type) to page dst[i], k and v:

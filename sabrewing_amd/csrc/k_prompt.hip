@@ -2,7 +2,7 @@
 // are made once, then out[s, h] = sum_t p_t v_t, p = softmax over t <= start + s of scale * q[s, h] . (k_t, r_t).
 //
 // Bf16, 32 heads of 128 + 64 and 128, rank 512: 2,048 tokens from position 6,000 on 433 to 476 us by the card (362 GFLOP, 836 to 760 TFLOP/s).  Traced,
-// where the launches take longer than back to back: the gathering 10, the expansion 112 (67 GFLOP: eight lots of 64 values are few to fill the pipe),
+// where the launches take longer than back to back: the gathering 9.5, the expansion 112 (67 GFLOP: eight lots of 64 values are few to fill the pipe),
 // the attention 358 (295 GFLOP: matrix instructions half of the cycles, vector ones -- exponentials -- the rest).  Heads of 192 and 256 are held as 256, one block
 // a CU: 747 us with 192 + 64 and 128, 1,108 with 256 + 64 and 256.  300 tokens of 16 heads from the beginning 33 us, its three launches' begins
 // and ends.
